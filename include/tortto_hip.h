@@ -451,6 +451,52 @@ int tt_nll_loss_fwd_f32(const float* logp, const long long* target, const float*
 int tt_nll_loss_bwd_f32(const float* g, const long long* target, const float* weight, const float* count,
                         float* dlogp, int R, int C, long long ignore_index, int reduction);
 
+/* ---- layer normalisation and logits over a vocabulary ------------------------------------------ */
+
+/* Rows are [R, D] resp. [R, V], contiguous.  Values named `void*` are float32 or float16 as their dtype argument says
+ * (the two of a call's tensors that share one are alike); everything else is float32, and so are all sums and
+ * statistics.  A result in float16 is rounded once, as it is stored. */
+enum { TT_F32 = 0, TT_F16 = 1 };
+
+/* Layer normalisation over the last D values (`LayerNorm`, autograd/grad_nn.py:993-1052): y = (x - mean) * rstd * w + b
+ * with the biased variance, rstd = 1 / sqrt(var + eps); w, b [D] or NULL (1, 0).  mean, rstd [R] are kept for the
+ * backward pass, or both NULL.  The backward writes what is not NULL of dx [R, D] and of dw, db [D], which are summed
+ * over the rows in an order that only the sizes decide. */
+int tt_layer_norm_fwd(const void* x, const float* w, const float* b, void* y, float* mean, float* rstd, double eps,
+                      int dtype, long long R, int D);
+int tt_layer_norm_bwd(const void* x, const void* dy, const float* w, const float* mean, const float* rstd, void* dx,
+                      float* dw, float* db, int dtype, long long R, int D);
+
+/* Of each row of logits x [R, V]: the log probability of its token, the entropy of its distribution, and the K largest
+ * log probabilities (0 <= K <= 64) with their places, best first, the lowest place first among equals.  tokens: int64 or
+ * int32 as token_bits says; negative ones count from the end.  No counterpart in the reference.
+ *   - a row whose token is ignore_index is not read: zeros, places -1, gradient 0;
+ *   - a token outside [-V, V) gives NaN for its log probability and its gradient row;
+ *   - a row of -inf alone: -inf, entropy 0, alternatives -inf, gradient 0;
+ *   - a NaN or +inf in a row gives NaN for all its values and -1 for its places.
+ * stats [R][2] are kept for the backward pass, or NULL.  The backward adds up the gradients of what the forward returned
+ * (each may be NULL) and writes dx [R, V]; entropy and top_index are the forward's. */
+int tt_token_log_prob_fwd(const void* x, const void* tokens, float* logp, float* entropy, float* top_logp,
+                          long long* top_index, float* stats, int dtype, int token_bits, long long ignore_index,
+                          long long R, int V, int K);
+int tt_token_log_prob_bwd(const void* x, const void* tokens, const float* stats, const float* entropy,
+                          const long long* top_index, const float* g_logp, const float* g_entropy, const float* g_top,
+                          void* dx, int dtype, int token_bits, long long ignore_index, long long R, int V, int K);
+
+/* Distillation of a student's logits x [R, V] from the K largest logits of a teacher (1 <= K <= 1024): with
+ * q = softmax(teacher / temperature) over a row's entries and p = softmax(x / temperature) over all V,
+ *   loss_r = temperature^2 sum_k q_k (log q_k - log p[index_k]),   dx_j = g temperature (p_j - sum_(k: index_k = j) q_k).
+ * index (int64 or int32 as index_bits says) < 0 is no entry; one from V on makes the row NaN.  Entries of one index add
+ * up.  A row without entries, or with -inf alone, has loss and gradient 0 and does not count.  reduction as in
+ * tt_nll_loss_fwd_f32; count [1] receives the number of rows that have a teacher, stats [R][2] are for the backward.
+ * No counterpart in the reference. */
+int tt_distill_fwd(const void* x, const void* teacher, const void* index, float* loss, float* stats, float* count,
+                   double temperature, int reduction, int dtype, int teacher_dtype, int index_bits, long long R, int V,
+                   int K);
+int tt_distill_bwd(const void* x, const void* teacher, const void* index, const float* stats, const float* count,
+                   const float* g, void* dx, double temperature, int reduction, int dtype, int teacher_dtype,
+                   int index_bits, long long R, int V, int K);
+
 /* ---- optimiser steps (optim/_functional.py:4-119) ---------------------------------------------- */
 
 /* One SGD update of a parameter in place (_functional.py:4-22): d = grad (+ weight_decay * param);

@@ -5,6 +5,7 @@ import warnings
 import numpy as np
 
 from .tensor import Tensor, float32
+from .xparray import hiparray
 
 
 def manual_seed(seed):
@@ -41,6 +42,18 @@ def tensor(data, requires_grad=False, dtype=None, copy=True, **kwargs):
     if dtype is None:
         dtype = getattr(data, 'dtype', float32)
     return Tensor(data, requires_grad=requires_grad, dtype=dtype, copy=copy, **kwargs)
+
+
+def as_tensor(data, requires_grad=False):
+    """A device tensor on the memory of an object with ``__cuda_array_interface__`` (a torch or CuPy array), without a
+    copy; see ``hiparray.borrow`` for what its owner has to keep to.  Tensors come back as they are."""
+    if isinstance(data, Tensor):
+        return data
+    array = hiparray.borrow(data)
+    out = Tensor(array, dtype=array._dtype, copy=False)
+    if requires_grad:
+        out.requires_grad = True
+    return out
 
 
 # ---- the few array functions the classifier head of the ResNet examples uses ----------------------

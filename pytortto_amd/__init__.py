@@ -11,12 +11,13 @@ __version__ = '0.1.0'
 import numpy as np
 
 from .xparray import nparray, hiparray
-from .tensor import Tensor, float16, float32, float64, int16, int32, int64
-from .VariableFunctions import (manual_seed, empty, zeros, ones, randn, tensor, transpose, swapaxes, swapdims,
+from .tensor import Tensor, backward, float16, float32, float64, int16, int32, int64
+from .VariableFunctions import (manual_seed, empty, zeros, ones, randn, tensor, as_tensor, transpose, swapaxes, swapdims,
                                 mean, flatten, mm, matmul)
 from .autograd import (no_grad, enable_grad, set_grad_enabled, is_grad_enabled, Function, AccumulateGrad,
                        ToCopy, Add, Convolution, TransposedConvolution, BatchNorm, Relu, LeakyRelu,
-                       MaxPool2DWithIndices, LogSoftmax, NllLoss, View, Transpose, Mm, Mean)
+                       MaxPool2DWithIndices, LogSoftmax, NllLoss, LayerNorm, TokenLogProb, DistillLoss,
+                       View, Transpose, Mm, Mean)
 from .serialization import save, load
 from . import nn
 from . import optim

@@ -13,6 +13,7 @@ from ._paths import LIB_PATH
 
 _P = c_void_p
 _I = c_int
+_L = ctypes.c_longlong
 
 # name -> argument types (every function returns int, except tt_last_error)
 PROTOTYPES = {
@@ -94,6 +95,12 @@ PROTOTYPES = {
     'tt_log_softmax_bwd_f32': [_P, _P, _P, _I, _I],
     'tt_nll_loss_fwd_f32': [_P, _P, _P, _P, _P, _I, _I, ctypes.c_longlong, _I],
     'tt_nll_loss_bwd_f32': [_P, _P, _P, _P, _P, _I, _I, ctypes.c_longlong, _I],
+    'tt_layer_norm_fwd': [_P] * 6 + [c_double, _I, _L, _I],
+    'tt_layer_norm_bwd': [_P] * 8 + [_I, _L, _I],
+    'tt_token_log_prob_fwd': [_P] * 7 + [_I, _I, _L, _L, _I, _I],
+    'tt_token_log_prob_bwd': [_P] * 9 + [_I, _I, _L, _L, _I, _I],
+    'tt_distill_fwd': [_P] * 6 + [c_double] + [_I] * 4 + [_L, _I, _I],
+    'tt_distill_bwd': [_P] * 7 + [c_double] + [_I] * 4 + [_L, _I, _I],
     'tt_sgd_step_f32': [_P, _P, _P, c_size_t, c_double, c_double, c_double, c_double, _I, _I],
     'tt_sgd_step_multi_f32': [_I, _P, _P, _P, _P, _P, c_double, c_double, c_double, c_double, _I],
     'tt_adam_step_f32': [_P, _P, _P, _P, _P, c_size_t, _I, c_double, c_double, c_double, c_double, c_double, _I, _I],

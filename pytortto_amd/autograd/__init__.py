@@ -4,3 +4,4 @@ from .helper import build_links, toposort, inplace_precheck, inplace_update
 from .grad_fcn import ToCopy, Add, Unsqueeze, Squeeze, View, Transpose, Mm, Mean
 from .grad_nn import (Convolution, TransposedConvolution, BatchNorm, Relu, LeakyRelu, MaxPool2DWithIndices,
                       LogSoftmax, NllLoss)
+from .grad_vocab import LayerNorm, TokenLogProb, DistillLoss

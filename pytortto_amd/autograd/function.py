@@ -208,12 +208,12 @@ def build_links(data, grad_fn, copy=False, _output_idx=0):
     return _Tensor(data, dtype=dtype, copy=copy)
 
 
-def toposort(end_node):
+def toposort(*end_nodes):
     """helper.py:53-82: yield nodes so that a node comes after everything that feeds gradient
     into it; nodes whose other consumers are not part of this backward pass are taken from
-    the ``waiting`` set once nothing else is ready."""
-    ready = [end_node]
-    waiting = set()
+    the ``waiting`` set once nothing else is ready.  Of several end nodes, one that others lead to waits for them."""
+    ready = [node for node in end_nodes if node.prev_function_counts == 0]
+    waiting = {node for node in end_nodes if node.prev_function_counts}
     while ready or waiting:
         node = ready.pop() if ready else waiting.pop()
         yield node

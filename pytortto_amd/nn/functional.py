@@ -4,6 +4,7 @@
 from ..autograd.grad_fcn import Squeeze, Unsqueeze
 from ..autograd.grad_nn import (BatchNorm, Convolution, LeakyRelu, LogSoftmax, MaxPool2DWithIndices, NllLoss, Relu,
                                 TransposedConvolution)
+from ..autograd.grad_vocab import DistillLoss, LayerNorm, TokenLogProb
 
 
 def pad(input, pad, mode='constant', value=0.0):
@@ -79,3 +80,33 @@ def linear(input, weight, bias):
     if bias is not None:
         return matmul(input, weight.T) + bias
     return matmul(input, weight.T)
+
+
+def layer_norm(input, normalized_shape, weight=None, bias=None, eps=1e-5):
+    """(input - mean) / sqrt(var + eps) * weight + bias over the trailing dimensions ``normalized_shape``.  The input is
+    float32 or float16, weight and bias are float32."""
+    if normalized_shape.__class__ is int:
+        normalized_shape = (normalized_shape,)
+    return LayerNorm.apply(input, weight, bias, normalized_shape=normalized_shape, eps=eps)
+
+
+def token_log_prob(input, tokens, top=0, ignore_index=-100):
+    """Of logits [..., V] and int64 or int32 tokens [...]: ``(logp, entropy)``, the log probability of each token and the
+    entropy of its distribution, in nats and float32; with ``top`` also ``(top_logp, top_index)`` [..., top], the best
+    alternatives, best first and the lowest index first among equals (at most 64).
+
+    Negative tokens count from the end.  A position whose token is ``ignore_index`` is not looked at: zeros, and -1 for
+    the indexes.  A token outside the vocabulary gives NaN, and so does a NaN or +inf among the logits (indexes -1).
+    Logits of -inf alone leave log probabilities of -inf, entropy 0 and no gradient.  ``tt.backward`` takes gradients of
+    several of the outputs in one pass."""
+    return TokenLogProb.apply(input, tokens=tokens, top=top, ignore_index=ignore_index)
+
+
+def distill_loss(input, teacher, index, temperature=1.0, reduction='mean'):
+    """Kullback-Leibler divergence, times temperature^2, of a student's distribution softmax(input / temperature) over V
+    classes from a teacher's over its K best: ``teacher`` [..., K] holds their logits (log probabilities do as well),
+    ``index`` [..., K] their classes, int64 or int32, and -1 where there is no entry.
+
+    Entries of one class add up.  Positions without an entry, or with -inf alone, have loss and gradient 0 and are not
+    counted by 'mean'; an index of V or more gives NaN.  Gradients flow to ``input`` only."""
+    return DistillLoss.apply(input, teacher=teacher, index=index, temperature=float(temperature), reduction=reduction)

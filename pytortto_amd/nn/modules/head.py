@@ -59,6 +59,34 @@ class Linear(Module):
         return F.linear(x, self.weight, self.bias)
 
 
+class LayerNorm(Module):
+    """Normalisation over the trailing dimensions (``src/tortto/nn/modules/normalization.py``); weight = 1, bias = 0."""
+
+    def __init__(self, normalized_shape, eps=1e-5, elementwise_affine=True, bias=True):
+        super().__init__()
+        shape = (normalized_shape,) if normalized_shape.__class__ is int else tuple(normalized_shape)
+        self.__dict__.update(normalized_shape=shape, eps=eps, elementwise_affine=elementwise_affine)
+        self.register_parameter('weight', Parameter(_vf.ones(shape)) if elementwise_affine else None)
+        self.register_parameter('bias', Parameter(_vf.zeros(shape)) if elementwise_affine and bias else None)
+
+    def extra_repr(self):
+        return f'{self.normalized_shape}, eps={self.eps}, elementwise_affine={self.elementwise_affine}'
+
+    def forward(self, inpt):
+        return F.layer_norm(inpt, self.normalized_shape, self.weight, self.bias, self.eps)
+
+
+class DistillLoss(Module):
+    """``F.distill_loss`` with its temperature and reduction kept."""
+
+    def __init__(self, temperature=1.0, reduction='mean'):
+        super().__init__()
+        self.temperature, self.reduction = temperature, reduction
+
+    def forward(self, inpt, teacher, index):
+        return F.distill_loss(inpt, teacher, index, self.temperature, self.reduction)
+
+
 class NLLLoss(Module):
     def __init__(self, weight=None, ignore_index=-100, reduction='mean'):
         super().__init__()

@@ -655,3 +655,112 @@ def nll_loss_bwd(g, logp_shape, target, weight, count, ignore_index, reduction):
     _hip.call('tt_nll_loss_bwd_f32', g.ptr, target.ptr, _ptr(weight), count.ptr, dlogp.ptr, r, c,
               int(ignore_index), _REDUCTIONS[reduction])
     return dlogp
+
+
+# ---- layer normalisation and logits over a vocabulary ---------------------------------------------
+
+_TYPES = {np.dtype(np.float32): 0, np.dtype(np.float16): 1}
+_INDEX_BITS = {np.dtype(np.int64): 64, np.dtype(np.int32): 32}
+MOST_ALTERNATIVES = 64
+MOST_TEACHER_ENTRIES = 1024
+
+
+def _kind(a, what):
+    kind = _TYPES.get(a._dtype)
+    if kind is None:
+        raise TypeError(f'{what} must be float32 or float16, got {a._dtype}')
+    return kind
+
+
+def _index_bits(a, what):
+    bits = _INDEX_BITS.get(a._dtype)
+    if bits is None:
+        raise TypeError(f'{what} must be int64 or int32, got {a._dtype}')
+    return bits
+
+
+def layer_norm_fwd(x, weight, bias, width, eps, keep):
+    """(y, mean, rstd) over the trailing ``width`` values; the statistics are None unless ``keep``."""
+    kind = _kind(x, 'the input of layer_norm')
+    _f32(weight, bias)
+    rows = x.size // width
+    y = hiparray.empty(x._shape, x._dtype)
+    mean, rstd = (hiparray.empty((rows,)), hiparray.empty((rows,))) if keep else (None, None)
+    if rows:
+        _hip.call('tt_layer_norm_fwd', x.ptr, _ptr(weight), _ptr(bias), y.ptr, _ptr(mean), _ptr(rstd), eps, kind, rows,
+                  width)
+    return y, mean, rstd
+
+
+def layer_norm_bwd(x, dy, weight, mean, rstd, width, need):
+    """(dx, dweight, dbias), each None unless needed."""
+    kind = _kind(x, 'the input of layer_norm')
+    if dy._dtype != x._dtype or dy._shape != x._shape:
+        raise TypeError(f'the gradient of layer_norm must be like its output, {x._dtype} {x._shape}, got {dy._dtype} '
+                        f'{dy._shape}')
+    rows = x.size // width
+    dx = hiparray.empty(x._shape, x._dtype) if need[0] else None
+    make = hiparray.empty if rows else hiparray.zeros
+    dw = make((width,)) if need[1] else None
+    db = make((width,)) if need[2] else None
+    if rows:
+        _hip.call('tt_layer_norm_bwd', x.ptr, dy.ptr, _ptr(weight), mean.ptr, rstd.ptr, _ptr(dx), _ptr(dw), _ptr(db),
+                  kind, rows, width)
+    return dx, dw, db
+
+
+def token_log_prob_fwd(x, tokens, top, ignore_index, keep):
+    """(logp, entropy, top_logp, top_index, stats); the alternatives are None without ``top``, the statistics unless
+    ``keep``."""
+    kind, bits = _kind(x, 'logits'), _index_bits(tokens, 'tokens')
+    rows, vocab = tokens.size, x._shape[-1]
+    logp, entropy = hiparray.empty(tokens._shape), hiparray.empty(tokens._shape)
+    top_logp = top_index = None
+    if top:
+        top_logp, top_index = hiparray.empty(tokens._shape + (top,)), hiparray.empty(tokens._shape + (top,), np.int64)
+    stats = hiparray.empty((rows, 2)) if keep else None
+    if rows:
+        _hip.call('tt_token_log_prob_fwd', x.ptr, tokens.ptr, logp.ptr, entropy.ptr, _ptr(top_logp), _ptr(top_index),
+                  _ptr(stats), kind, bits, ignore_index, rows, vocab, top)
+    return logp, entropy, top_logp, top_index, stats
+
+
+def token_log_prob_bwd(x, tokens, stats, entropy, top_index, gradients, top, ignore_index):
+    """dlogits from the gradients of (logp, entropy, top_logp), each of which may be None."""
+    _f32(*gradients)
+    rows = tokens.size
+    dx = hiparray.empty(x._shape, x._dtype)
+    if rows:
+        _hip.call('tt_token_log_prob_bwd', x.ptr, tokens.ptr, stats.ptr, entropy.ptr, _ptr(top_index),
+                  *[_ptr(g) for g in gradients], dx.ptr, _TYPES[x._dtype], _INDEX_BITS[tokens._dtype], ignore_index,
+                  rows, x._shape[-1], top)
+    return dx
+
+
+def distill_fwd(x, teacher, index, temperature, reduction):
+    """(loss, stats, count)."""
+    kinds, bits = (_kind(x, 'logits'), _kind(teacher, "the teacher's logits")), _index_bits(index, "the teacher's indexes")
+    red = _REDUCTIONS[reduction]
+    vocab, entries = x._shape[-1], index._shape[-1]
+    rows = index.size // entries
+    loss = hiparray.empty(x._shape[:-1] if red == 0 else ())
+    stats, count = hiparray.empty((rows, 2)), hiparray.empty((1,))
+    if rows:
+        _hip.call('tt_distill_fwd', x.ptr, teacher.ptr, index.ptr, loss.ptr, stats.ptr, count.ptr, temperature, red,
+                  *kinds, bits, rows, vocab, entries)
+    elif red:
+        loss.fill(0.0 if red == 1 else math.nan)
+    return loss, stats, count
+
+
+def distill_bwd(x, teacher, index, stats, count, g, temperature, reduction):
+    """dlogits."""
+    _f32(g)
+    entries = index._shape[-1]
+    rows = index.size // entries
+    dx = hiparray.empty(x._shape, x._dtype)
+    if rows:
+        _hip.call('tt_distill_bwd', x.ptr, teacher.ptr, index.ptr, stats.ptr, count.ptr, g.ptr, dx.ptr, temperature,
+                  _REDUCTIONS[reduction], _TYPES[x._dtype], _TYPES[teacher._dtype], _INDEX_BITS[index._dtype], rows,
+                  x._shape[-1], entries)
+    return dx

@@ -189,14 +189,26 @@ class Tensor:
     # ---- autograd ------------------------------------------------------------------------------
     def backward(self, gradient=None):
         """tensor.py:568-613."""
-        from .autograd.function import AccumulateGrad
-        from .autograd.helper import toposort
+        gradient = self._start_gradient(gradient)
+        if self.grad_fn:
+            self.grad_fn.grad[self._output_idx] = gradient
+            _propagate((self.grad_fn,))
+        else:
+            self._accumulate(gradient)
+
+    def _start_gradient(self, gradient):
+        """The array that a backward pass from here starts with."""
         if not self.requires_grad:
             raise RuntimeError('element 0 of tensors does not require grad and does not have a grad_fn')
         on_device = self.data.__class__ is hiparray
         if gradient is None:
-            one = np.ones((1,) * self.data.ndim, dtype=self.data.dtype)
-            gradient = hiparray(one) if on_device else one
+            shape = (1,) * self.data.ndim
+            if on_device and self.data._dtype == np.float32:
+                gradient = hiparray.empty(shape)
+                gradient.fill(1.0)              # (an upload would wait for all that has been launched)
+            else:
+                one = np.ones(shape, dtype=self.data.dtype)
+                gradient = hiparray(one) if on_device else one
         elif isinstance(gradient, Tensor):
             if gradient.device != self.device:
                 raise RuntimeError(f'invalid gradient at index 0 - expected device {self.device} '
@@ -206,29 +218,58 @@ class Tensor:
             gradient = gradient.data.lent() if on_device else gradient.data.copy().view(np.ndarray)
         if self.data.shape != gradient.shape:
             raise RuntimeError('grad can be implicitly created only for scalar outputs')
-        if self.grad_fn:
-            self.grad_fn.grad[self._output_idx] = gradient
-            for node in toposort(self.grad_fn):
-                grads = node.apply(*node.grad)
-                for i, (fn, idx) in enumerate(node.next_functions):   # empty for leaf accumulators
-                    g = grads[i]
-                    if g is None:
-                        continue
-                    if fn.grad[idx] is None:
-                        fn.grad[idx] = g if g.__class__ is hiparray else np.ascontiguousarray(g)
-                    elif fn.grad[idx].__class__ is hiparray and fn.grad[idx]._shared and g.__class__ is hiparray:
-                        # the first arrival is an alias of somebody else's gradient (hiparray.alias):
-                        # the sum goes to a new array instead of copying it and adding in place
-                        from . import ops
-                        fn.grad[idx] = ops.add(fn.grad[idx], g)
-                    else:
-                        fn.grad[idx] += g
-                node.clear()
+        return gradient
+
+    def _accumulate(self, gradient):
+        from .autograd.function import AccumulateGrad
+        acc = AccumulateGrad()
+        acc.variable = self
+        acc.grad = (gradient,)
+        acc.apply(*acc.grad)
+
+
+def _add_gradient(fn, idx, g):
+    if fn.grad[idx] is None:
+        fn.grad[idx] = g if g.__class__ is hiparray else np.ascontiguousarray(g)
+    elif fn.grad[idx].__class__ is hiparray and fn.grad[idx]._shared and g.__class__ is hiparray:
+        # the first arrival is an alias of somebody else's gradient (hiparray.alias):
+        # the sum goes to a new array instead of copying it and adding in place
+        from . import ops
+        fn.grad[idx] = ops.add(fn.grad[idx], g)
+    else:
+        fn.grad[idx] += g
+
+
+def _propagate(end_nodes):
+    from .autograd.helper import toposort
+    for node in toposort(*end_nodes):
+        grads = node.apply(*node.grad)
+        for i, (fn, idx) in enumerate(node.next_functions):   # empty for leaf accumulators
+            g = grads[i]
+            if g is not None:
+                _add_gradient(fn, idx, g)
+        node.clear()
+
+
+def backward(tensors, gradients=None):
+    """One backward pass from several tensors (the outputs of one operation, as a rule): ``gradients`` holds a
+    tensor for each, or None for a scalar.  Not in the reference, whose pass starts at one tensor."""
+    tensors = [tensors] if isinstance(tensors, Tensor) else list(tensors)
+    if isinstance(gradients, Tensor):
+        gradients = [gradients]
+    gradients = [None] * len(tensors) if gradients is None else list(gradients)
+    if len(gradients) != len(tensors):
+        raise RuntimeError(f'got {len(tensors)} tensors and {len(gradients)} gradients')
+    starts = [t._start_gradient(g) for t, g in zip(tensors, gradients)]
+    end_nodes = {}
+    for t, g in zip(tensors, starts):
+        if t.grad_fn:
+            _add_gradient(t.grad_fn, t._output_idx, g)
+            end_nodes[id(t.grad_fn)] = t.grad_fn
         else:
-            acc = AccumulateGrad()
-            acc.variable = self
-            acc.grad = (gradient,)
-            acc.apply(*acc.grad)
+            t._accumulate(g)
+    if end_nodes:
+        _propagate(end_nodes.values())
 
 
 class Parameter(Tensor):

@@ -153,6 +153,18 @@ class _Loan(_Buffer):
             _unfilled.discard(self)
 
 
+class _Borrowed(_Buffer):
+    """A block that somebody else allocated; ``owner`` is kept for as long as an array refers to it."""
+    __slots__ = ('owner',)
+
+    def __init__(self, ptr, nbytes, owner):
+        super().__init__(nbytes, lazy=True)
+        self._ptr, self.owner = ptr, owner
+
+    def __del__(self):
+        pass
+
+
 # buffers whose contents are still to be produced on demand, or lent by another (normally none or a handful: the
 # array of an absorbed BatchNorm or Add output lives only as long as somebody holds its tensor)
 _unfilled = weakref.WeakSet()
@@ -237,7 +249,33 @@ class hiparray:
     def empty_like(cls, other):
         return cls.empty(other.shape, other.dtype)
 
+    @classmethod
+    def borrow(cls, source):
+        """An array on the device memory of ``source``, an object with ``__cuda_array_interface__`` (a torch or
+        CuPy array); nothing is copied and ``source`` is kept alive.  Its writers must be done, or be ordered in
+        front of the library's stream, before the array is used; and memory is borrowed once, not as two arrays."""
+        about = source.__cuda_array_interface__
+        shape, dtype = tuple(about['shape']), np.dtype(about['typestr'])
+        nbytes = prod(shape) * dtype.itemsize
+        if about.get('mask') is not None:
+            raise ValueError('borrowed device memory cannot be masked')
+        strides = about.get('strides')
+        if strides is not None and nbytes:
+            whole = dtype.itemsize
+            for n, step in zip(reversed(shape), reversed(strides)):
+                if n != 1 and step != whole:
+                    raise ValueError(f'device arrays are C-contiguous, got strides {tuple(strides)} for shape {shape}')
+                whole *= n
+        return cls.on(_Borrowed(about['data'][0] or 0, nbytes, source) if nbytes else _Buffer(0), shape, dtype)
+
     # ---- ndarray-like attributes ----------------------------------------------------------
+    @property
+    def __cuda_array_interface__(self):
+        """For torch, CuPy and the like to use the memory in place (``torch.as_tensor(array, device='cuda')``); the
+        library's stream has to be waited for, or the device, before they read what it computes."""
+        return {'shape': self._shape, 'typestr': self._dtype.str, 'data': (self.ptr, False), 'strides': None,
+                'version': 2}
+
     @property
     def ptr(self):
         buf = self._buf
