@@ -489,13 +489,16 @@ int tt_token_log_prob_bwd(const void* x, const void* tokens, const float* stats,
  * index (int64 or int32 as index_bits says) < 0 is no entry; one from V on makes the row NaN.  Entries of one index add
  * up.  A row without entries, or with -inf alone, has loss and gradient 0 and does not count.  reduction as in
  * tt_nll_loss_fwd_f32; count [1] receives the number of rows that have a teacher, stats [R][2] are for the backward.
- * No counterpart in the reference. */
+ * No counterpart in the reference.
+ * Where tt_distill_ahead says yes the forward can write the gradient for g = 1 to dx in the visit that computes the loss
+ * (dx = NULL: it does not); the backward, told so by is_ahead and given that dx, then works for another g only. */
+int tt_distill_ahead(int* yes, int dtype, int reduction, long long R, int V);
 int tt_distill_fwd(const void* x, const void* teacher, const void* index, float* loss, float* stats, float* count,
-                   double temperature, int reduction, int dtype, int teacher_dtype, int index_bits, long long R, int V,
-                   int K);
+                   void* dx, double temperature, int reduction, int dtype, int teacher_dtype, int index_bits,
+                   long long R, int V, int K);
 int tt_distill_bwd(const void* x, const void* teacher, const void* index, const float* stats, const float* count,
-                   const float* g, void* dx, double temperature, int reduction, int dtype, int teacher_dtype,
-                   int index_bits, long long R, int V, int K);
+                   const float* g, void* dx, double temperature, int reduction, int is_ahead, int dtype,
+                   int teacher_dtype, int index_bits, long long R, int V, int K);
 
 /* ---- optimiser steps (optim/_functional.py:4-119) ---------------------------------------------- */
 

@@ -99,8 +99,9 @@ PROTOTYPES = {
     'tt_layer_norm_bwd': [_P] * 8 + [_I, _L, _I],
     'tt_token_log_prob_fwd': [_P] * 7 + [_I, _I, _L, _L, _I, _I],
     'tt_token_log_prob_bwd': [_P] * 9 + [_I, _I, _L, _L, _I, _I],
-    'tt_distill_fwd': [_P] * 6 + [c_double] + [_I] * 4 + [_L, _I, _I],
-    'tt_distill_bwd': [_P] * 7 + [c_double] + [_I] * 4 + [_L, _I, _I],
+    'tt_distill_ahead': [POINTER(c_int), _I, _I, _L, _I],
+    'tt_distill_fwd': [_P] * 7 + [c_double] + [_I] * 4 + [_L, _I, _I],
+    'tt_distill_bwd': [_P] * 7 + [c_double] + [_I] * 5 + [_L, _I, _I],
     'tt_sgd_step_f32': [_P, _P, _P, c_size_t, c_double, c_double, c_double, c_double, _I, _I],
     'tt_sgd_step_multi_f32': [_I, _P, _P, _P, _P, _P, c_double, c_double, c_double, c_double, _I],
     'tt_adam_step_f32': [_P, _P, _P, _P, _P, c_size_t, _I, c_double, c_double, c_double, c_double, c_double, _I, _I],

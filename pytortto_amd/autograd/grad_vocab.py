@@ -103,10 +103,11 @@ class DistillLoss(Function):
             raise ValueError(f'{params["reduction"]} is not a valid value for reduction')
         if not (math.isfinite(params['temperature']) and 1e-6 <= params['temperature'] <= 1e6):
             raise ValueError(f'the temperature must be in 1e-6 to 1e6, got {params["temperature"]}')
-        yd0, stats, count = ops.distill_fwd(xd0, td0, id0, params['temperature'], params['reduction'])
+        keep = ctx.requires_grad and is_grad_enabled()
+        yd0, stats, count, dx = ops.distill_fwd(xd0, td0, id0, params['temperature'], params['reduction'], keep)
         yt0 = build_links(yd0, grad_fn=ctx)
         ctx.save_for_backward(xt0, teacher, index)
-        ctx.params.update(stats=stats, count=count)
+        ctx.params.update(stats=stats, count=count, dx=dx)
         return yt0
 
     @staticmethod
@@ -114,4 +115,4 @@ class DistillLoss(Function):
         gd0, = grad_outputs
         x, teacher, index = ctx.saved_tensors
         p = ctx.params
-        return ops.distill_bwd(x, teacher, index, p['stats'], p['count'], gd0, p['temperature'], p['reduction'])
+        return ops.distill_bwd(x, teacher, index, p['stats'], p['count'], gd0, p['dx'], p['temperature'], p['reduction'])

@@ -737,30 +737,43 @@ def token_log_prob_bwd(x, tokens, stats, entropy, top_index, gradients, top, ign
     return dx
 
 
-def distill_fwd(x, teacher, index, temperature, reduction):
-    """(loss, stats, count)."""
+@functools.lru_cache(maxsize=1024)
+def _distill_ahead(kind, reduction, rows, vocab):
+    yes = ctypes.c_int()
+    _hip.call('tt_distill_ahead', ctypes.byref(yes), kind, reduction, rows, vocab)
+    return bool(yes.value)
+
+
+def distill_fwd(x, teacher, index, temperature, reduction, need_grad):
+    """(loss, stats, count, dx): with ``need_grad`` dx is the gradient for an incoming one of 1 where the forward pass
+    has it for one more write of the row; else None."""
     kinds, bits = (_kind(x, 'logits'), _kind(teacher, "the teacher's logits")), _index_bits(index, "the teacher's indexes")
     red = _REDUCTIONS[reduction]
     vocab, entries = x._shape[-1], index._shape[-1]
     rows = index.size // entries
     loss = hiparray.empty(x._shape[:-1] if red == 0 else ())
     stats, count = hiparray.empty((rows, 2)), hiparray.empty((1,))
+    dx = None
     if rows:
-        _hip.call('tt_distill_fwd', x.ptr, teacher.ptr, index.ptr, loss.ptr, stats.ptr, count.ptr, temperature, red,
-                  *kinds, bits, rows, vocab, entries)
+        if need_grad and _distill_ahead(kinds[0], red, rows, vocab):
+            dx = hiparray.empty(x._shape, x._dtype)
+        _hip.call('tt_distill_fwd', x.ptr, teacher.ptr, index.ptr, loss.ptr, stats.ptr, count.ptr, _ptr(dx), temperature,
+                  red, *kinds, bits, rows, vocab, entries)
     elif red:
         loss.fill(0.0 if red == 1 else math.nan)
-    return loss, stats, count
+    return loss, stats, count, dx
 
 
-def distill_bwd(x, teacher, index, stats, count, g, temperature, reduction):
-    """dlogits."""
+def distill_bwd(x, teacher, index, stats, count, g, dx, temperature, reduction):
+    """dlogits; ``dx`` is the forward's, or None."""
     _f32(g)
     entries = index._shape[-1]
     rows = index.size // entries
-    dx = hiparray.empty(x._shape, x._dtype)
+    ahead = dx is not None
+    if not ahead:
+        dx = hiparray.empty(x._shape, x._dtype)
     if rows:
         _hip.call('tt_distill_bwd', x.ptr, teacher.ptr, index.ptr, stats.ptr, count.ptr, g.ptr, dx.ptr, temperature,
-                  _REDUCTIONS[reduction], _TYPES[x._dtype], _TYPES[teacher._dtype], _INDEX_BITS[index._dtype], rows,
-                  x._shape[-1], entries)
+                  _REDUCTIONS[reduction], ahead, _TYPES[x._dtype], _TYPES[teacher._dtype], _INDEX_BITS[index._dtype],
+                  rows, x._shape[-1], entries)
     return dx

@@ -262,11 +262,11 @@ def test_refusals():
         F.distill_loss(x, t, _tensor(np.zeros((4, 3), np.int16)))
     from pytortto_amd import _hip
     p = x.data.ptr
-    good = [p, p, p, p, p, p, 1.0, 2, 0, 0, 64, 4, 8, 3]
-    for at, value, message in ((0, None, 'null pointer'), (0, p + 4, '16-byte aligned'), (6, 0.0, 'temperature must be'),
-                               (7, 3, 'reduction must be'), (8, 2, 'unknown type'), (9, -1, 'unknown type'),
-                               (10, 8, '32 or 64 bits'), (11, 0, 'rows must be'), (12, 0, 'vocabulary must have'),
-                               (13, 0, 'entries must be'), (13, 1025, 'entries must be')):
+    good = [p, p, p, p, p, p, None, 1.0, 2, 0, 0, 64, 4, 8, 3]
+    for at, value, message in ((0, None, 'null pointer'), (0, p + 4, '16-byte aligned'), (7, 0.0, 'temperature must be'),
+                               (8, 3, 'reduction must be'), (9, 2, 'unknown type'), (10, -1, 'unknown type'),
+                               (11, 8, '32 or 64 bits'), (12, 0, 'rows must be'), (13, 0, 'vocabulary must have'),
+                               (14, 0, 'entries must be'), (14, 1025, 'entries must be')):
         args = list(good)
         args[at] = value
         with pytest.raises(RuntimeError, match=message):
