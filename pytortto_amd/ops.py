@@ -13,7 +13,7 @@ from math import prod
 import numpy as np
 
 from . import _hip
-from .xparray import hiparray, poison
+from .xparray import hiparray, is_one, poison
 
 
 _F32 = np.dtype(np.float32)
@@ -685,7 +685,7 @@ def layer_norm_fwd(x, weight, bias, width, eps, keep):
     _f32(weight, bias)
     rows = x.size // width
     y = hiparray.empty(x._shape, x._dtype)
-    mean, rstd = (hiparray.empty((rows,)), hiparray.empty((rows,))) if keep else (None, None)
+    mean, rstd = hiparray.carve(((rows,), _F32), ((rows,), _F32)) if keep else (None, None)
     if rows:
         _hip.call('tt_layer_norm_fwd', x.ptr, _ptr(weight), _ptr(bias), y.ptr, _ptr(mean), _ptr(rstd), eps, kind, rows,
                   width)
@@ -700,9 +700,12 @@ def layer_norm_bwd(x, dy, weight, mean, rstd, width, need):
                         f'{dy._shape}')
     rows = x.size // width
     dx = hiparray.empty(x._shape, x._dtype) if need[0] else None
-    make = hiparray.empty if rows else hiparray.zeros
-    dw = make((width,)) if need[1] else None
-    db = make((width,)) if need[2] else None
+    if rows and need[1] and need[2]:
+        dw, db = hiparray.carve(((width,), _F32), ((width,), _F32))
+    else:
+        make = hiparray.empty if rows else hiparray.zeros
+        dw = make((width,)) if need[1] else None
+        db = make((width,)) if need[2] else None
     if rows:
         _hip.call('tt_layer_norm_bwd', x.ptr, dy.ptr, _ptr(weight), mean.ptr, rstd.ptr, _ptr(dx), _ptr(dw), _ptr(db),
                   kind, rows, width)
@@ -714,11 +717,14 @@ def token_log_prob_fwd(x, tokens, top, ignore_index, keep):
     ``keep``."""
     kind, bits = _kind(x, 'logits'), _index_bits(tokens, 'tokens')
     rows, vocab = tokens.size, x._shape[-1]
-    logp, entropy = hiparray.empty(tokens._shape), hiparray.empty(tokens._shape)
-    top_logp = top_index = None
+    wanted = [(tokens._shape, _F32), (tokens._shape, _F32)]
     if top:
-        top_logp, top_index = hiparray.empty(tokens._shape + (top,)), hiparray.empty(tokens._shape + (top,), np.int64)
-    stats = hiparray.empty((rows, 2)) if keep else None
+        wanted += [(tokens._shape + (top,), _F32), (tokens._shape + (top,), np.int64)]
+    if keep:
+        wanted.append(((rows, 2), _F32))
+    logp, entropy, *more = hiparray.carve(*wanted)
+    stats = more.pop() if keep else None
+    top_logp, top_index = more or (None, None)
     if rows:
         _hip.call('tt_token_log_prob_fwd', x.ptr, tokens.ptr, logp.ptr, entropy.ptr, _ptr(top_logp), _ptr(top_index),
                   _ptr(stats), kind, bits, ignore_index, rows, vocab, top)
@@ -751,8 +757,7 @@ def distill_fwd(x, teacher, index, temperature, reduction, need_grad):
     red = _REDUCTIONS[reduction]
     vocab, entries = x._shape[-1], index._shape[-1]
     rows = index.size // entries
-    loss = hiparray.empty(x._shape[:-1] if red == 0 else ())
-    stats, count = hiparray.empty((rows, 2)), hiparray.empty((1,))
+    loss, stats, count = hiparray.carve((x._shape[:-1] if red == 0 else (), _F32), ((rows, 2), _F32), ((1,), _F32))
     dx = None
     if rows:
         if need_grad and _distill_ahead(kinds[0], red, rows, vocab):
@@ -767,9 +772,11 @@ def distill_fwd(x, teacher, index, temperature, reduction, need_grad):
 def distill_bwd(x, teacher, index, stats, count, g, dx, temperature, reduction):
     """dlogits; ``dx`` is the forward's, or None."""
     _f32(g)
+    ahead = dx is not None
+    if ahead and is_one(g):
+        return dx
     entries = index._shape[-1]
     rows = index.size // entries
-    ahead = dx is not None
     if not ahead:
         dx = hiparray.empty(x._shape, x._dtype)
     if rows:

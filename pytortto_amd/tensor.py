@@ -202,12 +202,10 @@ class Tensor:
             raise RuntimeError('element 0 of tensors does not require grad and does not have a grad_fn')
         on_device = self.data.__class__ is hiparray
         if gradient is None:
-            shape = (1,) * self.data.ndim
             if on_device and self.data._dtype == np.float32:
-                gradient = hiparray.empty(shape)
-                gradient.fill(1.0)              # (an upload would wait for all that has been launched)
+                gradient = xparray.one(self.data.ndim)      # (an upload would wait for all that has been launched)
             else:
-                one = np.ones(shape, dtype=self.data.dtype)
+                one = np.ones((1,) * self.data.ndim, dtype=self.data.dtype)
                 gradient = hiparray(one) if on_device else one
         elif isinstance(gradient, Tensor):
             if gradient.device != self.device:

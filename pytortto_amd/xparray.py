@@ -57,6 +57,7 @@ class Device:
 
 
 _F32 = np.dtype(np.float32)
+_DTYPES = {}            # of array interfaces' type strings
 
 
 class _Buffer:
@@ -154,12 +155,12 @@ class _Loan(_Buffer):
 
 
 class _Borrowed(_Buffer):
-    """A block that somebody else allocated; ``owner`` is kept for as long as an array refers to it."""
+    """A block that somebody else allocated, or a part of another one; ``owner`` is kept for as long as an array refers
+    to it."""
     __slots__ = ('owner',)
 
     def __init__(self, ptr, nbytes, owner):
-        super().__init__(nbytes, lazy=True)
-        self._ptr, self.owner = ptr, owner
+        self._ptr, self.nbytes, self.owner, self.on_demand, self.deps = ptr, nbytes, owner, None, ()
 
     def __del__(self):
         pass
@@ -239,6 +240,17 @@ class hiparray:
         return self
 
     @classmethod
+    def carve(cls, *wanted):
+        """Arrays of the (shape, dtype) wanted on one block: what one operation returns together, for one allocation."""
+        dtypes = [_F32 if t is np.float32 else np.dtype(t) for _, t in wanted]
+        sizes = [prod(shape) * dtype.itemsize for (shape, _), dtype in zip(wanted, dtypes)]
+        block, at, out = _Buffer(sum(sizes) + 256 * len(sizes)), 0, []
+        for (shape, _), dtype, size in zip(wanted, dtypes, sizes):
+            out.append(cls.on(_Borrowed(block._ptr + at, size, block), shape, dtype))
+            at += (size + 255) & -256
+        return out
+
+    @classmethod
     def zeros(cls, shape, dtype=np.float32):
         out = cls.empty(shape, dtype)
         if out.nbytes:
@@ -255,7 +267,8 @@ class hiparray:
         CuPy array); nothing is copied and ``source`` is kept alive.  Its writers must be done, or be ordered in
         front of the library's stream, before the array is used; and memory is borrowed once, not as two arrays."""
         about = source.__cuda_array_interface__
-        shape, dtype = tuple(about['shape']), np.dtype(about['typestr'])
+        shape, kind = tuple(about['shape']), about['typestr']
+        dtype = _DTYPES.get(kind) or _DTYPES.setdefault(kind, np.dtype(kind))
         nbytes = prod(shape) * dtype.itemsize
         if about.get('mask') is not None:
             raise ValueError('borrowed device memory cannot be masked')
@@ -422,6 +435,26 @@ class hiparray:
         else:
             raise TypeError(f'device += is not defined for {other.__class__.__name__}')
         return self
+
+
+_one = None
+
+
+def one(ndim):
+    """The 1.0 that a backward pass starts with, ``ndim``-dimensional: always the same block, whose holders copy it
+    before they write (``own``)."""
+    global _one
+    if _one is None:
+        first = hiparray.empty(())
+        first.fill(1.0)
+        _one = first
+    out = _one.alias()
+    out._shape = (1,) * ndim
+    return out
+
+
+def is_one(a):
+    return _one is not None and a._buf is _one._buf
 
 
 def ascontiguousarray(a):

@@ -113,3 +113,28 @@ def test_the_plain_forms_gradients_are_those_of_their_values():
     for reduction in ('sum', 'mean'):
         _, (dz, _) = plain64.distill(x, teacher, index, 2.0, reduction)
         np.testing.assert_allclose(slope(lambda a: plain64.distill(a, teacher, index, 2.0, reduction)[0][0], x, v), (dz * v).sum(), rtol=1e-6)
+
+
+def test_the_ones_that_backward_passes_start_with(monkeypatch):
+    """One block, shared: who writes it gets a copy.  (Allocation and launches are recorded, not carried out.)"""
+    from pytortto_amd import _hip, xparray
+    calls = []
+
+    def call(name, *args):
+        calls.append(name)
+        if name == 'tt_malloc':
+            args[0]._obj.value = 4096 * (1 + len(calls))
+
+    monkeypatch.setattr(_hip, 'call', call)
+    monkeypatch.setattr(xparray, '_one', None)
+    monkeypatch.setattr(xparray._Buffer, '__del__', lambda self: None)
+    a, b = xparray.one(0), xparray.one(2)
+    assert a.shape == () and b.shape == (1, 1) and a.ptr == b.ptr and calls == ['tt_malloc', 'tt_fill_f32']
+    assert xparray.is_one(a) and xparray.is_one(b) and not xparray.is_one(hiparray.empty((1,)))
+    b += 1.0
+    assert b.ptr != a.ptr and not xparray.is_one(b) and xparray.is_one(xparray.one(1))
+    assert calls[-2:] == ['tt_memcpy_d2d', 'tt_add_scalar_f32']
+    first, second, third = hiparray.carve(((3,), np.float32), ((0, 2), np.float32), ((2, 2), np.int64))
+    assert first.ptr % 256 == second.ptr % 256 == third.ptr % 256 == 0 and third.ptr >= first.ptr + 12
+    assert first._buf.owner is third._buf.owner and third.nbytes == 32 and third.dtype == np.int64
+    assert third.ptr + third.nbytes <= first._buf.owner._ptr + first._buf.owner.nbytes
