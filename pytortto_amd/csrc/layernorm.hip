@@ -218,8 +218,19 @@ __global__ __launch_bounds__(1024) void ln_join(const float* __restrict__ parts,
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   const size_t c = (size_t)blockIdx.x * kWave + lane;
   double s = 0.0;
-  if (c < 2 * (size_t)D)
-    for (int k = wave; k < blocks; k += 16) s += (double)parts[(size_t)k * 2 * D + c];
+  if (c < 2 * (size_t)D) {
+    const float* __restrict__ p = parts + c;
+    const size_t step = 2 * (size_t)D;
+    int k = wave;
+    for (; k + 7 * 16 < blocks; k += 8 * 16) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = p[(k + i * 16) * step];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += (double)v[i];
+    }
+    for (; k < blocks; k += 16) s += (double)p[k * step];
+  }
   sums[wave][lane] = s;
   __syncthreads();
   if (wave || c >= 2 * (size_t)D) return;

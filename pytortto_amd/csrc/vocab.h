@@ -13,57 +13,55 @@ namespace tt {
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr double kLog2e = 1.44269504088896340736;
 
-// Rows begin at any multiple of the type: a row is read as the aligned packs that cover it.  Element i of pack j is
-// column j * n + i - skip; the first and the last pack may hold columns of the neighbours, and those two are then read
-// value by value, so that nothing outside the row is touched.
+// Rows begin at any multiple of the type.  The aligned packs that lie in a row altogether, [first, end), are read and
+// written whole; element i of pack j is column j n + i - skip.  The columns in front of them (`head`, n - 1 at most)
+// and behind them (`tail`, from tail_at on) go one by one, so nothing outside the row is touched.
 template <typename T>
 struct LogitRow {
-  typedef typename Pack<T>::type P;
   static constexpr int n = Pack<T>::n;
-  const P* at;        // the pack that holds column 0
+  const char* at;     // where pack 0, which holds column 0, begins
+  size_t start;       // element offset of column 0
   int skip, V;
-  int packs;          // that cover the row
-  int whole0, whole1; // [whole0, whole1): the packs that lie in the row altogether
+  int first, end;
+  int head, tail, tail_at;
 
-  __device__ __forceinline__ LogitRow(const T* x, size_t row, int V_) : V(V_) {
-    const size_t first = row * (size_t)V;       // (x itself is 16-byte aligned)
-    skip = (int)(first % n);
-    at = reinterpret_cast<const P*>(x) + first / n;
-    packs = (V + skip + n - 1) / n;
-    whole0 = skip ? 1 : 0;
-    whole1 = (V + skip) / n;
+  __device__ __forceinline__ LogitRow(const T* x, size_t row, int V_) : start(row * (size_t)V_), V(V_) {
+    skip = (int)(start % n);                    // (x itself is 16-byte aligned)
+    at = reinterpret_cast<const char*>(x + (start - skip));
+    first = skip ? 1 : 0;
+    end = (V + skip) / n;
+    head = skip ? n - skip : 0;
+    head = head < V ? head : V;
+    tail_at = end * n - skip;
+    tail_at = tail_at > head ? tail_at : head;
+    tail = V - tail_at;
+  }
+  __device__ __forceinline__ Words pack(int j) const {
+    return *reinterpret_cast<const Words*>(at + (unsigned)j * 16u);
   }
   __device__ __forceinline__ int column(int j) const { return j * n - skip; }
-  __device__ __forceinline__ P read(int j) const {
-    if (j >= whole0 && j < whole1) return at[j];
-    P p;
-#pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const int c = column(j) + i;
-      p[i] = c >= 0 && c < V ? reinterpret_cast<const T*>(at)[(ptrdiff_t)c + skip] : (T)-INFINITY;
-    }
-    return p;
-  }
 };
 
 template <typename T>
-__device__ __forceinline__ void write_pack(const LogitRow<T>& r, T* dx_at, int j, const typename Pack<T>::type& p) {
-  if (j >= r.whole0 && j < r.whole1) {
-    __builtin_nontemporal_store(p, reinterpret_cast<typename Pack<T>::type*>(dx_at) + j);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < Pack<T>::n; ++i) {
-    const int c = r.column(j) + i;
-    if (c >= 0 && c < r.V) dx_at[(ptrdiff_t)c + r.skip] = p[i];
-  }
+__device__ __forceinline__ void write_pack(const LogitRow<T>& r, T* dx, int j, const Words& p) {
+  char* at = reinterpret_cast<char*>(dx + (r.start - r.skip));
+  __builtin_nontemporal_store(p, reinterpret_cast<Words*>(at + (unsigned)j * 16u));
 }
 
-// Where the aligned packs of a row begin in an array laid out like the logits.
-template <typename T>
-__device__ __forceinline__ T* packs_of(T* dx, size_t row, int V) {
-  return dx + (row * (size_t)V) / Pack<T>::n * Pack<T>::n;
-}
+// The part of a row that split `split` of `splits` works on: whole packs [p0, p1), the head with the first split, the
+// tail with the last.
+struct Share {
+  int p0, p1;
+  int head, tail;
+  template <typename T>
+  __device__ __forceinline__ Share(const LogitRow<T>& r, int split, int splits) {
+    const int packs = r.end > r.first ? r.end - r.first : 0, per = (packs + splits - 1) / splits;
+    p0 = r.first + (split * per < packs ? split * per : packs);
+    p1 = r.first + ((split + 1) * per < packs ? (split + 1) * per : packs);
+    head = split == 0 ? r.head : 0;
+    tail = split == splits - 1 ? r.tail : 0;
+  }
+};
 
 // Running maximum and sums of a softmax: s = sum 2^d, t = sum 2^d d with d = (z - m) c.  No value yet: m = -inf.
 struct Stat {
@@ -77,51 +75,117 @@ __device__ __forceinline__ float anchor(float m) { return m == -INFINITY ? 0.f :
 // 2^d d where d may be -inf; the clamp changes no product, for 2^-200 is zero.
 __device__ __forceinline__ float floor_at(float d) { return fmaxf(d, -200.f); }
 
+// d of a value, (z - m) c.  Halves cannot overflow z c, and take one instruction for their widening, the product and the
+// difference; every d of a row has the same rounded m c then, which drops out of all that is made of them.
+__device__ __forceinline__ float rounded(float m, float c) {
+#pragma clang fp contract(off)
+  return m * c;
+}
+__device__ __forceinline__ float rounded_between(float m, float to, float c) {
+#pragma clang fp contract(off)
+  return m * c - to * c;        // (fused, equal ones would differ by the rounding)
+}
+template <typename T>
+__device__ __forceinline__ float bits(float z, float m, float c) {
+  return sizeof(T) == 2 ? fmaf(z, c, -rounded(m, c)) : (z - m) * c;
+}
+
 // Moves the sums of `a` to another, larger maximum.
-template <bool ENTROPY>
+template <typename T, bool ENTROPY>
 __device__ __forceinline__ void rescale(Stat& a, float m, float c) {
-  const float d = (a.m - anchor(m)) * c, f = pow2(d);
+  const float to = anchor(m), d = sizeof(T) == 2 ? rounded_between(a.m, to, c) : (a.m - to) * c, f = pow2(d);
   if (ENTROPY) a.t = f * fmaf(a.s, floor_at(d), a.t);
   a.s *= f;
   a.m = m;
 }
 
-// N values at once: one comparison of maxima and at most one rescaling for all of them.  A NaN, or an infinity, which
-// is taken from itself, ends up in s.
-template <int N, bool ENTROPY>
-__device__ __forceinline__ bool add_values(Stat& a, const float (&z)[N], float c) {
-  float most = z[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) most = fmaxf(most, z[i]);
+// Adds N values of which `most` is the largest: at most one rescaling for all of them.  A NaN, or an infinity, which is
+// taken from itself, ends up in s.  Returns whether the maximum rose.
+template <typename T, int N, bool ENTROPY>
+__device__ __forceinline__ bool add_values(Stat& a, const float (&z)[N], float most, float c) {
   const bool rises = most > a.m;
-  if (rises) rescale<ENTROPY>(a, most, c);
+  if (rises) rescale<T, ENTROPY>(a, most, c);
   const float m = anchor(a.m);
-  float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f;
+  float s[2] = {}, t[2] = {};
 #pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const float d0 = (z[i] - m) * c, e0 = pow2(d0);
-    s0 += e0;
-    if (ENTROPY) t0 = fmaf(e0, floor_at(d0), t0);
-    if (i + 1 < N) {
-      const float d1 = (z[i + 1] - m) * c, e1 = pow2(d1);
-      s1 += e1;
-      if (ENTROPY) t1 = fmaf(e1, floor_at(d1), t1);
-    }
+  for (int i = 0; i < N; ++i) {
+    const float d = bits<T>(z[i], m, c), e = pow2(d);
+    s[i % 2] += e;
+    if (ENTROPY) t[i % 2] = fmaf(e, floor_at(d), t[i % 2]);
   }
-  a.s += s0 + s1;
-  if (ENTROPY) a.t += t0 + t1;
+  a.s += s[0] + s[1];
+  if (ENTROPY) a.t += t[0] + t[1];
   return rises;
+}
+
+template <typename T, int N, bool ENTROPY>
+__device__ __forceinline__ bool add_packs(Stat& a, const Words* p, float c) {
+  constexpr int n = Pack<T>::n;
+  float z[N * n];
+#pragma unroll
+  for (int i = 0; i < N; ++i) unpack<T>(z + i * n, p[i]);
+  return add_values<T, N * n, ENTROPY>(a, z, pack_max<T, N>(p), c);
+}
+template <typename T, bool ENTROPY>
+__device__ __forceinline__ bool add_value(Stat& a, float value, float c) {
+  const float z[1] = {value};
+  return add_values<T, 1, ENTROPY>(a, z, value, c);
+}
+
+constexpr int kUnroll = 4;      // packs that a thread has on their way at once in the streaming loops
+
+// A thread's share of a row: thread `lane` of G takes packs p0 + lane + i G, one column of the head in front of them and
+// one of the tail behind them, so that it sees its columns in ascending order.  `best` is told what holds the first
+// of its largest values: a group of kUnroll packs by its first one, kHead or kTail.
+constexpr int kNothing = -1, kHead = -2, kTail = -3;
+
+// (PACKS = false: the head and the tail only.)
+template <typename T, int G, bool ENTROPY, bool PACKS = true>
+__device__ __forceinline__ void scan(Stat& a, int& best, const T* x, const LogitRow<T>& r, const Share& h, int lane,
+                                     float c) {
+  if (lane < h.head) {
+    add_value<T, ENTROPY>(a, widen(x[r.start + lane]), c);
+    best = kHead;
+  }
+  for (int j = h.p0 + lane; PACKS && j < h.p1; j += kUnroll * G) {
+    Words p[kUnroll];
+    if (j + (kUnroll - 1) * G < h.p1) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) p[u] = r.pack(j + u * G);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        p[u] = Words(Pack<T>::lowest);
+        if (j + u * G < h.p1) p[u] = r.pack(j + u * G);
+      }
+    }
+    if (add_packs<T, kUnroll, ENTROPY>(a, p, c) || best == kNothing) best = j;
+  }
+  if (lane < h.tail && (add_value<T, ENTROPY>(a, widen(x[r.start + r.tail_at + lane]), c) || best == kNothing))
+    best = kTail;
 }
 
 // The statistics of all G threads of a row: first the maximum, then each thread's sums moved to it and added up.
 // part: LDS of 3 * G / 64 floats.
-template <int G, bool ENTROPY>
+template <typename T, int G, bool ENTROPY>
 __device__ __forceinline__ Stat row_join(Stat a, float c, float* part) {
   const float m = row_max<G>(a.m, part);
-  rescale<ENTROPY>(a, m, c);
+  rescale<T, ENTROPY>(a, m, c);
   a.s = row_sum<G>(a.s, part + G / kWave);
   if (ENTROPY) a.t = row_sum<G>(a.t, part + 2 * (G / kWave));
   return a;
+}
+
+struct Scale {
+  float c;            // log2(e) / temperature
+  float inverse;      // 1 / temperature
+  float temperature;
+};
+
+// log p of a value, in nats.  (In bits a float32 that is its type's lowest would overflow.)
+template <typename T>
+__device__ __forceinline__ float log_p(float z, float m, float log_s, const Scale& sc) {
+  return (sizeof(T) == 2 ? bits<T>(z, m, sc.c) * kLn2 : (z - m) * sc.inverse) - log_s * kLn2;
 }
 
 // log2 of the sum, 0 for an empty row; a NaN stays.

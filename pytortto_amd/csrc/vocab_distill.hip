@@ -5,26 +5,23 @@
 
 namespace {
 
+using tt::kUnroll;
 using tt::kWave;
 using tt::LogitRow;
 using tt::Pack;
+using tt::Scale;
+using tt::Share;
 using tt::Stat;
+using tt::Words;
 
 constexpr int kThreads = 256;
 constexpr int kMostTeacher = 1024;
-constexpr int kUnroll = 4;
-constexpr int kCountBlocks = 256;
+constexpr int kMostSplitRows = 8192;    // fewer rows than this may be shared by blocks
 
 struct Teacher {
   const void* logits;
   const void* index;
   int half, wide, K;
-};
-
-struct Scale {
-  float c;            // log2(e) / T
-  float inverse;      // 1 / T
-  float temperature;
 };
 
 // The teacher's entry k of a row: its logit, -inf where there is none, NaN for an index behind the vocabulary.
@@ -34,247 +31,335 @@ __device__ __forceinline__ float teacher_entry(const Teacher& te, size_t at, int
   return i < 0 ? -INFINITY : i >= V ? NAN : tt::read_value(te.logits, at, te.half);
 }
 
-// The teacher's distribution of a row: weight[k] = q_k and place[k], LDS of K each.
+// A row's teacher in LDS, K entries each: their probabilities q, their places, the student's logits there, and a
+// queue for each of the G threads that write the row's gradient (below).
+struct Entries {
+  float* weight;
+  int* place;
+  float* logit;
+  int* next;
+  int* queue;
+};
+constexpr int kEntryBytes = 16;
+
+template <int G>
+__device__ __forceinline__ Entries entries_of(float* lds, int K, int sub) {
+  float* at = lds + (size_t)sub * (4 * K + G);
+  return {at, (int*)(at + K), at + 2 * K, (int*)(at + 3 * K), (int*)(at + 4 * K)};
+}
+template <int G>
+size_t entries_bytes(int K, int rows) {
+  return ((size_t)K * kEntryBytes + G * sizeof(int)) * rows;
+}
+
 struct TeacherSum {
   float s;            // at least 1: the row has a teacher; 0: it has none; NaN: it cannot be computed
   float q_log_q;      // sum_k q_k log2 q_k
 };
 
-template <int G>
-__device__ __forceinline__ TeacherSum read_teacher(const Teacher& te, size_t row, int V, float c, int lane,
-                                                   float* weight, int* place, float* part) {
+template <typename T, int G>
+__device__ __forceinline__ TeacherSum read_teacher(const Teacher& te, const T* x, const LogitRow<T>& r, size_t row,
+                                                   float c, int lane, const Entries& e, float* part) {
   Stat a = {-INFINITY, 0.f, 0.f};
+  e.queue[lane] = -1;
   for (int k = lane; k < te.K; k += G) {
     int i;
-    const float z[1] = {teacher_entry(te, row * te.K + k, V, &i)};
-    weight[k] = z[0];
-    place[k] = i;
-    tt::add_values<1, true>(a, z, c);
+    const float z = teacher_entry(te, row * te.K + k, r.V, &i);
+    e.weight[k] = z;
+    e.place[k] = i;
+    e.logit[k] = tt::widen(x[r.start + i]);
+    tt::add_value<float, true>(a, z, c);
   }
-  a = tt::row_join<G, true>(a, c, part);
+  a = tt::row_join<float, G, true>(a, c, part);
   const float log_s = tt::log_sum(a), m = tt::anchor(a.m);
-  for (int k = lane; k < te.K; k += G) weight[k] = a.s == 0.f ? 0.f : tt::pow2((weight[k] - m) * c - log_s);
+  for (int k = lane; k < te.K; k += G) e.weight[k] = a.s == 0.f ? 0.f : tt::pow2((e.weight[k] - m) * c - log_s);
   tt::sync_row<G>();
   return {a.s, a.s == 0.f ? 0.f : a.t / a.s - log_s};
 }
 
-// sum_k q_k (-log p_(i_k)) of a row; every thread gets it.
+// This thread's part of sum_k q_k (-log p_(i_k)).
 template <typename T, int G>
-__device__ __forceinline__ float cross_entropy(const T* x, size_t row, int V, const Stat& a, float log_s, float inverse,
-                                               int K, int lane, const float* weight, const int* place, float* part) {
+__device__ __forceinline__ float cross_entropy(const Entries& e, int K, int lane, const Stat& a, float log_s,
+                                               const Scale& sc) {
   float s = 0.f;
   for (int k = lane; k < K; k += G) {
-    const float w = weight[k];
-    if (w != 0.f)
-      s -= w * ((tt::widen(x[row * (size_t)V + place[k]]) - tt::anchor(a.m)) * inverse - log_s * tt::kLn2);
+    const float w = e.weight[k];
+    if (w != 0.f) s -= w * tt::log_p<T>(e.logit[k], tt::anchor(a.m), log_s, sc);
   }
-  return tt::row_sum<G>(s, part);
+  return s;
 }
 
-// What a row leaves behind: its loss, whether it counts, and what the backward pass needs.  A row without a teacher has
-// m = -inf there, as one without any possible class: no gradient.
-__device__ __forceinline__ void write_row(float* loss, float* counted, float2* stats, size_t row, const Stat& a,
-                                          float log_s, const TeacherSum& te, float cross, const Scale& sc) {
-  const bool none = te.s == 0.f;
-  loss[row] = none ? 0.f : fmaf(te.q_log_q, tt::kLn2, cross) * (sc.temperature * sc.temperature);
-  counted[row] = none ? 0.f : 1.f;
-  stats[row] = make_float2(none ? -INFINITY : a.m, te.s == te.s ? log_s : te.s);
-}
-
-// The gradient at the teacher's entries, over what has been written there without q: of a row's packs [v0, v1).
+// The gradient at the teacher's entries has q in it, which the threads that write a row's packs do not know.  Each such
+// value is queued for the thread that writes its pack, which stores it after that: a thread's own stores stay in order,
+// so nobody waits for them.  The values go where the logits were.
 template <typename T, int G>
-__device__ __forceinline__ void fix_entries(const T* x, T* dx, const LogitRow<T>& r, size_t row, int v0, int v1, int K,
-                                            int lane, const float* weight, const int* place, float m, float log_s,
-                                            float c, float scale) {
-  tt::stores_done();
-  tt::sync_row<G>();
+__device__ __forceinline__ void queue_entries(const Entries& e, const LogitRow<T>& r, const Share& s, int K, int lane,
+                                              float m, float log_s, float c, float scale) {
   for (int k = lane; k < K; k += G) {
-    const int j = place[k], pack = (j + r.skip) / Pack<T>::n;
-    if (pack < v0 || pack >= v1 || weight[k] == 0.f) continue;
+    const int j = e.place[k], pack = (j + r.skip) / Pack<T>::n;
+    if (e.weight[k] == 0.f) continue;
+    int owner;
+    if (j < r.head) {
+      if (s.head == 0) continue;
+      owner = j;
+    } else if (j >= r.tail_at) {
+      if (s.tail == 0) continue;
+      owner = s.head + j - r.tail_at;
+    } else {
+      if (pack < s.p0 || pack >= s.p1) continue;
+      owner = (pack - s.p0) % G;
+    }
     float q = 0.f;
-    for (int i = 0; i < K; ++i) q += place[i] == j ? weight[i] : 0.f;
-    const size_t at = row * (size_t)r.V + j;
-    dx[at] = (T)(scale * (tt::pow2((tt::widen(x[at]) - m) * c - log_s) - q));
+    for (int i = 0; i < K; ++i) q += e.place[i] == j ? e.weight[i] : 0.f;
+    e.logit[k] = scale * (tt::pow2(tt::bits<T>(e.logit[k], m, c) - log_s) - q);
+    e.next[k] = atomicExch(&e.queue[owner], k);
   }
+  tt::sync_row<G>();
+}
+template <typename T>
+__device__ __forceinline__ void store_queued(const Entries& e, T* dx, const LogitRow<T>& r, int lane) {
+  asm volatile("" ::: "memory");      // (behind the packs' stores for the compiler too, to which they are another type)
+  for (int k = e.queue[lane]; k >= 0; k = e.next[k]) dx[r.start + e.place[k]] = (T)e.logit[k];
+}
+
+// What the rows leave behind, and what the last of them makes of it.
+struct Out {
+  float* loss;        // of each row
+  float* counted;     // 1 of a row with a teacher, else 0
+  float2* stats;      // for the backward pass
+  float* total;       // the rows' sum, or over the count for the mean; NULL: not wanted
+  float* count;       // how many rows have a teacher
+  int mean;
+};
+
+// A row without a teacher has m = -inf for the backward pass, as one without any possible class: no gradient.
+__device__ __forceinline__ void write_row(const Out& o, size_t row, const Stat& a, float log_s, const TeacherSum& te,
+                                          float cross, const Scale& sc) {
+  const bool none = te.s == 0.f;
+  tt::share(o.loss + row, none ? 0.f : fmaf(te.q_log_q, tt::kLn2, cross) * (sc.temperature * sc.temperature));
+  tt::share(o.counted + row, none ? 0.f : 1.f);
+  o.stats[row] = make_float2(none ? -INFINITY : a.m, te.s == te.s ? log_s : te.s);
+}
+
+// The rows' losses added up by one block, in 64 bits and in an order that the sizes alone decide.
+template <int BLOCK>
+__device__ __forceinline__ void add_rows(const Out& o, int R, double* part) {
+  double s = 0.0, n = 0.0;
+  for (int r = threadIdx.x; r < R; r += BLOCK) {
+    s += (double)tt::shared(o.loss + r);
+    n += (double)tt::shared(o.counted + r);
+  }
+  s = tt::row_sum<BLOCK>(s, part);
+  n = tt::row_sum<BLOCK>(n, part + BLOCK / kWave);
+  if (threadIdx.x == 0) {
+    if (o.total) o.total[0] = (float)(o.mean ? s / n : s);
+    o.count[0] = (float)n;
+  }
+}
+
+// scale p of a pack's values.  FOLD, for scale > 0: halves, whose rounding hides it, take log2(scale) into the exponent.
+template <typename T, bool FOLD>
+__device__ __forceinline__ Words gradient_pack(const Words& p, float m, float log_s, float c, float scale) {
+  float z[Pack<T>::n];
+  tt::unpack<T>(z, p);
+  const float add = log2f(scale) - log_s - tt::rounded(m, c);
+#pragma unroll
+  for (int i = 0; i < Pack<T>::n; ++i)
+    z[i] = FOLD && sizeof(T) == 2 ? tt::pow2(fmaf(z[i], c, add)) : scale * tt::pow2(tt::bits<T>(z[i], m, c) - log_s);
+  return tt::pack<T>(z);
+}
+
+// The values of NV packs: their maximum first, then their sum, so that there is no chain of rescaled sums.  The packs are
+// opaque to the compiler in between, which would otherwise hold all their widened values from one loop to the other.
+template <typename T, int NV>
+__device__ __forceinline__ void add_kept(Stat& a, Words (&kept)[NV], float c) {
+  constexpr int n = Pack<T>::n;
+  const float most = tt::pack_max<T, NV>(kept);
+  if (most > a.m) tt::rescale<T, false>(a, most, c);
+  const float m = tt::anchor(a.m);
+  float s[4] = {};
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    asm volatile("" : "+v"(kept[u]));
+    float z[n];
+    tt::unpack<T>(z, kept[u]);
+#pragma unroll
+    for (int i = 0; i < n; ++i) s[i % 4] += tt::pow2(tt::bits<T>(z[i], m, c));
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  a.s += (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 template <typename T>
-__device__ __forceinline__ typename Pack<T>::type gradient_pack(const typename Pack<T>::type& p, float m, float log_s,
-                                                                float c, float scale) {
-  typename Pack<T>::type q;
-#pragma unroll
-  for (int i = 0; i < Pack<T>::n; ++i) q[i] = (T)(scale * tt::pow2((tt::widen(p[i]) - m) * c - log_s));
-  return q;
-}
-
-// Adds packs j, j + G, ... (N of them, those below v1) to the statistics.
-template <typename T, int N>
-__device__ __forceinline__ void add_packs(Stat& a, const typename Pack<T>::type (&p)[N], float c) {
-  constexpr int n = Pack<T>::n;
-  float z[N * n];
-#pragma unroll
-  for (int i = 0; i < N * n; ++i) z[i] = tt::widen(p[i / n][i % n]);
-  tt::add_values<N * n, false>(a, z, c);
-}
-
-template <typename T, int G>
-__device__ __forceinline__ void scan(Stat& a, const LogitRow<T>& r, int v0, int v1, int lane, float c) {
-  typedef typename Pack<T>::type P;
-  const int whole1 = v1 < r.whole1 ? v1 : r.whole1;
-  for (int j = v0 + lane; j < v1; j += kUnroll * G) {
-    P p[kUnroll];
-    if (j >= r.whole0 && j + (kUnroll - 1) * G < whole1) {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) p[u] = r.at[j + u * G];
-    } else {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) p[u] = j + u * G < v1 ? r.read(j + u * G) : P((T)-INFINITY);
-    }
-    add_packs<T, kUnroll>(a, p, c);
+__device__ __forceinline__ void write_loose(const T* x, T* dx, const LogitRow<T>& r, const Share& s, int lane,
+                                            bool none, float m, float log_s, float c, float scale) {
+  if (lane < s.head + s.tail) {
+    const size_t at = r.start + (lane < s.head ? lane : r.tail_at + lane - s.head);
+    dx[at] = none ? (T)0.f : (T)(scale * tt::pow2(tt::bits<T>(tt::widen(x[at]), m, c) - log_s));
   }
+}
+
+__device__ __forceinline__ bool has_teacher(const Teacher& te, size_t row, int V) {
+  for (int k = 0; k < te.K; ++k) {        // (the first entry decides, as a rule)
+    int i;
+    if (teacher_entry(te, row * te.K + k, V, &i) != -INFINITY) return true;
+  }
+  return false;
 }
 
 // How many rows have a teacher, in parts: one whole number for each block.
+constexpr int kCountBlocks = 256;
 __global__ __launch_bounds__(kThreads) void distill_count(Teacher te, int* __restrict__ parts, int R, int V) {
+  constexpr int kLanes = 16;              // to a row
   __shared__ int part[kThreads / kWave];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x % kLanes, shift = (threadIdx.x & (kWave - 1)) / kLanes * kLanes;
   int n = 0;
-  for (long long row = (long long)blockIdx.x * 4 + wave; row < R; row += (long long)gridDim.x * 4) {
+  for (long long row = ((long long)blockIdx.x * kThreads + threadIdx.x) / kLanes; row < R;
+       row += (long long)gridDim.x * (kThreads / kLanes)) {
     bool any = false;
-    for (int k = lane; k < te.K; k += kWave) {
+    for (int k = lane; k < te.K; k += kLanes) {
       int i;
       any |= teacher_entry(te, row * te.K + k, V, &i) != -INFINITY;
     }
-    n += __any(any) ? 1 : 0;
+    const unsigned long long rows = __ballot(any);
+    if (lane == 0 && (rows >> shift & 0xffffu) != 0) ++n;
   }
-  if (lane == 0) part[wave] = n;
-  __syncthreads();
-  if (threadIdx.x == 0) parts[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
+  n = tt::row_sum<kThreads>(n, part);
+  if (threadIdx.x == 0) parts[blockIdx.x] = n;
 }
 
-// Rows of G threads each, kept in registers as far as NV packs to a thread reach: loss, statistics and, with GRAD, the
-// gradient for an incoming gradient of one, which then costs one read and one write of the row.  `count_parts`: for
-// the mean.
-template <typename T, int G, int NV, bool GRAD>
-__global__ __launch_bounds__(G < kThreads ? kThreads : G) void distill_rows(const T* __restrict__ x, Teacher te,
-                                                                           float* __restrict__ loss,
-                                                                           float* __restrict__ counted,
-                                                                           float2* __restrict__ stats, T* dx,
-                                                                           const int* __restrict__ count_parts,
+__device__ unsigned distill_done;       // blocks of a launch that are done, and splits of each row: zero between launches
+__device__ unsigned distill_tickets[kMostSplitRows];
+
+// Rows of G threads each: loss, statistics and, with GRAD, the gradient for an incoming gradient of one.  For that the
+// row is kept in registers, NV packs to a thread, and costs one read and one write; of a longer row (LONG) the rest is
+// read a second time.  For the mean's gradient the rows with a teacher are counted first: by each block, or from
+// `count_parts`.
+template <typename T, int G, int NV, bool LONG, bool GRAD>
+__global__ __launch_bounds__(G < kThreads ? kThreads : G) void distill_rows(const T* __restrict__ x, Teacher te, Out o,
+                                                                           T* dx, const int* __restrict__ count_parts,
                                                                            Scale sc, int R, int V) {
   constexpr int kBlock = G < kThreads ? kThreads : G, kRows = kBlock / G;
-  typedef typename Pack<T>::type P;
   extern __shared__ float lds[];
   __shared__ float part[kRows][3 * (G / kWave)];
   __shared__ float more[kRows][4 * (G / kWave)];
+  __shared__ double sums[2 * (kBlock / kWave)];
+  __shared__ bool last;
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
-  float* weight = lds + sub * 2 * te.K;
-  int* place = (int*)(weight + te.K);
+  const Entries e = entries_of<G>(lds, te.K, sub);
   float scale = sc.temperature;
-  if (GRAD && count_parts) {
+  if (GRAD && o.mean) {
     int n = 0;
-    for (int i = lane; i < kCountBlocks; i += G) n += count_parts[i];
-    scale /= (float)tt::row_sum<G>(n, (int*)part[sub]);
-    tt::sync_row<G>();
+    if (count_parts) {
+      for (int i = threadIdx.x; i < kCountBlocks; i += kBlock) n += count_parts[i];
+    } else {
+      for (int i = threadIdx.x; i < R; i += kBlock) n += has_teacher(te, i, V) ? 1 : 0;
+    }
+    scale /= (float)tt::row_sum<kBlock>(n, (int*)sums);
   }
   for (long long row = (long long)blockIdx.x * kRows + sub; row < R; row += (long long)gridDim.x * kRows) {
     const LogitRow<T> r(x, row, V);
-    P kept[NV];
-    // (a thread's packs beyond the row are -inf, which adds nothing)
+    const Share all(r, 0, 1);
+    Words kept[NV ? NV : 1];
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      const int j = lane + u * G;
-      kept[u] = j < r.packs ? r.read(j) : P((T)-INFINITY);
+      kept[u] = Words(Pack<T>::lowest);
+      if (all.p0 + lane + u * G < all.p1) kept[u] = r.pack(all.p0 + lane + u * G);
     }
-    const TeacherSum ts = read_teacher<G>(te, row, V, sc.c, lane, weight, place, part[sub]);
+    const TeacherSum ts = read_teacher<T, G>(te, x, r, row, sc.c, lane, e, part[sub]);
     Stat a = {-INFINITY, 0.f, 0.f};
-    if constexpr (NV % 4 == 0) {
-#pragma unroll
-      for (int u = 0; u < NV; u += 4) add_packs<T, 4>(a, reinterpret_cast<const P(&)[4]>(kept[u]), sc.c);
-    } else {
-      add_packs<T, NV>(a, kept, sc.c);
-    }
-    scan<T, G>(a, r, NV * G, r.packs, lane, sc.c);
-    a = tt::row_join<G, false>(a, sc.c, more[sub]);
+    Share rest = all;
+    rest.p0 = LONG && all.p0 + NV * G < all.p1 ? all.p0 + NV * G : all.p1;
+    int best;
+    tt::scan<T, G, false, LONG>(a, best, x, r, rest, lane, sc.c);
+    if constexpr (NV > 0) add_kept<T, NV>(a, kept, sc.c);
+    a = tt::row_join<T, G, false>(a, sc.c, more[sub]);
     const float log_s = tt::log_sum(a);
-    const float cross = cross_entropy<T, G>(x, row, V, a, log_s, sc.inverse, te.K, lane, weight, place,
-                                            more[sub] + 3 * (G / kWave));
-    if (lane == 0) write_row(loss, counted, stats, row, a, log_s, ts, cross, sc);
+    float cross = cross_entropy<T, G>(e, te.K, lane, a, log_s, sc);
     if constexpr (GRAD) {
-      T* out = tt::packs_of(dx, row, V);
       const bool none = ts.s == 0.f || a.m == -INFINITY;
-      const float by = ts.s == ts.s ? scale : ts.s, l = log_s;
+      const float by = ts.s == ts.s ? scale : ts.s;
+      if (!none) queue_entries<T, G>(e, r, all, te.K, lane, a.m, log_s, sc.c, by);
+      int own = all.p0 + lane;        // (opaque as the packs are: no address is held from the reads to here)
+      asm volatile("" : "+v"(own));
 #pragma unroll
       for (int u = 0; u < NV; ++u) {
-        const int j = lane + u * G;
-        if (j < r.packs) tt::write_pack(r, out, j, none ? P((T)0.f) : gradient_pack<T>(kept[u], a.m, l, sc.c, by));
+        asm volatile("" : "+v"(kept[u]));
+        const int j = own + u * G;
+        if (j < all.p1) {
+          const Words q = none ? Words(0u) : gradient_pack<T, true>(kept[u], a.m, log_s, sc.c, by);
+          tt::write_pack(r, dx, j, q);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      for (int j = lane + NV * G; j < r.packs; j += G)
-        tt::write_pack(r, out, j, none ? P((T)0.f) : gradient_pack<T>(r.read(j), a.m, l, sc.c, by));
-      if (!none) fix_entries<T, G>(x, dx, r, row, 0, r.packs, te.K, lane, weight, place, a.m, l, sc.c, by);
+      if constexpr (LONG)
+        for (int j = rest.p0 + lane; j < rest.p1; j += kUnroll * G) {
+          Words p[kUnroll];
+#pragma unroll
+          for (int u = 0; u < kUnroll; ++u)
+            if (j + u * G < rest.p1) p[u] = r.pack(j + u * G);
+#pragma unroll
+          for (int u = 0; u < kUnroll; ++u)
+            if (j + u * G < rest.p1)
+              tt::write_pack(r, dx, j + u * G, none ? Words(0u) : gradient_pack<T, true>(p[u], a.m, log_s, sc.c, by));
+        }
+      write_loose(x, dx, r, all, lane, none, a.m, log_s, sc.c, by);
+      store_queued(e, dx, r, lane);
     }
+    cross = tt::row_sum<G>(cross, more[sub] + 3 * (G / kWave));
+    if (lane == 0) write_row(o, row, a, log_s, ts, cross, sc);
     tt::sync_row<G>();
   }
+  tt::stores_done();
+  __syncthreads();
+  if (threadIdx.x == 0) last = tt::last_ticket(&distill_done, gridDim.x);
+  __syncthreads();
+  if (last) add_rows<kBlock>(o, R, sums);
 }
 
-// Few long rows: `splits` blocks to a row, each with the sums of its share of the packs; distill_join puts them
-// together.
+// Few long rows: `splits` blocks to a row, each with the sums of its share; the one that comes last puts them together,
+// and the one whose row is the last of all adds up the rows.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void distill_split(const T* __restrict__ x, float2* __restrict__ stat_part,
-                                                          Scale sc, int splits, int V) {
-  __shared__ float part[3 * (kThreads / kWave)];
-  const int row = blockIdx.x / splits, split = blockIdx.x % splits;
-  const LogitRow<T> r(x, row, V);
-  const int per = (r.packs + splits - 1) / splits;
-  const int v0 = split * per, v1 = v0 + per < r.packs ? v0 + per : r.packs;
-  Stat a = {-INFINITY, 0.f, 0.f};
-  scan<T, kThreads>(a, r, v0, v1, threadIdx.x, sc.c);
-  a = tt::row_join<kThreads, false>(a, sc.c, part);
-  if (threadIdx.x == 0) stat_part[blockIdx.x] = make_float2(a.m, a.s);
-}
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void distill_join(const T* __restrict__ x, Teacher te,
-                                                         const float2* __restrict__ stat_part,
-                                                         float* __restrict__ loss, float* __restrict__ counted,
-                                                         float2* __restrict__ stats, Scale sc, int splits, int V) {
+__global__ __launch_bounds__(kThreads) void distill_split(const T* __restrict__ x, Teacher te, Out o, float* stat_part,
+                                                          Scale sc, int splits, int R, int V) {
   constexpr int G = kThreads;
   extern __shared__ float lds[];
   __shared__ float part[3 * (G / kWave)];
   __shared__ float more[4 * (G / kWave)];
-  const size_t row = blockIdx.x;
-  float* weight = lds;
-  int* place = (int*)(lds + te.K);
+  __shared__ double sums[2 * (G / kWave)];
+  __shared__ bool last;
+  const int split = blockIdx.x % splits, lane = threadIdx.x;
+  const size_t row = blockIdx.x / splits;
+  const Entries e = entries_of<G>(lds, te.K, 0);
+  const LogitRow<T> r(x, row, V);
   Stat a = {-INFINITY, 0.f, 0.f};
-  if (threadIdx.x < splits) {
-    const float2 v = stat_part[row * splits + threadIdx.x];
-    a.m = v.x;
-    a.s = v.y;
+  int best;
+  tt::scan<T, G, false>(a, best, x, r, Share(r, split, splits), lane, sc.c);
+  a = tt::row_join<T, G, false>(a, sc.c, part);
+  if (lane == 0) {
+    tt::share(stat_part + (size_t)blockIdx.x * 2, a.m);
+    tt::share(stat_part + (size_t)blockIdx.x * 2 + 1, a.s);
+    tt::stores_done();
+    last = tt::last_ticket(&distill_tickets[row], splits);
   }
-  const TeacherSum ts = read_teacher<G>(te, row, V, sc.c, threadIdx.x, weight, place, part);
-  a = tt::row_join<G, false>(a, sc.c, more);
-  const float log_s = tt::log_sum(a);
-  const float cross = cross_entropy<T, G>(x, row, V, a, log_s, sc.inverse, te.K, threadIdx.x, weight, place,
-                                          more + 3 * (G / kWave));
-  if (threadIdx.x == 0) write_row(loss, counted, stats, row, a, log_s, ts, cross, sc);
-}
-
-// out[0] = sum of the rows' losses, over count[0], the number of rows with a teacher, if `mean`.  One block.
-__global__ __launch_bounds__(1024) void distill_total(const float* __restrict__ loss, const float* __restrict__ counted,
-                                                      float* __restrict__ out, float* __restrict__ count, int R,
-                                                      int mean) {
-  __shared__ double part[2][16];
-  double s = 0.0, n = 0.0;
-  for (int r = threadIdx.x; r < R; r += 1024) {
-    s += (double)loss[r];
-    n += (double)counted[r];
+  __syncthreads();
+  if (!last) return;
+  Stat whole = {-INFINITY, 0.f, 0.f};
+  if (lane < splits) {
+    whole.m = tt::shared(stat_part + (row * splits + lane) * 2);
+    whole.s = tt::shared(stat_part + (row * splits + lane) * 2 + 1);
   }
-  s = tt::row_sum<1024>(s, part[0]);
-  n = tt::row_sum<1024>(n, part[1]);
-  if (threadIdx.x == 0) {
-    if (out) out[0] = (float)(mean ? s / n : s);
-    count[0] = (float)n;
+  const TeacherSum ts = read_teacher<T, G>(te, x, r, row, sc.c, lane, e, part);
+  whole = tt::row_join<T, G, false>(whole, sc.c, more);
+  const float log_s = tt::log_sum(whole);
+  const float cross = tt::row_sum<G>(cross_entropy<T, G>(e, te.K, lane, whole, log_s, sc), more + 3 * (G / kWave));
+  if (lane == 0) {
+    write_row(o, row, whole, log_s, ts, cross, sc);
+    tt::stores_done();
+    last = tt::last_ticket(&distill_done, R);
   }
+  __syncthreads();
+  if (last) add_rows<G>(o, R, sums);
 }
 
 // The gradient from the kept statistics.  With `ahead` the forward pass has written it for an incoming gradient of one
@@ -286,39 +371,38 @@ __global__ __launch_bounds__(kThreads) void distill_bwd(const T* __restrict__ x,
                                                         T* dx, Scale sc, int reduction, int ahead, int splits, int R,
                                                         int V) {
   constexpr int kRows = kThreads / G;
-  typedef typename Pack<T>::type P;
   if (ahead && g[0] == 1.f) return;
   extern __shared__ float lds[];
   __shared__ float part[kRows][3 * (G / kWave)];
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
-  float* weight = lds + sub * 2 * te.K;
-  int* place = (int*)(weight + te.K);
+  const Entries e = entries_of<G>(lds, te.K, sub);
   const long long items = (long long)R * splits;
   for (long long item = (long long)blockIdx.x * kRows + sub; item < items; item += (long long)gridDim.x * kRows) {
-    const size_t row = item / splits;
-    const int split = (int)(item % splits);
+    const size_t row = R - 1 - item / splits;     // (what the forward pass read last may still be cached)
     const LogitRow<T> r(x, row, V);
-    T* out = tt::packs_of(dx, row, V);
-    const int per = (r.packs + splits - 1) / splits;
-    const int v0 = split * per, v1 = v0 + per < r.packs ? v0 + per : r.packs;
+    const Share s(r, (int)(item % splits), splits);
     const float2 st = stats[row];
-    if (st.x == -INFINITY) {
-      for (int j = v0 + lane; j < v1; j += G) tt::write_pack(r, out, j, P((T)0.f));
-      continue;
-    }
+    const bool none = st.x == -INFINITY;
     float scale = sc.temperature * (reduction == 0 ? g[row] : g[0]);
     if (reduction == 2) scale /= count[0];
-    for (int j = v0 + lane; j < v1; j += kUnroll * G) {
-      P p[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (j + u * G < v1) p[u] = r.read(j + u * G);
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (j + u * G < v1) tt::write_pack(r, out, j + u * G, gradient_pack<T>(p[u], st.x, st.y, sc.c, scale));
+    if (none) {
+      e.queue[lane] = -1;
+    } else {
+      read_teacher<T, G>(te, x, r, row, sc.c, lane, e, part[sub]);
+      queue_entries<T, G>(e, r, s, te.K, lane, st.x, st.y, sc.c, scale);
     }
-    read_teacher<G>(te, row, V, sc.c, lane, weight, place, part[sub]);
-    fix_entries<T, G>(x, dx, r, row, v0, v1, te.K, lane, weight, place, st.x, st.y, sc.c, scale);
+    for (int j = s.p0 + lane; j < s.p1; j += kUnroll * G) {
+      Words p[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (!none && j + u * G < s.p1) p[u] = r.pack(j + u * G);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (j + u * G < s.p1)
+          tt::write_pack(r, dx, j + u * G, none ? Words(0u) : gradient_pack<T, false>(p[u], st.x, st.y, sc.c, scale));
+    }
+    write_loose(x, dx, r, s, lane, none, st.x, st.y, sc.c, scale);
+    store_queued(e, dx, r, lane);
     tt::sync_row<G>();
   }
 }
@@ -341,8 +425,10 @@ int check(const char* fn, int dtype, int teacher_dtype, int index_bits, double t
 
 unsigned grid_for(long long blocks, long long most) { return (unsigned)(blocks < most ? blocks : most); }
 
-// Rows of up to this many packs go to a wave each, which keeps them in registers.
-constexpr int kWavePacks = 8 * kWave;
+// Rows of up to this many packs go to a wave each, which keeps them in registers; four of them share a block's LDS, where
+// the teacher's entries have to fit.
+constexpr int kWavePacks = 8 * kWave, kWaveEntries = 256;
+bool by_waves(int packs, int K) { return packs <= kWavePacks && K <= kWaveEntries; }
 
 int packs_for(int V, int dtype) { return dtype == TT_F32 ? (V + 3) / 4 : (V + 7) / 8; }
 
@@ -366,21 +452,31 @@ bool ahead(int dtype, int reduction, long long R, int V) {
 }
 
 template <typename T, bool GRAD>
-int launch_rows(const T* x, const Teacher& te, float* loss, float* counted, float* stats, T* dx, const int* count_parts,
-                const Scale& sc, int R, int V, int packs) {
+int launch_rows(const T* x, const Teacher& te, const Out& o, T* dx, const int* count_parts, const Scale& sc, int R,
+                int V, int packs) {
   hipStream_t st = tt::stream();
-  float2* s = (float2*)stats;
-  const size_t lds = (size_t)te.K * 8;
-  const int cus = tt::compute_units();
-  if (packs <= kWavePacks)
-    distill_rows<T, kWave, 8, GRAD><<<grid_for((R + 3LL) / 4, 16 * cus), kThreads, 4 * lds, st>>>(
-        x, te, loss, counted, s, dx, count_parts, sc, R, V);
-  else if (packs <= 8 * 256)
-    distill_rows<T, 256, 8, GRAD><<<grid_for(R, 16 * cus), 256, lds, st>>>(x, te, loss, counted, s, dx, count_parts, sc,
-                                                                          R, V);
-  else
-    distill_rows<T, 1024, 8, GRAD><<<grid_for(R, 16 * cus), 1024, lds, st>>>(x, te, loss, counted, s, dx, count_parts,
-                                                                            sc, R, V);
+  const long long most = 16 * tt::compute_units();
+  const size_t wave_lds = entries_bytes<kWave>(te.K, kThreads / kWave);
+  if constexpr (!GRAD) {
+    if (by_waves(packs, te.K))
+      distill_rows<T, kWave, 0, true, false><<<grid_for((R + 3LL) / 4, most), kThreads, wave_lds, st>>>(
+          x, te, o, dx, count_parts, sc, R, V);
+    else
+      distill_rows<T, 256, 0, true, false><<<grid_for(R, most), 256, entries_bytes<256>(te.K, 1), st>>>(
+          x, te, o, dx, count_parts, sc, R, V);
+  } else if (by_waves(packs, te.K)) {
+    distill_rows<T, kWave, 8, false, true><<<grid_for((R + 3LL) / 4, most), kThreads, wave_lds, st>>>(
+        x, te, o, dx, count_parts, sc, R, V);
+  } else if (packs <= 8 * 256) {
+    distill_rows<T, 256, 8, false, true><<<grid_for(R, most), 256, entries_bytes<256>(te.K, 1), st>>>(
+        x, te, o, dx, count_parts, sc, R, V);
+  } else if (packs <= 16 * 512) {
+    distill_rows<T, 512, 16, false, true><<<grid_for(R, most), 512, entries_bytes<512>(te.K, 1), st>>>(
+        x, te, o, dx, count_parts, sc, R, V);
+  } else {
+    distill_rows<T, 1024, 16, true, true><<<grid_for(R, most), 1024, entries_bytes<1024>(te.K, 1), st>>>(
+        x, te, o, dx, count_parts, sc, R, V);
+  }
   TT_LAUNCH_CHECK();
   return 0;
 }
@@ -397,31 +493,25 @@ int forward(const T* x, const Teacher& te, float* loss, float* stats, float* cou
   const int packs = (V + Pack<T>::n - 1) / Pack<T>::n;
   const int splits = whole_rows(R, packs) ? 1 : splits_for(R, packs);
   void* ws;
-  if (tt::workspace(((size_t)R * 2 + kCountBlocks) * sizeof(float) + (size_t)R * splits * sizeof(float2), &ws))
-    return -1;
-  float2* stat_part = (float2*)ws;
-  float* counted = (float*)(stat_part + (size_t)R * splits);
+  if (tt::workspace(((size_t)R * 2 + kCountBlocks + (size_t)R * splits * 2) * sizeof(float), &ws)) return -1;
+  float* stat_part = (float*)ws;
+  float* counted = stat_part + (size_t)R * splits * 2;
   int* parts = (int*)(counted + R);
-  float* rows = reduction == 0 ? loss : (float*)(parts + kCountBlocks);
+  const Out o = {reduction == 0 ? loss : (float*)(parts + kCountBlocks), counted, (float2*)stats,
+                 reduction == 0 ? nullptr : loss, count, reduction == 2};
   if (splits > 1) {
-    distill_split<T><<<(unsigned)(R * splits), kThreads, 0, st>>>(x, stat_part, sc, splits, V);
+    distill_split<T><<<(unsigned)(R * splits), kThreads, entries_bytes<kThreads>(te.K, 1), st>>>(x, te, o, stat_part, sc, splits, R, V);
     TT_LAUNCH_CHECK();
-    distill_join<T><<<R, kThreads, (size_t)te.K * 8, st>>>(x, te, stat_part, rows, counted, (float2*)stats, sc, splits,
-                                                           V);
-    TT_LAUNCH_CHECK();
-  } else if (dx) {
-    if (reduction == 2) {
-      distill_count<<<kCountBlocks, kThreads, 0, st>>>(te, parts, R, V);
-      TT_LAUNCH_CHECK();
-    }
-    if (launch_rows<T, true>(x, te, rows, counted, stats, dx, reduction == 2 ? parts : nullptr, sc, R, V, packs))
-      return -1;
-  } else {
-    if (launch_rows<T, false>(x, te, rows, counted, stats, dx, nullptr, sc, R, V, packs)) return -1;
+    return 0;
   }
-  distill_total<<<1, 1024, 0, st>>>(rows, counted, reduction == 0 ? nullptr : loss, count, R, reduction == 2);
-  TT_LAUNCH_CHECK();
-  return 0;
+  if (!dx) return launch_rows<T, false>(x, te, o, dx, nullptr, sc, R, V, packs);
+  // a block counts this many rows by itself in the time of a launch
+  const bool counts_itself = R <= 1024;
+  if (reduction == 2 && !counts_itself) {
+    distill_count<<<kCountBlocks, kThreads, 0, st>>>(te, parts, R, V);
+    TT_LAUNCH_CHECK();
+  }
+  return launch_rows<T, true>(x, te, o, dx, counts_itself ? nullptr : parts, sc, R, V, packs);
 }
 
 template <typename T>
@@ -430,13 +520,14 @@ int backward(const T* x, const Teacher& te, const float* stats, const float* cou
   hipStream_t st = tt::stream();
   const Scale sc = scale_for(temperature);
   const int packs = (V + Pack<T>::n - 1) / Pack<T>::n;
-  const size_t lds = (size_t)te.K * 8;
-  if (packs <= kWavePacks) {
-    distill_bwd<T, kWave><<<grid_for((R + 3LL) / 4, 16 * tt::compute_units()), kThreads, 4 * lds, st>>>(
+  if (by_waves(packs, te.K)) {
+    distill_bwd<T, kWave><<<grid_for((R + 3LL) / 4, 16 * tt::compute_units()), kThreads,
+                            entries_bytes<kWave>(te.K, kThreads / kWave), st>>>(
         x, te, (const float2*)stats, count, g, dx, sc, reduction, is_ahead, 1, R, V);
   } else {
     const int splits = splits_for(R, packs);
-    distill_bwd<T, kThreads><<<grid_for((long long)R * splits, 16 * tt::compute_units()), kThreads, lds, st>>>(
+    distill_bwd<T, kThreads><<<grid_for((long long)R * splits, 16 * tt::compute_units()), kThreads,
+                               entries_bytes<kThreads>(te.K, 1), st>>>(
         x, te, (const float2*)stats, count, g, dx, sc, reduction, is_ahead, splits, R, V);
   }
   TT_LAUNCH_CHECK();

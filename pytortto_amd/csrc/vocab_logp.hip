@@ -2,16 +2,21 @@
 // backward (vocab.h has the formulas).
 #include "vocab.h"
 
+#include <type_traits>
+
 namespace {
 
+using tt::kUnroll;
 using tt::kWave;
 using tt::LogitRow;
 using tt::Pack;
+using tt::Share;
 using tt::Stat;
 
 constexpr int kThreads = 256;
+constexpr tt::Scale kPlain = {(float)tt::kLog2e, 1.f, 1.f};
 constexpr int kMostTop = 64;
-constexpr int kUnroll = 4;
+constexpr int kMostSplitRows = 8192;    // fewer rows than this may be shared by blocks
 
 // ---- the best alternatives -------------------------------------------------------------------------
 //
@@ -51,16 +56,20 @@ __device__ __forceinline__ Key wave_sort(Key k) {
   return k;
 }
 
+constexpr int most(int a, int b) { return a > b ? a : b; }
+
 template <int G, int n>
 struct TopSpace {
-  static constexpr int room = G * n + kMostTop;     // what one round can add to K kept candidates
+  // what one round can add to K kept candidates; what the lists of the splits can add up to
+  static constexpr int room = most(G * n + kMostTop, G == kWave ? 0 : kMostTop * (kMostTop + 1) / 2);
   Key cand[room];
-  Key heads[G / kWave * kMostTop];
+  Key heads[G];
   Key best[kMostTop];
   int owner[kMostTop];
   int count, owners;
   Key bound;
 };
+struct NoSpace {};
 
 // Of `count` keys in `cand` the K largest, largest first, to `best` (zeros where there are fewer).
 template <int G, int n>
@@ -76,11 +85,33 @@ __device__ __forceinline__ void rank_candidates(TopSpace<G, n>& s, int lane, int
   tt::sync_row<G>();
 }
 
-// Packs [v0, v1) of the row by the G threads, thread `lane` on v0 + lane + i G; `mine` is the key of its best value, or
-// zero.  Leaves the K best in s.best.
+// The key of a thread's best value, from where scan() says that it stands; zero of a thread without values.
 template <typename T, int G>
-__device__ __forceinline__ void select_top(TopSpace<G, Pack<T>::n>& s, const LogitRow<T>& r, int v0, int v1, int lane,
-                                           Key mine, int K) {
+__device__ __forceinline__ Key best_key(const T* x, const LogitRow<T>& r, const Share& h, int lane, int best) {
+  if (best == tt::kNothing) return 0;
+  if (best == tt::kHead) return make_key(tt::widen(x[r.start + lane]), lane);
+  if (best == tt::kTail) return make_key(tt::widen(x[r.start + r.tail_at + lane]), r.tail_at + lane);
+  Key mine = 0;
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int j = best + u * G;
+    if (j < h.p1) {
+      float z[Pack<T>::n];
+      tt::unpack<T>(z, r.pack(j));
+#pragma unroll
+      for (int i = 0; i < Pack<T>::n; ++i) {
+        const Key k = make_key(z[i], r.column(j) + i);
+        mine = k > mine ? k : mine;
+      }
+    }
+  }
+  return mine;
+}
+
+// Leaves the K best of a share in s.best; `mine` is the key of this thread's best value, or zero.
+template <typename T, int G>
+__device__ __forceinline__ void select_top(TopSpace<G, Pack<T>::n>& s, const T* x, const LogitRow<T>& r, const Share& h,
+                                           int lane, Key mine, int K) {
   constexpr int n = Pack<T>::n;
   const Key sorted = wave_sort(mine);
   const int in_wave = lane & (kWave - 1), lists = G / kWave;
@@ -90,37 +121,46 @@ __device__ __forceinline__ void select_top(TopSpace<G, Pack<T>::n>& s, const Log
     s.bound = 0;
   }
   tt::sync_row<G>();
-  for (int i = lane; i < lists * K; i += G) {       // (at most one each: K <= 64)
-    const Key k = s.heads[i];
+  if (lane < lists * K) {                           // (K <= 64: at most one key to a thread)
+    const Key k = s.heads[lane];
     int rank = 0;
     for (int o = 0; o < lists * K; ++o) rank += s.heads[o] > k;
     if (k != 0 && rank < K) {
-      s.owner[rank] = ((key_place(k) + r.skip) / n - v0) % G;
+      const int c = key_place(k);
+      s.owner[rank] = c < r.head ? c : c >= r.tail_at ? c - r.tail_at : ((c + r.skip) / n - h.p0) % G;
       atomicAdd(&s.owners, 1);
       if (rank == K - 1) s.bound = k;
     }
   }
   tt::sync_row<G>();
-  const int rounds = (v1 - v0 + G - 1) / G, pairs = s.owners * rounds;
+  // every owner's packs, and its column of the head and of the tail
+  const int rounds = (h.p1 - h.p0 + G - 1) / G, steps = rounds + 2, pairs = s.owners * steps;
   Key bound = s.bound;
   int count = 0;
-  for (int p0 = 0; p0 < pairs; p0 += G) {
-    const int p = p0 + lane;
-    if (p < pairs) {
-      const int j = v0 + s.owner[p / rounds] + p % rounds * G;
-      if (j < v1) {
-        const typename Pack<T>::type q = r.read(j);
+  for (int q0 = 0; q0 < pairs; q0 += G) {
+    const int q = q0 + lane;
+    if (q < pairs) {
+      const int owner = s.owner[q / steps], step = q % steps;
+      if (step < rounds) {
+        const int j = h.p0 + owner + step * G;
+        if (j < h.p1) {
+          float z[n];
+          tt::unpack<T>(z, r.pack(j));
 #pragma unroll
-        for (int i = 0; i < n; ++i) {
-          const int c = r.column(j) + i;
-          const Key k = make_key(tt::widen(q[i]), c);
-          if (c >= 0 && c < r.V && k >= bound) s.cand[atomicAdd(&s.count, 1)] = k;
+          for (int i = 0; i < n; ++i) {
+            const Key k = make_key(z[i], r.column(j) + i);
+            if (k >= bound) s.cand[atomicAdd(&s.count, 1)] = k;
+          }
         }
+      } else if (owner < (step == rounds ? h.head : h.tail)) {
+        const int c = (step == rounds ? 0 : r.tail_at) + owner;
+        const Key k = make_key(tt::widen(x[r.start + c]), c);
+        if (k >= bound) s.cand[atomicAdd(&s.count, 1)] = k;
       }
     }
     tt::sync_row<G>();
     count = s.count;
-    if (count > kMostTop && p0 + G < pairs) {       // another round might not fit: keep the K best of these
+    if (count > kMostTop && q0 + G < pairs) {       // another round might not fit: keep the K best of these
       rank_candidates(s, lane, count, K);
       for (int k = lane; k < K; k += G) s.cand[k] = s.best[k];
       bound = s.best[K - 1] > bound ? s.best[K - 1] : bound;
@@ -129,6 +169,38 @@ __device__ __forceinline__ void select_top(TopSpace<G, Pack<T>::n>& s, const Log
     tt::sync_row<G>();
   }
   rank_candidates(s, lane, count, K);
+}
+
+// The K best of `splits` sorted lists of K keys.  The list whose head has rank i holds at most K - i of them, and those
+// reach the K-th head: at most K (K + 1) / 2 candidates.
+template <int G, int n>
+__device__ __forceinline__ void join_top(TopSpace<G, n>& s, const Key* lists, int splits, int lane, int K) {
+  const Key head = lane < splits ? tt::shared(lists + (size_t)lane * K) : 0;
+  s.heads[lane] = head;
+  if (lane == 0) {
+    s.count = s.owners = 0;
+    s.bound = 0;
+  }
+  __syncthreads();
+  if (head != 0) {
+    int rank = 0;
+    for (int i = 0; i < splits; ++i) rank += s.heads[i] > head;
+    if (rank < K) {
+      s.owner[rank] = lane;
+      atomicAdd(&s.owners, 1);
+      if (rank == K - 1) s.bound = head;
+    }
+  }
+  __syncthreads();
+  for (int q = lane; q < s.owners * K; q += G) {
+    const int rank = q / K, k = q % K;
+    if (k < K - rank) {
+      const Key key = tt::shared(lists + (size_t)s.owner[rank] * K + k);
+      if (key != 0 && key >= s.bound) s.cand[atomicAdd(&s.count, 1)] = key;
+    }
+  }
+  __syncthreads();
+  rank_candidates(s, lane, s.count, K);
 }
 
 // ---- forward ---------------------------------------------------------------------------------------
@@ -163,71 +235,27 @@ __device__ __forceinline__ void write_ignored(const ForwardOut& o, size_t row, i
   }
 }
 
-template <int G>
+template <typename T, int G>
 __device__ __forceinline__ void write_row(const ForwardOut& o, size_t row, int lane, const Stat& a, bool is_token,
                                           float z_token, const Key* best, int K) {
   const float log_s = tt::log_sum(a), m = tt::anchor(a.m);
   if (lane == 0) {
-    o.logp[row] = is_token ? (z_token - m) - log_s * tt::kLn2 : NAN;
+    o.logp[row] = is_token ? tt::log_p<T>(z_token, m, log_s, kPlain) : NAN;
     o.entropy[row] = a.s == 0.f ? 0.f : (log_s - a.t / a.s) * tt::kLn2;
     if (o.stats) o.stats[row] = make_float2(a.m, log_s);
   }
   const bool fine = a.s == a.s;
   for (int k = lane; k < K; k += G) {
-    o.top_logp[row * K + k] = fine ? (key_value(best[k]) - m) - log_s * tt::kLn2 : NAN;
+    o.top_logp[row * K + k] = fine ? tt::log_p<T>(key_value(best[k]), m, log_s, kPlain) : NAN;
     o.top_index[row * K + k] = fine ? key_place(best[k]) : -1;
   }
-}
-
-// The statistics of packs [v0, v1), and with TOP the key of this thread's best value.
-template <typename T, int G, bool TOP>
-__device__ __forceinline__ Stat scan(const LogitRow<T>& r, int v0, int v1, int lane, float c, Key& mine) {
-  constexpr int n = Pack<T>::n;
-  typedef typename Pack<T>::type P;
-  Stat a = {-INFINITY, 0.f, 0.f};
-  int best = -1;
-  const int whole1 = v1 < r.whole1 ? v1 : r.whole1;
-  for (int j = v0 + lane; j < v1; j += kUnroll * G) {
-    P p[kUnroll];
-    if (j >= r.whole0 && j + (kUnroll - 1) * G < whole1) {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) p[u] = r.at[j + u * G];
-    } else {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) p[u] = j + u * G < v1 ? r.read(j + u * G) : P((T)-INFINITY);
-    }
-    float z[kUnroll * n];
-#pragma unroll
-    for (int i = 0; i < kUnroll * n; ++i) z[i] = tt::widen(p[i / n][i % n]);
-    const bool rises = tt::add_values<kUnroll * n, true>(a, z, c);
-    if (TOP && (rises || best < 0)) best = j;
-  }
-  if (TOP) {
-    mine = 0;
-    if (best >= 0) {
-#pragma unroll
-      for (int u = kUnroll - 1; u >= 0; --u) {
-        const int j = best + u * G;
-        if (j < v1) {
-          const P p = r.read(j);
-#pragma unroll
-          for (int i = n - 1; i >= 0; --i) {
-            const int col = r.column(j) + i;
-            const Key k = make_key(tt::widen(p[i]), col);
-            if (col >= 0 && col < r.V && k > mine) mine = k;
-          }
-        }
-      }
-    }
-  }
-  return a;
 }
 
 template <typename T, int G, bool TOP>
 __global__ __launch_bounds__(kThreads) void logp_rows(const T* __restrict__ x, ForwardOut o, int R, int V, int K) {
   constexpr int kRows = kThreads / G;
   __shared__ float part[kRows][3 * (G / kWave)];
-  __shared__ TopSpace<TOP ? G : kWave, TOP ? Pack<T>::n : 1> space[TOP ? kRows : 1];
+  __shared__ std::conditional_t<TOP, TopSpace<G, Pack<T>::n>, NoSpace> space[kRows];
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
   const float c = (float)tt::kLog2e;
   for (long long row = (long long)blockIdx.x * kRows + sub; row < R; row += (long long)gridDim.x * kRows) {
@@ -237,89 +265,79 @@ __global__ __launch_bounds__(kThreads) void logp_rows(const T* __restrict__ x, F
       continue;
     }
     const LogitRow<T> r(x, row, V);
+    const Share h(r, 0, 1);
     const long long t = token_place(t0, V);
-    const float z_token = lane == 0 && t >= 0 ? tt::widen(x[row * (size_t)V + t]) : 0.f;
-    Key mine;
-    Stat a = scan<T, G, TOP>(r, 0, r.packs, lane, c, mine);
-    a = tt::row_join<G, true>(a, c, part[sub]);
-    if constexpr (TOP) select_top<T, G>(space[sub], r, 0, r.packs, lane, mine, K);
-    if constexpr (TOP) write_row<G>(o, row, lane, a, t >= 0, z_token, space[sub].best, K);
-    else write_row<G>(o, row, lane, a, t >= 0, z_token, nullptr, 0);
+    const float z_token = lane == 0 && t >= 0 ? tt::widen(x[r.start + t]) : 0.f;
+    Stat a = {-INFINITY, 0.f, 0.f};
+    int best = tt::kNothing;
+    tt::scan<T, G, true>(a, best, x, r, h, lane, c);
+    Key mine = 0;
+    if constexpr (TOP) mine = best_key<T, G>(x, r, h, lane, best);
+    a = tt::row_join<T, G, true>(a, c, part[sub]);
+    if constexpr (TOP) {
+      select_top<T, G>(space[sub], x, r, h, lane, mine, K);
+      write_row<T, G>(o, row, lane, a, t >= 0, z_token, space[sub].best, K);
+    } else {
+      write_row<T, G>(o, row, lane, a, t >= 0, z_token, nullptr, 0);
+    }
     tt::sync_row<G>();
   }
 }
 
-// Few long rows: `splits` blocks to a row, each with its share of the packs; logp_join puts them together.
-template <typename T, bool TOP>
-__global__ __launch_bounds__(kThreads) void logp_split(const T* __restrict__ x, const void* __restrict__ tokens,
-                                                       int wide, long long ignored, Stat* __restrict__ stat_part,
-                                                       Key* __restrict__ key_part, int splits, int V, int K) {
-  constexpr int G = kThreads;
-  __shared__ float part[3 * (G / kWave)];
-  __shared__ TopSpace<TOP ? G : kWave, TOP ? Pack<T>::n : 1> space;
-  const int row = blockIdx.x / splits, split = blockIdx.x % splits, lane = threadIdx.x;
-  if (tt::read_index(tokens, row, wide) == ignored) return;
-  const LogitRow<T> r(x, row, V);
-  const int per = (r.packs + splits - 1) / splits;
-  const int v0 = split * per, v1 = v0 + per < r.packs ? v0 + per : r.packs;     // (v0 may lie behind the last pack)
-  Key mine;
-  Stat a = scan<T, G, TOP>(r, v0, v1, lane, (float)tt::kLog2e, mine);
-  a = tt::row_join<G, true>(a, (float)tt::kLog2e, part);
-  if (lane == 0) stat_part[blockIdx.x] = a;
-  if constexpr (TOP) {
-    select_top<T, G>(space, r, v0, v1, lane, mine, K);
-    for (int k = lane; k < K; k += G) key_part[(size_t)blockIdx.x * K + k] = space.best[k];
-  }
-}
+// How many splits of a row are done; zero between launches.
+__device__ unsigned logp_tickets[kMostSplitRows];
 
-// One block to a row.  The splits' lists of keys are sorted, so the list whose head has rank i holds at most K - i of
-// the K best, and those reach the K-th head: at most K (K + 1) / 2 candidates.
+// Few long rows: `splits` blocks to a row, each with its share; the one that comes last puts the shares together.
 template <typename T, bool TOP>
-__global__ __launch_bounds__(kThreads) void logp_join(const T* __restrict__ x, ForwardOut o,
-                                                      const Stat* __restrict__ stat_part,
-                                                      const Key* __restrict__ key_part, int splits, int V, int K) {
+__global__ __launch_bounds__(kThreads) void logp_split(const T* __restrict__ x, ForwardOut o, float* stat_part,
+                                                       Key* key_part, int splits, int V, int K) {
   constexpr int G = kThreads;
   __shared__ float part[3 * (G / kWave)];
-  __shared__ Key heads[TOP ? G : 1];
-  typedef TopSpace<TOP ? G : kWave, TOP ? 8 : 1> Space;
-  static_assert(!TOP || kMostTop * (kMostTop + 1) / 2 <= Space::room, "the lists' candidates fit");
-  __shared__ Space space;
-  const int lane = threadIdx.x;
-  const size_t row = blockIdx.x;
+  __shared__ float more[3 * (G / kWave)];
+  __shared__ std::conditional_t<TOP, TopSpace<G, Pack<T>::n>, NoSpace> space;
+  __shared__ bool last;
+  const float c = (float)tt::kLog2e;
+  const int split = blockIdx.x % splits, lane = threadIdx.x;
+  const size_t row = blockIdx.x / splits;
   const long long t0 = tt::read_index(o.tokens, row, o.wide);
   if (t0 == o.ignored) {
-    write_ignored<G>(o, row, lane, K);
+    if (split == 0) write_ignored<G>(o, row, lane, K);
     return;
   }
-  const long long t = token_place(t0, V);
-  const float z_token = lane == 0 && t >= 0 ? tt::widen(x[row * (size_t)V + t]) : 0.f;
+  const LogitRow<T> r(x, row, V);
+  const Share h(r, split, splits);
   Stat a = {-INFINITY, 0.f, 0.f};
-  if (lane < splits) a = stat_part[row * splits + lane];
-  a = tt::row_join<G, true>(a, (float)tt::kLog2e, part);
+  int best = tt::kNothing;
+  tt::scan<T, G, true>(a, best, x, r, h, lane, c);
+  Key mine = 0;
+  if constexpr (TOP) mine = best_key<T, G>(x, r, h, lane, best);
+  a = tt::row_join<T, G, true>(a, c, part);
+  if constexpr (TOP) select_top<T, G>(space, x, r, h, lane, mine, K);
+  if (lane < kWave) {
+    float* mine_part = stat_part + (size_t)blockIdx.x * 3;
+    if (lane < 3) tt::share(mine_part + lane, lane == 0 ? a.m : lane == 1 ? a.s : a.t);
+    if constexpr (TOP)
+      if (lane < K) tt::share(key_part + (size_t)blockIdx.x * K + lane, space.best[lane]);
+    tt::stores_done();
+    if (lane == 0) last = tt::last_ticket(&logp_tickets[row], splits);
+  }
+  __syncthreads();
+  if (!last) return;
+  const long long t = token_place(t0, V);
+  const float z_token = lane == 0 && t >= 0 ? tt::widen(x[r.start + t]) : 0.f;
+  Stat all = {-INFINITY, 0.f, 0.f};
+  if (lane < splits) {
+    const float* p = stat_part + (row * splits + lane) * 3;
+    all.m = tt::shared(p);
+    all.s = tt::shared(p + 1);
+    all.t = tt::shared(p + 2);
+  }
+  all = tt::row_join<T, G, true>(all, c, more);
   if constexpr (TOP) {
-    const Key* keys = key_part + row * (size_t)splits * K;
-    const Key head = lane < splits ? keys[(size_t)lane * K] : 0;
-    heads[lane] = head;
-    if (lane == 0) {
-      space.count = 0;
-      space.bound = 0;
-    }
-    __syncthreads();
-    int rank = 0;
-    for (int i = 0; i < splits; ++i) rank += heads[i] > head;
-    if (head != 0 && rank == K - 1) space.bound = head;
-    __syncthreads();
-    if (head != 0 && rank < K)
-      for (int k = 0; k < K - rank; ++k) {
-        const Key key = keys[(size_t)lane * K + k];
-        if (key == 0 || key < space.bound) break;
-        space.cand[atomicAdd(&space.count, 1)] = key;
-      }
-    __syncthreads();
-    rank_candidates(space, lane, space.count, K);
-    write_row<G>(o, row, lane, a, t >= 0, z_token, space.best, K);
+    join_top(space, key_part + row * (size_t)splits * K, splits, lane, K);
+    write_row<T, G>(o, row, lane, all, t >= 0, z_token, space.best, K);
   } else {
-    write_row<G>(o, row, lane, a, t >= 0, z_token, nullptr, 0);
+    write_row<T, G>(o, row, lane, all, t >= 0, z_token, nullptr, 0);
   }
 }
 
@@ -337,70 +355,77 @@ struct BackwardIn {
   long long ignored;
 };
 
-// dz_j = -p_j (a + sum_k c_k + h (log p_j + H)) + a [j = t] + sum_k c_k [j = i_k].
-// A block (or wave, G = 64) writes packs [v0, v1) of a row without the last two terms, and then the few values that
-// have them once more.
+// dz_j = -p_j (a + sum_k c_k + h (log p_j + H)) + a [j = t] + sum_k c_k [j = i_k]
+template <typename T>
+struct RowGradient {
+  float m, log_s, total, h, H;
+  __device__ __forceinline__ float operator()(float z, float extra) const {
+    const float d = tt::bits<T>(z, m, (float)tt::kLog2e) - log_s;
+    return fmaf(-tt::pow2(d), fmaf(h, fmaf(tt::floor_at(d), tt::kLn2, H), total), extra);
+  }
+};
+
+// G threads write a share of a row without the last two terms, and then the few values that have them once more.
+// Rows go last to first: what the forward pass read last may still be in the memory-side cache.
 template <typename T, int G>
-__global__ __launch_bounds__(kThreads) void logp_bwd(const T* __restrict__ x, BackwardIn in, T* __restrict__ dx,
-                                                     int splits, int R, int V, int K) {
+__global__ __launch_bounds__(kThreads) void logp_bwd(const T* __restrict__ x, BackwardIn in, T* dx, int splits, int R,
+                                                     int V, int K) {
   constexpr int kRows = kThreads / G, n = Pack<T>::n;
-  typedef typename Pack<T>::type P;
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
-  const float c = (float)tt::kLog2e;
   const long long items = (long long)R * splits;
   for (long long item = (long long)blockIdx.x * kRows + sub; item < items; item += (long long)gridDim.x * kRows) {
-    const long long row = item / splits;
-    const int split = (int)(item % splits);
+    const size_t row = R - 1 - item / splits;
     const LogitRow<T> r(x, row, V);
-    T* out = tt::packs_of(dx, row, V);
-    const int per = (r.packs + splits - 1) / splits;
-    const int v0 = split * per, v1 = v0 + per < r.packs ? v0 + per : r.packs;
+    const Share s(r, (int)(item % splits), splits);
     const long long t0 = tt::read_index(in.tokens, row, in.wide), t = token_place(t0, V);
     const float2 st = in.stats[row];
-    if (t0 == in.ignored || st.x == -INFINITY) {
-      for (int j = v0 + lane; j < v1; j += G) tt::write_pack(r, out, j, P((T)0.f));
-      continue;
-    }
-    const float a = in.g_logp ? in.g_logp[row] : 0.f, h = in.g_entropy ? in.g_entropy[row] : 0.f;
-    const float H = in.entropy[row];
-    float total = in.g_logp && t < 0 ? NAN : a;
-    if (in.g_top) {
-      const int at = threadIdx.x & (kWave - 1);
-      total += tt::wave_sum(at < K ? in.g_top[row * K + at] : 0.f);
-    }
-    for (int j = v0 + lane; j < v1; j += kUnroll * G) {
-      P p[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (j + u * G < v1) p[u] = r.read(j + u * G);
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        if (j + u * G >= v1) continue;
-        P q;
-#pragma unroll
-        for (int i = 0; i < n; ++i) {
-          const float d = (tt::widen(p[u][i]) - st.x) * c - st.y;
-          q[i] = (T)(-tt::pow2(d) * fmaf(h, fmaf(tt::floor_at(d), tt::kLn2, H), total));
-        }
-        tt::write_pack(r, out, j + u * G, q);
+    const bool none = t0 == in.ignored || st.x == -INFINITY, given = in.g_logp && t >= 0;
+    RowGradient<T> g = {st.x, st.y, 0.f, 0.f, 0.f};
+    float a = 0.f;
+    if (!none) {
+      a = in.g_logp ? in.g_logp[row] : 0.f;
+      g.h = in.g_entropy ? in.g_entropy[row] : 0.f;
+      g.H = in.entropy[row];
+      g.total = in.g_logp && t < 0 ? NAN : a;
+      if (in.g_top) {
+        const int at = threadIdx.x & (kWave - 1);
+        g.total += tt::wave_sum(at < K ? in.g_top[row * K + at] : 0.f);
       }
     }
-    const int fixes = (in.g_logp && t >= 0 ? 1 : 0) + (in.g_top ? K : 0);
+    for (int j = s.p0 + lane; j < s.p1; j += kUnroll * G) {
+      tt::Words p[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (!none && j + u * G < s.p1) p[u] = r.pack(j + u * G);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        if (j + u * G >= s.p1) continue;
+        float z[n];
+        tt::unpack<T>(z, p[u]);
+#pragma unroll
+        for (int i = 0; i < n; ++i) z[i] = g(z[i], 0.f);
+        tt::write_pack(r, dx, j + u * G, none ? tt::Words(0u) : tt::pack<T>(z));
+      }
+    }
+    if (lane < s.head + s.tail) {
+      const size_t at = r.start + (lane < s.head ? lane : r.tail_at + lane - s.head);
+      dx[at] = none ? (T)0.f : (T)g(tt::widen(x[at]), 0.f);
+    }
+    const int fixes = none ? 0 : (given ? 1 : 0) + (in.g_top ? K : 0);
     if (fixes == 0) continue;
     // what is stored below goes over what was stored above: that has to have left first
     tt::stores_done();
     tt::sync_row<G>();
     for (int f = lane; f < fixes; f += G) {
-      const bool given = in.g_logp && t >= 0;
       const long long j = given && f == 0 ? t : in.top_index[row * K + f - (given ? 1 : 0)];
       const int pack = (int)((j + r.skip) / n);
-      if (j < 0 || pack < v0 || pack >= v1) continue;
+      const bool here = j < r.head ? s.head > 0 : j >= r.tail_at ? s.tail > 0 : pack >= s.p0 && pack < s.p1;
+      if (j < 0 || !here) continue;
       float extra = given && j == t ? a : 0.f;      // summed first: what cancels here leaves no rounding behind
       if (in.g_top)
         for (int k = 0; k < K; ++k)
           if (in.top_index[row * K + k] == j) extra += in.g_top[row * K + k];
-      const float d = (tt::widen(x[row * (size_t)V + j]) - st.x) * c - st.y;
-      dx[row * (size_t)V + j] = (T)fmaf(-tt::pow2(d), fmaf(h, fmaf(tt::floor_at(d), tt::kLn2, H), total), extra);
+      dx[r.start + j] = (T)g(tt::widen(x[r.start + j]), extra);
     }
     tt::sync_row<G>();
   }
@@ -436,24 +461,14 @@ template <typename T>
 int forward(const T* x, const ForwardOut& o, int R, int V, int K) {
   hipStream_t st = tt::stream();
   const int packs = (V + Pack<T>::n - 1) / Pack<T>::n;
-  const int splits = packs <= kWavePacks ? 1 : splits_for(R, packs);
+  const int splits = packs <= kWavePacks || R > kMostSplitRows ? 1 : splits_for(R, packs);
   if (splits > 1) {
     void* ws;
-    const size_t parts = (size_t)R * splits, stat_bytes = (parts * sizeof(Stat) + 255) / 256 * 256;
+    const size_t parts = (size_t)R * splits, stat_bytes = (parts * 3 * sizeof(float) + 255) / 256 * 256;
     if (tt::workspace(stat_bytes + parts * K * sizeof(Key), &ws)) return -1;
-    Stat* stat_part = (Stat*)ws;
-    Key* key_part = (Key*)((char*)ws + stat_bytes);
-    if (K) {
-      logp_split<T, true><<<(unsigned)parts, kThreads, 0, st>>>(x, o.tokens, o.wide, o.ignored, stat_part, key_part,
-                                                                splits, V, K);
-      TT_LAUNCH_CHECK();
-      logp_join<T, true><<<R, kThreads, 0, st>>>(x, o, stat_part, key_part, splits, V, K);
-    } else {
-      logp_split<T, false><<<(unsigned)parts, kThreads, 0, st>>>(x, o.tokens, o.wide, o.ignored, stat_part, key_part,
-                                                                 splits, V, K);
-      TT_LAUNCH_CHECK();
-      logp_join<T, false><<<R, kThreads, 0, st>>>(x, o, stat_part, key_part, splits, V, K);
-    }
+    Key* keys = (Key*)((char*)ws + stat_bytes);
+    if (K) logp_split<T, true><<<(unsigned)parts, kThreads, 0, st>>>(x, o, (float*)ws, keys, splits, V, K);
+    else logp_split<T, false><<<(unsigned)parts, kThreads, 0, st>>>(x, o, (float*)ws, keys, splits, V, K);
   } else if (packs <= kWavePacks) {
     const unsigned grid = grid_for((R + 3LL) / 4);
     if (K) logp_rows<T, kWave, true><<<grid, kThreads, 0, st>>>(x, o, R, V, K);
