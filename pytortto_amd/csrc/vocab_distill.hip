@@ -231,12 +231,16 @@ __global__ __launch_bounds__(kThreads) void distill_count(Teacher te, int* __res
 __device__ unsigned distill_done;       // blocks of a launch that are done, and splits of each row: zero between launches
 __device__ unsigned distill_tickets[kMostSplitRows];
 
+// Of a longer row than the registers hold, LDS takes this many packs more of each thread; the loop over them and what is
+// left has few registers.
+constexpr int kShelf = 8, kPair = 2;
+
 // Rows of G threads each: loss, statistics and, with GRAD, the gradient for an incoming gradient of one.  For that the
-// row is kept in registers, NV packs to a thread, and costs one read and one write; of a longer row (LONG) the rest is
-// read a second time.  For the mean's gradient the rows with a teacher are counted first: by each block, or from
+// row is kept in registers, NV packs to a thread, and costs one read and one write; of a longer row (LONG) kShelf packs
+// more go to LDS and the rest is read a second time.  For the mean's gradient the rows with a teacher are counted first: by each block, or from
 // `count_parts`.
 template <typename T, int G, int NV, bool LONG, bool GRAD>
-__global__ __launch_bounds__(G < kThreads ? kThreads : G) void distill_rows(const T* __restrict__ x, Teacher te, Out o,
+__global__ __launch_bounds__(G < kThreads ? kThreads : G, G == 512 ? 4 : 1) void distill_rows(const T* __restrict__ x, Teacher te, Out o,
                                                                            T* dx, const int* __restrict__ count_parts,
                                                                            Scale sc, int R, int V) {
   constexpr int kBlock = G < kThreads ? kThreads : G, kRows = kBlock / G;
@@ -246,7 +250,8 @@ __global__ __launch_bounds__(G < kThreads ? kThreads : G) void distill_rows(cons
   __shared__ double sums[2 * (kBlock / kWave)];
   __shared__ bool last;
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
-  const Entries e = entries_of<G>(lds, te.K, sub);
+  Words* shelf = reinterpret_cast<Words*>(lds);
+  const Entries e = entries_of<G>(lds + (LONG && GRAD ? kShelf * G * 4 : 0), te.K, sub);
   float scale = sc.temperature;
   if (GRAD && o.mean) {
     int n = 0;
@@ -271,8 +276,22 @@ __global__ __launch_bounds__(G < kThreads ? kThreads : G) void distill_rows(cons
     Share rest = all;
     rest.p0 = LONG && all.p0 + NV * G < all.p1 ? all.p0 + NV * G : all.p1;
     int best;
-    tt::scan<T, G, false, LONG>(a, best, x, r, rest, lane, sc.c);
+    tt::scan<T, G, false, LONG && !GRAD>(a, best, x, r, rest, lane, sc.c);
     if constexpr (NV > 0) add_kept<T, NV>(a, kept, sc.c);
+    if constexpr (LONG && GRAD)
+      for (int j = rest.p0 + lane, i = 0; j < rest.p1; j += kPair * G, i += kPair) {
+        Words p[kPair];
+#pragma unroll
+        for (int u = 0; u < kPair; ++u) {
+          p[u] = Words(Pack<T>::lowest);
+          if (j + u * G < rest.p1) p[u] = r.pack(j + u * G);
+        }
+        if (i < kShelf) {
+#pragma unroll
+          for (int u = 0; u < kPair; ++u) shelf[(i + u) * G + lane] = p[u];
+        }
+        tt::add_packs<T, kPair, false>(a, p, sc.c);
+      }
     a = tt::row_join<T, G, false>(a, sc.c, more[sub]);
     const float log_s = tt::log_sum(a);
     float cross = cross_entropy<T, G>(e, te.K, lane, a, log_s, sc);
@@ -293,13 +312,13 @@ __global__ __launch_bounds__(G < kThreads ? kThreads : G) void distill_rows(cons
         __builtin_amdgcn_sched_barrier(0);
       }
       if constexpr (LONG)
-        for (int j = rest.p0 + lane; j < rest.p1; j += kUnroll * G) {
-          Words p[kUnroll];
+        for (int j = rest.p0 + lane, i = 0; j < rest.p1; j += kPair * G, i += kPair) {
+          Words p[kPair];
 #pragma unroll
-          for (int u = 0; u < kUnroll; ++u)
-            if (j + u * G < rest.p1) p[u] = r.pack(j + u * G);
+          for (int u = 0; u < kPair; ++u)
+            if (j + u * G < rest.p1) p[u] = i < kShelf ? shelf[(i + u) * G + lane] : r.pack(j + u * G);
 #pragma unroll
-          for (int u = 0; u < kUnroll; ++u)
+          for (int u = 0; u < kPair; ++u)
             if (j + u * G < rest.p1)
               tt::write_pack(r, dx, j + u * G, none ? Words(0u) : gradient_pack<T, true>(p[u], a.m, log_s, sc.c, by));
         }
@@ -474,7 +493,7 @@ int launch_rows(const T* x, const Teacher& te, const Out& o, T* dx, const int* c
     distill_rows<T, 512, 16, false, true><<<grid_for(R, most), 512, entries_bytes<512>(te.K, 1), st>>>(
         x, te, o, dx, count_parts, sc, R, V);
   } else {
-    distill_rows<T, 1024, 16, true, true><<<grid_for(R, most), 1024, entries_bytes<1024>(te.K, 1), st>>>(
+    distill_rows<T, 512, 16, true, true><<<grid_for(R, most), 512, entries_bytes<512>(te.K, 1) + kShelf * 512 * 16, st>>>(
         x, te, o, dx, count_parts, sc, R, V);
   }
   TT_LAUNCH_CHECK();
