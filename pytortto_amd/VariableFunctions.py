@@ -50,7 +50,7 @@ def as_tensor(data, requires_grad=False):
     if isinstance(data, Tensor):
         return data
     array = hiparray.borrow(data)
-    out = Tensor(array, dtype=array._dtype, copy=False)
+    out = Tensor(array, dtype=array._dtype)
     if requires_grad:
         out.requires_grad = True
     return out

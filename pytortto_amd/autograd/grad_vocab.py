@@ -26,7 +26,8 @@ class LayerNorm(Function):
         xd0 = xt0.data
         shape, eps = tuple(params['normalized_shape']), params['eps']
         _device_only('layer_norm', xd0)
-        w, b = (None if t is None else t.data for t in (xt1, xt2))
+        w = None if xt1 is None else xt1.data
+        b = None if xt2 is None else xt2.data
         _same_device('layer_norm', w, b)
         if not shape or xd0.shape[-len(shape):] != shape:
             raise RuntimeError(f'Given normalized_shape={list(shape)}, expected input with shape '
@@ -39,19 +40,17 @@ class LayerNorm(Function):
                 raise RuntimeError(f'Expected {name} to be of same shape as normalized_shape, but got {name} of shape '
                                    f'{list(d.shape)} and normalized_shape = {list(shape)}')
         keep = ctx.requires_grad and is_grad_enabled()
-        yd0, mean, rstd = ops.layer_norm_fwd(xd0, w, b, width, eps, keep)
+        yd0, stats = ops.layer_norm_fwd(xd0, w, b, width, eps, keep)
         yt0 = build_links(yd0, grad_fn=ctx)
         ctx.save_for_backward(xt0, xt1)
-        ctx.params = {'mean': mean, 'rstd': rstd, 'shape': shape}
+        ctx.params = {'stats': stats, 'shape': shape}
         return yt0
 
     @staticmethod
     def backward(ctx, *grad_outputs):
         gd0, = grad_outputs
         xd0, w = ctx.saved_tensors
-        p = ctx.params
-        dx, dw, db = ops.layer_norm_bwd(xd0, gd0, w, p['mean'], p['rstd'], prod(p['shape']), ctx.needs_input_grad)
-        return dx, None if dw is None else dw.reshape(p['shape']), None if db is None else db.reshape(p['shape'])
+        return ops.layer_norm_bwd(xd0, gd0, w, ctx.params['stats'], ctx.params['shape'], ctx.needs_input_grad)
 
 
 class TokenLogProb(Function):

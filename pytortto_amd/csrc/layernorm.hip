@@ -65,49 +65,67 @@ __device__ __forceinline__ void read_parameters(float (&v)[n], const float* w, i
   for (int i = 0; i < n; ++i) v[i] = w && q * n + i < D ? w[(size_t)q * n + i] : other;
 }
 
-// Sums over the G threads of a row: a part of a wave, a wave, or a block.
-template <int G>
-__device__ __forceinline__ float group_sum(float v, float* part) {
-  if (G > kWave) return tt::row_sum<(G > kWave ? G : kWave)>(v, part);
+// Sums of N values over the threads of a row: G of a wave, or (G = 0) the whole waves of one y of the block.  part: LDS of
+// 16 N floats of this call's own.
+template <int G, int N>
+__device__ __forceinline__ void group_sum(float (&v)[N], float* part) {
 #pragma unroll
-  for (int off = (G < kWave ? G : kWave) / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
-  return v;
+  for (int off = (G ? G : kWave) / 2; off > 0; off >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], off, kWave);
+  if (G) return;
+  const int waves = blockDim.x / kWave;
+  part += threadIdx.y * waves * N;
+  if ((threadIdx.x & (kWave - 1)) == 0)
+#pragma unroll
+    for (int k = 0; k < N; ++k) part[(threadIdx.x >> 6) * N + k] = v[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = part[k];
+  for (int i = 1; i < waves; ++i)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] += part[i * N + k];
 }
 
-template <typename T, int G, int NV, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void ln_fwd(const T* __restrict__ x, const float* __restrict__ w,
-                                                const float* __restrict__ b, T* __restrict__ y,
-                                                float* __restrict__ mean, float* __restrict__ rstd, int R, int D,
-                                                float eps) {
-  constexpr int n = Loose<T>::n, kRows = BLOCK / G, kParts = G > kWave ? G / kWave : 1;
+constexpr int kMostBlock = 1024, kFwdBlock = 256, kBwdBlock = 512;    // threads: G = 0 at most, G > 0 forward, backward
+
+template <typename T, int G, int NV>
+__global__ __launch_bounds__(G ? kFwdBlock : kMostBlock) void ln_fwd(const T* __restrict__ x,
+                                                                    const float* __restrict__ w,
+                                                                    const float* __restrict__ b, T* __restrict__ y,
+                                                                    float* __restrict__ mean, float* __restrict__ rstd,
+                                                                    int R, int D, float eps) {
+  constexpr int n = Loose<T>::n, kRows = G ? kFwdBlock / (G ? G : 1) : 1;
   typedef typename Loose<T>::type P;
-  __shared__ float part[2][kParts];
-  const int lane = threadIdx.x % G, sub = threadIdx.x / G, packs = (D + n - 1) / n;
+  __shared__ float part[2][G ? 1 : kMostBlock / kWave];
+  const int stride = G ? G : (int)blockDim.x, lane = threadIdx.x % stride, sub = G ? threadIdx.x / stride : 0;
+  const int packs = (D + n - 1) / n;
   for (long long row = (long long)blockIdx.x * kRows + sub; row < R; row += (long long)gridDim.x * kRows) {
     const T* __restrict__ p = x + row * (size_t)D;
     P v[NV];
-    float s = 0.f;
+    float s[1] = {}, sq[1] = {};
 #pragma unroll
-    for (int u = 0; u < NV; ++u) v[u] = lane + u * G < packs ? read_columns(p, lane + u * G, D) : P((T)0.f);
+    for (int u = 0; u < NV; ++u) v[u] = lane + u * stride < packs ? read_columns(p, lane + u * stride, D) : P((T)0.f);
 #pragma unroll
     for (int u = 0; u < NV; ++u)
 #pragma unroll
-      for (int i = 0; i < n; ++i) s += tt::widen(v[u][i]);
-    const float m = group_sum<G>(s, part[0]) / (float)D;
-    float sq = 0.f;
+      for (int i = 0; i < n; ++i) s[0] += tt::widen(v[u][i]);
+    group_sum<G>(s, part[0]);
+    const float m = s[0] / (float)D;
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      const int left = D - (lane + u * G) * n;      // columns of the row from this pack on
+      const int left = D - (lane + u * stride) * n;     // columns of the row from this pack on
 #pragma unroll
       for (int i = 0; i < n; ++i) {
         const float d = i < left ? tt::widen(v[u][i]) - m : 0.f;
-        sq = fmaf(d, d, sq);
+        sq[0] = fmaf(d, d, sq[0]);
       }
     }
-    const float r = 1.f / sqrtf(group_sum<G>(sq, part[1]) / (float)D + eps);
+    group_sum<G>(sq, part[1]);
+    const float r = 1.f / sqrtf(sq[0] / (float)D + eps);
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      const int q = lane + u * G;
+      const int q = lane + u * stride;
       if (q >= packs) break;
       float wv[n], bv[n];
       read_parameters(wv, w, q, D, 1.f);
@@ -124,89 +142,112 @@ __global__ __launch_bounds__(BLOCK) void ln_fwd(const T* __restrict__ x, const f
   }
 }
 
-// parts: [blocks][2][D], a block's sums for dw and db, or NULL when neither is wanted.
-template <typename T, int G, int NV, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void ln_bwd(const T* __restrict__ x, const T* __restrict__ dy,
-                                                const float* __restrict__ w, const float* __restrict__ mean,
-                                                const float* __restrict__ rstd, T* __restrict__ dx,
-                                                float* __restrict__ parts, int R, int D) {
-  constexpr int n = Loose<T>::n, kRows = BLOCK / G, kParts = G > kWave ? G / kWave : 1;
+__device__ unsigned ln_done;      // blocks of a launch that have left their sums: zero between launches
+
+// parts: [blocks][2][D], a block's sums for dw and db (NULL when neither is wanted).  One block writes dw and db itself;
+// of few blocks with few columns (`joins`) the last adds them up, which saves a launch.
+template <typename T, int G, int NV>
+__global__ __launch_bounds__(G ? kBwdBlock : kMostBlock) void ln_bwd(const T* __restrict__ x, const T* __restrict__ dy,
+                                                                    const float* __restrict__ w,
+                                                                    const float* __restrict__ mean,
+                                                                    const float* __restrict__ rstd, T* __restrict__ dx,
+                                                                    float* parts, float* dw_out, float* db_out,
+                                                                    int joins, int R, int D) {
+  constexpr int n = Loose<T>::n;
   typedef typename Loose<T>::type P;
-  __shared__ float part[2][kParts];
-  const int lane = threadIdx.x % G, sub = threadIdx.x / G, packs = (D + n - 1) / n;
-  float dw[NV][n], db[NV][n];
+  __shared__ float part[2][G ? 1 : 2 * (kMostBlock / kWave)];
+  const int stride = G ? G : (int)blockDim.x, rows = G ? kBwdBlock / (G ? G : 1) : (int)blockDim.y;
+  const int lane = G ? threadIdx.x % stride : threadIdx.x, sub = G ? threadIdx.x / stride : threadIdx.y;
+  const int thread = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
+  const int all_packs = (D + n - 1) / n;
+  float sums[2][NV][n] = {};        // dw, db
+  float wv[NV][n];
 #pragma unroll
-  for (int u = 0; u < NV; ++u)
-#pragma unroll
-    for (int i = 0; i < n; ++i) dw[u][i] = db[u][i] = 0.f;
-  for (long long row = (long long)blockIdx.x * kRows + sub; row < R; row += (long long)gridDim.x * kRows) {
+  for (int u = 0; u < NV; ++u) read_parameters(wv[u], lane + u * stride < all_packs ? w : nullptr, lane + u * stride, D, 1.f);
+  int turn = 0;
+  // (all rows of a block go round together, for the barriers: one behind the last has no packs)
+  for (long long row0 = (long long)blockIdx.x * rows; row0 < R; row0 += (long long)gridDim.x * rows, turn ^= 1) {
+    const long long row = row0 + sub < R ? row0 + sub : R - 1;
+    const int packs = row0 + sub < R ? all_packs : 0;
     const size_t base = row * (size_t)D;
     P xv[NV], gv[NV];
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      const int q = lane + u * G;
+      const int q = lane + u * stride;
       xv[u] = q < packs ? read_columns(x + base, q, D) : P((T)0.f);
       gv[u] = q < packs ? read_columns(dy + base, q, D) : P((T)0.f);
     }
     const float m = mean[row], r = rstd[row];
-    float sh = 0.f, shn = 0.f;
+    float of[2] = {};                 // h, h n
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      const int q = lane + u * G;
-      if (q >= packs) break;
-      float wv[n];
-      read_parameters(wv, w, q, D, 1.f);
+      if (lane + u * stride >= packs) break;
 #pragma unroll
       for (int i = 0; i < n; ++i) {       // (behind the last column dy is 0 and adds nothing)
-        const float g = tt::widen(gv[u][i]), nn = (tt::widen(xv[u][i]) - m) * r, h = g * wv[i];
-        sh += h;
-        shn = fmaf(h, nn, shn);
-        dw[u][i] = fmaf(g, nn, dw[u][i]);
-        db[u][i] += g;
+        const float g = tt::widen(gv[u][i]), nn = (tt::widen(xv[u][i]) - m) * r, h = g * wv[u][i];
+        of[0] += h;
+        of[1] = fmaf(h, nn, of[1]);
+        sums[0][u][i] = fmaf(g, nn, sums[0][u][i]);
+        sums[1][u][i] += g;
       }
     }
     if (!dx) continue;
-    const float mh = group_sum<G>(sh, part[0]) / (float)D, mhn = group_sum<G>(shn, part[1]) / (float)D;
+    group_sum<G>(of, part[turn]);     // (in turns: one barrier to a row)
+    const float mh = of[0] / (float)D, mhn = of[1] / (float)D;
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      const int q = lane + u * G;
+      const int q = lane + u * stride;
       if (q >= packs) break;
-      float wv[n];
-      read_parameters(wv, w, q, D, 1.f);
       P o;
 #pragma unroll
       for (int i = 0; i < n; ++i) {
         const float nn = (tt::widen(xv[u][i]) - m) * r;
-        o[i] = (T)(r * (tt::widen(gv[u][i]) * wv[i] - mh - nn * mhn));
+        o[i] = (T)(r * (tt::widen(gv[u][i]) * wv[u][i] - mh - nn * mhn));
       }
       write_columns(dx + base, q, D, o);
     }
   }
-  if (!parts) return;
-  // this block's rows: one sum of dw and db for each column, pack by pack
-  __shared__ float sums[kRows > 1 ? BLOCK * n : 1];
-  float* __restrict__ out = parts + (size_t)blockIdx.x * 2 * D;
+  if (!dw_out && !db_out) return;
+  const bool alone = gridDim.x == 1;
+  float* out[2] = {alone ? dw_out : parts + (size_t)blockIdx.x * 2 * D,
+                   alone ? db_out : parts + (size_t)blockIdx.x * 2 * D + D};
+  auto leave = [&](int which, int c, float s) {
+    if (c >= D || !out[which]) return;
+    if (joins) tt::share(out[which] + c, s);
+    else out[which][c] = s;
+  };
+  // this block's rows: one sum for each column, pack by pack
+  __shared__ float all[kBwdBlock * n];     // (more threads than that are one row's)
 #pragma unroll
-  for (int u = 0; u < NV; ++u) {
+  for (int u = 0; u < 2 * NV; ++u) {
+    const int which = u & 1, first = (u >> 1) * stride;
+    if (rows == 1) {
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      if (kRows == 1) {
-        const int q = lane + u * G;
+      for (int i = 0; i < n; ++i) leave(which, (lane + first) * n + i, sums[which][u >> 1][i]);
+    } else {
+      __syncthreads();
 #pragma unroll
-        for (int i = 0; i < n; ++i)
-          if (q * n + i < D) out[which * D + q * n + i] = which ? db[u][i] : dw[u][i];
-      } else {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < n; ++i) sums[threadIdx.x * n + i] = which ? db[u][i] : dw[u][i];
-        __syncthreads();
-        for (int c = threadIdx.x; c < G * n; c += BLOCK) {
-          float s = 0.f;
-          for (int k = 0; k < kRows; ++k) s += sums[k * G * n + c];
-          if (u * G * n + c < D) out[which * D + u * G * n + c] = s;
-        }
+      for (int i = 0; i < n; ++i) all[thread * n + i] = sums[which][u >> 1][i];
+      __syncthreads();
+      for (int c = thread; c < stride * n; c += threads) {
+        float s = 0.f;
+        for (int k = 0; k < rows; ++k) s += all[k * stride * n + c];
+        leave(which, first * n + c, s);
       }
     }
+  }
+  if (!joins) return;
+  __shared__ bool last;
+  tt::stores_done();
+  __syncthreads();
+  if (thread == 0) last = tt::last_ticket(&ln_done, gridDim.x);
+  __syncthreads();
+  if (!last) return;
+  for (int c = thread; c < 2 * D; c += threads) {
+    double s = 0.0;
+    for (int k = 0; k < (int)gridDim.x; ++k) s += (double)tt::shared(parts + (size_t)k * 2 * D + c);
+    float* to = c < D ? dw_out : db_out;
+    if (to) to[c < D ? c : c - D] = (float)s;
   }
 }
 
@@ -369,9 +410,11 @@ unsigned grid_for(long long rows, int rows_per_block, long long most) {
   return (unsigned)(blocks < most ? blocks : most);
 }
 
-template <typename T, int G, int NV, int BLOCK>
+template <typename T, int G, int NV>
 int launch_fwd(const T* x, const float* w, const float* b, T* y, float* mean, float* rstd, float eps, int R, int D) {
-  ln_fwd<T, G, NV, BLOCK><<<grid_for(R, BLOCK / G, 1 << 22), BLOCK, 0, tt::stream()>>>(x, w, b, y, mean, rstd, R, D, eps);
+  const int packs = (D + Loose<T>::n - 1) / Loose<T>::n;
+  const int block = G ? kFwdBlock : (packs + NV * kWave - 1) / (NV * kWave) * kWave, rows = G ? kFwdBlock / (G ? G : 1) : 1;
+  ln_fwd<T, G, NV><<<grid_for(R, rows, 1 << 22), block, 0, tt::stream()>>>(x, w, b, y, mean, rstd, R, D, eps);
   TT_LAUNCH_CHECK();
   return 0;
 }
@@ -379,35 +422,54 @@ int launch_fwd(const T* x, const float* w, const float* b, T* y, float* mean, fl
 template <typename T>
 int forward(const T* x, const float* w, const float* b, T* y, float* mean, float* rstd, float eps, int R, int D) {
   const int packs = (D + Loose<T>::n - 1) / Loose<T>::n;
-  if (packs <= 16) return launch_fwd<T, 16, 1, 256>(x, w, b, y, mean, rstd, eps, R, D);
-  if (packs <= 32) return launch_fwd<T, 32, 1, 256>(x, w, b, y, mean, rstd, eps, R, D);
-  if (packs <= 64) return launch_fwd<T, 64, 1, 256>(x, w, b, y, mean, rstd, eps, R, D);
-  if (packs <= 128) return launch_fwd<T, 64, 2, 256>(x, w, b, y, mean, rstd, eps, R, D);
-  if (packs <= 256) return launch_fwd<T, 64, 4, 256>(x, w, b, y, mean, rstd, eps, R, D);
-  if (packs <= 512) return launch_fwd<T, 256, 2, 256>(x, w, b, y, mean, rstd, eps, R, D);
-  if (packs <= 1024) return launch_fwd<T, 256, 4, 256>(x, w, b, y, mean, rstd, eps, R, D);
-  if (packs <= 2048) return launch_fwd<T, 1024, 2, 1024>(x, w, b, y, mean, rstd, eps, R, D);
-  if (packs <= 4096) return launch_fwd<T, 1024, 4, 1024>(x, w, b, y, mean, rstd, eps, R, D);
+#define TT_LN_FWD(G, NV) return launch_fwd<T, G, NV>(x, w, b, y, mean, rstd, eps, R, D)
+  if (packs <= 4) TT_LN_FWD(4, 1);
+  if (packs <= 8) TT_LN_FWD(8, 1);
+  if (packs <= 16) TT_LN_FWD(8, 2);
+  if (packs <= 24) TT_LN_FWD(8, 3);
+  if (packs <= 32) TT_LN_FWD(16, 2);
+  if (packs <= 48) TT_LN_FWD(16, 3);
+  if (packs <= 64) TT_LN_FWD(32, 2);
+  if (packs <= 96) TT_LN_FWD(32, 3);
+  if (packs <= 128) TT_LN_FWD(64, 2);
+  if (packs <= 192) TT_LN_FWD(64, 3);
+  if (packs <= 256) TT_LN_FWD(64, 4);
+  if (packs <= 512) TT_LN_FWD(0, 2);
+  if (packs <= 768) TT_LN_FWD(0, 3);
+  if (packs <= 4096) TT_LN_FWD(0, 4);
+#undef TT_LN_FWD
   ln_fwd_long<T><<<grid_for(R, 1, 1 << 20), kLong, 0, tt::stream()>>>(x, w, b, y, mean, rstd, R, D, eps);
   TT_LAUNCH_CHECK();
   return 0;
 }
 
-template <typename T, int G, int NV, int BLOCK>
+int launch_join(const float* parts, float* dw, float* db, int D, int blocks) {
+  ln_join<<<(2 * (unsigned)D + kWave - 1) / kWave, 1024, 0, tt::stream()>>>(parts, dw, db, D, blocks);
+  TT_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename T, int G, int NV>
 int launch_bwd(const T* x, const T* dy, const float* w, const float* mean, const float* rstd, T* dx, float* dw,
                float* db, int R, int D) {
-  hipStream_t st = tt::stream();
-  const unsigned grid = grid_for(R, BLOCK / G, tt::compute_units() * (1024 / BLOCK));
+  const int packs = (D + Loose<T>::n - 1) / Loose<T>::n;
+  // a row's threads, and as many rows as fill the block, which leaves one set of sums
+  const int along = G ? kBwdBlock : (packs + NV * kWave - 1) / (NV * kWave) * kWave;
+  const int rows = G ? kBwdBlock / (G ? G : 1) : along < kBwdBlock ? kBwdBlock / along : 1;
+  const dim3 block(along, G ? 1 : rows);
+  // as many blocks as the device holds at once: more of them would only leave more sums
+  static int resident[kMostBlock / kWave + 1];
+  int& per_unit = resident[along / kWave];
+  if (per_unit == 0)
+    TT_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_unit, ln_bwd<T, G, NV>, block.x * block.y, 0));
+  const unsigned grid = grid_for(R, rows, (long long)tt::compute_units() * (per_unit > 0 ? per_unit : 1));
+  const bool sums = dw || db, joins = sums && grid > 1 && (long long)grid * D <= 16384;
   void* ws = nullptr;
-  if (dw || db)
+  if (sums && grid > 1)
     if (tt::workspace((size_t)grid * 2 * D * sizeof(float), &ws)) return -1;
-  ln_bwd<T, G, NV, BLOCK><<<grid, BLOCK, 0, st>>>(x, dy, w, mean, rstd, dx, (float*)ws, R, D);
+  ln_bwd<T, G, NV><<<grid, block, 0, tt::stream()>>>(x, dy, w, mean, rstd, dx, (float*)ws, dw, db, joins, R, D);
   TT_LAUNCH_CHECK();
-  if (dw || db) {
-    ln_join<<<(2 * D + kWave - 1) / kWave, 1024, 0, st>>>((const float*)ws, dw, db, D, grid);
-    TT_LAUNCH_CHECK();
-  }
-  return 0;
+  return sums && grid > 1 && !joins ? launch_join((const float*)ws, dw, db, D, grid) : 0;
 }
 
 template <typename T>
@@ -415,16 +477,24 @@ int backward(const T* x, const T* dy, const float* w, const float* mean, const f
              int R, int D) {
   constexpr bool wide = sizeof(T) == 4;
   const int packs = (D + Loose<T>::n - 1) / Loose<T>::n;
-  if (packs <= 16) return launch_bwd<T, 16, 1, 512>(x, dy, w, mean, rstd, dx, dw, db, R, D);
-  if (packs <= 32) return launch_bwd<T, 32, 1, 512>(x, dy, w, mean, rstd, dx, dw, db, R, D);
-  if (packs <= 64) return launch_bwd<T, 64, 1, 512>(x, dy, w, mean, rstd, dx, dw, db, R, D);
-  if (packs <= 128) return launch_bwd<T, 64, 2, 512>(x, dy, w, mean, rstd, dx, dw, db, R, D);
-  if (packs <= 256) return launch_bwd<T, 64, 4, 512>(x, dy, w, mean, rstd, dx, dw, db, R, D);
-  if (packs <= 512) return launch_bwd<T, 512, 1, 512>(x, dy, w, mean, rstd, dx, dw, db, R, D);
-  if (packs <= 1024) return launch_bwd<T, 512, 2, 512>(x, dy, w, mean, rstd, dx, dw, db, R, D);
-  if (packs <= 2048) return launch_bwd<T, 1024, 2, 1024>(x, dy, w, mean, rstd, dx, dw, db, R, D);
-  if constexpr (wide)
-    if (packs <= 4096) return launch_bwd<T, 1024, 4, 1024>(x, dy, w, mean, rstd, dx, dw, db, R, D);
+#define TT_LN_BWD(G, NV) return launch_bwd<T, G, NV>(x, dy, w, mean, rstd, dx, dw, db, R, D)
+  if (packs <= 4) TT_LN_BWD(4, 1);
+  if (packs <= 8) TT_LN_BWD(8, 1);
+  if (packs <= 16) TT_LN_BWD(16, 1);
+  if (packs <= 24) TT_LN_BWD(8, 3);
+  if (packs <= 32) TT_LN_BWD(32, 1);
+  if (packs <= 48) TT_LN_BWD(16, 3);
+  if (packs <= 64) TT_LN_BWD(64, 1);
+  if (wide && packs <= 96) TT_LN_BWD(32, 3);
+  if (wide && packs <= 128) TT_LN_BWD(64, 2);
+  if (wide && packs <= 192) TT_LN_BWD(64, 3);
+  if (packs <= 512) TT_LN_BWD(0, 1);
+  if (packs <= 2048) TT_LN_BWD(0, 2);
+  if constexpr (wide) {
+    if (packs <= 3072) TT_LN_BWD(0, 3);
+    if (packs <= 4096) TT_LN_BWD(0, 4);
+  }
+#undef TT_LN_BWD
   hipStream_t st = tt::stream();
   if (dx) {
     ln_bwd_long<T><<<grid_for(R, 1, 1 << 20), kLong, 0, st>>>(x, dy, w, mean, rstd, dx, R, D);
@@ -440,8 +510,7 @@ int backward(const T* x, const T* dy, const float* w, const float* mean, const f
     if (tt::workspace((size_t)splits * 2 * D * sizeof(float), &ws)) return -1;
     ln_parts_long<T><<<dim3(columns, splits), 256, 0, st>>>(x, dy, mean, rstd, (float*)ws, R, D, per);
     TT_LAUNCH_CHECK();
-    ln_join<<<(2 * (unsigned)D + kWave - 1) / kWave, 1024, 0, st>>>((const float*)ws, dw, db, D, splits);
-    TT_LAUNCH_CHECK();
+    return launch_join((const float*)ws, dw, db, D, splits);
   }
   return 0;
 }

@@ -680,35 +680,40 @@ def _index_bits(a, what):
 
 
 def layer_norm_fwd(x, weight, bias, width, eps, keep):
-    """(y, mean, rstd) over the trailing ``width`` values; the statistics are None unless ``keep``."""
+    """(y, stats) over the trailing ``width`` values; the statistics, every row's mean and then every row's reciprocal
+    deviation, are None unless ``keep``."""
     kind = _kind(x, 'the input of layer_norm')
     _f32(weight, bias)
     rows = x.size // width
     y = hiparray.empty(x._shape, x._dtype)
-    mean, rstd = hiparray.carve(((rows,), _F32), ((rows,), _F32)) if keep else (None, None)
+    stats = mean = rstd = None
+    if keep:
+        stats = hiparray.empty((2, rows))
+        mean = stats.ptr
+        rstd = mean + 4 * rows
     if rows:
-        _hip.call('tt_layer_norm_fwd', x.ptr, _ptr(weight), _ptr(bias), y.ptr, _ptr(mean), _ptr(rstd), eps, kind, rows,
-                  width)
-    return y, mean, rstd
+        _hip.call('tt_layer_norm_fwd', x.ptr, _ptr(weight), _ptr(bias), y.ptr, mean, rstd, eps, kind, rows, width)
+    return y, stats
 
 
-def layer_norm_bwd(x, dy, weight, mean, rstd, width, need):
+def layer_norm_bwd(x, dy, weight, stats, shape, need):
     """(dx, dweight, dbias), each None unless needed."""
-    kind = _kind(x, 'the input of layer_norm')
     if dy._dtype != x._dtype or dy._shape != x._shape:
         raise TypeError(f'the gradient of layer_norm must be like its output, {x._dtype} {x._shape}, got {dy._dtype} '
                         f'{dy._shape}')
-    rows = x.size // width
+    rows = stats._shape[1]
     dx = hiparray.empty(x._shape, x._dtype) if need[0] else None
+    dw = db = None
     if rows and need[1] and need[2]:
-        dw, db = hiparray.carve(((width,), _F32), ((width,), _F32))
+        dw, db = hiparray.carve((shape, _F32), (shape, _F32))
     else:
         make = hiparray.empty if rows else hiparray.zeros
-        dw = make((width,)) if need[1] else None
-        db = make((width,)) if need[2] else None
+        dw = make(shape) if need[1] else None
+        db = make(shape) if need[2] else None
     if rows:
-        _hip.call('tt_layer_norm_bwd', x.ptr, dy.ptr, _ptr(weight), mean.ptr, rstd.ptr, _ptr(dx), _ptr(dw), _ptr(db),
-                  kind, rows, width)
+        mean = stats.ptr
+        _hip.call('tt_layer_norm_bwd', x.ptr, dy.ptr, _ptr(weight), mean, mean + 4 * rows, _ptr(dx), _ptr(dw), _ptr(db),
+                  _TYPES[x._dtype], rows, prod(shape))
     return dx, dw, db
 
 

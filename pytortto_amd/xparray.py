@@ -268,7 +268,9 @@ class hiparray:
         front of the library's stream, before the array is used; and memory is borrowed once, not as two arrays."""
         about = source.__cuda_array_interface__
         shape, kind = tuple(about['shape']), about['typestr']
-        dtype = _DTYPES.get(kind) or _DTYPES.setdefault(kind, np.dtype(kind))
+        dtype = _DTYPES.get(kind)
+        if dtype is None:
+            dtype = _DTYPES[kind] = np.dtype(kind)
         nbytes = prod(shape) * dtype.itemsize
         if about.get('mask') is not None:
             raise ValueError('borrowed device memory cannot be masked')
@@ -279,7 +281,7 @@ class hiparray:
                 if n != 1 and step != whole:
                     raise ValueError(f'device arrays are C-contiguous, got strides {tuple(strides)} for shape {shape}')
                 whole *= n
-        return cls.on(_Borrowed(about['data'][0] or 0, nbytes, source) if nbytes else _Buffer(0), shape, dtype)
+        return cls.on(_Borrowed(about['data'][0] or 0, nbytes, source), shape, dtype)
 
     # ---- ndarray-like attributes ----------------------------------------------------------
     @property
