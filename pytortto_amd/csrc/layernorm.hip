@@ -217,7 +217,7 @@ __global__ __launch_bounds__(G ? kBwdBlock : kMostBlock) void ln_bwd(const T* __
     else out[which][c] = s;
   };
   // this block's rows: one sum for each column, pack by pack
-  __shared__ float all[kBwdBlock * n];     // (more threads than that are one row's)
+  __shared__ float all[(G || sizeof(T) == 4 ? kBwdBlock : kMostBlock) * n];    // (as many threads as have several rows)
 #pragma unroll
   for (int u = 0; u < 2 * NV; ++u) {
     const int which = u & 1, first = (u >> 1) * stride;
@@ -453,9 +453,12 @@ template <typename T, int G, int NV>
 int launch_bwd(const T* x, const T* dy, const float* w, const float* mean, const float* rstd, T* dx, float* dw,
                float* db, int R, int D) {
   const int packs = (D + Loose<T>::n - 1) / Loose<T>::n;
-  // a row's threads, and as many rows as fill the block, which leaves one set of sums
+  // a row's threads, and as many rows as fill the block, which leaves one set of sums.  (Long rows of halves, whose sums
+  // weigh as much as a dozen of them: blocks of 1024 threads, 8192 columns 65 -> 55 us at 2^25 values; of float32, or
+  // short ones, 512: 1024 columns of halves 46 us, 53 with 1024 threads)
   const int along = G ? kBwdBlock : (packs + NV * kWave - 1) / (NV * kWave) * kWave;
-  const int rows = G ? kBwdBlock / (G ? G : 1) : along < kBwdBlock ? kBwdBlock / along : 1;
+  const int fill = sizeof(T) == 2 && along > 256 ? kMostBlock : kBwdBlock;
+  const int rows = G ? kBwdBlock / (G ? G : 1) : along < fill ? fill / along : 1;
   const dim3 block(along, G ? 1 : rows);
   // as many blocks as the device holds at once: more of them would only leave more sums
   static int resident[kMostBlock / kWave + 1];
@@ -488,8 +491,8 @@ int backward(const T* x, const T* dy, const float* w, const float* mean, const f
   if (wide && packs <= 96) TT_LN_BWD(32, 3);
   if (wide && packs <= 128) TT_LN_BWD(64, 2);
   if (wide && packs <= 192) TT_LN_BWD(64, 3);
-  if (packs <= 512) TT_LN_BWD(0, 1);
-  if (packs <= 2048) TT_LN_BWD(0, 2);
+  if (packs <= 256) TT_LN_BWD(0, 1);
+  if (packs <= (wide ? 512 : 2048)) TT_LN_BWD(0, 2);
   if constexpr (wide) {
     if (packs <= 3072) TT_LN_BWD(0, 3);
     if (packs <= 4096) TT_LN_BWD(0, 4);
