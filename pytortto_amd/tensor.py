@@ -208,7 +208,7 @@ class Tensor:
                 one = np.ones((1,) * self.data.ndim, dtype=self.data.dtype)
                 gradient = hiparray(one) if on_device else one
         elif isinstance(gradient, Tensor):
-            if gradient.device != self.device:
+            if (gradient.data.__class__ is hiparray) is not on_device:
                 raise RuntimeError(f'invalid gradient at index 0 - expected device {self.device} '
                                    f'but got {gradient.device}')
             # not copied up front: the nodes read it, and whoever keeps or writes it makes a copy (256 channels of

@@ -57,6 +57,7 @@ class Device:
 
 
 _F32 = np.dtype(np.float32)
+_void_p, _byref = ctypes.c_void_p, ctypes.byref
 _DTYPES = {}            # of array interfaces' type strings
 
 
@@ -76,8 +77,8 @@ class _Buffer:
             self._allocate()
 
     def _allocate(self):
-        p = ctypes.c_void_p()
-        _hip.call('tt_malloc', ctypes.byref(p), self.nbytes)
+        p = _void_p()
+        _hip.call('tt_malloc', _byref(p), self.nbytes)
         self._ptr = p.value or 0
 
     def fill_on_demand(self, fill, operands):
@@ -114,7 +115,7 @@ class _Buffer:
     def __del__(self):
         try:
             if self._ptr:
-                _hip.load_library().tt_free(ctypes.c_void_p(self._ptr))
+                _hip._lib.tt_free(self._ptr)
                 self._ptr = 0
         except Exception:   # interpreter shutdown
             pass
@@ -242,13 +243,16 @@ class hiparray:
     @classmethod
     def carve(cls, *wanted):
         """Arrays of the (shape, dtype) wanted on one block: what one operation returns together, for one allocation."""
-        dtypes = [_F32 if t is np.float32 else np.dtype(t) for _, t in wanted]
-        sizes = [prod(shape) * dtype.itemsize for (shape, _), dtype in zip(wanted, dtypes)]
-        block, at, out = _Buffer(sum(sizes) + 256 * len(sizes)), 0, []
-        for (shape, _), dtype, size in zip(wanted, dtypes, sizes):
-            out.append(cls.on(_Borrowed(block._ptr + at, size, block), shape, dtype))
+        ends, at = [], 0
+        for shape, dtype in wanted:
+            if dtype.__class__ is type:
+                dtype = np.dtype(dtype)
+            size = prod(shape) * dtype.itemsize
+            ends.append((shape, dtype, size, at))
             at += (size + 255) & -256
-        return out
+        block = _Buffer(at)
+        first = block._ptr
+        return [cls.on(_Borrowed(first + start, size, block), shape, dtype) for shape, dtype, size, start in ends]
 
     @classmethod
     def zeros(cls, shape, dtype=np.float32):
