@@ -142,7 +142,7 @@ __global__ __launch_bounds__(G ? kFwdBlock : kMostBlock) void ln_fwd(const T* __
   }
 }
 
-__device__ unsigned ln_done;      // blocks of a launch that have left their sums: zero between launches
+__device__ tt::Ticket ln_done;     // blocks of a launch that have left their sums: zero between launches
 
 // parts: [blocks][2][D], a block's sums for dw and db (NULL when neither is wanted).  One block writes dw and db itself;
 // of few blocks with few columns (`joins`) the last adds them up, which saves a launch.

@@ -2,7 +2,6 @@
 // log probabilities and distillation (vocab.hip).  Values are widened to float32 as they are read; sums and
 // statistics are float32 or wider, and a result is rounded once, to its own type, as it is stored.
 //
-// G threads work on a row: a wave (G = 64, several rows to a block, no block barrier) or a block.
 #pragma once
 #include "tt_common.h"
 
@@ -56,10 +55,10 @@ __device__ __forceinline__ Words pack(const float* z) {
   return __builtin_bit_cast(Words, v);
 }
 
-// Whether the threads of a row are a wave of a larger block or the block itself.
+// G threads work on a row: a part of a wave, a wave, or a block of G threads.
 template <int G>
 __device__ __forceinline__ void sync_row() {
-  if (G == kWave) {
+  if (G <= kWave) {
     // LDS operations of one wave run in order: only the compiler has to keep them so
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -68,45 +67,72 @@ __device__ __forceinline__ void sync_row() {
   }
 }
 
-// Waits until this wave's stores have left for memory: what another wave of the block stores to the same place after
-// the next sync_row comes later.
+// Waits until this wave's stores have left for memory.
 __device__ __forceinline__ void stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-template <typename V>
-__device__ __forceinline__ V wave_sum(V v) {
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
-  return v;
+struct Plus {
+  template <typename V>
+  __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
+};
+struct Larger {
+  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+
+// The value of another lane of the sixteen, by a cross-lane move of the vector unit (a tenth of the time that one through
+// LDS takes): 0xB1 and 0x4E exchange neighbours and pairs, 0x141 and 0x140 mirror eight and sixteen lanes.
+template <int CTRL, typename V>
+__device__ __forceinline__ V across(V v) {
+  static_assert(sizeof(V) == 4 || sizeof(V) == 8, "words");
+  if constexpr (sizeof(V) == 4) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+  } else {
+    const int2 w = __builtin_bit_cast(int2, v);
+    return __builtin_bit_cast(V, make_int2(__builtin_amdgcn_mov_dpp(w.x, CTRL, 0xf, 0xf, true),
+                                           __builtin_amdgcn_mov_dpp(w.y, CTRL, 0xf, 0xf, true)));
+  }
 }
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, kWave));
+template <typename V>
+__device__ __forceinline__ V lane_value(V v, int lane) {
+  if constexpr (sizeof(V) == 4) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+  } else {
+    const int2 w = __builtin_bit_cast(int2, v);
+    return __builtin_bit_cast(V, make_int2(__builtin_amdgcn_readlane(w.x, lane), __builtin_amdgcn_readlane(w.y, lane)));
+  }
+}
+
+// v of G lanes of a wave together (G a power of two to 64), in an order that is the same for all of them.
+template <int G, typename V, typename Op>
+__device__ __forceinline__ V lanes_reduce(V v, Op op) {
+  if (G >= 2) v = op(v, across<0xB1>(v));
+  if (G >= 4) v = op(v, across<0x4E>(v));
+  if (G >= 8) v = op(v, across<0x141>(v));
+  if (G >= 16) v = op(v, across<0x140>(v));
+  if (G == 32) v = op(v, __shfl_xor(v, 16, kWave));
+  if (G == 64) v = op(op(lane_value(v, 0), lane_value(v, 16)), op(lane_value(v, 32), lane_value(v, 48)));
   return v;
 }
 
-// Sum over the G threads of a row; every thread gets it.  `part` is LDS of G / 64 values of this row's own; it is
+// The same over the G threads of a row.  `part` is LDS of G / 64 values of this row's own (none for G <= 64); it is
 // written before and read after one barrier, so two calls in a row need different ones.
-template <int G, typename V>
-__device__ __forceinline__ V row_sum(V v, V* part) {
-  v = wave_sum(v);
-  if (G == kWave) return v;
+template <int G, typename V, typename Op>
+__device__ __forceinline__ V row_reduce(V v, V* part, Op op) {
+  v = lanes_reduce<(G < kWave ? G : kWave)>(v, op);
+  if (G <= kWave) return v;
   if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x >> 6] = v;
   __syncthreads();
   V s = part[0];
 #pragma unroll
-  for (int i = 1; i < G / kWave; ++i) s += part[i];
+  for (int i = 1; i < G / kWave; ++i) s = op(s, part[i]);
   return s;
+}
+template <int G, typename V>
+__device__ __forceinline__ V row_sum(V v, V* part) {
+  return row_reduce<G>(v, part, Plus());
 }
 template <int G>
 __device__ __forceinline__ float row_max(float v, float* part) {
-  v = wave_max(v);
-  if (G == kWave) return v;
-  if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float s = part[0];
-#pragma unroll
-  for (int i = 1; i < G / kWave; ++i) s = fmaxf(s, part[i]);
-  return s;
+  return row_reduce<G>(v, part, Larger());
 }
 
 // What blocks of one launch leave for the block that comes last.  The stores and loads are device-wide ones, which go
@@ -119,13 +145,25 @@ template <typename V>
 __device__ __forceinline__ V shared(const V* p) {
   return __hip_atomic_load(const_cast<V*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+// A counter of blocks that are done, zero between launches.  Blocks that count at one address wait for each other, some
+// 9 ns each (4096 of them 38 us), so counters stand in lines of their own, and blocks of one large launch count in two
+// steps, in kBranches groups and then the groups (3 us).
+struct alignas(128) Ticket {
+  unsigned n;
+};
+constexpr unsigned kBranches = 32;
 // True for the last of `all` callers, for whom everything the others shared is there; the counter is zero again then.
 // One thread of a block calls it, after what the block shares.
-__device__ __forceinline__ bool last_ticket(unsigned* counter, unsigned all) {
+__device__ __forceinline__ bool last_ticket(Ticket* t, unsigned all) {
   asm volatile("" ::: "memory");
-  const bool last = atomicInc(counter, all - 1) == all - 1;
+  const bool last = atomicInc(&t->n, all - 1) == all - 1;
   asm volatile("" ::: "memory");
   return last;
+}
+// The same for caller number `at`, with 1 + kBranches counters.
+__device__ __forceinline__ bool last_ticket(Ticket* t, unsigned at, unsigned all) {
+  const unsigned groups = all < kBranches ? all : kBranches, group = at % groups;
+  return last_ticket(t + 1 + group, all / groups + (group < all % groups ? 1 : 0)) && last_ticket(t, groups);
 }
 
 // An index array of 64 or 32 bits, and a value array of float16 or float32.

@@ -134,45 +134,51 @@ __device__ __forceinline__ bool add_value(Stat& a, float value, float c) {
 
 constexpr int kUnroll = 4;      // packs that a thread has on their way at once in the streaming loops
 
-// A thread's share of a row: thread `lane` of G takes packs p0 + lane + i G, one column of the head in front of them and
-// one of the tail behind them, so that it sees its columns in ascending order.  `best` is told what holds the first
-// of its largest values: a group of kUnroll packs by its first one, kHead or kTail.
-constexpr int kNothing = -1, kHead = -2, kTail = -3;
+// The columns outside the whole packs, of which thread `lane` of G takes lane, lane + G, ...
+template <typename T>
+__device__ __forceinline__ int loose_column(const LogitRow<T>& r, const Share& h, int i) {
+  return i < h.head ? i : r.tail_at + i - h.head;
+}
 
-// (PACKS = false: the head and the tail only.)
+// A thread's share of a row: packs p0 + lane + i G in ascending order, then its loose columns (PACKS = false: these only).
+// `best` is told the first pack of those, kUnroll at most and G apart, that hold the first of the packs' largest values;
+// kNothing: none is above -inf.
+constexpr int kNothing = -1;
+
 template <typename T, int G, bool ENTROPY, bool PACKS = true>
 __device__ __forceinline__ void scan(Stat& a, int& best, const T* x, const LogitRow<T>& r, const Share& h, int lane,
                                      float c) {
-  if (lane < h.head) {
-    add_value<T, ENTROPY>(a, widen(x[r.start + lane]), c);
-    best = kHead;
-  }
-  for (int j = h.p0 + lane; PACKS && j < h.p1; j += kUnroll * G) {
+  for (int j0 = h.p0; PACKS && j0 < h.p1; j0 += kUnroll * G) {
+    const int j = j0 + lane;
     Words p[kUnroll];
-    if (j + (kUnroll - 1) * G < h.p1) {
+    if (j0 + kUnroll * G <= h.p1) {
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) p[u] = r.pack(j + u * G);
+      if (add_packs<T, kUnroll, ENTROPY>(a, p, c)) best = j;
     } else {
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
         p[u] = Words(Pack<T>::lowest);
         if (j + u * G < h.p1) p[u] = r.pack(j + u * G);
       }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (j0 + u * G < h.p1 && add_packs<T, 1, ENTROPY>(a, p + u, c)) best = j + u * G;
     }
-    if (add_packs<T, kUnroll, ENTROPY>(a, p, c) || best == kNothing) best = j;
   }
-  if (lane < h.tail && (add_value<T, ENTROPY>(a, widen(x[r.start + r.tail_at + lane]), c) || best == kNothing))
-    best = kTail;
+  for (int i = lane; i < h.head + h.tail; i += G)
+    add_value<T, ENTROPY>(a, widen(x[r.start + loose_column(r, h, i)]), c);
 }
 
 // The statistics of all G threads of a row: first the maximum, then each thread's sums moved to it and added up.
-// part: LDS of 3 * G / 64 floats.
+// part: LDS of 3 G / 64 floats.
 template <typename T, int G, bool ENTROPY>
 __device__ __forceinline__ Stat row_join(Stat a, float c, float* part) {
+  constexpr int kParts = G > kWave ? G / kWave : 0;
   const float m = row_max<G>(a.m, part);
   rescale<T, ENTROPY>(a, m, c);
-  a.s = row_sum<G>(a.s, part + G / kWave);
-  if (ENTROPY) a.t = row_sum<G>(a.t, part + 2 * (G / kWave));
+  a.s = row_sum<G>(a.s, part + kParts);
+  if (ENTROPY) a.t = row_sum<G>(a.t, part + 2 * kParts);
   return a;
 }
 
@@ -187,6 +193,9 @@ template <typename T>
 __device__ __forceinline__ float log_p(float z, float m, float log_s, const Scale& sc) {
   return (sizeof(T) == 2 ? bits<T>(z, m, sc.c) * kLn2 : (z - m) * sc.inverse) - log_s * kLn2;
 }
+
+// LDS floats of `sums` sums over a row.
+constexpr int parts_of(int G, int sums) { return G > kWave ? sums * (G / kWave) : 1; }
 
 // log2 of the sum, 0 for an empty row; a NaN stays.
 __device__ __forceinline__ float log_sum(const Stat& a) { return a.s > 0.f ? log2f(a.s) : a.s; }

@@ -16,7 +16,7 @@ using tt::Words;
 
 constexpr int kThreads = 256;
 constexpr int kMostTeacher = 1024;
-constexpr int kMostSplitRows = 8192;    // fewer rows than this may be shared by blocks
+constexpr int kMostSplitRows = 2048;    // rows that may be shared by blocks
 
 struct Teacher {
   const void* logits;
@@ -40,16 +40,18 @@ struct Entries {
   int* next;
   int* queue;
 };
-constexpr int kEntryBytes = 16;
+// K rounded up, so that places can be read sixteen bytes at a time.
+__host__ __device__ __forceinline__ int whole(int K) { return (K + 3) / 4 * 4; }
 
 template <int G>
 __device__ __forceinline__ Entries entries_of(float* lds, int K, int sub) {
-  float* at = lds + (size_t)sub * (4 * K + G);
-  return {at, (int*)(at + K), at + 2 * K, (int*)(at + 3 * K), (int*)(at + 4 * K)};
+  const int n = whole(K);
+  float* at = lds + (size_t)sub * (4 * n + G);
+  return {at, (int*)(at + n), at + 2 * n, (int*)(at + 3 * n), (int*)(at + 4 * n)};
 }
 template <int G>
 size_t entries_bytes(int K, int rows) {
-  return ((size_t)K * kEntryBytes + G * sizeof(int)) * rows;
+  return ((size_t)whole(K) * 4 + G) * sizeof(float) * rows;
 }
 
 struct TeacherSum {
@@ -62,6 +64,7 @@ __device__ __forceinline__ TeacherSum read_teacher(const Teacher& te, const T* x
                                                    float c, int lane, const Entries& e, float* part) {
   Stat a = {-INFINITY, 0.f, 0.f};
   e.queue[lane] = -1;
+  if (lane < whole(te.K) - te.K) e.place[te.K + lane] = -1;
   for (int k = lane; k < te.K; k += G) {
     int i;
     const float z = teacher_entry(te, row * te.K + k, r.V, &i);
@@ -101,16 +104,24 @@ __device__ __forceinline__ void queue_entries(const Entries& e, const LogitRow<T
     int owner;
     if (j < r.head) {
       if (s.head == 0) continue;
-      owner = j;
+      owner = j % G;
     } else if (j >= r.tail_at) {
       if (s.tail == 0) continue;
-      owner = s.head + j - r.tail_at;
+      owner = (s.head + j - r.tail_at) % G;
     } else {
       if (pack < s.p0 || pack >= s.p1) continue;
       owner = (pack - s.p0) % G;
     }
-    float q = 0.f;
-    for (int i = 0; i < K; ++i) q += e.place[i] == j ? e.weight[i] : 0.f;
+    int same = 0;
+    for (int i = 0; i < K; i += 4) {
+      const int4 p = *reinterpret_cast<const int4*>(e.place + i);
+      same += (p.x == j) + (p.y == j) + (p.z == j) + (p.w == j);
+    }
+    float q = e.weight[k];
+    if (same > 1) {
+      q = 0.f;
+      for (int i = 0; i < K; ++i) q += e.place[i] == j ? e.weight[i] : 0.f;
+    }
     e.logit[k] = scale * (tt::pow2(tt::bits<T>(e.logit[k], m, c) - log_s) - q);
     e.next[k] = atomicExch(&e.queue[owner], k);
   }
@@ -122,38 +133,52 @@ __device__ __forceinline__ void store_queued(const Entries& e, T* dx, const Logi
   for (int k = e.queue[lane]; k >= 0; k = e.next[k]) dx[r.start + e.place[k]] = (T)e.logit[k];
 }
 
-// What the rows leave behind, and what the last of them makes of it.
+// What the rows leave behind, and what the last block makes of it.
 struct Out {
-  float* loss;        // of each row
-  float* counted;     // 1 of a row with a teacher, else 0
+  float* loss;        // of each row, where that is wanted
   float2* stats;      // for the backward pass
+  double* sums;       // of each block's rows: their losses, and how many have a teacher
   float* total;       // the rows' sum, or over the count for the mean; NULL: not wanted
   float* count;       // how many rows have a teacher
   int mean;
 };
 
 // A row without a teacher has m = -inf for the backward pass, as one without any possible class: no gradient.
-__device__ __forceinline__ void write_row(const Out& o, size_t row, const Stat& a, float log_s, const TeacherSum& te,
-                                          float cross, const Scale& sc) {
+__device__ __forceinline__ double write_row(const Out& o, size_t row, const Stat& a, float log_s, const TeacherSum& te,
+                                            float cross, const Scale& sc) {
   const bool none = te.s == 0.f;
-  tt::share(o.loss + row, none ? 0.f : fmaf(te.q_log_q, tt::kLn2, cross) * (sc.temperature * sc.temperature));
-  tt::share(o.counted + row, none ? 0.f : 1.f);
+  const float loss = none ? 0.f : fmaf(te.q_log_q, tt::kLn2, cross) * (sc.temperature * sc.temperature);
+  if (o.loss) o.loss[row] = loss;
   o.stats[row] = make_float2(none ? -INFINITY : a.m, te.s == te.s ? log_s : te.s);
+  return loss;
 }
 
-// The rows' losses added up by one block, in 64 bits and in an order that the sizes alone decide.
+// The block's number `at` of `all` is done with its rows.  The one that comes last adds up what they all leave, in 64
+// bits and in an order that the sizes alone decide.  `part` is LDS of 2 BLOCK / 64 values.
 template <int BLOCK>
-__device__ __forceinline__ void add_rows(const Out& o, int R, double* part) {
-  double s = 0.0, n = 0.0;
-  for (int r = threadIdx.x; r < R; r += BLOCK) {
-    s += (double)tt::shared(o.loss + r);
-    n += (double)tt::shared(o.counted + r);
-  }
-  s = tt::row_sum<BLOCK>(s, part);
-  n = tt::row_sum<BLOCK>(n, part + BLOCK / kWave);
+__device__ __forceinline__ void add_up(const Out& o, tt::Ticket* done, unsigned at, unsigned all, double loss, double rows,
+                                       double* part) {
+  __shared__ bool last;
+  loss = tt::row_sum<BLOCK>(loss, part);
+  rows = tt::row_sum<BLOCK>(rows, part + BLOCK / kWave);
   if (threadIdx.x == 0) {
-    if (o.total) o.total[0] = (float)(o.mean ? s / n : s);
-    o.count[0] = (float)n;
+    tt::share(o.sums + 2 * (size_t)at, loss);
+    tt::share(o.sums + 2 * (size_t)at + 1, rows);
+    tt::stores_done();
+    last = tt::last_ticket(done, at, all);
+  }
+  __syncthreads();
+  if (!last) return;
+  loss = rows = 0.0;
+  for (unsigned i = threadIdx.x; i < all; i += BLOCK) {
+    loss += tt::shared(o.sums + 2 * (size_t)i);
+    rows += tt::shared(o.sums + 2 * (size_t)i + 1);
+  }
+  loss = tt::row_sum<BLOCK>(loss, part);
+  rows = tt::row_sum<BLOCK>(rows, part + BLOCK / kWave);
+  if (threadIdx.x == 0) {
+    if (o.total) o.total[0] = (float)(o.mean ? loss / rows : loss);
+    o.count[0] = (float)rows;
   }
 }
 
@@ -169,10 +194,10 @@ __device__ __forceinline__ Words gradient_pack(const Words& p, float m, float lo
   return tt::pack<T>(z);
 }
 
-// The values of NV packs: their maximum first, then their sum, so that there is no chain of rescaled sums.  The packs are
+// The values of NV packs, or the first `packs` of them: their maximum first, then their sum, so that there is no chain of rescaled sums.  The packs are
 // opaque to the compiler in between, which would otherwise hold all their widened values from one loop to the other.
 template <typename T, int NV>
-__device__ __forceinline__ void add_kept(Stat& a, Words (&kept)[NV], float c) {
+__device__ __forceinline__ void add_kept(Stat& a, Words (&kept)[NV], int packs, float c) {
   constexpr int n = Pack<T>::n;
   const float most = tt::pack_max<T, NV>(kept);
   if (most > a.m) tt::rescale<T, false>(a, most, c);
@@ -181,6 +206,7 @@ __device__ __forceinline__ void add_kept(Stat& a, Words (&kept)[NV], float c) {
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
     asm volatile("" : "+v"(kept[u]));
+    if (u >= packs) continue;
     float z[n];
     tt::unpack<T>(z, kept[u]);
 #pragma unroll
@@ -190,11 +216,11 @@ __device__ __forceinline__ void add_kept(Stat& a, Words (&kept)[NV], float c) {
   a.s += (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-template <typename T>
+template <typename T, int G>
 __device__ __forceinline__ void write_loose(const T* x, T* dx, const LogitRow<T>& r, const Share& s, int lane,
                                             bool none, float m, float log_s, float c, float scale) {
-  if (lane < s.head + s.tail) {
-    const size_t at = r.start + (lane < s.head ? lane : r.tail_at + lane - s.head);
+  for (int i = lane; i < s.head + s.tail; i += G) {
+    const size_t at = r.start + tt::loose_column(r, s, i);
     dx[at] = none ? (T)0.f : (T)(scale * tt::pow2(tt::bits<T>(tt::widen(x[at]), m, c) - log_s));
   }
 }
@@ -228,8 +254,7 @@ __global__ __launch_bounds__(kThreads) void distill_count(Teacher te, int* __res
   if (threadIdx.x == 0) parts[blockIdx.x] = n;
 }
 
-__device__ unsigned distill_done;       // blocks of a launch that are done, and splits of each row: zero between launches
-__device__ unsigned distill_tickets[kMostSplitRows];
+__device__ tt::Ticket distill_done[1 + tt::kBranches], distill_tickets[kMostSplitRows];
 
 // Of a longer row than the registers hold, LDS takes this many packs more of each thread; the loop over them and what is
 // left has few registers.
@@ -245,13 +270,13 @@ __global__ __launch_bounds__(G < kThreads ? kThreads : G, G == 512 ? 4 : 1) void
                                                                            Scale sc, int R, int V) {
   constexpr int kBlock = G < kThreads ? kThreads : G, kRows = kBlock / G;
   extern __shared__ float lds[];
-  __shared__ float part[kRows][3 * (G / kWave)];
-  __shared__ float more[kRows][4 * (G / kWave)];
+  __shared__ float part[kRows][tt::parts_of(G, 3)];
+  __shared__ float more[kRows][tt::parts_of(G, 4)];
   __shared__ double sums[2 * (kBlock / kWave)];
-  __shared__ bool last;
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
   Words* shelf = reinterpret_cast<Words*>(lds);
   const Entries e = entries_of<G>(lds + (LONG && GRAD ? kShelf * G * 4 : 0), te.K, sub);
+  double losses = 0.0, rows = 0.0;
   float scale = sc.temperature;
   if (GRAD && o.mean) {
     int n = 0;
@@ -277,7 +302,7 @@ __global__ __launch_bounds__(G < kThreads ? kThreads : G, G == 512 ? 4 : 1) void
     rest.p0 = LONG && all.p0 + NV * G < all.p1 ? all.p0 + NV * G : all.p1;
     int best;
     tt::scan<T, G, false, LONG && !GRAD>(a, best, x, r, rest, lane, sc.c);
-    if constexpr (NV > 0) add_kept<T, NV>(a, kept, sc.c);
+    if constexpr (NV > 0) add_kept<T, NV>(a, kept, G > kWave ? NV : (all.p1 - all.p0 + G - 1) / G, sc.c);
     if constexpr (LONG && GRAD)
       for (int j = rest.p0 + lane, i = 0; j < rest.p1; j += kPair * G, i += kPair) {
         Words p[kPair];
@@ -322,18 +347,18 @@ __global__ __launch_bounds__(G < kThreads ? kThreads : G, G == 512 ? 4 : 1) void
             if (j + u * G < rest.p1)
               tt::write_pack(r, dx, j + u * G, none ? Words(0u) : gradient_pack<T, true>(p[u], a.m, log_s, sc.c, by));
         }
-      write_loose(x, dx, r, all, lane, none, a.m, log_s, sc.c, by);
+      write_loose<T, G>(x, dx, r, all, lane, none, a.m, log_s, sc.c, by);
       store_queued(e, dx, r, lane);
     }
-    cross = tt::row_sum<G>(cross, more[sub] + 3 * (G / kWave));
-    if (lane == 0) write_row(o, row, a, log_s, ts, cross, sc);
+    cross = tt::row_sum<G>(cross, more[sub] + tt::parts_of(G, 3) % tt::parts_of(G, 4));
+    if (lane == 0) {
+      losses += write_row(o, row, a, log_s, ts, cross, sc);
+      rows += ts.s == 0.f ? 0.0 : 1.0;
+    }
     tt::sync_row<G>();
   }
-  tt::stores_done();
   __syncthreads();
-  if (threadIdx.x == 0) last = tt::last_ticket(&distill_done, gridDim.x);
-  __syncthreads();
-  if (last) add_rows<kBlock>(o, R, sums);
+  add_up<kBlock>(o, distill_done, blockIdx.x, gridDim.x, losses, rows, sums);
 }
 
 // Few long rows: `splits` blocks to a row, each with the sums of its share; the one that comes last puts them together,
@@ -359,7 +384,7 @@ __global__ __launch_bounds__(kThreads) void distill_split(const T* __restrict__ 
     tt::share(stat_part + (size_t)blockIdx.x * 2, a.m);
     tt::share(stat_part + (size_t)blockIdx.x * 2 + 1, a.s);
     tt::stores_done();
-    last = tt::last_ticket(&distill_tickets[row], splits);
+    last = tt::last_ticket(distill_tickets + row, splits);
   }
   __syncthreads();
   if (!last) return;
@@ -372,13 +397,8 @@ __global__ __launch_bounds__(kThreads) void distill_split(const T* __restrict__ 
   whole = tt::row_join<T, G, false>(whole, sc.c, more);
   const float log_s = tt::log_sum(whole);
   const float cross = tt::row_sum<G>(cross_entropy<T, G>(e, te.K, lane, whole, log_s, sc), more + 3 * (G / kWave));
-  if (lane == 0) {
-    write_row(o, row, whole, log_s, ts, cross, sc);
-    tt::stores_done();
-    last = tt::last_ticket(&distill_done, R);
-  }
-  __syncthreads();
-  if (last) add_rows<G>(o, R, sums);
+  const double loss = lane == 0 ? write_row(o, row, whole, log_s, ts, cross, sc) : 0.0;
+  add_up<G>(o, distill_done, row, R, loss, lane == 0 && ts.s != 0.f ? 1.0 : 0.0, sums);
 }
 
 // The gradient from the kept statistics.  With `ahead` the forward pass has written it for an incoming gradient of one
@@ -392,7 +412,7 @@ __global__ __launch_bounds__(kThreads) void distill_bwd(const T* __restrict__ x,
   constexpr int kRows = kThreads / G;
   if (ahead && g[0] == 1.f) return;
   extern __shared__ float lds[];
-  __shared__ float part[kRows][3 * (G / kWave)];
+  __shared__ float part[kRows][tt::parts_of(G, 3)];
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
   const Entries e = entries_of<G>(lds, te.K, sub);
   const long long items = (long long)R * splits;
@@ -420,7 +440,7 @@ __global__ __launch_bounds__(kThreads) void distill_bwd(const T* __restrict__ x,
         if (j + u * G < s.p1)
           tt::write_pack(r, dx, j + u * G, none ? Words(0u) : gradient_pack<T, false>(p[u], st.x, st.y, sc.c, scale));
     }
-    write_loose(x, dx, r, s, lane, none, st.x, st.y, sc.c, scale);
+    write_loose<T, G>(x, dx, r, s, lane, none, st.x, st.y, sc.c, scale);
     store_queued(e, dx, r, lane);
     tt::sync_row<G>();
   }
@@ -442,12 +462,16 @@ int check(const char* fn, int dtype, int teacher_dtype, int index_bits, double t
   return 0;
 }
 
+constexpr long long kMostBlocks = 16;      // of a launch, to a compute unit; they take rows in turn
 unsigned grid_for(long long blocks, long long most) { return (unsigned)(blocks < most ? blocks : most); }
 
-// Rows of up to this many packs go to a wave each, which keeps them in registers; four of them share a block's LDS, where
-// the teacher's entries have to fit.
-constexpr int kWavePacks = 8 * kWave, kWaveEntries = 256;
+// Rows of up to kWavePacks packs go to a wave each, which keeps them in registers; four of them share a block's LDS, where
+// the teacher's entries have to fit.  (22369 rows of 3000 in float32 with their gradient: 124 us, by blocks 190 us.)
+// Short ones go to kLanes lanes each: 131072 rows of 100 with 32 entries take 83 us, by waves 310 us.
+constexpr int kWavePacks = 16 * kWave, kWaveEntries = 256;
 bool by_waves(int packs, int K) { return packs <= kWavePacks && K <= kWaveEntries; }
+constexpr int kLanes = 16, kLanesPacks = 8 * kLanes, kLanesEntries = 64;
+bool by_lanes(int packs, int K) { return packs <= kLanesPacks && K <= kLanesEntries; }
 
 int packs_for(int V, int dtype) { return dtype == TT_F32 ? (V + 3) / 4 : (V + 7) / 8; }
 
@@ -461,7 +485,9 @@ int splits_for(long long R, int packs) {
 }
 
 // A row to a block, or a wave, from this many rows on (two blocks of 1024 threads to a unit); fewer long rows are split.
-bool whole_rows(long long R, int packs) { return packs <= kWavePacks || R >= tt::compute_units(); }
+bool whole_rows(long long R, int packs) {
+  return packs <= kWavePacks || R >= tt::compute_units() || R > kMostSplitRows;
+}
 
 // Whether the forward pass writes the gradient too, for an incoming gradient of one: where a row's own block does it
 // (the row is then read once for both), and that gradient is the likely one.  A loss for each row is weighted by its
@@ -474,15 +500,27 @@ template <typename T, bool GRAD>
 int launch_rows(const T* x, const Teacher& te, const Out& o, T* dx, const int* count_parts, const Scale& sc, int R,
                 int V, int packs) {
   hipStream_t st = tt::stream();
-  const long long most = 16 * tt::compute_units();
+  const long long most = kMostBlocks * tt::compute_units();
   const size_t wave_lds = entries_bytes<kWave>(te.K, kThreads / kWave);
-  if constexpr (!GRAD) {
+  constexpr int kRows = kThreads / kLanes;
+  if (GRAD && by_lanes(packs, te.K) && packs <= 2 * kLanes) {
+    distill_rows<T, kLanes, 2, false, true>
+        <<<grid_for((R + kRows - 1LL) / kRows, most), kThreads, entries_bytes<kLanes>(te.K, kRows), st>>>(
+            x, te, o, dx, count_parts, sc, R, V);
+  } else if (by_lanes(packs, te.K)) {
+    distill_rows<T, kLanes, GRAD ? 8 : 0, !GRAD, GRAD>
+        <<<grid_for((R + kRows - 1LL) / kRows, most), kThreads, entries_bytes<kLanes>(te.K, kRows), st>>>(
+            x, te, o, dx, count_parts, sc, R, V);
+  } else if constexpr (!GRAD) {
     if (by_waves(packs, te.K))
       distill_rows<T, kWave, 0, true, false><<<grid_for((R + 3LL) / 4, most), kThreads, wave_lds, st>>>(
           x, te, o, dx, count_parts, sc, R, V);
     else
       distill_rows<T, 256, 0, true, false><<<grid_for(R, most), 256, entries_bytes<256>(te.K, 1), st>>>(
           x, te, o, dx, count_parts, sc, R, V);
+  } else if (by_waves(packs, te.K) && packs > 8 * kWave) {
+    distill_rows<T, kWave, 16, false, true><<<grid_for((R + 3LL) / 4, most), kThreads, wave_lds, st>>>(
+        x, te, o, dx, count_parts, sc, R, V);
   } else if (by_waves(packs, te.K)) {
     distill_rows<T, kWave, 8, false, true><<<grid_for((R + 3LL) / 4, most), kThreads, wave_lds, st>>>(
         x, te, o, dx, count_parts, sc, R, V);
@@ -511,15 +549,17 @@ int forward(const T* x, const Teacher& te, float* loss, float* stats, float* cou
   const Scale sc = scale_for(temperature);
   const int packs = (V + Pack<T>::n - 1) / Pack<T>::n;
   const int splits = whole_rows(R, packs) ? 1 : splits_for(R, packs);
+  const size_t blocks = splits > 1 ? R : kMostBlocks * (size_t)tt::compute_units();
   void* ws;
-  if (tt::workspace(((size_t)R * 2 + kCountBlocks + (size_t)R * splits * 2) * sizeof(float), &ws)) return -1;
-  float* stat_part = (float*)ws;
-  float* counted = stat_part + (size_t)R * splits * 2;
-  int* parts = (int*)(counted + R);
-  const Out o = {reduction == 0 ? loss : (float*)(parts + kCountBlocks), counted, (float2*)stats,
-                 reduction == 0 ? nullptr : loss, count, reduction == 2};
+  if (tt::workspace(blocks * 2 * sizeof(double) + (kCountBlocks + (size_t)R * splits * 2) * sizeof(float), &ws)) return -1;
+  double* sums = (double*)ws;
+  int* parts = (int*)(sums + 2 * blocks);
+  float* stat_part = (float*)(parts + kCountBlocks);
+  const Out o = {reduction == 0 ? loss : nullptr, (float2*)stats, sums, reduction == 0 ? nullptr : loss, count,
+                 reduction == 2};
   if (splits > 1) {
-    distill_split<T><<<(unsigned)(R * splits), kThreads, entries_bytes<kThreads>(te.K, 1), st>>>(x, te, o, stat_part, sc, splits, R, V);
+    distill_split<T><<<(unsigned)(R * splits), kThreads, entries_bytes<kThreads>(te.K, 1), st>>>(x, te, o, stat_part, sc,
+                                                                                              splits, R, V);
     TT_LAUNCH_CHECK();
     return 0;
   }
@@ -539,13 +579,18 @@ int backward(const T* x, const Teacher& te, const float* stats, const float* cou
   hipStream_t st = tt::stream();
   const Scale sc = scale_for(temperature);
   const int packs = (V + Pack<T>::n - 1) / Pack<T>::n;
-  if (by_waves(packs, te.K)) {
-    distill_bwd<T, kWave><<<grid_for((R + 3LL) / 4, 16 * tt::compute_units()), kThreads,
+  if (by_lanes(packs, te.K)) {
+    constexpr int kRows = kThreads / kLanes;
+    distill_bwd<T, kLanes><<<grid_for((R + kRows - 1LL) / kRows, kMostBlocks * tt::compute_units()), kThreads,
+                             entries_bytes<kLanes>(te.K, kRows), st>>>(
+        x, te, (const float2*)stats, count, g, dx, sc, reduction, is_ahead, 1, R, V);
+  } else if (by_waves(packs, te.K)) {
+    distill_bwd<T, kWave><<<grid_for((R + 3LL) / 4, kMostBlocks * tt::compute_units()), kThreads,
                             entries_bytes<kWave>(te.K, kThreads / kWave), st>>>(
         x, te, (const float2*)stats, count, g, dx, sc, reduction, is_ahead, 1, R, V);
   } else {
     const int splits = splits_for(R, packs);
-    distill_bwd<T, kThreads><<<grid_for((long long)R * splits, 16 * tt::compute_units()), kThreads,
+    distill_bwd<T, kThreads><<<grid_for((long long)R * splits, kMostBlocks * tt::compute_units()), kThreads,
                                entries_bytes<kThreads>(te.K, 1), st>>>(
         x, te, (const float2*)stats, count, g, dx, sc, reduction, is_ahead, splits, R, V);
   }

@@ -2,6 +2,7 @@
 // backward (vocab.h has the formulas).
 #include "vocab.h"
 
+#include <climits>
 #include <type_traits>
 
 namespace {
@@ -12,48 +13,36 @@ using tt::LogitRow;
 using tt::Pack;
 using tt::Share;
 using tt::Stat;
+using tt::Words;
 
 constexpr int kThreads = 256;
 constexpr tt::Scale kPlain = {(float)tt::kLog2e, 1.f, 1.f};
 constexpr int kMostTop = 64;
-constexpr int kMostSplitRows = 8192;    // fewer rows than this may be shared by blocks
+constexpr int kMostSplitRows = 2048;    // rows that may be shared by blocks
 
 // ---- the best alternatives -------------------------------------------------------------------------
 //
-// One pass keeps, beside the sums, each thread's largest value and where it stood first.  Of the G threads' best values
-// the K largest name K owners, and the K-th of them is a bound: a value above it lies with an owner, for every other
-// thread's best is below.  So the owners' packs alone are read again, a few thousand values of a row that has just come
-// through the cache, and what reaches the bound (K values and few more, unless the row is laid out against it) is
-// ranked by counting.  Values and places make keys without ties, so the answer does not depend on the order in which
-// candidates arrive.
+// One pass keeps, beside the sums, each thread's largest value.  Of the G threads' largest values the K-th largest is a
+// bound: K threads reach it, and what no thread's largest value reaches is no candidate.  So the packs of these K owners
+// alone are read again, a few thousand values of a row that has just come through the cache, and what reaches the bound
+// (K values and few more, unless the row is laid out against it) is ranked by counting.  Values and places make keys
+// without ties, so the answer does not depend on the order in which candidates arrive.
 
 typedef unsigned long long Key;
 
-// A value and its place as one number that orders by value, then by the lower place.  -0 counts as 0.
-__device__ __forceinline__ Key make_key(float z, int place) {
+// A value as a number that orders alike, above zero.  -0 counts as 0.
+__device__ __forceinline__ unsigned order_of(float z) {
   const unsigned b = __float_as_uint(z + 0.f);
-  const unsigned order = b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
-  return ((Key)order << 32) | (0xffffffffu - (unsigned)place);
+  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+// A value and its place as one number that orders by value, then by the lower place.
+__device__ __forceinline__ Key make_key(float z, int place) {
+  return ((Key)order_of(z) << 32) | (0xffffffffu - (unsigned)place);
 }
 __device__ __forceinline__ int key_place(Key k) { return (int)(0xffffffffu - (unsigned)k); }
 __device__ __forceinline__ float key_value(Key k) {
   const unsigned order = (unsigned)(k >> 32);
   return __uint_as_float(order ^ ((order >> 31) ? 0x80000000u : 0xffffffffu));
-}
-
-// The keys of a wave, largest first.
-__device__ __forceinline__ Key wave_sort(Key k) {
-  const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-  for (int size = 2; size <= kWave; size <<= 1) {
-#pragma unroll
-    for (int off = size >> 1; off > 0; off >>= 1) {
-      const Key o = __shfl_xor(k, off, kWave);
-      const bool lower = (lane & off) == 0, down = (lane & size) == 0;
-      k = (o > k) == (lower == down) ? o : k;
-    }
-  }
-  return k;
 }
 
 constexpr int most(int a, int b) { return a > b ? a : b; }
@@ -64,6 +53,7 @@ struct TopSpace {
   static constexpr int room = most(G * n + kMostTop, G == kWave ? 0 : kMostTop * (kMostTop + 1) / 2);
   Key cand[room];
   Key heads[G];
+  alignas(16) unsigned largest[G];
   Key best[kMostTop];
   int owner[kMostTop];
   int count, owners;
@@ -76,25 +66,30 @@ template <int G, int n>
 __device__ __forceinline__ void rank_candidates(TopSpace<G, n>& s, int lane, int count, int K) {
   for (int k = lane; k < K; k += G) s.best[k] = 0;
   tt::sync_row<G>();
-  for (int i = lane; i < count; i += G) {
-    const Key mine = s.cand[i];
+  if (G == kWave && count <= kWave) {       // a key to a lane
+    const Key mine = lane < count ? s.cand[lane] : 0;
     int rank = 0;
-    for (int k = 0; k < count; ++k) rank += s.cand[k] > mine;
-    if (rank < K) s.best[rank] = mine;
+    for (int k = 0; k < count; ++k) rank += tt::lane_value(mine, k) > mine;
+    if (lane < count && rank < K) s.best[rank] = mine;
+  } else {
+    for (int i = lane; i < count; i += G) {
+      const Key mine = s.cand[i];
+      int rank = 0;
+      for (int k = 0; k < count; ++k) rank += s.cand[k] > mine;
+      if (rank < K) s.best[rank] = mine;
+    }
   }
   tt::sync_row<G>();
 }
 
-// The key of a thread's best value, from where scan() says that it stands; zero of a thread without values.
+// The key of a thread's best value; `best` is what scan() says.
 template <typename T, int G>
 __device__ __forceinline__ Key best_key(const T* x, const LogitRow<T>& r, const Share& h, int lane, int best) {
-  if (best == tt::kNothing) return 0;
-  if (best == tt::kHead) return make_key(tt::widen(x[r.start + lane]), lane);
-  if (best == tt::kTail) return make_key(tt::widen(x[r.start + r.tail_at + lane]), r.tail_at + lane);
   Key mine = 0;
+  const int from = best == tt::kNothing ? h.p0 + lane : best;
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int j = best + u * G;
+    const int j = from + u * G;
     if (j < h.p1) {
       float z[Pack<T>::n];
       tt::unpack<T>(z, r.pack(j));
@@ -105,68 +100,161 @@ __device__ __forceinline__ Key best_key(const T* x, const LogitRow<T>& r, const 
       }
     }
   }
+  if (lane < h.head + h.tail) {
+    const int i = tt::loose_column(r, h, lane);
+    const Key k = make_key(tt::widen(x[r.start + i]), i);
+    mine = k > mine ? k : mine;
+  }
   return mine;
 }
 
-// Leaves the K best of a share in s.best; `mine` is the key of this thread's best value, or zero.
+// Names the owners in s.owner, as many as it returns, and leaves the bound in `bound`.  The K-th largest value is built
+// bit by bit from the top, each time counting the threads that reach it.  Most often K of them alone do after some bits,
+// which is near enough unless K is most of G.
+template <typename T, int G>
+__device__ __forceinline__ int name_owners(TopSpace<G, Pack<T>::n>& s, const T* x, const LogitRow<T>& r, const Share& h,
+                                           int lane, float largest, int best, int K, Key& bound) {
+  constexpr int kLists = G / kWave, kLowest = sizeof(T) == 2 ? 13 : 0;     // (a widened half has 13 bits alike below)
+  const int in_wave = lane & (kWave - 1);
+  const bool any = h.p0 + lane < h.p1 || lane < h.head + h.tail;
+  const unsigned own = any ? order_of(largest) : 0u;
+  unsigned v[kLists] = {own};
+  if (lane == 0) s.count = s.owners = 0;
+  if constexpr (G > kWave) {
+    static_assert(kLists == 4, "a wave reads the block's values as 16 bytes a lane");
+    s.largest[lane] = own;
+    tt::sync_row<G>();
+    const uint4 all = *reinterpret_cast<const uint4*>(&s.largest[in_wave * kLists]);
+    v[0] = all.x, v[1] = all.y, v[2] = all.z, v[3] = all.w;
+  }
+  unsigned reach = 0;
+  int have = G;
+  for (int bit = 31; bit >= kLowest && (have != K || 2 * K > G); --bit) {
+    const unsigned next = reach | 1u << bit;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kLists; ++i) n += __popcll(__ballot(v[i] >= next));
+    if (n >= K) {
+      reach = next;
+      have = n;
+    }
+  }
+  bound = (Key)reach << 32;
+  if (have == K || reach == 0) {        // (0: fewer than K threads have values at all, and each of those is an owner)
+    reach = reach ? reach : 1u;
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < kLists; ++i) {
+      const unsigned long long who = __ballot(v[i] >= reach);
+      const int slot = at + __builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)who, 0));
+      if (v[i] >= reach && lane < kWave) s.owner[slot] = in_wave * kLists + i;
+      at += __popcll(who);
+    }
+    tt::sync_row<G>();
+    return at;
+  }
+  // more than K threads reach the K-th largest value: those with the lowest places are the owners
+  const Key mine = own >= reach ? best_key<T, G>(x, r, h, lane, best) : 0;
+  s.heads[lane] = mine;
+  tt::sync_row<G>();
+  if (mine != 0) {
+    int rank = 0;
+    for (int i = 0; i < G; ++i) rank += s.heads[i] > mine;
+    if (rank < K) s.owner[rank] = lane;
+    if (rank == K - 1) s.bound = mine;
+  }
+  tt::sync_row<G>();
+  bound = s.bound;
+  return K;
+}
+
+// The owners' packs and loose columns, numbered: an owner's have numbers from its own on, up to a power of two.
+template <typename T, int G>
+struct Again {
+  static constexpr int n = Pack<T>::n, kNone = INT_MIN;
+  int rounds, shift, all;
+  __device__ __forceinline__ Again(const Share& h, int owners) : rounds((h.p1 - h.p0 + G - 1) / G) {
+    shift = 32 - __builtin_clz(rounds | 1);       // 2^shift > rounds
+    all = owners << shift;
+  }
+  // what number q is: a pack, or -1 - c for a column, or kNone
+  __device__ __forceinline__ int place(const TopSpace<G, n>& s, const LogitRow<T>& r, const Share& h, int q) const {
+    if (q >= all) return kNone;
+    const int owner = s.owner[q >> shift], step = q & ((1 << shift) - 1);
+    if (step == rounds) return owner < h.head + h.tail ? -1 - tt::loose_column(r, h, owner) : kNone;
+    const int j = h.p0 + owner + step * G;
+    return step < rounds && j < h.p1 ? j : kNone;
+  }
+  // Appends the keys that reach the bound.  A wave of its own counts them in a register.
+  static __device__ __forceinline__ void offer(TopSpace<G, n>& s, int& count, bool any, float z, int column, Key bound) {
+    const Key k = make_key(z, column);
+    const bool is = any && k >= bound;
+    if constexpr (G == kWave) {
+      const unsigned long long who = __ballot(is);
+      if (who == 0) return;
+      const int at = count + __builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)who, 0));
+      if (is && at < TopSpace<G, n>::room) s.cand[at] = k;
+      count += __popcll(who);
+    } else if (is) {
+      const int at = atomicAdd(&s.count, 1);
+      if (at < TopSpace<G, n>::room) s.cand[at] = k;
+    }
+  }
+  static __device__ __forceinline__ void collect(TopSpace<G, n>& s, int& count, const T* x, const LogitRow<T>& r, int at,
+                                                 const Words& p, Key bound) {
+    float z[n];
+    tt::unpack<T>(z, p);
+#pragma unroll
+    for (int i = 0; i < n; ++i) offer(s, count, at >= 0, z[i], r.column(at) + i, bound);
+    const bool loose = at < 0 && at != kNone;
+    offer(s, count, loose, loose ? tt::widen(x[r.start - 1 - at]) : 0.f, -1 - at, bound);
+  }
+};
+
+// Leaves the K best of a share in s.best; `largest` is this thread's largest value and `best` what scan() says of it.
 template <typename T, int G>
 __device__ __forceinline__ void select_top(TopSpace<G, Pack<T>::n>& s, const T* x, const LogitRow<T>& r, const Share& h,
-                                           int lane, Key mine, int K) {
-  constexpr int n = Pack<T>::n;
-  const Key sorted = wave_sort(mine);
-  const int in_wave = lane & (kWave - 1), lists = G / kWave;
-  if (in_wave < K) s.heads[(lane >> 6) * K + in_wave] = sorted;
-  if (lane == 0) {
-    s.count = s.owners = 0;
-    s.bound = 0;
-  }
-  tt::sync_row<G>();
-  if (lane < lists * K) {                           // (K <= 64: at most one key to a thread)
-    const Key k = s.heads[lane];
-    int rank = 0;
-    for (int o = 0; o < lists * K; ++o) rank += s.heads[o] > k;
-    if (k != 0 && rank < K) {
-      const int c = key_place(k);
-      s.owner[rank] = c < r.head ? c : c >= r.tail_at ? c - r.tail_at : ((c + r.skip) / n - h.p0) % G;
-      atomicAdd(&s.owners, 1);
-      if (rank == K - 1) s.bound = k;
-    }
-  }
-  tt::sync_row<G>();
-  // every owner's packs, and its column of the head and of the tail
-  const int rounds = (h.p1 - h.p0 + G - 1) / G, steps = rounds + 2, pairs = s.owners * steps;
-  Key bound = s.bound;
+                                           int lane, float largest, int best, int K) {
+  typedef Again<T, G> A;
+  Key bound;
+  const A again(h, name_owners<T, G>(s, x, r, h, lane, largest, best, K, bound));
   int count = 0;
-  for (int q0 = 0; q0 < pairs; q0 += G) {
-    const int q = q0 + lane;
-    if (q < pairs) {
-      const int owner = s.owner[q / steps], step = q % steps;
-      if (step < rounds) {
-        const int j = h.p0 + owner + step * G;
-        if (j < h.p1) {
-          float z[n];
-          tt::unpack<T>(z, r.pack(j));
+  for (int q0 = 0; q0 < again.all; q0 += kUnroll * G) {
+    int at[kUnroll];
+    Words p[kUnroll];
 #pragma unroll
-          for (int i = 0; i < n; ++i) {
-            const Key k = make_key(z[i], r.column(j) + i);
-            if (k >= bound) s.cand[atomicAdd(&s.count, 1)] = k;
-          }
-        }
-      } else if (owner < (step == rounds ? h.head : h.tail)) {
-        const int c = (step == rounds ? 0 : r.tail_at) + owner;
-        const Key k = make_key(tt::widen(x[r.start + c]), c);
-        if (k >= bound) s.cand[atomicAdd(&s.count, 1)] = k;
+    for (int u = 0; u < kUnroll; ++u) {
+      at[u] = again.place(s, r, h, q0 + u * G + lane);
+      p[u] = Words(Pack<T>::lowest);
+      if (at[u] >= 0) p[u] = r.pack(at[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (q0 + u * G < again.all) A::collect(s, count, x, r, at[u], p[u], bound);
+  }
+  tt::sync_row<G>();
+  if (G > kWave) count = s.count;
+  if (count > TopSpace<G, Pack<T>::n>::room) {        // once more, with the K best of each round kept
+    tt::sync_row<G>();
+    if (lane == 0) s.count = 0;
+    count = 0;
+    tt::sync_row<G>();
+    for (int q0 = 0; q0 < again.all; q0 += G) {
+      const int at = again.place(s, r, h, q0 + lane);
+      Words p = Words(Pack<T>::lowest);
+      if (at >= 0) p = r.pack(at);
+      A::collect(s, count, x, r, at, p, bound);
+      tt::sync_row<G>();
+      if (G > kWave) count = s.count;
+      if (count > kMostTop && q0 + G < again.all) {
+        rank_candidates(s, lane, count, K);
+        for (int k = lane; k < K; k += G) s.cand[k] = s.best[k];
+        bound = s.best[K - 1] > bound ? s.best[K - 1] : bound;
+        if (lane == 0) s.count = K;
+        count = K;
       }
+      tt::sync_row<G>();
     }
-    tt::sync_row<G>();
-    count = s.count;
-    if (count > kMostTop && q0 + G < pairs) {       // another round might not fit: keep the K best of these
-      rank_candidates(s, lane, count, K);
-      for (int k = lane; k < K; k += G) s.cand[k] = s.best[k];
-      bound = s.best[K - 1] > bound ? s.best[K - 1] : bound;
-      if (lane == 0) s.count = K;
-    }
-    tt::sync_row<G>();
   }
   rank_candidates(s, lane, count, K);
 }
@@ -254,7 +342,7 @@ __device__ __forceinline__ void write_row(const ForwardOut& o, size_t row, int l
 template <typename T, int G, bool TOP>
 __global__ __launch_bounds__(kThreads) void logp_rows(const T* __restrict__ x, ForwardOut o, int R, int V, int K) {
   constexpr int kRows = kThreads / G;
-  __shared__ float part[kRows][3 * (G / kWave)];
+  __shared__ float part[kRows][tt::parts_of(G, 3)];
   __shared__ std::conditional_t<TOP, TopSpace<G, Pack<T>::n>, NoSpace> space[kRows];
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
   const float c = (float)tt::kLog2e;
@@ -271,11 +359,10 @@ __global__ __launch_bounds__(kThreads) void logp_rows(const T* __restrict__ x, F
     Stat a = {-INFINITY, 0.f, 0.f};
     int best = tt::kNothing;
     tt::scan<T, G, true>(a, best, x, r, h, lane, c);
-    Key mine = 0;
-    if constexpr (TOP) mine = best_key<T, G>(x, r, h, lane, best);
+    const float largest = a.m;
     a = tt::row_join<T, G, true>(a, c, part[sub]);
     if constexpr (TOP) {
-      select_top<T, G>(space[sub], x, r, h, lane, mine, K);
+      select_top<T, G>(space[sub], x, r, h, lane, largest, best, K);
       write_row<T, G>(o, row, lane, a, t >= 0, z_token, space[sub].best, K);
     } else {
       write_row<T, G>(o, row, lane, a, t >= 0, z_token, nullptr, 0);
@@ -284,8 +371,7 @@ __global__ __launch_bounds__(kThreads) void logp_rows(const T* __restrict__ x, F
   }
 }
 
-// How many splits of a row are done; zero between launches.
-__device__ unsigned logp_tickets[kMostSplitRows];
+__device__ tt::Ticket logp_tickets[kMostSplitRows];       // the splits of each row that are done
 
 // Few long rows: `splits` blocks to a row, each with its share; the one that comes last puts the shares together.
 template <typename T, bool TOP>
@@ -309,17 +395,16 @@ __global__ __launch_bounds__(kThreads) void logp_split(const T* __restrict__ x, 
   Stat a = {-INFINITY, 0.f, 0.f};
   int best = tt::kNothing;
   tt::scan<T, G, true>(a, best, x, r, h, lane, c);
-  Key mine = 0;
-  if constexpr (TOP) mine = best_key<T, G>(x, r, h, lane, best);
+  const float largest = a.m;
   a = tt::row_join<T, G, true>(a, c, part);
-  if constexpr (TOP) select_top<T, G>(space, x, r, h, lane, mine, K);
+  if constexpr (TOP) select_top<T, G>(space, x, r, h, lane, largest, best, K);
   if (lane < kWave) {
     float* mine_part = stat_part + (size_t)blockIdx.x * 3;
     if (lane < 3) tt::share(mine_part + lane, lane == 0 ? a.m : lane == 1 ? a.s : a.t);
     if constexpr (TOP)
       if (lane < K) tt::share(key_part + (size_t)blockIdx.x * K + lane, space.best[lane]);
     tt::stores_done();
-    if (lane == 0) last = tt::last_ticket(&logp_tickets[row], splits);
+    if (lane == 0) last = tt::last_ticket(logp_tickets + row, splits);
   }
   __syncthreads();
   if (!last) return;
@@ -388,8 +473,10 @@ __global__ __launch_bounds__(kThreads) void logp_bwd(const T* __restrict__ x, Ba
       g.H = in.entropy[row];
       g.total = in.g_logp && t < 0 ? NAN : a;
       if (in.g_top) {
-        const int at = threadIdx.x & (kWave - 1);
-        g.total += tt::wave_sum(at < K ? in.g_top[row * K + at] : 0.f);
+        constexpr int kLanes = G < kWave ? G : kWave;
+        float sum = 0.f;
+        for (int k = lane % kLanes; k < K; k += kLanes) sum += in.g_top[row * K + k];
+        g.total += tt::lanes_reduce<kLanes>(sum, tt::Plus());
       }
     }
     for (int j = s.p0 + lane; j < s.p1; j += kUnroll * G) {
@@ -407,8 +494,8 @@ __global__ __launch_bounds__(kThreads) void logp_bwd(const T* __restrict__ x, Ba
         tt::write_pack(r, dx, j + u * G, none ? tt::Words(0u) : tt::pack<T>(z));
       }
     }
-    if (lane < s.head + s.tail) {
-      const size_t at = r.start + (lane < s.head ? lane : r.tail_at + lane - s.head);
+    for (int i = lane; i < s.head + s.tail; i += G) {
+      const size_t at = r.start + tt::loose_column(r, s, i);
       dx[at] = none ? (T)0.f : (T)g(tt::widen(x[at]), 0.f);
     }
     const int fixes = none ? 0 : (given ? 1 : 0) + (in.g_top ? K : 0);
@@ -445,8 +532,17 @@ int check(const char* fn, int dtype, int index_bits, long long R, int V, int K) 
 
 unsigned grid_for(long long blocks) { return (unsigned)(blocks < (1 << 22) ? blocks : (1 << 22)); }
 
-// Rows of up to this many packs go to a wave each, longer ones to a block.
-constexpr int kWavePacks = 1024;
+// Rows of up to kWavePacks packs go to a wave each, short ones to some of its lanes, so that a wave has several rows on
+// their way; longer ones go to a block.  Measured on 131072 rows of float32, a wave against eight lanes: of 10 values 60
+// and 9 us, of 300 values 58 and 31 us forward; and backward, where more lanes store wider pieces, 8 against 16 lanes: of
+// 37 values 17 and 25 us, of 100 values 31 and 29 us, of 300 values 105 and 79 us (a wave: 125 us).  67108 rows of 1000
+// are level.  With kWaveTop alternatives and more a block of four times as many threads has a closer bound (22369 rows of
+// 3000 with 64: 1062 us by waves, 205 us by blocks).
+constexpr int kLanesPacks = 128, kFewPacks = 16, kWavePacks = 1024, kWaveTop = 32;
+template <int G>
+unsigned row_grid(long long R) {
+  return grid_for((R + kThreads / G - 1) / (kThreads / G));
+}
 
 // How many blocks share a row: as many as fill the device eight times, each with kUnroll packs to a thread at least.
 int splits_for(long long R, int packs) {
@@ -469,10 +565,11 @@ int forward(const T* x, const ForwardOut& o, int R, int V, int K) {
     Key* keys = (Key*)((char*)ws + stat_bytes);
     if (K) logp_split<T, true><<<(unsigned)parts, kThreads, 0, st>>>(x, o, (float*)ws, keys, splits, V, K);
     else logp_split<T, false><<<(unsigned)parts, kThreads, 0, st>>>(x, o, (float*)ws, keys, splits, V, K);
-  } else if (packs <= kWavePacks) {
-    const unsigned grid = grid_for((R + 3LL) / 4);
-    if (K) logp_rows<T, kWave, true><<<grid, kThreads, 0, st>>>(x, o, R, V, K);
-    else logp_rows<T, kWave, false><<<grid, kThreads, 0, st>>>(x, o, R, V, K);
+  } else if (packs <= kLanesPacks && K == 0) {
+    logp_rows<T, 8, false><<<row_grid<8>(R), kThreads, 0, st>>>(x, o, R, V, K);
+  } else if (packs <= kWavePacks && K <= kWaveTop) {
+    if (K) logp_rows<T, kWave, true><<<row_grid<kWave>(R), kThreads, 0, st>>>(x, o, R, V, K);
+    else logp_rows<T, kWave, false><<<row_grid<kWave>(R), kThreads, 0, st>>>(x, o, R, V, K);
   } else {
     if (K) logp_rows<T, kThreads, true><<<grid_for(R), kThreads, 0, st>>>(x, o, R, V, K);
     else logp_rows<T, kThreads, false><<<grid_for(R), kThreads, 0, st>>>(x, o, R, V, K);
@@ -485,8 +582,12 @@ template <typename T>
 int backward(const T* x, const BackwardIn& in, T* dx, int R, int V, int K) {
   hipStream_t st = tt::stream();
   const int packs = (V + Pack<T>::n - 1) / Pack<T>::n;
-  if (packs <= kWavePacks) {
-    logp_bwd<T, kWave><<<grid_for((R + 3LL) / 4), kThreads, 0, st>>>(x, in, dx, 1, R, V, K);
+  if (packs <= kFewPacks) {
+    logp_bwd<T, 8><<<row_grid<8>(R), kThreads, 0, st>>>(x, in, dx, 1, R, V, K);
+  } else if (packs <= kLanesPacks) {
+    logp_bwd<T, 16><<<row_grid<16>(R), kThreads, 0, st>>>(x, in, dx, 1, R, V, K);
+  } else if (packs <= kWavePacks) {
+    logp_bwd<T, kWave><<<row_grid<kWave>(R), kThreads, 0, st>>>(x, in, dx, 1, R, V, K);
   } else {
     const int splits = splits_for(R, packs);
     logp_bwd<T, kThreads><<<grid_for((long long)R * splits), kThreads, 0, st>>>(x, in, dx, splits, R, V, K);
