@@ -47,6 +47,9 @@ __device__ __forceinline__ float key_value(Key k) {
 
 constexpr int most(int a, int b) { return a > b ? a : b; }
 
+// More than K owners do no harm; up to this many more may be named, as halves, which are often equal, tend to.
+constexpr int kMore = 32;
+
 template <int G, int n>
 struct TopSpace {
   // what one round can add to K kept candidates; what the lists of the splits can add up to
@@ -55,7 +58,7 @@ struct TopSpace {
   Key heads[G];
   alignas(16) unsigned largest[G];
   Key best[kMostTop];
-  int owner[kMostTop];
+  int owner[kMostTop + kMore];
   int count, owners;
   Key bound;
 };
@@ -87,17 +90,14 @@ template <typename T, int G>
 __device__ __forceinline__ Key best_key(const T* x, const LogitRow<T>& r, const Share& h, int lane, int best) {
   Key mine = 0;
   const int from = best == tt::kNothing ? h.p0 + lane : best;
+#pragma unroll 1
+  for (int j = from; j < from + kUnroll * G && j < h.p1; j += G) {
+    float z[Pack<T>::n];
+    tt::unpack<T>(z, r.pack(j));
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const int j = from + u * G;
-    if (j < h.p1) {
-      float z[Pack<T>::n];
-      tt::unpack<T>(z, r.pack(j));
-#pragma unroll
-      for (int i = 0; i < Pack<T>::n; ++i) {
-        const Key k = make_key(z[i], r.column(j) + i);
-        mine = k > mine ? k : mine;
-      }
+    for (int i = 0; i < Pack<T>::n; ++i) {
+      const Key k = make_key(z[i], r.column(j) + i);
+      mine = k > mine ? k : mine;
     }
   }
   if (lane < h.head + h.tail) {
@@ -140,7 +140,7 @@ __device__ __forceinline__ int name_owners(TopSpace<G, Pack<T>::n>& s, const T* 
     }
   }
   bound = (Key)reach << 32;
-  if (have == K || reach == 0) {        // (0: fewer than K threads have values at all, and each of those is an owner)
+  if (have <= K + kMore || reach == 0) {        // (0: fewer than K threads have values at all, and each of those is an owner)
     reach = reach ? reach : 1u;
     int at = 0;
 #pragma unroll
@@ -153,7 +153,7 @@ __device__ __forceinline__ int name_owners(TopSpace<G, Pack<T>::n>& s, const T* 
     tt::sync_row<G>();
     return at;
   }
-  // more than K threads reach the K-th largest value: those with the lowest places are the owners
+  // many threads reach the K-th largest value: those with the lowest places are the owners
   const Key mine = own >= reach ? best_key<T, G>(x, r, h, lane, best) : 0;
   s.heads[lane] = mine;
   tt::sync_row<G>();
@@ -215,46 +215,45 @@ struct Again {
 template <typename T, int G>
 __device__ __forceinline__ void select_top(TopSpace<G, Pack<T>::n>& s, const T* x, const LogitRow<T>& r, const Share& h,
                                            int lane, float largest, int best, int K) {
-  typedef Again<T, G> A;
   Key bound;
-  const A again(h, name_owners<T, G>(s, x, r, h, lane, largest, best, K, bound));
+  const Again<T, G> again(h, name_owners<T, G>(s, x, r, h, lane, largest, best, K, bound));
   int count = 0;
-  for (int q0 = 0; q0 < again.all; q0 += kUnroll * G) {
-    int at[kUnroll];
-    Words p[kUnroll];
+  constexpr int kAgain = 2;       // packs on their way at once
+  // If there is no room for all candidates, the second time keeps the K best after each step.
+  for (bool careful = false;; careful = true) {
+    for (int q0 = 0; q0 < again.all; q0 += kAgain * G) {
+      int at[kAgain];
+      Words p[kAgain];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      at[u] = again.place(s, r, h, q0 + u * G + lane);
-      p[u] = Words(Pack<T>::lowest);
-      if (at[u] >= 0) p[u] = r.pack(at[u]);
+      for (int u = 0; u < kAgain; ++u) {
+        at[u] = again.place(s, r, h, q0 + u * G + lane);
+        p[u] = Words(Pack<T>::lowest);
+        if (at[u] >= 0) p[u] = r.pack(at[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kAgain; ++u) {
+        if (q0 + u * G >= again.all) continue;
+        Again<T, G>::collect(s, count, x, r, at[u], p[u], bound);
+        if (!careful) continue;
+        tt::sync_row<G>();
+        if (G > kWave) count = s.count;
+        if (count > kMostTop) {
+          rank_candidates(s, lane, count, K);
+          for (int k = lane; k < K; k += G) s.cand[k] = s.best[k];
+          bound = s.best[K - 1] > bound ? s.best[K - 1] : bound;
+          if (lane == 0) s.count = K;
+          count = K;
+        }
+        tt::sync_row<G>();
+      }
     }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (q0 + u * G < again.all) A::collect(s, count, x, r, at[u], p[u], bound);
-  }
-  tt::sync_row<G>();
-  if (G > kWave) count = s.count;
-  if (count > TopSpace<G, Pack<T>::n>::room) {        // once more, with the K best of each round kept
+    tt::sync_row<G>();
+    if (G > kWave) count = s.count;
+    if (count <= TopSpace<G, Pack<T>::n>::room) break;
     tt::sync_row<G>();
     if (lane == 0) s.count = 0;
     count = 0;
     tt::sync_row<G>();
-    for (int q0 = 0; q0 < again.all; q0 += G) {
-      const int at = again.place(s, r, h, q0 + lane);
-      Words p = Words(Pack<T>::lowest);
-      if (at >= 0) p = r.pack(at);
-      A::collect(s, count, x, r, at, p, bound);
-      tt::sync_row<G>();
-      if (G > kWave) count = s.count;
-      if (count > kMostTop && q0 + G < again.all) {
-        rank_candidates(s, lane, count, K);
-        for (int k = lane; k < K; k += G) s.cand[k] = s.best[k];
-        bound = s.best[K - 1] > bound ? s.best[K - 1] : bound;
-        if (lane == 0) s.count = K;
-        count = K;
-      }
-      tt::sync_row<G>();
-    }
   }
   rank_candidates(s, lane, count, K);
 }
