@@ -55,6 +55,9 @@ int tt_memcpy_d2h(void* dst_host, const void* src_dev, size_t bytes);   /* synch
 int tt_memcpy_d2d(void* dst_dev, const void* src_dev, size_t bytes);    /* stream-ordered */
 int tt_memset(void* dst_dev, int byte_value, size_t bytes);             /* stream-ordered */
 int tt_sync(void);
+/* What is launched from here on waits for what another stream of the device has been given so far (1: the default
+ * stream, 2: the default stream of the calling thread, else a hipStream_t). */
+int tt_wait_stream(unsigned long long stream);
 
 /* HIP events on the library stream, for timing kernels from the host side. */
 int tt_event_create(void** event);

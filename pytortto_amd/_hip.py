@@ -28,6 +28,7 @@ PROTOTYPES = {
     'tt_memcpy_d2d': [_P, _P, c_size_t],
     'tt_memset': [_P, _I, c_size_t],
     'tt_sync': [],
+    'tt_wait_stream': [ctypes.c_ulonglong],
     'tt_set_conv_math': [_I],
     'tt_get_conv_math': [POINTER(c_int)],
     'tt_set_conv_dense_cell_min_tiles': [_I],

@@ -349,6 +349,19 @@ int tt_conv2d_dgrad_bf16x3(const float* dy, const float* w, const float* bias, f
   return tt_conv2d_dgrad_f32(dy, w, bias, dx, N, C, Hx, Wx, K, R, S_, sh, sw, ph, pw, dh, dw, groups, P, Q);
 }
 
+int tt_wait_stream(unsigned long long stream) {
+  TT_REQUIRE_INIT();
+  TT_REQUIRE(stream != 0, "tt_wait_stream: 0 is no stream (1: the default stream, 2: the calling thread's)");
+  const hipStream_t other = stream == 1 ? nullptr : stream == 2 ? hipStreamPerThread : (hipStream_t)stream;
+  hipEvent_t event;
+  TT_HIP(hipEventCreateWithFlags(&event, hipEventDisableTiming));
+  hipError_t e = hipEventRecord(event, other);
+  if (e == hipSuccess) e = hipStreamWaitEvent(S().stream, event, 0);
+  (void)hipEventDestroy(event);       // (released once it has passed)
+  TT_HIP(e);
+  return 0;
+}
+
 int tt_sync(void) {
   TT_REQUIRE_INIT();
   TT_HIP(hipStreamSynchronize(S().stream));

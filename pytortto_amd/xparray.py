@@ -268,8 +268,10 @@ class hiparray:
     @classmethod
     def borrow(cls, source):
         """An array on the device memory of ``source``, an object with ``__cuda_array_interface__`` (a torch or
-        CuPy array); nothing is copied and ``source`` is kept alive.  Its writers must be done, or be ordered in
-        front of the library's stream, before the array is used; and memory is borrowed once, not as two arrays."""
+        CuPy array); nothing is copied and ``source`` is kept alive with the array.  Where the interface names the
+        stream of its writers, the library's waits for it; where it does not (torch), they must be done, or be ordered
+        in front of the library's stream, before the array is used.  The memory must not be given to others before what
+        reads it here is done, and it is borrowed once, not as two arrays."""
         about = source.__cuda_array_interface__
         shape, kind = tuple(about['shape']), about['typestr']
         dtype = _DTYPES.get(kind)
@@ -278,6 +280,8 @@ class hiparray:
         nbytes = prod(shape) * dtype.itemsize
         if about.get('mask') is not None:
             raise ValueError('borrowed device memory cannot be masked')
+        if about.get('stream') is not None:
+            _hip.call('tt_wait_stream', about['stream'])
         strides = about.get('strides')
         if strides is not None and nbytes:
             whole = dtype.itemsize
