@@ -127,10 +127,57 @@ __device__ __forceinline__ void queue_entries(const Entries& e, const LogitRow<T
   }
   tt::sync_row<G>();
 }
+// Of its queue a thread takes the first P entries of packs into registers, and into the packs as it writes them; `rest`
+// is stored behind the packs.  (A lone value costs memory a piece of 64 bytes: 131072 rows of 300 with 32 entries take
+// 104 us with P = 4 and 131 us with none.  Of long rows they are few, so P = 0.)
+template <int G>
+constexpr int kPatches = G < kWave ? 4 : G == kWave ? 2 : 0;
+template <int P>
+struct Patches {
+  int at[P ? P : 1];
+  float value[P ? P : 1];
+  int rest;
+};
+template <typename T, int P>
+__device__ __forceinline__ Patches<P> take_queued(const Entries& e, const LogitRow<T>& r, int lane) {
+  Patches<P> t;
+  int k = e.queue[lane];
+  t.rest = k;
+  if constexpr (P > 0) {
+    t.rest = -1;
+#pragma unroll
+    for (int i = 0; i < P; ++i) t.at[i] = -1;
+    for (int taken = 0; k >= 0;) {
+      const int j = e.place[k], next = e.next[k];
+      if (taken < P && j >= r.head && j < r.tail_at) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          t.at[i] = i == taken ? j + r.skip : t.at[i];
+          t.value[i] = i == taken ? e.logit[k] : t.value[i];
+        }
+        ++taken;
+      } else {
+        e.next[k] = t.rest;
+        t.rest = k;
+      }
+      k = next;
+    }
+  }
+  return t;
+}
+template <typename T, int P>
+__device__ __forceinline__ void patch(float (&z)[Pack<T>::n], const Patches<P>& t, int j) {
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int i0 = t.at[p] - j * Pack<T>::n;
+#pragma unroll
+    for (int i = 0; i < Pack<T>::n; ++i) z[i] = i0 == i ? t.value[p] : z[i];
+  }
+}
 template <typename T>
-__device__ __forceinline__ void store_queued(const Entries& e, T* dx, const LogitRow<T>& r, int lane) {
+__device__ __forceinline__ void store_rest(const Entries& e, T* dx, const LogitRow<T>& r, int rest) {
   asm volatile("" ::: "memory");      // (behind the packs' stores for the compiler too, to which they are another type)
-  for (int k = e.queue[lane]; k >= 0; k = e.next[k]) dx[r.start + e.place[k]] = (T)e.logit[k];
+  for (int k = rest; k >= 0; k = e.next[k]) dx[r.start + e.place[k]] = (T)e.logit[k];
 }
 
 // What the rows leave behind, and what the last block makes of it.
@@ -182,15 +229,18 @@ __device__ __forceinline__ void add_up(const Out& o, tt::Ticket* done, unsigned 
   }
 }
 
-// scale p of a pack's values.  FOLD, for scale > 0: halves, whose rounding hides it, take log2(scale) into the exponent.
-template <typename T, bool FOLD>
-__device__ __forceinline__ Words gradient_pack(const Words& p, float m, float log_s, float c, float scale) {
+// scale p of the values of pack j, and the patches.  FOLD, for scale > 0: halves, whose rounding hides it, take
+// log2(scale) into the exponent.
+template <typename T, bool FOLD, int P>
+__device__ __forceinline__ Words gradient_pack(const Words& p, const Patches<P>& t, int j, float m, float log_s, float c,
+                                               float scale) {
   float z[Pack<T>::n];
   tt::unpack<T>(z, p);
   const float add = log2f(scale) - log_s - tt::rounded(m, c);
 #pragma unroll
   for (int i = 0; i < Pack<T>::n; ++i)
     z[i] = FOLD && sizeof(T) == 2 ? tt::pow2(fmaf(z[i], c, add)) : scale * tt::pow2(tt::bits<T>(z[i], m, c) - log_s);
+  patch<T, P>(z, t, j);
   return tt::pack<T>(z);
 }
 
@@ -269,7 +319,7 @@ __global__ __launch_bounds__(G < kThreads ? kThreads : G, G == 512 ? 4 : 1) void
                                                                            T* dx, const int* __restrict__ count_parts,
                                                                            Scale sc, int R, int V) {
   constexpr int kBlock = G < kThreads ? kThreads : G, kRows = kBlock / G;
-  extern __shared__ float lds[];
+  extern __shared__ __attribute__((aligned(16))) float lds[];
   __shared__ float part[kRows][tt::parts_of(G, 3)];
   __shared__ float more[kRows][tt::parts_of(G, 4)];
   __shared__ double sums[2 * (kBlock / kWave)];
@@ -324,6 +374,7 @@ __global__ __launch_bounds__(G < kThreads ? kThreads : G, G == 512 ? 4 : 1) void
       const bool none = ts.s == 0.f || a.m == -INFINITY;
       const float by = ts.s == ts.s ? scale : ts.s;
       if (!none) queue_entries<T, G>(e, r, all, te.K, lane, a.m, log_s, sc.c, by);
+      const Patches<kPatches<G>> patches = take_queued<T, kPatches<G>>(e, r, lane);
       int own = all.p0 + lane;        // (opaque as the packs are: no address is held from the reads to here)
       asm volatile("" : "+v"(own));
 #pragma unroll
@@ -331,7 +382,7 @@ __global__ __launch_bounds__(G < kThreads ? kThreads : G, G == 512 ? 4 : 1) void
         asm volatile("" : "+v"(kept[u]));
         const int j = own + u * G;
         if (j < all.p1) {
-          const Words q = none ? Words(0u) : gradient_pack<T, true>(kept[u], a.m, log_s, sc.c, by);
+          const Words q = none ? Words(0u) : gradient_pack<T, true>(kept[u], patches, j, a.m, log_s, sc.c, by);
           tt::write_pack(r, dx, j, q);
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -345,10 +396,11 @@ __global__ __launch_bounds__(G < kThreads ? kThreads : G, G == 512 ? 4 : 1) void
 #pragma unroll
           for (int u = 0; u < kPair; ++u)
             if (j + u * G < rest.p1)
-              tt::write_pack(r, dx, j + u * G, none ? Words(0u) : gradient_pack<T, true>(p[u], a.m, log_s, sc.c, by));
+              tt::write_pack(r, dx, j + u * G,
+                             none ? Words(0u) : gradient_pack<T, true>(p[u], patches, j + u * G, a.m, log_s, sc.c, by));
         }
       write_loose<T, G>(x, dx, r, all, lane, none, a.m, log_s, sc.c, by);
-      store_queued(e, dx, r, lane);
+      store_rest(e, dx, r, patches.rest);
     }
     cross = tt::row_sum<G>(cross, more[sub] + tt::parts_of(G, 3) % tt::parts_of(G, 4));
     if (lane == 0) {
@@ -367,7 +419,7 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void distill_split(const T* __restrict__ x, Teacher te, Out o, float* stat_part,
                                                           Scale sc, int splits, int R, int V) {
   constexpr int G = kThreads;
-  extern __shared__ float lds[];
+  extern __shared__ __attribute__((aligned(16))) float lds[];
   __shared__ float part[3 * (G / kWave)];
   __shared__ float more[4 * (G / kWave)];
   __shared__ double sums[2 * (G / kWave)];
@@ -411,7 +463,7 @@ __global__ __launch_bounds__(kThreads) void distill_bwd(const T* __restrict__ x,
                                                         int V) {
   constexpr int kRows = kThreads / G;
   if (ahead && g[0] == 1.f) return;
-  extern __shared__ float lds[];
+  extern __shared__ __attribute__((aligned(16))) float lds[];
   __shared__ float part[kRows][tt::parts_of(G, 3)];
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
   const Entries e = entries_of<G>(lds, te.K, sub);
@@ -430,6 +482,7 @@ __global__ __launch_bounds__(kThreads) void distill_bwd(const T* __restrict__ x,
       read_teacher<T, G>(te, x, r, row, sc.c, lane, e, part[sub]);
       queue_entries<T, G>(e, r, s, te.K, lane, st.x, st.y, sc.c, scale);
     }
+    const Patches<kPatches<G>> patches = take_queued<T, kPatches<G>>(e, r, lane);
     for (int j = s.p0 + lane; j < s.p1; j += kUnroll * G) {
       Words p[kUnroll];
 #pragma unroll
@@ -438,10 +491,11 @@ __global__ __launch_bounds__(kThreads) void distill_bwd(const T* __restrict__ x,
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u)
         if (j + u * G < s.p1)
-          tt::write_pack(r, dx, j + u * G, none ? Words(0u) : gradient_pack<T, false>(p[u], st.x, st.y, sc.c, scale));
+          tt::write_pack(r, dx, j + u * G,
+                         none ? Words(0u) : gradient_pack<T, false>(p[u], patches, j + u * G, st.x, st.y, sc.c, scale));
     }
     write_loose<T, G>(x, dx, r, s, lane, none, st.x, st.y, sc.c, scale);
-    store_queued(e, dx, r, lane);
+    store_rest(e, dx, r, patches.rest);
     tt::sync_row<G>();
   }
 }
