@@ -70,9 +70,7 @@ __device__ __forceinline__ void read_parameters(float (&v)[n], const float* w, i
 template <int G, int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float* part) {
 #pragma unroll
-  for (int off = (G ? G : kWave) / 2; off > 0; off >>= 1)
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], off, kWave);
+  for (int k = 0; k < N; ++k) v[k] = tt::lanes_reduce<(G ? G : kWave)>(v[k], tt::Plus());
   if (G) return;
   const int waves = blockDim.x / kWave;
   part += threadIdx.y * waves * N;
