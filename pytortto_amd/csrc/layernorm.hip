@@ -432,6 +432,7 @@ int forward(const T* x, const float* w, const float* b, T* y, float* mean, float
   if (packs <= 128) TT_LN_FWD(64, 2);
   if (packs <= 192) TT_LN_FWD(64, 3);
   if (packs <= 256) TT_LN_FWD(64, 4);
+  if (sizeof(T) == 4 && packs <= 320) TT_LN_FWD(64, 5);       // 1025 columns 68 -> 55 us at 2^25 values, 1200: 55 -> 51
   if (packs <= 512) TT_LN_FWD(0, 2);
   if (packs <= 768) TT_LN_FWD(0, 3);
   if (packs <= 4096) TT_LN_FWD(0, 4);
@@ -452,10 +453,11 @@ int launch_bwd(const T* x, const T* dy, const float* w, const float* mean, const
                float* db, int R, int D) {
   const int packs = (D + Loose<T>::n - 1) / Loose<T>::n;
   // a row's threads, and as many rows as fill the block, which leaves one set of sums.  (Long rows of halves, whose sums
-  // weigh as much as a dozen of them: blocks of 1024 threads, 8192 columns 65 -> 55 us at 2^25 values; of float32, or
-  // short ones, 512: 1024 columns of halves 46 us, 53 with 1024 threads)
+  // weigh as much as a dozen of them: blocks of 1024 threads, 8192 columns 65 -> 55 us at 2^25 values; and rows of three
+  // waves, five of which leave fewer threads idle than two: 1025 columns 93 -> 78 us.  Of float32, or of other short ones,
+  // 512: 1024 columns of halves 46 us, 53 with 1024 threads)
   const int along = G ? kBwdBlock : (packs + NV * kWave - 1) / (NV * kWave) * kWave;
-  const int fill = sizeof(T) == 2 && along > 256 ? kMostBlock : kBwdBlock;
+  const int fill = sizeof(T) == 2 && (along > 256 || along == 192) ? kMostBlock : kBwdBlock;
   const int rows = G ? kBwdBlock / (G ? G : 1) : along < fill ? fill / along : 1;
   const dim3 block(along, G ? 1 : rows);
   // as many blocks as the device holds at once: more of them would only leave more sums
@@ -490,6 +492,7 @@ int backward(const T* x, const T* dy, const float* w, const float* mean, const f
   if (wide && packs <= 128) TT_LN_BWD(64, 2);
   if (wide && packs <= 192) TT_LN_BWD(64, 3);
   if (packs <= 256) TT_LN_BWD(0, 1);
+  if (wide && packs <= 384) TT_LN_BWD(0, 3);      // (with NV = 2: three waves; 1025 columns 115 -> 85 us, 1536: 90 -> 80)
   if (packs <= (wide ? 512 : 2048)) TT_LN_BWD(0, 2);
   if constexpr (wide) {
     if (packs <= 3072) TT_LN_BWD(0, 3);
