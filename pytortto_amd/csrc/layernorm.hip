@@ -215,7 +215,8 @@ __global__ __launch_bounds__(G ? kBwdBlock : kMostBlock) void ln_bwd(const T* __
     else out[which][c] = s;
   };
   // this block's rows: one sum for each column, pack by pack
-  __shared__ float all[(G || sizeof(T) == 4 ? kBwdBlock : kMostBlock) * n];    // (as many threads as have several rows)
+  __shared__ __attribute__((aligned(16))) float all[(G || sizeof(T) == 4 ? kBwdBlock : kMostBlock) * n];
+  // (values of as many threads as have several rows)
 #pragma unroll
   for (int u = 0; u < 2 * NV; ++u) {
     const int which = u & 1, first = (u >> 1) * stride;
@@ -241,9 +242,28 @@ __global__ __launch_bounds__(G ? kBwdBlock : kMostBlock) void ln_bwd(const T* __
   if (thread == 0) last = tt::last_ticket(&ln_done, gridDim.x);
   __syncthreads();
   if (!last) return;
-  for (int c = thread; c < 2 * D; c += threads) {
+  // as many threads to a column as there are, each with every so manieth block's sum, four on their way
+  double* sums64 = reinterpret_cast<double*>(all);
+  const int ways = 2 * D < threads ? threads / (2 * D) : 1, used = 2 * D < threads ? 2 * D : threads;
+  for (int c0 = 0; c0 < 2 * D; c0 += used) {
+    const int c = c0 + thread % used, way = thread / used;
     double s = 0.0;
-    for (int k = 0; k < (int)gridDim.x; ++k) s += (double)tt::shared(parts + (size_t)k * 2 * D + c);
+    if (way < ways && c < 2 * D)
+      for (int k = way; k < (int)gridDim.x; k += 4 * ways) {
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = 0.f;
+          if (k + i * ways < (int)gridDim.x) v[i] = tt::shared(parts + (size_t)(k + i * ways) * 2 * D + c);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s += (double)v[i];
+      }
+    __syncthreads();
+    sums64[thread] = s;
+    __syncthreads();
+    if (way || c >= 2 * D) continue;
+    for (int k = 1; k < ways; ++k) s += sums64[k * used + thread];
     float* to = c < D ? dw_out : db_out;
     if (to) to[c < D ? c : c - D] = (float)s;
   }
@@ -492,11 +512,15 @@ int backward(const T* x, const T* dy, const float* w, const float* mean, const f
   if (wide && packs <= 128) TT_LN_BWD(64, 2);
   if (wide && packs <= 192) TT_LN_BWD(64, 3);
   if (packs <= 256) TT_LN_BWD(0, 1);
-  if (wide && packs <= 384) TT_LN_BWD(0, 3);      // (with NV = 2: three waves; 1025 columns 115 -> 85 us, 1536: 90 -> 80)
-  if (packs <= (wide ? 512 : 2048)) TT_LN_BWD(0, 2);
+  // (float32: three packs to a thread but where they leave an odd number of waves, of which a unit then holds fewer.  1025
+  // columns 115 us at 2^25 values with two, 85 with three; 3300 columns 101 with three, 86 with four)
   if constexpr (wide) {
+    if (packs > 384 && packs <= 512) TT_LN_BWD(0, 2);
+    if (packs > 768 && packs <= 960) TT_LN_BWD(0, 4);
     if (packs <= 3072) TT_LN_BWD(0, 3);
     if (packs <= 4096) TT_LN_BWD(0, 4);
+  } else {
+    if (packs <= 2048) TT_LN_BWD(0, 2);
   }
 #undef TT_LN_BWD
   hipStream_t st = tt::stream();
