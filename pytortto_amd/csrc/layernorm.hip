@@ -486,7 +486,12 @@ int launch_bwd(const T* x, const T* dy, const float* w, const float* mean, const
   if (per_unit == 0)
     TT_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_unit, ln_bwd<T, G, NV>, block.x * block.y, 0));
   const unsigned grid = grid_for(R, rows, (long long)tt::compute_units() * (per_unit > 0 ? per_unit : 1));
-  const bool sums = dw || db, joins = sums && grid > 1 && (long long)grid * D <= 16384;
+  const bool sums = dw || db;
+  // the last block joins what takes it a few rounds of loads (10 blocks of 1024 columns: 8.7 us, 11.6 with a launch more;
+  // 10 of 1537 columns, in 21 rounds: 16.6 and 11.8)
+  const int threads = block.x * block.y, ways = 2 * D < threads ? threads / (2 * D) : 1;
+  const long long rounds = (2 * (long long)D + threads - 1) / threads * ((grid + 4 * ways - 1) / (4 * ways));
+  const bool joins = sums && grid > 1 && rounds <= 8;
   void* ws = nullptr;
   if (sums && grid > 1)
     if (tt::workspace((size_t)grid * 2 * D * sizeof(float), &ws)) return -1;

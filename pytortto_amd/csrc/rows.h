@@ -1,7 +1,6 @@
-// What the kernels over rows of float32 or float16 values share: layer normalisation (layernorm.hip), token
-// log probabilities and distillation (vocab.hip).  Values are widened to float32 as they are read; sums and
-// statistics are float32 or wider, and a result is rounded once, to its own type, as it is stored.
-//
+// What the kernels over rows of float32 or float16 values share: layer normalisation (layernorm.hip), token log
+// probabilities and distillation (vocab_logp.hip, vocab_distill.hip).  Values are widened to float32 as they are read;
+// sums and statistics are float32 or wider, and a result is rounded once, to its own type, as it is stored.
 #pragma once
 #include "tt_common.h"
 
@@ -12,8 +11,8 @@ namespace tt {
 __device__ __forceinline__ float widen(float v) { return v; }
 __device__ __forceinline__ float widen(_Float16 v) { return (float)v; }
 
-// Sixteen bytes of a row.  They are kept as four words until their values are wanted: as a vector of halves the compiler
-// would give every value a register of its own.
+// Sixteen bytes of a row.  They are kept as four words until their values are wanted: as a vector of halves the
+// compiler would give every value a register of its own.
 typedef unsigned Words __attribute__((ext_vector_type(4)));
 template <typename T>
 struct Pack;
@@ -78,8 +77,8 @@ struct Larger {
   __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
 };
 
-// The value of another lane of the sixteen, by a cross-lane move of the vector unit (a tenth of the time that one through
-// LDS takes): 0xB1 and 0x4E exchange neighbours and pairs, 0x141 and 0x140 mirror eight and sixteen lanes.
+// The value of another lane of the sixteen, by a cross-lane move of the vector unit (a tenth of the time that one
+// through LDS takes): 0xB1 and 0x4E exchange neighbours and pairs, 0x141 and 0x140 mirror eight and sixteen lanes.
 template <int CTRL, typename V>
 __device__ __forceinline__ V across(V v) {
   static_assert(sizeof(V) == 4 || sizeof(V) == 8, "words");

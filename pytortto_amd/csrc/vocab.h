@@ -5,6 +5,8 @@
 //   log p_j = (z_j - m) / temperature - ln S          H = (log2 S - sum_j 2^(d_j) d_j / S) ln 2
 // The pair (m, log2 S) is kept for the backward pass.  The two are not added up: of a row that a mask has left with
 // nothing but the type's lowest value, log2 S would be lost beside m.
+// One pass keeps a thread's maximum and its sums to that maximum.  A thread takes kUnroll packs at a time, so a rescaling
+// costs one exponential for 16 or 32 values, and the sums of G threads are moved to the row's maximum at the end.
 #pragma once
 #include "rows.h"
 
@@ -133,6 +135,15 @@ __device__ __forceinline__ bool add_value(Stat& a, float value, float c) {
 }
 
 constexpr int kUnroll = 4;      // packs that a thread has on their way at once in the streaming loops
+
+// How many blocks of `threads` share a row: as many as come to `fill` for each compute unit, each with `least` packs.
+inline int splits_for(long long R, int packs, int threads, int fill, int least) {
+  long long want = ((long long)fill * compute_units() + R - 1) / R;
+  const long long most = (packs + least - 1) / least;
+  if (want > most) want = most;
+  if (want > threads) want = threads;
+  return want < 1 ? 1 : (int)want;
+}
 
 // The columns outside the whole packs, of which thread `lane` of G takes lane, lane + G, ...
 template <typename T>

@@ -529,19 +529,23 @@ bool by_lanes(int packs, int K) { return packs <= kLanesPacks && K <= kLanesEntr
 
 int packs_for(int V, int dtype) { return dtype == TT_F32 ? (V + 3) / 4 : (V + 7) / 8; }
 
-// How many blocks share a row: as many as fill the device eight times, each with kUnroll packs to a thread at least.
-int splits_for(long long R, int packs) {
-  long long want = (8LL * tt::compute_units() + R - 1) / R;
-  const long long most = (packs + kUnroll * kThreads - 1) / (kUnroll * kThreads);
-  if (want > most) want = most;
-  if (want > kThreads) want = kThreads;
-  return want < 1 ? 1 : (int)want;
+// Rows shared by blocks, as for log probabilities; where the backward pass has more, it has fewer than there, for each
+// block reads the row's teacher (1300 rows of 50021 with 32 entries: 127 -> 115 us; with as many as there 110, but 300 rows
+// of 50021 take 27 us instead of 24).
+int forward_splits(long long R, int packs) {
+  if (packs <= kWavePacks || R > kMostSplitRows) return 1;
+  return tt::splits_for(R, packs, kThreads, 8, kUnroll * kThreads);
+}
+int backward_splits(long long R, int packs) {
+  const int few = tt::splits_for(R, packs, kThreads, 8, kUnroll * kThreads);
+  const int many = tt::splits_for(R, packs, kThreads, 16, 4 * kUnroll * kThreads);
+  return few > many ? few : many;
 }
 
-// A row to a block, or a wave, from this many rows on (two blocks of 1024 threads to a unit); fewer long rows are split.
-bool whole_rows(long long R, int packs) {
-  return packs <= kWavePacks || R >= tt::compute_units() || R > kMostSplitRows;
-}
+// A row to a block, loss and gradient in one visit: while it fits the registers, which saves two launches (20 rows of
+// 10000: 10 us, 15 us shared by blocks), and longer ones from half as many rows as there are units on (140 rows of 131072
+// 42 and 46 us, 80 rows 35 and 33 us).
+bool whole_rows(long long R, int packs) { return packs <= 16 * 512 || 2 * R >= tt::compute_units(); }
 
 // Whether the forward pass writes the gradient too, for an incoming gradient of one: where a row's own block does it
 // (the row is then read once for both), and that gradient is the likely one.  A loss for each row is weighted by its
@@ -602,7 +606,7 @@ int forward(const T* x, const Teacher& te, float* loss, float* stats, float* cou
   hipStream_t st = tt::stream();
   const Scale sc = scale_for(temperature);
   const int packs = (V + Pack<T>::n - 1) / Pack<T>::n;
-  const int splits = whole_rows(R, packs) ? 1 : splits_for(R, packs);
+  const int splits = dx ? 1 : forward_splits(R, packs);
   const size_t blocks = splits > 1 ? R : kMostBlocks * (size_t)tt::compute_units();
   void* ws;
   if (tt::workspace(blocks * 2 * sizeof(double) + (kCountBlocks + (size_t)R * splits * 2) * sizeof(float), &ws)) return -1;
@@ -643,7 +647,7 @@ int backward(const T* x, const Teacher& te, const float* stats, const float* cou
                             entries_bytes<kWave>(te.K, kThreads / kWave), st>>>(
         x, te, (const float2*)stats, count, g, dx, sc, reduction, is_ahead, 1, R, V);
   } else {
-    const int splits = splits_for(R, packs);
+    const int splits = backward_splits(R, packs);
     distill_bwd<T, kThreads><<<grid_for((long long)R * splits, kMostBlocks * tt::compute_units()), kThreads,
                                entries_bytes<kThreads>(te.K, 1), st>>>(
         x, te, (const float2*)stats, count, g, dx, sc, reduction, is_ahead, splits, R, V);

@@ -543,20 +543,25 @@ unsigned row_grid(long long R) {
   return grid_for((R + kThreads / G - 1) / (kThreads / G));
 }
 
-// How many blocks share a row: as many as fill the device eight times, each with kUnroll packs to a thread at least.
-int splits_for(long long R, int packs) {
-  long long want = (8LL * tt::compute_units() + R - 1) / R;
-  const long long most = (packs + kUnroll * kThreads - 1) / (kUnroll * kThreads);
-  if (want > most) want = most;
-  if (want > kThreads) want = kThreads;
-  return want < 1 ? 1 : (int)want;
+// Rows shared by blocks: eight blocks to a compute unit, with kUnroll packs to a thread at least (300 rows of 50021 take
+// 14.2 us, with four or sixteen 14.5 and 15.2; one row of 32768 is read in 7.6 us).
+int forward_splits(long long R, int packs) {
+  if (packs <= kWavePacks || R > kMostSplitRows) return 1;
+  return tt::splits_for(R, packs, kThreads, 8, kUnroll * kThreads);
+}
+// The blocks of the backward pass share nothing, and more of them end more evenly: 32 to a unit, of twice as many packs,
+// where that is more (1300 rows of 50021: 123 -> 98 us; 8000 rows of 8191, which stay whole, take 102 us and would take 107).
+int backward_splits(long long R, int packs) {
+  const int few = tt::splits_for(R, packs, kThreads, 8, kUnroll * kThreads);
+  const int many = tt::splits_for(R, packs, kThreads, 32, 2 * kUnroll * kThreads);
+  return few > many ? few : many;
 }
 
 template <typename T>
 int forward(const T* x, const ForwardOut& o, int R, int V, int K) {
   hipStream_t st = tt::stream();
   const int packs = (V + Pack<T>::n - 1) / Pack<T>::n;
-  const int splits = packs <= kWavePacks || R > kMostSplitRows ? 1 : splits_for(R, packs);
+  const int splits = forward_splits(R, packs);
   if (splits > 1) {
     void* ws;
     const size_t parts = (size_t)R * splits, stat_bytes = (parts * 3 * sizeof(float) + 255) / 256 * 256;
@@ -588,7 +593,7 @@ int backward(const T* x, const BackwardIn& in, T* dx, int R, int V, int K) {
   } else if (packs <= kWavePacks) {
     logp_bwd<T, kWave><<<row_grid<kWave>(R), kThreads, 0, st>>>(x, in, dx, 1, R, V, K);
   } else {
-    const int splits = splits_for(R, packs);
+    const int splits = backward_splits(R, packs);
     logp_bwd<T, kThreads><<<grid_for((long long)R * splits), kThreads, 0, st>>>(x, in, dx, splits, R, V, K);
   }
   TT_LAUNCH_CHECK();
