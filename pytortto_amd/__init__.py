@@ -2,7 +2,8 @@
 
 Mirrors the names of samrere/pytortto that the path sits behind: ``tensor``, ``Tensor``,
 ``manual_seed``, ``randn``/``zeros``/``ones``, ``no_grad``, ``nn.Conv2d``, ``nn.ConvTranspose2d``,
-``nn.BatchNorm2d``, ``nn.functional.conv2d`` / ``conv_transpose2d`` / ``batch_norm``.
+``nn.BatchNorm2d``, ``nn.functional.conv2d`` / ``conv_transpose2d`` / ``batch_norm``; and, for models over a
+vocabulary, ``nn.LayerNorm``, ``nn.functional.token_log_prob`` and ``nn.DistillLoss``.
 ``.cuda()`` moves data into device arrays owned through ``libtortto_hip.so``; every computation
 on them runs in hand-written HIP kernels.  Importing this package does not touch the GPU.
 """

@@ -1,12 +1,17 @@
 // Layer normalisation of rows: y = (x - mean) / sqrt(var + eps) * w + b, its gradient dx and the reductions over the
-// rows that give dw and db.  x, y, dy and dx are float32 or float16, everything else float32.
+// rows that give dw and db. x, y, dy and dx are float32 or float16, everything else float32.
 //
 //   n = (x - mean) rstd,  h = dy w,  dx = rstd (h - mean(h) - n mean(h n)),  dw = sum_rows dy n,  db = sum_rows dy
 //
 // G threads hold a row in registers, NV sixteen-byte packs each, so a row is read once whatever is summed over it: the
-// variance is that of the values less their mean, not a difference of squares.  The backward kernel walks a block's
-// rows and keeps each thread's columns of dw and db in registers on the way; they are added up over the rows of a block
-// in LDS, and over the blocks by ln_join.  Rows longer than the registers hold are read again (the *_long kernels).
+// variance is that of the values less their mean, not a difference of squares. The backward kernel walks a block's rows
+// and keeps each thread's columns of dw and db in registers on the way; they are added up over the rows of a block in
+// LDS, and over the blocks by ln_join. Rows longer than the registers hold are read again (the *_long kernels).
+//
+// Memory bounds them: 2^25 float32 values take 49 to 55 us forward and 79 to 85 us backward (4.9 to 5.5 TB/s, a large
+// copy 5.0 to 5.6) in rows of 24 to 5000; float16 24 to 28 and 44 to 55 us (3.7 to 5.4 TB/s), rows that begin off
+// sixteen bytes up to half as much more. What is left to lose are idle lanes, where a row's packs do not fill its
+// waves, and the blocks' sums.
 #include "rows.h"
 
 namespace {
@@ -65,8 +70,8 @@ __device__ __forceinline__ void read_parameters(float (&v)[n], const float* w, i
   for (int i = 0; i < n; ++i) v[i] = w && q * n + i < D ? w[(size_t)q * n + i] : other;
 }
 
-// Sums of N values over the threads of a row: G of a wave, or (G = 0) the whole waves of one y of the block.  part: LDS of
-// 16 N floats of this call's own.
+// Sums of N values over the threads of a row: G of a wave, or (G = 0) the whole waves of one y of the block.  part: LDS
+// of 16 N floats of this call's own.
 template <int G, int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float* part) {
 #pragma unroll
@@ -142,7 +147,7 @@ __global__ __launch_bounds__(G ? kFwdBlock : kMostBlock) void ln_fwd(const T* __
 
 __device__ tt::Ticket ln_done;     // blocks of a launch that have left their sums: zero between launches
 
-// parts: [blocks][2][D], a block's sums for dw and db (NULL when neither is wanted).  One block writes dw and db itself;
+// parts: [blocks][2][D], a block's sums for dw and db (NULL when neither is wanted). One block writes dw and db itself;
 // of few blocks with few columns (`joins`) the last adds them up, which saves a launch.
 template <typename T, int G, int NV>
 __global__ __launch_bounds__(G ? kBwdBlock : kMostBlock) void ln_bwd(const T* __restrict__ x, const T* __restrict__ dy,
@@ -161,7 +166,8 @@ __global__ __launch_bounds__(G ? kBwdBlock : kMostBlock) void ln_bwd(const T* __
   float sums[2][NV][n] = {};        // dw, db
   float wv[NV][n];
 #pragma unroll
-  for (int u = 0; u < NV; ++u) read_parameters(wv[u], lane + u * stride < all_packs ? w : nullptr, lane + u * stride, D, 1.f);
+  for (int u = 0; u < NV; ++u)
+    read_parameters(wv[u], lane + u * stride < all_packs ? w : nullptr, lane + u * stride, D, 1.f);
   int turn = 0;
   // (all rows of a block go round together, for the barriers: one behind the last has no packs)
   for (long long row0 = (long long)blockIdx.x * rows; row0 < R; row0 += (long long)gridDim.x * rows, turn ^= 1) {
@@ -431,7 +437,8 @@ unsigned grid_for(long long rows, int rows_per_block, long long most) {
 template <typename T, int G, int NV>
 int launch_fwd(const T* x, const float* w, const float* b, T* y, float* mean, float* rstd, float eps, int R, int D) {
   const int packs = (D + Loose<T>::n - 1) / Loose<T>::n;
-  const int block = G ? kFwdBlock : (packs + NV * kWave - 1) / (NV * kWave) * kWave, rows = G ? kFwdBlock / (G ? G : 1) : 1;
+  const int block = G ? kFwdBlock : (packs + NV * kWave - 1) / (NV * kWave) * kWave;
+  const int rows = G ? kFwdBlock / (G ? G : 1) : 1;
   ln_fwd<T, G, NV><<<grid_for(R, rows, 1 << 22), block, 0, tt::stream()>>>(x, w, b, y, mean, rstd, R, D, eps);
   TT_LAUNCH_CHECK();
   return 0;
@@ -472,10 +479,10 @@ template <typename T, int G, int NV>
 int launch_bwd(const T* x, const T* dy, const float* w, const float* mean, const float* rstd, T* dx, float* dw,
                float* db, int R, int D) {
   const int packs = (D + Loose<T>::n - 1) / Loose<T>::n;
-  // a row's threads, and as many rows as fill the block, which leaves one set of sums.  (Long rows of halves, whose sums
-  // weigh as much as a dozen of them: blocks of 1024 threads, 8192 columns 65 -> 55 us at 2^25 values; and rows of three
-  // waves, five of which leave fewer threads idle than two: 1025 columns 93 -> 78 us.  Of float32, or of other short ones,
-  // 512: 1024 columns of halves 46 us, 53 with 1024 threads)
+  // a row's threads, and as many rows as fill the block, which leaves one set of sums. (Long rows of halves, whose sums
+  // weigh as much as a dozen of them: blocks of 1024 threads, 8192 columns 65 -> 55 us at 2^25 values; and rows of
+  // three waves, five of which leave fewer threads idle than two: 1025 columns 93 -> 78 us. Of float32, or of other
+  // short ones, 512: 1024 columns of halves 46 us, 53 with 1024 threads)
   const int along = G ? kBwdBlock : (packs + NV * kWave - 1) / (NV * kWave) * kWave;
   const int fill = sizeof(T) == 2 && (along > 256 || along == 192) ? kMostBlock : kBwdBlock;
   const int rows = G ? kBwdBlock / (G ? G : 1) : along < fill ? fill / along : 1;
@@ -487,8 +494,8 @@ int launch_bwd(const T* x, const T* dy, const float* w, const float* mean, const
     TT_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_unit, ln_bwd<T, G, NV>, block.x * block.y, 0));
   const unsigned grid = grid_for(R, rows, (long long)tt::compute_units() * (per_unit > 0 ? per_unit : 1));
   const bool sums = dw || db;
-  // the last block joins what takes it a few rounds of loads (10 blocks of 1024 columns: 8.7 us, 11.6 with a launch more;
-  // 10 of 1537 columns, in 21 rounds: 16.6 and 11.8)
+  // the last block joins what takes it a few rounds of loads (10 blocks of 1024 columns: 8.7 us, 11.6 with a launch
+  // more; 10 of 1537 columns, in 21 rounds: 16.6 and 11.8)
   const int threads = block.x * block.y, ways = 2 * D < threads ? threads / (2 * D) : 1;
   const long long rounds = (2 * (long long)D + threads - 1) / threads * ((grid + 4 * ways - 1) / (4 * ways));
   const bool joins = sums && grid > 1 && rounds <= 8;
@@ -517,8 +524,8 @@ int backward(const T* x, const T* dy, const float* w, const float* mean, const f
   if (wide && packs <= 128) TT_LN_BWD(64, 2);
   if (wide && packs <= 192) TT_LN_BWD(64, 3);
   if (packs <= 256) TT_LN_BWD(0, 1);
-  // (float32: three packs to a thread but where they leave an odd number of waves, of which a unit then holds fewer.  1025
-  // columns 115 us at 2^25 values with two, 85 with three; 3300 columns 101 with three, 86 with four)
+  // (float32: three packs to a thread but where they leave an odd number of waves, of which a unit then holds fewer.
+  // 1025 columns 115 us at 2^25 values with two, 85 with three; 3300 columns 101 with three, 86 with four)
   if constexpr (wide) {
     if (packs > 384 && packs <= 512) TT_LN_BWD(0, 2);
     if (packs > 768 && packs <= 960) TT_LN_BWD(0, 4);

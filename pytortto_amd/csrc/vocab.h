@@ -5,8 +5,8 @@
 //   log p_j = (z_j - m) / temperature - ln S          H = (log2 S - sum_j 2^(d_j) d_j / S) ln 2
 // The pair (m, log2 S) is kept for the backward pass.  The two are not added up: of a row that a mask has left with
 // nothing but the type's lowest value, log2 S would be lost beside m.
-// One pass keeps a thread's maximum and its sums to that maximum.  A thread takes kUnroll packs at a time, so a rescaling
-// costs one exponential for 16 or 32 values, and the sums of G threads are moved to the row's maximum at the end.
+// One pass keeps a thread's maximum and its sums to that maximum.  A thread takes kUnroll packs at a time, so a
+// rescaling costs one exponential for 16 or 32 values, and the sums of G threads move to the row's maximum at the end.
 #pragma once
 #include "rows.h"
 
@@ -77,8 +77,8 @@ __device__ __forceinline__ float anchor(float m) { return m == -INFINITY ? 0.f :
 // 2^d d where d may be -inf; the clamp changes no product, for 2^-200 is zero.
 __device__ __forceinline__ float floor_at(float d) { return fmaxf(d, -200.f); }
 
-// d of a value, (z - m) c.  Halves cannot overflow z c, and take one instruction for their widening, the product and the
-// difference; every d of a row has the same rounded m c then, which drops out of all that is made of them.
+// d of a value, (z - m) c.  Halves cannot overflow z c, and take one instruction for their widening, the product and
+// the difference; every d of a row has the same rounded m c then, which drops out of all that is made of them.
 __device__ __forceinline__ float rounded(float m, float c) {
 #pragma clang fp contract(off)
   return m * c;
@@ -151,9 +151,9 @@ __device__ __forceinline__ int loose_column(const LogitRow<T>& r, const Share& h
   return i < h.head ? i : r.tail_at + i - h.head;
 }
 
-// A thread's share of a row: packs p0 + lane + i G in ascending order, then its loose columns (PACKS = false: these only).
-// `best` is told the first pack of those, kUnroll at most and G apart, that hold the first of the packs' largest values;
-// kNothing: none is above -inf.
+// A thread's share of a row: packs p0 + lane + i G in ascending order, then its loose columns (PACKS = false: these
+// only).  `best` is told the first pack of those, kUnroll at most and G apart, that hold the first of the packs'
+// largest values; kNothing: none is above -inf.
 constexpr int kNothing = -1;
 
 template <typename T, int G, bool ENTROPY, bool PACKS = true>

@@ -1,6 +1,13 @@
 // Distillation of a student's logits from the K best of a teacher, forward and backward (vocab.h has the statistics):
 //   q = softmax(teacher / T) over a row's entries,  p = softmax(x / T) over all V
 //   loss_r = T^2 sum_k q_k (log q_k - log p_(i_k)),   dx_j = g T (p_j - sum_(k: i_k = j) q_k)
+//
+// Memory bounds them, and the fewest bytes are one read and one write of the row: the gradient for an incoming gradient
+// of one is written in the visit that reads the row for the loss (4096x32768 float32 with 32 entries: 1074 MB in 205
+// us, 5.2 TB/s, where a large copy reaches 5.0 to 5.6).  Of rows longer than registers and LDS hold the rest is read
+// twice (1024x131072 float16 with 64 entries: 604 MB instead of 537, in 121 us, 5.0 TB/s; the vector units are busy for
+// 36 % of that).  Short rows are bound by the latency of their teacher: index, then the logit there (131072 rows of 100
+// with 32 entries: 35 us, 57 with the gradient).
 #include "vocab.h"
 
 namespace {
@@ -203,8 +210,8 @@ __device__ __forceinline__ double write_row(const Out& o, size_t row, const Stat
 // The block's number `at` of `all` is done with its rows.  The one that comes last adds up what they all leave, in 64
 // bits and in an order that the sizes alone decide.  `part` is LDS of 2 BLOCK / 64 values.
 template <int BLOCK>
-__device__ __forceinline__ void add_up(const Out& o, tt::Ticket* done, unsigned at, unsigned all, double loss, double rows,
-                                       double* part) {
+__device__ __forceinline__ void add_up(const Out& o, tt::Ticket* done, unsigned at, unsigned all, double loss,
+                                       double rows, double* part) {
   __shared__ bool last;
   loss = tt::row_sum<BLOCK>(loss, part);
   rows = tt::row_sum<BLOCK>(rows, part + BLOCK / kWave);
@@ -232,8 +239,8 @@ __device__ __forceinline__ void add_up(const Out& o, tt::Ticket* done, unsigned 
 // scale p of the values of pack j, and the patches.  FOLD, for scale > 0: halves, whose rounding hides it, take
 // log2(scale) into the exponent.
 template <typename T, bool FOLD, int P>
-__device__ __forceinline__ Words gradient_pack(const Words& p, const Patches<P>& t, int j, float m, float log_s, float c,
-                                               float scale) {
+__device__ __forceinline__ Words gradient_pack(const Words& p, const Patches<P>& t, int j, float m, float log_s,
+                                               float c, float scale) {
   float z[Pack<T>::n];
   tt::unpack<T>(z, p);
   const float add = log2f(scale) - log_s - tt::rounded(m, c);
@@ -244,8 +251,9 @@ __device__ __forceinline__ Words gradient_pack(const Words& p, const Patches<P>&
   return tt::pack<T>(z);
 }
 
-// The values of NV packs, or the first `packs` of them: their maximum first, then their sum, so that there is no chain of rescaled sums.  The packs are
-// opaque to the compiler in between, which would otherwise hold all their widened values from one loop to the other.
+// The values of NV packs, or the first `packs` of them: their maximum first, then their sum, so that there is no chain
+// of rescaled sums. The packs are opaque to the compiler in between, which would otherwise hold all their widened
+// values from one loop to the other.
 template <typename T, int NV>
 __device__ __forceinline__ void add_kept(Stat& a, Words (&kept)[NV], int packs, float c) {
   constexpr int n = Pack<T>::n;
@@ -306,18 +314,17 @@ __global__ __launch_bounds__(kThreads) void distill_count(Teacher te, int* __res
 
 __device__ tt::Ticket distill_done[1 + tt::kBranches], distill_tickets[kMostSplitRows];
 
-// Of a longer row than the registers hold, LDS takes this many packs more of each thread; the loop over them and what is
-// left has few registers.
+// Of a longer row than the registers hold, LDS takes this many packs more of each thread (1024x131072 float16: 143 us
+// without, 124 with them); the loop over them and what is left has few registers.
 constexpr int kShelf = 8, kPair = 2;
 
-// Rows of G threads each: loss, statistics and, with GRAD, the gradient for an incoming gradient of one.  For that the
+// Rows of G threads each: loss, statistics and, with GRAD, the gradient for an incoming gradient of one. For that the
 // row is kept in registers, NV packs to a thread, and costs one read and one write; of a longer row (LONG) kShelf packs
-// more go to LDS and the rest is read a second time.  For the mean's gradient the rows with a teacher are counted first: by each block, or from
-// `count_parts`.
+// more go to LDS and the rest is read a second time. For the mean's gradient the rows with a teacher are counted first:
+// by each block, or from `count_parts`.
 template <typename T, int G, int NV, bool LONG, bool GRAD>
-__global__ __launch_bounds__(G < kThreads ? kThreads : G, G == 512 ? 4 : 1) void distill_rows(const T* __restrict__ x, Teacher te, Out o,
-                                                                           T* dx, const int* __restrict__ count_parts,
-                                                                           Scale sc, int R, int V) {
+__global__ __launch_bounds__(G < kThreads ? kThreads : G, G == 512 ? 4 : 1) void distill_rows(
+    const T* __restrict__ x, Teacher te, Out o, T* dx, const int* __restrict__ count_parts, Scale sc, int R, int V) {
   constexpr int kBlock = G < kThreads ? kThreads : G, kRows = kBlock / G;
   extern __shared__ __attribute__((aligned(16))) float lds[];
   __shared__ float part[kRows][tt::parts_of(G, 3)];
@@ -519,9 +526,9 @@ int check(const char* fn, int dtype, int teacher_dtype, int index_bits, double t
 constexpr long long kMostBlocks = 16;      // of a launch, to a compute unit; they take rows in turn
 unsigned grid_for(long long blocks, long long most) { return (unsigned)(blocks < most ? blocks : most); }
 
-// Rows of up to kWavePacks packs go to a wave each, which keeps them in registers; four of them share a block's LDS, where
-// the teacher's entries have to fit.  (22369 rows of 3000 in float32 with their gradient: 124 us, by blocks 190 us.)
-// Short ones go to kLanes lanes each: 131072 rows of 100 with 32 entries take 83 us, by waves 310 us.
+// Rows of up to kWavePacks packs go to a wave each, which keeps them in registers; four of them share a block's LDS,
+// where the teacher's entries have to fit. (22369 rows of 3000 in float32 with 32 entries and their gradient: 113 us,
+// by blocks 190.) Short ones go to kLanes lanes each: 131072 rows of 100 with 32 entries take 57 us, by waves 310.
 constexpr int kWavePacks = 16 * kWave, kWaveEntries = 256;
 bool by_waves(int packs, int K) { return packs <= kWavePacks && K <= kWaveEntries; }
 constexpr int kLanes = 16, kLanesPacks = 8 * kLanes, kLanesEntries = 64;
@@ -530,8 +537,8 @@ bool by_lanes(int packs, int K) { return packs <= kLanesPacks && K <= kLanesEntr
 int packs_for(int V, int dtype) { return dtype == TT_F32 ? (V + 3) / 4 : (V + 7) / 8; }
 
 // Rows shared by blocks, as for log probabilities; where the backward pass has more, it has fewer than there, for each
-// block reads the row's teacher (1300 rows of 50021 with 32 entries: 127 -> 115 us; with as many as there 110, but 300 rows
-// of 50021 take 27 us instead of 24).
+// block reads the row's teacher (1300 rows of 50021 with 32 entries: 127 -> 115 us; with as many as there 110, but 300
+// rows of 50021 take 27 us instead of 24).
 int forward_splits(long long R, int packs) {
   if (packs <= kWavePacks || R > kMostSplitRows) return 1;
   return tt::splits_for(R, packs, kThreads, 8, kUnroll * kThreads);
@@ -543,8 +550,8 @@ int backward_splits(long long R, int packs) {
 }
 
 // A row to a block, loss and gradient in one visit: while it fits the registers, which saves two launches (20 rows of
-// 10000: 10 us, 15 us shared by blocks), and longer ones from half as many rows as there are units on (140 rows of 131072
-// 42 and 46 us, 80 rows 35 and 33 us).
+// 10000: 10 us, 15 us shared by blocks), and longer ones from half as many rows as there are units on (140 rows of
+// 131072 42 and 46 us, 80 rows 35 and 33 us).
 bool whole_rows(long long R, int packs) { return packs <= 16 * 512 || 2 * R >= tt::compute_units(); }
 
 // Whether the forward pass writes the gradient too, for an incoming gradient of one: where a row's own block does it
@@ -589,8 +596,8 @@ int launch_rows(const T* x, const Teacher& te, const Out& o, T* dx, const int* c
     distill_rows<T, 512, 16, false, true><<<grid_for(R, most), 512, entries_bytes<512>(te.K, 1), st>>>(
         x, te, o, dx, count_parts, sc, R, V);
   } else {
-    distill_rows<T, 512, 16, true, true><<<grid_for(R, most), 512, entries_bytes<512>(te.K, 1) + kShelf * 512 * 16, st>>>(
-        x, te, o, dx, count_parts, sc, R, V);
+    const size_t lds = entries_bytes<512>(te.K, 1) + kShelf * 512 * sizeof(Words);
+    distill_rows<T, 512, 16, true, true><<<grid_for(R, most), 512, lds, st>>>(x, te, o, dx, count_parts, sc, R, V);
   }
   TT_LAUNCH_CHECK();
   return 0;
@@ -608,21 +615,23 @@ int forward(const T* x, const Teacher& te, float* loss, float* stats, float* cou
   const int packs = (V + Pack<T>::n - 1) / Pack<T>::n;
   const int splits = dx ? 1 : forward_splits(R, packs);
   const size_t blocks = splits > 1 ? R : kMostBlocks * (size_t)tt::compute_units();
+  const size_t words = kCountBlocks + (size_t)R * splits * 2;
   void* ws;
-  if (tt::workspace(blocks * 2 * sizeof(double) + (kCountBlocks + (size_t)R * splits * 2) * sizeof(float), &ws)) return -1;
+  if (tt::workspace(blocks * 2 * sizeof(double) + words * sizeof(float), &ws)) return -1;
   double* sums = (double*)ws;
   int* parts = (int*)(sums + 2 * blocks);
   float* stat_part = (float*)(parts + kCountBlocks);
   const Out o = {reduction == 0 ? loss : nullptr, (float2*)stats, sums, reduction == 0 ? nullptr : loss, count,
                  reduction == 2};
   if (splits > 1) {
-    distill_split<T><<<(unsigned)(R * splits), kThreads, entries_bytes<kThreads>(te.K, 1), st>>>(x, te, o, stat_part, sc,
-                                                                                              splits, R, V);
+    distill_split<T><<<(unsigned)(R * splits), kThreads, entries_bytes<kThreads>(te.K, 1), st>>>(
+        x, te, o, stat_part, sc, splits, R, V);
     TT_LAUNCH_CHECK();
     return 0;
   }
   if (!dx) return launch_rows<T, false>(x, te, o, dx, nullptr, sc, R, V, packs);
-  // a block counts this many rows by itself in the time of a launch
+  // each block counts this many rows by itself in the time of a launch (900 rows of 1000: 10.5 and 12.5 us, 1500 rows:
+  // 13.3 and 12.4)
   const bool counts_itself = R <= 1024;
   if (reduction == 2 && !counts_itself) {
     distill_count<<<kCountBlocks, kThreads, 0, st>>>(te, parts, R, V);

@@ -1,5 +1,11 @@
 // Log probabilities of given tokens, with the entropy and the best alternatives of each row of logits, forward and
 // backward (vocab.h has the formulas).
+//
+// Memory bounds them: the forward pass reads the logits once (4096x32768 float32 in 88 us, 6.1 TB/s, where a plain read
+// reaches 6.2), the backward pass reads them once more and writes as much (2047x50021 float32: 819 MB in 132 us, 6.2
+// TB/s). What little there is to do for a row of a decoding step is bound by latency: reading a share, a ticket,
+// joining the shares (1x32768: 7.4 us, 10.5 with five alternatives; 48x131072 float16 with twenty: 16 us, 7.6 with
+// none).
 #include "vocab.h"
 
 #include <climits>
@@ -23,10 +29,11 @@ constexpr int kMostSplitRows = 2048;    // rows that may be shared by blocks
 // ---- the best alternatives -------------------------------------------------------------------------
 //
 // One pass keeps, beside the sums, each thread's largest value.  Of the G threads' largest values the K-th largest is a
-// bound: K threads reach it, and what no thread's largest value reaches is no candidate.  So the packs of these K owners
-// alone are read again, a few thousand values of a row that has just come through the cache, and what reaches the bound
-// (K values and few more, unless the row is laid out against it) is ranked by counting.  Values and places make keys
-// without ties, so the answer does not depend on the order in which candidates arrive.
+// bound: K threads reach it, and what no thread's largest value reaches is no candidate.  So the packs of these K
+// owners alone are read again, a few thousand values of a row that has just come through the cache, and what reaches
+// the bound (K values and few more, unless the row is laid out against it) is ranked by counting.  Values and places
+// make keys without ties, so the answer does not depend on the order in which candidates arrive.  (1341 rows of 50021
+// in float32: 52 us with no alternatives, 59 with five, 71 with twenty, 110 with 64.)
 
 typedef unsigned long long Key;
 
@@ -46,6 +53,10 @@ __device__ __forceinline__ float key_value(Key k) {
 }
 
 constexpr int most(int a, int b) { return a > b ? a : b; }
+// how many of these lanes come before this one
+__device__ __forceinline__ int lanes_below(unsigned long long who) {
+  return __builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)who, 0));
+}
 
 // More than K owners do no harm; up to this many more may be named, as halves, which are often equal, tend to.
 constexpr int kMore = 32;
@@ -108,8 +119,9 @@ __device__ __forceinline__ Key best_key(const T* x, const LogitRow<T>& r, const 
   return mine;
 }
 
-// Names the owners in s.owner, as many as it returns, and leaves the bound in `bound`.  The K-th largest value is built
-// bit by bit from the top, each time counting the threads that reach it.  Most often K of them alone do after some bits,
+// Names the owners in s.owner, as many as it returns, and leaves the bound in `bound`. The K-th largest value is built
+// bit by bit from the top, each time counting the threads that reach it: some 12 steps of a few scalar instructions,
+// where sorting the threads' values took 21 of exchanges through LDS. Most often K of them alone do after some bits,
 // which is near enough unless K is most of G.
 template <typename T, int G>
 __device__ __forceinline__ int name_owners(TopSpace<G, Pack<T>::n>& s, const T* x, const LogitRow<T>& r, const Share& h,
@@ -140,13 +152,13 @@ __device__ __forceinline__ int name_owners(TopSpace<G, Pack<T>::n>& s, const T* 
     }
   }
   bound = (Key)reach << 32;
-  if (have <= K + kMore || reach == 0) {        // (0: fewer than K threads have values at all, and each of those is an owner)
-    reach = reach ? reach : 1u;
+  if (have <= K + kMore || reach == 0) {
+    reach = reach ? reach : 1u;         // (0: fewer than K threads have values at all, and each of those is an owner)
     int at = 0;
 #pragma unroll
     for (int i = 0; i < kLists; ++i) {
       const unsigned long long who = __ballot(v[i] >= reach);
-      const int slot = at + __builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)who, 0));
+      const int slot = at + lanes_below(who);
       if (v[i] >= reach && lane < kWave) s.owner[slot] = in_wave * kLists + i;
       at += __popcll(who);
     }
@@ -186,13 +198,14 @@ struct Again {
     return step < rounds && j < h.p1 ? j : kNone;
   }
   // Appends the keys that reach the bound.  A wave of its own counts them in a register.
-  static __device__ __forceinline__ void offer(TopSpace<G, n>& s, int& count, bool any, float z, int column, Key bound) {
+  static __device__ __forceinline__ void offer(TopSpace<G, n>& s, int& count, bool any, float z, int column,
+                                               Key bound) {
     const Key k = make_key(z, column);
     const bool is = any && k >= bound;
     if constexpr (G == kWave) {
       const unsigned long long who = __ballot(is);
       if (who == 0) return;
-      const int at = count + __builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)who, 0));
+      const int at = count + lanes_below(who);
       if (is && at < TopSpace<G, n>::room) s.cand[at] = k;
       count += __popcll(who);
     } else if (is) {
@@ -200,8 +213,8 @@ struct Again {
       if (at < TopSpace<G, n>::room) s.cand[at] = k;
     }
   }
-  static __device__ __forceinline__ void collect(TopSpace<G, n>& s, int& count, const T* x, const LogitRow<T>& r, int at,
-                                                 const Words& p, Key bound) {
+  static __device__ __forceinline__ void collect(TopSpace<G, n>& s, int& count, const T* x, const LogitRow<T>& r,
+                                                 int at, const Words& p, Key bound) {
     float z[n];
     tt::unpack<T>(z, p);
 #pragma unroll
@@ -532,25 +545,26 @@ int check(const char* fn, int dtype, int index_bits, long long R, int V, int K) 
 unsigned grid_for(long long blocks) { return (unsigned)(blocks < (1 << 22) ? blocks : (1 << 22)); }
 
 // Rows of up to kWavePacks packs go to a wave each, short ones to some of its lanes, so that a wave has several rows on
-// their way; longer ones go to a block.  Measured on 131072 rows of float32, a wave against eight lanes: of 10 values 60
-// and 9 us, of 300 values 58 and 31 us forward; and backward, where more lanes store wider pieces, 8 against 16 lanes: of
-// 37 values 17 and 25 us, of 100 values 31 and 29 us, of 300 values 105 and 79 us (a wave: 125 us).  67108 rows of 1000
-// are level.  With kWaveTop alternatives and more a block of four times as many threads has a closer bound (22369 rows of
-// 3000 with 64: 1062 us by waves, 205 us by blocks).
+// their way; longer ones go to a block.  131072 rows of float32, a wave against eight lanes: of 10 values 60 and 9 us,
+// of 300 values 58 and 31 us forward; and backward, where more lanes store wider pieces, 8 against 16 lanes: of 37
+// values 17 and 25 us, of 100 values 31 and 29 us, of 300 values 105 and 79 us (a wave: 125 us); 67108 rows of 1000 are
+// level.  With more than kWaveTop alternatives a block, of four times as many threads, has a closer bound (22369 rows
+// of 3000 with 64: 1062 us by waves, 240 us by blocks).
 constexpr int kLanesPacks = 128, kFewPacks = 16, kWavePacks = 1024, kWaveTop = 32;
 template <int G>
 unsigned row_grid(long long R) {
   return grid_for((R + kThreads / G - 1) / (kThreads / G));
 }
 
-// Rows shared by blocks: eight blocks to a compute unit, with kUnroll packs to a thread at least (300 rows of 50021 take
-// 14.2 us, with four or sixteen 14.5 and 15.2; one row of 32768 is read in 7.6 us).
+// Rows shared by blocks: eight blocks to a compute unit, with kUnroll packs to a thread at least (300 rows of 50021
+// take 14.2 us, with four or sixteen 14.5 and 15.2; one row of 32768 is read in 7.6 us).
 int forward_splits(long long R, int packs) {
   if (packs <= kWavePacks || R > kMostSplitRows) return 1;
   return tt::splits_for(R, packs, kThreads, 8, kUnroll * kThreads);
 }
-// The blocks of the backward pass share nothing, and more of them end more evenly: 32 to a unit, of twice as many packs,
-// where that is more (1300 rows of 50021: 123 -> 98 us; 8000 rows of 8191, which stay whole, take 102 us and would take 107).
+// The blocks of the backward pass share nothing, and more of them end more evenly: 32 to a unit, of twice as many
+// packs, where that is more (1300 rows of 50021: 123 -> 98 us; 8000 rows of 8191, which stay whole, take 102 us and
+// would take 107).
 int backward_splits(long long R, int packs) {
   const int few = tt::splits_for(R, packs, kThreads, 8, kUnroll * kThreads);
   const int many = tt::splits_for(R, packs, kThreads, 32, 2 * kUnroll * kThreads);
