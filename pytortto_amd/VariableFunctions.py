@@ -49,8 +49,7 @@ def as_tensor(data, requires_grad=False):
     copy; see ``hiparray.borrow`` for what its owner has to keep to.  Tensors come back as they are."""
     if isinstance(data, Tensor):
         return data
-    array = hiparray.borrow(data)
-    out = Tensor(array, dtype=array._dtype)
+    out = Tensor.on(hiparray.borrow(data))
     if requires_grad:
         out.requires_grad = True
     return out

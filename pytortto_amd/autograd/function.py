@@ -63,6 +63,15 @@ class BackwardFunction(FunctionBase):
 
 
 class AccumulateGrad(BackwardFunction):
+    next_functions = ()
+    done = False        # its gradient of this pass is where it belongs
+
+    def accumulate(self, g):
+        self.grad[0] = g
+        self.apply(g)
+        self.grad[0] = None
+        self.done = True
+
     def apply(self, *args):
         """function.py:70-93: first gradient is stored (contiguous), later ones are added."""
         var = self.variable
@@ -92,9 +101,8 @@ def _link(t, grad_fn, output_idx):
     if grad_fn is None:             # leaf: gradients end in an accumulator
         acc = AccumulateGrad()
         acc.variable = t
-        acc.prev_function_counts += 1
+        acc.prev_function_counts = 1
         acc.grad = [None]
-        acc.next_functions = tuple()
         return acc, 0
     grad_fn.prev_function_counts += 1
     return grad_fn, output_idx
@@ -201,7 +209,13 @@ def build_links(data, grad_fn, copy=False, _output_idx=0):
     global _Tensor
     if _Tensor is None:                 # tensor.py imports this module's users
         from ..tensor import Tensor as _Tensor
-    dtype = data._dtype if data.__class__ is xparray.hiparray else getattr(data, 'dtype', None)
+    if data.__class__ is xparray.hiparray:
+        if grad_fn.requires_grad and grad_mode._enabled:
+            if grad_fn.sources is not None:
+                grad_fn.hang()
+            return _Tensor.on(data, True, grad_fn, _output_idx)
+        return _Tensor.on(data)
+    dtype = getattr(data, 'dtype', None)
     if grad_fn.requires_grad and grad_mode._enabled:
         grad_fn.hang()
         return _Tensor(data, requires_grad=True, dtype=dtype, copy=copy, grad_fn=grad_fn, _output_idx=_output_idx)
@@ -221,7 +235,9 @@ def toposort(*end_nodes):
             if fn is None:
                 continue
             fn.prev_function_counts -= 1
-            if fn.prev_function_counts == 0:
+            if fn.__class__ is AccumulateGrad and fn.done:
+                fn.done = False
+            elif fn.prev_function_counts == 0:
                 ready.append(fn)
                 waiting.discard(fn)
             else:

@@ -32,6 +32,14 @@ class Tensor:
         self._requires_grad = requires_grad
         self._output_idx = kwargs.get('_output_idx')
 
+    @classmethod
+    def on(cls, array, requires_grad=False, grad_fn=None, output_idx=None):
+        """A tensor on a device array as it is."""
+        self = cls.__new__(cls)
+        self.data, self.grad, self.grad_fn, self._requires_grad, self._output_idx = \
+            array, None, grad_fn, requires_grad, output_idx
+        return self
+
     # ---- properties --------------------------------------------------------------------------
     @property
     def _version(self):
@@ -238,14 +246,23 @@ def _add_gradient(fn, idx, g):
         fn.grad[idx] += g
 
 
+_graph = None
+
+
 def _propagate(end_nodes):
-    from .autograd.helper import toposort
-    for node in toposort(*end_nodes):
+    global _graph
+    if _graph is None:                  # function.py's users import this module
+        from .autograd import function as _graph
+    for node in _graph.toposort(*end_nodes):
         grads = node.apply(*node.grad)
-        for i, (fn, idx) in enumerate(node.next_functions):   # empty for leaf accumulators
-            g = grads[i]
-            if g is not None:
-                _add_gradient(fn, idx, g)
+        if grads is not None:           # (a leaf's accumulator returns nothing)
+            for (fn, idx), g in zip(node.next_functions, grads):
+                if g is None:
+                    continue
+                if fn.__class__ is _graph.AccumulateGrad and fn.prev_function_counts == 1:
+                    fn.accumulate(g)    # nothing else leads there: not a node to wait for
+                else:
+                    _add_gradient(fn, idx, g)
         node.clear()
 
 

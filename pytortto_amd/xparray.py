@@ -273,18 +273,20 @@ class hiparray:
         in front of the library's stream, before the array is used.  The memory must not be given to others before what
         reads it here is done, and it is borrowed once, not as two arrays."""
         about = source.__cuda_array_interface__
-        shape, kind = tuple(about['shape']), about['typestr']
-        dtype = _DTYPES.get(kind)
-        if dtype is None:
-            dtype = _DTYPES[kind] = np.dtype(kind)
-        nbytes = prod(shape) * dtype.itemsize
-        if about.get('mask') is not None:
+        shape, kind, get = tuple(about['shape']), about['typestr'], about.get
+        known = _DTYPES.get(kind)
+        if known is None:
+            known = np.dtype(kind)
+            known = _DTYPES[kind] = known, known.itemsize
+        dtype, itemsize = known
+        nbytes = prod(shape) * itemsize
+        if get('mask') is not None:
             raise ValueError('borrowed device memory cannot be masked')
-        if about.get('stream') is not None:
+        if get('stream') is not None:
             _hip.call('tt_wait_stream', about['stream'])
-        strides = about.get('strides')
+        strides = get('strides')
         if strides is not None and nbytes:
-            whole = dtype.itemsize
+            whole = itemsize
             for n, step in zip(reversed(shape), reversed(strides)):
                 if n != 1 and step != whole:
                     raise ValueError(f'device arrays are C-contiguous, got strides {tuple(strides)} for shape {shape}')
