@@ -46,6 +46,10 @@ __device__ __forceinline__ unsigned order_of(float z) {
 __device__ __forceinline__ Key make_key(float z, int place) {
   return ((Key)order_of(z) << 32) | (0xffffffffu - (unsigned)place);
 }
+// The value that a bound of keys has at least.  (Orders below that of -inf belong to no value.)
+__device__ __forceinline__ float least_value(unsigned order) {
+  return order <= 0x007fffffu ? -INFINITY : __uint_as_float(order ^ ((order >> 31) ? 0x80000000u : 0xffffffffu));
+}
 __device__ __forceinline__ int key_place(Key k) { return (int)(0xffffffffu - (unsigned)k); }
 __device__ __forceinline__ float key_value(Key k) {
   const unsigned order = (unsigned)(k >> 32);
@@ -119,14 +123,32 @@ __device__ __forceinline__ Key best_key(const T* x, const LogitRow<T>& r, const 
   return mine;
 }
 
-// Names the owners in s.owner, as many as it returns, and leaves the bound in `bound`. The K-th largest value is built
-// bit by bit from the top, each time counting the threads that reach it: some 12 steps of a few scalar instructions,
-// where sorting the threads' values took 21 of exchanges through LDS. Most often K of them alone do after some bits,
-// which is near enough unless K is most of G.
+// What K of the numbers reach, LISTS of a lane: built bit by bit from the top, each time counting those that reach it, some
+// 12 steps of a few scalar instructions, where sorting them took 21 of exchanges through LDS.  `have` is how many do: K
+// alone do most often after some bits, which is near enough unless K is most of them.
+template <typename T, int LISTS>
+__device__ __forceinline__ unsigned reached_by(const unsigned (&v)[LISTS], int K, int& have) {
+  constexpr int kLowest = sizeof(T) == 2 ? 13 : 0;     // (a widened half has 13 bits alike below)
+  unsigned reach = 0;
+  have = LISTS * kWave;
+  for (int bit = 31; bit >= kLowest && (have != K || 2 * K > LISTS * kWave); --bit) {
+    const unsigned next = reach | 1u << bit;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < LISTS; ++i) n += __popcll(__ballot(v[i] >= next));
+    if (n >= K) {
+      reach = next;
+      have = n;
+    }
+  }
+  return reach;
+}
+
+// Names the owners in s.owner, as many as it returns, and leaves the bound in `bound`.
 template <typename T, int G>
 __device__ __forceinline__ int name_owners(TopSpace<G, Pack<T>::n>& s, const T* x, const LogitRow<T>& r, const Share& h,
                                            int lane, float largest, int best, int K, Key& bound) {
-  constexpr int kLists = G / kWave, kLowest = sizeof(T) == 2 ? 13 : 0;     // (a widened half has 13 bits alike below)
+  constexpr int kLists = G / kWave;
   const int in_wave = lane & (kWave - 1);
   const bool any = h.p0 + lane < h.p1 || lane < h.head + h.tail;
   const unsigned own = any ? order_of(largest) : 0u;
@@ -139,18 +161,8 @@ __device__ __forceinline__ int name_owners(TopSpace<G, Pack<T>::n>& s, const T* 
     const uint4 all = *reinterpret_cast<const uint4*>(&s.largest[in_wave * kLists]);
     v[0] = all.x, v[1] = all.y, v[2] = all.z, v[3] = all.w;
   }
-  unsigned reach = 0;
-  int have = G;
-  for (int bit = 31; bit >= kLowest && (have != K || 2 * K > G); --bit) {
-    const unsigned next = reach | 1u << bit;
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < kLists; ++i) n += __popcll(__ballot(v[i] >= next));
-    if (n >= K) {
-      reach = next;
-      have = n;
-    }
-  }
+  int have;
+  unsigned reach = reached_by<T, kLists>(v, K, have);
   bound = (Key)reach << 32;
   if (have <= K + kMore || reach == 0) {
     reach = reach ? reach : 1u;         // (0: fewer than K threads have values at all, and each of those is an owner)
@@ -271,6 +283,39 @@ __device__ __forceinline__ void select_top(TopSpace<G, Pack<T>::n>& s, const T* 
   rank_candidates(s, lane, count, K);
 }
 
+// The same for a row that a wave keeps in registers, `kept` packs and one loose value to a lane: all that reach the bound
+// are at hand, and nothing is read again.
+template <typename T, int NV>
+__device__ __forceinline__ void select_kept(TopSpace<kWave, Pack<T>::n>& s, const T* x, const LogitRow<T>& r,
+                                            const Share& h, int lane, const Words (&kept)[NV], float loose, float largest,
+                                            int best, int K) {
+  constexpr int n = Pack<T>::n;
+  const bool any = h.p0 + lane < h.p1 || lane < h.head + h.tail;
+  const unsigned v[1] = {any ? order_of(largest) : 0u};
+  int have, count = 0;
+  const float least = least_value(reached_by<T, 1>(v, K, have));
+  auto offer = [&](bool is, float z, int column) {
+    const unsigned long long who = __ballot(is);
+    if (who == 0) return;
+    const int at = count + lanes_below(who);
+    if (is && at < TopSpace<kWave, n>::room) s.cand[at] = make_key(z, column);
+    count += __popcll(who);
+  };
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    const int j = h.p0 + lane + u * kWave;
+    const bool has = j < h.p1 && tt::pack_max<T, 1>(&kept[u]) >= least;
+    if (__ballot(has) == 0) continue;
+    float z[n];
+    tt::unpack<T>(z, kept[u]);
+#pragma unroll
+    for (int i = 0; i < n; ++i) offer(has && z[i] >= least, z[i], r.column(j) + i);
+  }
+  offer(lane < h.head + h.tail && loose >= least, loose, tt::loose_column(r, h, lane));
+  if (count > TopSpace<kWave, n>::room) return select_top<T, kWave>(s, x, r, h, lane, largest, best, K);
+  rank_candidates(s, lane, count, K);
+}
+
 // The K best of `splits` sorted lists of K keys.  The list whose head has rank i holds at most K - i of them, and those
 // reach the K-th head: at most K (K + 1) / 2 candidates.
 template <int G, int n>
@@ -351,29 +396,48 @@ __device__ __forceinline__ void write_row(const ForwardOut& o, size_t row, int l
   }
 }
 
-template <typename T, int G, bool TOP>
+// NV > 0: a wave keeps its row, NV packs to a lane.
+template <typename T, int G, bool TOP, int NV = 0>
 __global__ __launch_bounds__(kThreads) void logp_rows(const T* __restrict__ x, ForwardOut o, int R, int V, int K) {
-  constexpr int kRows = kThreads / G;
+  constexpr int kRows = kThreads / G, kKept = NV < kUnroll ? NV : kUnroll;      // (of a lane's packs taken together)
   __shared__ float part[kRows][tt::parts_of(G, 3)];
   __shared__ std::conditional_t<TOP, TopSpace<G, Pack<T>::n>, NoSpace> space[kRows];
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
   const float c = (float)tt::kLog2e;
   for (long long row = (long long)blockIdx.x * kRows + sub; row < R; row += (long long)gridDim.x * kRows) {
+    const LogitRow<T> r(x, row, V);
+    const Share h(r, 0, 1);
+    Words kept[NV ? NV : 1];            // (on their way together with the token)
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      kept[u] = Words(Pack<T>::lowest);
+      if (h.p0 + lane + u * G < h.p1) kept[u] = r.pack(h.p0 + lane + u * G);
+    }
+    float loose = -INFINITY;
+    if (NV > 0 && lane < h.head + h.tail) loose = tt::widen(x[r.start + tt::loose_column(r, h, lane)]);
     const long long t0 = tt::read_index(o.tokens, row, o.wide);
     if (t0 == o.ignored) {
       write_ignored<G>(o, row, lane, K);
       continue;
     }
-    const LogitRow<T> r(x, row, V);
-    const Share h(r, 0, 1);
     const long long t = token_place(t0, V);
     const float z_token = lane == 0 && t >= 0 ? tt::widen(x[r.start + t]) : 0.f;
     Stat a = {-INFINITY, 0.f, 0.f};
     int best = tt::kNothing;
-    tt::scan<T, G, true>(a, best, x, r, h, lane, c);
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int u = 0; u < NV; u += kKept)
+        if (h.p0 + u * G < h.p1 && tt::add_packs<T, kKept, true>(a, kept + u, c)) best = h.p0 + lane + u * G;
+      tt::add_value<T, true>(a, loose, c);
+    } else {
+      tt::scan<T, G, true>(a, best, x, r, h, lane, c);
+    }
     const float largest = a.m;
     a = tt::row_join<T, G, true>(a, c, part[sub]);
-    if constexpr (TOP) {
+    if constexpr (NV > 0) {
+      select_kept<T, NV>(space[sub], x, r, h, lane, kept, loose, largest, best, K);
+      write_row<T, G>(o, row, lane, a, t >= 0, z_token, space[sub].best, K);
+    } else if constexpr (TOP) {
       select_top<T, G>(space[sub], x, r, h, lane, largest, best, K);
       write_row<T, G>(o, row, lane, a, t >= 0, z_token, space[sub].best, K);
     } else {
@@ -586,8 +650,11 @@ int forward(const T* x, const ForwardOut& o, int R, int V, int K) {
   } else if (packs <= kLanesPacks && K == 0) {
     logp_rows<T, 8, false><<<row_grid<8>(R), kThreads, 0, st>>>(x, o, R, V, K);
   } else if (packs <= kWavePacks && K <= kWaveTop) {
-    if (K) logp_rows<T, kWave, true><<<row_grid<kWave>(R), kThreads, 0, st>>>(x, o, R, V, K);
-    else logp_rows<T, kWave, false><<<row_grid<kWave>(R), kThreads, 0, st>>>(x, o, R, V, K);
+    const unsigned grid = row_grid<kWave>(R);
+    if (K && packs <= 2 * kWave) logp_rows<T, kWave, true, 2><<<grid, kThreads, 0, st>>>(x, o, R, V, K);
+    else if (K && packs <= 4 * kWave) logp_rows<T, kWave, true, 4><<<grid, kThreads, 0, st>>>(x, o, R, V, K);
+    else if (K) logp_rows<T, kWave, true><<<grid, kThreads, 0, st>>>(x, o, R, V, K);
+    else logp_rows<T, kWave, false><<<grid, kThreads, 0, st>>>(x, o, R, V, K);
   } else {
     if (K) logp_rows<T, kThreads, true><<<grid_for(R), kThreads, 0, st>>>(x, o, R, V, K);
     else logp_rows<T, kThreads, false><<<grid_for(R), kThreads, 0, st>>>(x, o, R, V, K);
