@@ -66,6 +66,13 @@ __device__ __forceinline__ void sync_row() {
   }
 }
 
+// Which row of its block a thread works on; the compiler is told where that is the same for a whole wave.
+template <int G>
+__device__ __forceinline__ int row_of_block() {
+  const int sub = threadIdx.x / G;
+  return G < kWave ? sub : __builtin_amdgcn_readfirstlane(sub);
+}
+
 // Waits until this wave's stores have left for memory.
 __device__ __forceinline__ void stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 

@@ -330,7 +330,7 @@ __global__ __launch_bounds__(G < kThreads ? kThreads : G, G == 512 ? 4 : 1) void
   __shared__ float part[kRows][tt::parts_of(G, 3)];
   __shared__ float more[kRows][tt::parts_of(G, 4)];
   __shared__ double sums[2 * (kBlock / kWave)];
-  const int lane = threadIdx.x % G, sub = threadIdx.x / G;
+  const int lane = threadIdx.x % G, sub = tt::row_of_block<G>();
   Words* shelf = reinterpret_cast<Words*>(lds);
   const Entries e = entries_of<G>(lds + (LONG && GRAD ? kShelf * G * 4 : 0), te.K, sub);
   double losses = 0.0, rows = 0.0;
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(kThreads) void distill_bwd(const T* __restrict__ x,
   if (ahead && g[0] == 1.f) return;
   extern __shared__ __attribute__((aligned(16))) float lds[];
   __shared__ float part[kRows][tt::parts_of(G, 3)];
-  const int lane = threadIdx.x % G, sub = threadIdx.x / G;
+  const int lane = threadIdx.x % G, sub = tt::row_of_block<G>();
   const Entries e = entries_of<G>(lds, te.K, sub);
   const long long items = (long long)R * splits;
   for (long long item = (long long)blockIdx.x * kRows + sub; item < items; item += (long long)gridDim.x * kRows) {

@@ -402,7 +402,7 @@ __global__ __launch_bounds__(kThreads) void logp_rows(const T* __restrict__ x, F
   constexpr int kRows = kThreads / G, kKept = NV < kUnroll ? NV : kUnroll;      // (of a lane's packs taken together)
   __shared__ float part[kRows][tt::parts_of(G, 3)];
   __shared__ std::conditional_t<TOP, TopSpace<G, Pack<T>::n>, NoSpace> space[kRows];
-  const int lane = threadIdx.x % G, sub = threadIdx.x / G;
+  const int lane = threadIdx.x % G, sub = tt::row_of_block<G>();
   const float c = (float)tt::kLog2e;
   for (long long row = (long long)blockIdx.x * kRows + sub; row < R; row += (long long)gridDim.x * kRows) {
     const LogitRow<T> r(x, row, V);
@@ -532,7 +532,7 @@ template <typename T, int G>
 __global__ __launch_bounds__(kThreads) void logp_bwd(const T* __restrict__ x, BackwardIn in, T* dx, int splits, int R,
                                                      int V, int K) {
   constexpr int kRows = kThreads / G, n = Pack<T>::n;
-  const int lane = threadIdx.x % G, sub = threadIdx.x / G;
+  const int lane = threadIdx.x % G, sub = tt::row_of_block<G>();
   const long long items = (long long)R * splits;
   for (long long item = (long long)blockIdx.x * kRows + sub; item < items; item += (long long)gridDim.x * kRows) {
     const size_t row = R - 1 - item / splits;
