@@ -101,7 +101,8 @@ __global__ __launch_bounds__(G ? kFwdBlock : kMostBlock) void ln_fwd(const T* __
   constexpr int n = Loose<T>::n, kRows = G ? kFwdBlock / (G ? G : 1) : 1;
   typedef typename Loose<T>::type P;
   __shared__ float part[2][G ? 1 : kMostBlock / kWave];
-  const int stride = G ? G : (int)blockDim.x, lane = threadIdx.x % stride, sub = G ? threadIdx.x / stride : 0;
+  const int stride = G ? G : (int)blockDim.x, lane = threadIdx.x % stride;
+  const int sub = G ? tt::row_of_block<G ? G : 1>() : 0;
   const int packs = (D + n - 1) / n;
   for (long long row = (long long)blockIdx.x * kRows + sub; row < R; row += (long long)gridDim.x * kRows) {
     const T* __restrict__ p = x + row * (size_t)D;
@@ -160,7 +161,8 @@ __global__ __launch_bounds__(G ? kBwdBlock : kMostBlock) void ln_bwd(const T* __
   typedef typename Loose<T>::type P;
   __shared__ float part[2][G ? 1 : 2 * (kMostBlock / kWave)];
   const int stride = G ? G : (int)blockDim.x, rows = G ? kBwdBlock / (G ? G : 1) : (int)blockDim.y;
-  const int lane = G ? threadIdx.x % stride : threadIdx.x, sub = G ? threadIdx.x / stride : threadIdx.y;
+  const int lane = G ? threadIdx.x % stride : threadIdx.x;
+  const int sub = G ? tt::row_of_block<G ? G : 1>() : __builtin_amdgcn_readfirstlane(threadIdx.y);
   const int thread = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
   const int all_packs = (D + n - 1) / n;
   float sums[2][NV][n] = {};        // dw, db
