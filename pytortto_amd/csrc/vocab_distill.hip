@@ -23,7 +23,7 @@ using tt::Words;
 
 constexpr int kThreads = 256;
 constexpr int kMostTeacher = 1024;
-constexpr int kMostSplitRows = 2048;    // rows that may be shared by blocks
+constexpr int kMostSplitRows = 255;     // rows that may be shared by blocks
 
 struct Teacher {
   const void* logits;
@@ -536,13 +536,15 @@ bool by_lanes(int packs, int K) { return packs <= kLanesPacks && K <= kLanesEntr
 
 int packs_for(int V, int dtype) { return dtype == TT_F32 ? (V + 3) / 4 : (V + 7) / 8; }
 
-// Rows shared by blocks, as for log probabilities; where the backward pass has more, it has fewer than there, for each
-// block reads the row's teacher (1300 rows of 50021 with 32 entries: 127 -> 115 us; with as many as there 110, but 300
-// rows of 50021 take 27 us instead of 24).
+// Rows shared by blocks, where they are fewer than units: the block that joins a row reads its teacher last. (300 rows
+// of 50021 take 15.8 us whole and 17.8 shared, 512 of 131072 49 and 54; 100 of 131072 25 and 16 us.)
 int forward_splits(long long R, int packs) {
   if (packs <= kWavePacks || R > kMostSplitRows) return 1;
   return tt::splits_for(R, packs, kThreads, 8, kUnroll * kThreads);
 }
+// Where the backward pass has more than those, it has fewer than that of log probabilities, for each block reads the
+// row's teacher (1300 rows of 50021 with 32 entries: 127 -> 115 us; with as many as there 110, but 300 rows of 50021
+// take 27 us instead of 24).
 int backward_splits(long long R, int packs) {
   const int few = tt::splits_for(R, packs, kThreads, 8, kUnroll * kThreads);
   const int many = tt::splits_for(R, packs, kThreads, 16, 4 * kUnroll * kThreads);

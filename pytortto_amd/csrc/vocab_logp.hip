@@ -123,9 +123,9 @@ __device__ __forceinline__ Key best_key(const T* x, const LogitRow<T>& r, const 
   return mine;
 }
 
-// What K of the numbers reach, LISTS of a lane: built bit by bit from the top, each time counting those that reach it, some
-// 12 steps of a few scalar instructions, where sorting them took 21 of exchanges through LDS.  `have` is how many do: K
-// alone do most often after some bits, which is near enough unless K is most of them.
+// What K of the numbers reach, LISTS of a lane: built bit by bit from the top, each time counting those that reach it,
+// some 12 steps of a few scalar instructions, where sorting them took 21 of exchanges through LDS. `have` is how many
+// do: K alone do most often after some bits, which is near enough unless K is most of them.
 template <typename T, int LISTS>
 __device__ __forceinline__ unsigned reached_by(const unsigned (&v)[LISTS], int K, int& have) {
   constexpr int kLowest = sizeof(T) == 2 ? 13 : 0;     // (a widened half has 13 bits alike below)
@@ -283,8 +283,8 @@ __device__ __forceinline__ void select_top(TopSpace<G, Pack<T>::n>& s, const T* 
   rank_candidates(s, lane, count, K);
 }
 
-// The same for a row that a wave keeps in registers, `kept` packs and one loose value to a lane: all that reach the bound
-// are at hand, and nothing is read again.
+// The same for a row that a wave keeps in registers, `kept` packs and one loose value to a lane: all that reach the
+// bound are at hand, and nothing is read again.
 template <typename T, int NV>
 __device__ __forceinline__ void select_kept(TopSpace<kWave, Pack<T>::n>& s, const T* x, const LogitRow<T>& r,
                                             const Share& h, int lane, const Words (&kept)[NV], float loose, float largest,
