@@ -540,7 +540,7 @@ int packs_for(int V, int dtype) { return dtype == TT_F32 ? (V + 3) / 4 : (V + 7)
 // of 50021 take 15.8 us whole and 17.8 shared, 512 of 131072 49 and 54; 100 of 131072 25 and 16 us.)
 int forward_splits(long long R, int packs) {
   if (packs <= kWavePacks || R > kMostSplitRows) return 1;
-  return tt::splits_for(R, packs, kThreads, 8, kUnroll * kThreads);
+  return tt::splits_for(R, packs, kThreads, 2, kUnroll * kThreads);
 }
 // Where the backward pass has more than those, it has fewer than that of log probabilities, for each block reads the
 // row's teacher (1300 rows of 50021 with 32 entries: 127 -> 115 us; with as many as there 110, but 300 rows of 50021

@@ -24,7 +24,7 @@ using tt::Words;
 constexpr int kThreads = 256;
 constexpr tt::Scale kPlain = {(float)tt::kLog2e, 1.f, 1.f};
 constexpr int kMostTop = 64;
-constexpr int kMostSplitRows = 2048;    // rows that may be shared by blocks
+constexpr int kMostSplitRows = 255;     // rows that may be shared by blocks
 
 // ---- the best alternatives -------------------------------------------------------------------------
 //
@@ -620,11 +620,12 @@ unsigned row_grid(long long R) {
   return grid_for((R + kThreads / G - 1) / (kThreads / G));
 }
 
-// Rows shared by blocks: eight blocks to a compute unit, with kUnroll packs to a thread at least (300 rows of 50021
-// take 14.2 us, with four or sixteen 14.5 and 15.2; one row of 32768 is read in 7.6 us).
+// Rows shared by blocks, where they are fewer than units: two blocks to a unit, with kUnroll packs to a thread at least
+// (200 rows of 50021 with twenty alternatives take 19 us, with eight blocks to a unit 25; 1000 rows of 9000 with ten 14
+// us whole and 25 shared by two; one row of 32768 is read in 7.6 us, 100 of 131072 in 13, 24 if they stay whole).
 int forward_splits(long long R, int packs) {
   if (packs <= kWavePacks || R > kMostSplitRows) return 1;
-  return tt::splits_for(R, packs, kThreads, 8, kUnroll * kThreads);
+  return tt::splits_for(R, packs, kThreads, 2, kUnroll * kThreads);
 }
 // The blocks of the backward pass share nothing, and more of them end more evenly: 32 to a unit, of twice as many
 // packs, where that is more (1300 rows of 50021: 123 -> 98 us; 8000 rows of 8191, which stay whole, take 102 us and
