@@ -5,8 +5,8 @@
 // Memory bounds them, and the fewest bytes are one read and one write of the row: the gradient for an incoming gradient
 // of one is written in the visit that reads the row for the loss (4096x32768 float32 with 32 entries: 1074 MB in 205
 // us, 5.2 TB/s, where a large copy reaches 5.0 to 5.6).  Of rows longer than registers and LDS hold the rest is read
-// twice (1024x131072 float16 with 64 entries: 604 MB instead of 537, in 121 us, 5.0 TB/s; the vector units are busy for
-// 36 % of that).  Short rows are bound by the latency of their teacher: index, then the logit there (131072 rows of 100
+// twice (1024x131072 float16 with 64 entries: 604 MB instead of 537, in 115 us, 5.2 TB/s; the vector units are busy for
+// 38 % of that).  Short rows are bound by the latency of their teacher: index, then the logit there (131072 rows of 100
 // with 32 entries: 35 us, 57 with the gradient).
 #include "vocab.h"
 

@@ -2,9 +2,9 @@
 // backward (vocab.h has the formulas).
 //
 // Memory bounds them: the forward pass reads the logits once (4096x32768 float32 in 88 us, 6.1 TB/s, where a plain read
-// reaches 6.2), the backward pass reads them once more and writes as much (2047x50021 float32: 819 MB in 132 us, 6.2
+// reaches 6.2), the backward pass reads them once more and writes as much (2047x50021 float32: 819 MB in 136 us, 6.0
 // TB/s). What little there is to do for a row of a decoding step is bound by latency: reading a share, a ticket,
-// joining the shares (1x32768: 7.4 us, 10.5 with five alternatives; 48x131072 float16 with twenty: 16 us, 7.6 with
+// joining the shares (1x32768: 7.4 us, 10.5 with five alternatives; 48x131072 float16 with twenty: 17 us, 8 with
 // none).
 #include "vocab.h"
 
@@ -32,8 +32,8 @@ constexpr int kMostSplitRows = 255;     // rows that may be shared by blocks
 // bound: K threads reach it, and what no thread's largest value reaches is no candidate.  So the packs of these K
 // owners alone are read again, a few thousand values of a row that has just come through the cache, and what reaches
 // the bound (K values and few more, unless the row is laid out against it) is ranked by counting.  Values and places
-// make keys without ties, so the answer does not depend on the order in which candidates arrive.  (1341 rows of 50021
-// in float32: 52 us with no alternatives, 59 with five, 71 with twenty, 110 with 64.)
+// make keys without ties, so the answer does not depend on the order in which candidates arrive.  (512 rows of 131072
+// in float32: 46 us with no alternatives, 55 with five, 73 with twenty.)
 
 typedef unsigned long long Key;
 
