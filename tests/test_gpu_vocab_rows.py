@@ -72,6 +72,22 @@ def test_more_candidates_than_room(top, dtype):
         logp._compare(z.astype(dtype), rng.integers(0, vocab, rows), top, grads=False)
 
 
+@BOTH
+@pytest.mark.parametrize('top', [1, 5, 20, 32, 33])
+@pytest.mark.parametrize('packs', [1, 9, 64, 100, 128, 129, 200, 256, 257])
+def test_equal_values_in_rows_of_a_wave(packs, top, dtype):
+    """More values reach the bound than a wave has room for: equal ones, whose places decide."""
+    vocab = packs * _packs(dtype) - (packs > 1)
+    rng = np.random.default_rng(packs)
+    j = np.arange(vocab)
+    low = np.finfo(dtype).min
+    rows = [np.zeros(vocab), np.full(vocab, -np.inf), np.full(vocab, low), j % 2, -(j % 3), rng.integers(0, 2, vocab),
+            np.where(j < vocab // 2, -np.inf, 1.0), np.where(rng.random(vocab) < 0.1, 3.0, low), np.where(j % 64 < 40, 2.0, 0),
+            np.where(j == vocab - 1, 5.0, -np.inf), rng.standard_normal(vocab)]
+    z = np.stack(rows).astype(dtype)
+    logp._compare(z, rng.integers(0, vocab, len(rows)), min(top, vocab), grads=False)
+
+
 def test_counters_are_zero_again():
     """Launches of different numbers of blocks in turn, each of which counts its blocks."""
     for rows, vocab in ((1, 40000), (2000, 40), (3, 200000), (33, 9001), (700, 100), (31, 300), (4000, 20)):
