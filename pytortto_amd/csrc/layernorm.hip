@@ -90,6 +90,7 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float* part) {
     for (int k = 0; k < N; ++k) v[k] += part[i * N + k];
 }
 
+constexpr int kFlight = 16;       // loads that a thread of the joining block has on their way
 constexpr int kMostBlock = 1024, kFwdBlock = 256, kBwdBlock = 512;    // threads: G = 0 at most, G > 0 forward, backward
 
 template <typename T, int G, int NV>
@@ -250,22 +251,22 @@ __global__ __launch_bounds__(G ? kBwdBlock : kMostBlock) void ln_bwd(const T* __
   if (thread == 0) last = tt::last_ticket(&ln_done, gridDim.x);
   __syncthreads();
   if (!last) return;
-  // as many threads to a column as there are, each with every so manieth block's sum, four on their way
+  // as many threads to a column as there are, each with every so manieth block's sum, kFlight on their way
   double* sums64 = reinterpret_cast<double*>(all);
   const int ways = 2 * D < threads ? threads / (2 * D) : 1, used = 2 * D < threads ? 2 * D : threads;
   for (int c0 = 0; c0 < 2 * D; c0 += used) {
     const int c = c0 + thread % used, way = thread / used;
     double s = 0.0;
     if (way < ways && c < 2 * D)
-      for (int k = way; k < (int)gridDim.x; k += 4 * ways) {
-        float v[4];
+      for (int k = way; k < (int)gridDim.x; k += kFlight * ways) {
+        float v[kFlight];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kFlight; ++i) {
           v[i] = 0.f;
           if (k + i * ways < (int)gridDim.x) v[i] = tt::shared(parts + (size_t)(k + i * ways) * 2 * D + c);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s += (double)v[i];
+        for (int i = 0; i < kFlight; ++i) s += (double)v[i];
       }
     __syncthreads();
     sums64[thread] = s;
@@ -496,11 +497,12 @@ int launch_bwd(const T* x, const T* dy, const float* w, const float* mean, const
     TT_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_unit, ln_bwd<T, G, NV>, block.x * block.y, 0));
   const unsigned grid = grid_for(R, rows, (long long)tt::compute_units() * (per_unit > 0 ? per_unit : 1));
   const bool sums = dw || db;
-  // the last block joins what takes it a few rounds of loads (10 blocks of 1024 columns: 8.7 us, 11.6 with a launch
-  // more; 10 of 1537 columns, in 21 rounds: 16.6 and 11.8)
+  // the last block joins what takes it a few rounds of loads: that saves the host a launch, 3 us, for a little more of
+  // the device's time (300 rows of 256: 7.0 us, 6.4 with the launch, 5000 of 96: 11.4 and 10.5; 300 of 512, in six
+  // rounds, 10.9 and 6.9)
   const int threads = block.x * block.y, ways = 2 * D < threads ? threads / (2 * D) : 1;
-  const long long rounds = (2 * (long long)D + threads - 1) / threads * ((grid + 4 * ways - 1) / (4 * ways));
-  const bool joins = sums && grid > 1 && rounds <= 8;
+  const long long rounds = (2 * (long long)D + threads - 1) / threads * ((grid + kFlight * ways - 1) / (kFlight * ways));
+  const bool joins = sums && grid > 1 && rounds <= 3;
   void* ws = nullptr;
   if (sums && grid > 1)
     if (tt::workspace((size_t)grid * 2 * D * sizeof(float), &ws)) return -1;
