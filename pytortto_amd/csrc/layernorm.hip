@@ -465,7 +465,7 @@ int forward(const T* x, const float* w, const float* b, T* y, float* mean, float
   if (sizeof(T) == 4 && packs <= 320) TT_LN_FWD(64, 5);       // 1025 columns 68 -> 55 us at 2^25 values, 1200: 55 -> 51
   if (packs <= 512) TT_LN_FWD(0, 2);
   if (packs <= 768) TT_LN_FWD(0, 3);
-  if (packs <= 4096) TT_LN_FWD(0, 4);
+  if (packs <= 4 * kMostBlock) TT_LN_FWD(0, 4);
 #undef TT_LN_FWD
   ln_fwd_long<T><<<grid_for(R, 1, 1 << 20), kLong, 0, tt::stream()>>>(x, w, b, y, mean, rstd, R, D, eps);
   TT_LAUNCH_CHECK();
@@ -533,10 +533,10 @@ int backward(const T* x, const T* dy, const float* w, const float* mean, const f
   if constexpr (wide) {
     if (packs > 384 && packs <= 512) TT_LN_BWD(0, 2);
     if (packs > 768 && packs <= 960) TT_LN_BWD(0, 4);
-    if (packs <= 3072) TT_LN_BWD(0, 3);
-    if (packs <= 4096) TT_LN_BWD(0, 4);
+    if (packs <= 3 * kMostBlock) TT_LN_BWD(0, 3);
+    if (packs <= 4 * kMostBlock) TT_LN_BWD(0, 4);
   } else {
-    if (packs <= 2048) TT_LN_BWD(0, 2);
+    if (packs <= 2 * kMostBlock) TT_LN_BWD(0, 2);
   }
 #undef TT_LN_BWD
   hipStream_t st = tt::stream();
