@@ -42,10 +42,28 @@ __device__ __forceinline__ typename Loose<T>::type read_columns(const T* row, in
   return p;
 }
 template <typename T>
-__device__ __forceinline__ void write_columns(T* row, int q, int D, const typename Loose<T>::type& p) {
+__device__ __forceinline__ bool whole_lines(int D) {
+  return D % (128 / (int)sizeof(T)) == 0;
+}
+// `passing`: on its way to memory at once, past the caches, which then hold more of what is read. Float32 rows that end
+// inside a line of memory are better left to the cache, which puts the pieces of a line together (72 columns forward:
+// 53 us at 2^25 values, 87 passing; 2500 columns 49 and 50; of whole lines, 16000 columns, 72 and 66). Halves always
+// pass (385 columns 36 us, 37 if they do not).
+template <typename T>
+__device__ __forceinline__ void write_columns(T* row, int q, int D, const typename Loose<T>::type& p,
+                                              bool passing = true) {
   constexpr int n = Loose<T>::n;
   if (q * n + n <= D) {
-    __builtin_nontemporal_store(p, reinterpret_cast<typename Loose<T>::type*>(row + (size_t)q * n));
+    typename Loose<T>::type* at = reinterpret_cast<typename Loose<T>::type*>(row + (size_t)q * n);
+    if (sizeof(T) == 2) {
+      __builtin_nontemporal_store(p, at);
+    } else if (passing) {
+      asm volatile("" ::: "memory");        // (or the compiler makes one store of the two, that does not pass)
+      __builtin_nontemporal_store(p, at);
+      asm volatile("" ::: "memory");
+    } else {
+      *at = p;
+    }
     return;
   }
 #pragma unroll
@@ -105,6 +123,7 @@ __global__ __launch_bounds__(G ? kFwdBlock : kMostBlock) void ln_fwd(const T* __
   const int stride = G ? G : (int)blockDim.x, lane = threadIdx.x % stride;
   const int sub = G ? tt::row_of_block<G ? G : 1>() : 0;
   const int packs = (D + n - 1) / n;
+  const bool passing = whole_lines<T>(D);
   for (long long row = (long long)blockIdx.x * kRows + sub; row < R; row += (long long)gridDim.x * kRows) {
     const T* __restrict__ p = x + row * (size_t)D;
     P v[NV];
@@ -138,7 +157,7 @@ __global__ __launch_bounds__(G ? kFwdBlock : kMostBlock) void ln_fwd(const T* __
       P o;
 #pragma unroll
       for (int i = 0; i < n; ++i) o[i] = (T)fmaf((tt::widen(v[u][i]) - m) * r, wv[i], bv[i]);
-      write_columns(y + row * (size_t)D, q, D, o);
+      write_columns(y + row * (size_t)D, q, D, o, passing);
     }
     if (mean && lane == 0) {
       mean[row] = m;
@@ -166,6 +185,7 @@ __global__ __launch_bounds__(G ? kBwdBlock : kMostBlock) void ln_bwd(const T* __
   const int sub = G ? tt::row_of_block<G ? G : 1>() : __builtin_amdgcn_readfirstlane(threadIdx.y);
   const int thread = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
   const int all_packs = (D + n - 1) / n;
+  const bool passing = G == 0 || G > 16 || whole_lines<T>(D);   // (132 columns 91 us, 84 not passing)
   float sums[2][NV][n] = {};        // dw, db
   float wv[NV][n];
 #pragma unroll
@@ -211,7 +231,7 @@ __global__ __launch_bounds__(G ? kBwdBlock : kMostBlock) void ln_bwd(const T* __
         const float nn = (tt::widen(xv[u][i]) - m) * r;
         o[i] = (T)(r * (tt::widen(gv[u][i]) * wv[u][i] - mh - nn * mhn));
       }
-      write_columns(dx + base, q, D, o);
+      write_columns(dx + base, q, D, o, passing);
     }
   }
   if (!dw_out && !db_out) return;
@@ -520,7 +540,6 @@ int backward(const T* x, const T* dy, const float* w, const float* mean, const f
   if (packs <= 4) TT_LN_BWD(4, 1);
   if (packs <= 8) TT_LN_BWD(8, 1);
   if (packs <= 16) TT_LN_BWD(16, 1);
-  if (packs <= 24) TT_LN_BWD(8, 3);
   if (packs <= 32) TT_LN_BWD(32, 1);
   if (packs <= 48) TT_LN_BWD(16, 3);
   if (packs <= 64) TT_LN_BWD(64, 1);
