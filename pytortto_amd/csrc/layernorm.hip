@@ -8,10 +8,10 @@
 // and keeps each thread's columns of dw and db in registers on the way; they are added up over the rows of a block in
 // LDS, and over the blocks by ln_join. Rows longer than the registers hold are read again (the *_long kernels).
 //
-// Memory bounds them: 2^25 float32 values take 49 to 55 us forward and 79 to 85 us backward (4.9 to 5.5 TB/s, a large
-// copy 5.0 to 5.6) in rows of 24 to 5000; float16 24 to 28 and 44 to 55 us (3.7 to 5.4 TB/s), rows that begin off
-// sixteen bytes up to half as much more. What is left to lose are idle lanes, where a row's packs do not fill its
-// waves, and the blocks' sums.
+// Memory bounds them: 2^25 float32 values take 45 to 61 us forward and 77 to 85 us backward (4.4 to 6.0 and 4.7 to 5.2
+// TB/s, a large copy 5.0 to 5.6) in rows of 24 to 4096, 1537 columns 65 and 84; float16 23 to 39 us and 42 to 78 us,
+// where rows that begin off sixteen bytes take up to half as much more.  What is left to lose are idle lanes, where a
+// row's packs do not fill its waves, and the blocks' sums.
 #include "rows.h"
 
 namespace {
