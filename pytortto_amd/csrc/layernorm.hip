@@ -46,9 +46,10 @@ __device__ __forceinline__ bool whole_lines(int D) {
   return D % (128 / (int)sizeof(T)) == 0;
 }
 // `passing`: on its way to memory at once, past the caches, which then hold more of what is read. Float32 rows that end
-// inside a line of memory are better left to the cache, which puts the pieces of a line together (72 columns forward:
-// 53 us at 2^25 values, 87 passing; 2500 columns 49 and 50; of whole lines, 16000 columns, 72 and 66). Halves always
-// pass (385 columns 36 us, 37 if they do not).
+// inside a line of memory and have a part of a wave each, so that its pieces come from several instructions, are better
+// left to the cache, which puts them together (forward at 2^27 values: 72 columns 209 us, 394 passing, 264 columns 215
+// and 226; but 2500 columns, a block to a row, 210 and 199). Halves always pass (385 columns at 2^25 values 36 us, 37 if
+// they do not).
 template <typename T>
 __device__ __forceinline__ void write_columns(T* row, int q, int D, const typename Loose<T>::type& p,
                                               bool passing = true) {
@@ -123,7 +124,7 @@ __global__ __launch_bounds__(G ? kFwdBlock : kMostBlock) void ln_fwd(const T* __
   const int stride = G ? G : (int)blockDim.x, lane = threadIdx.x % stride;
   const int sub = G ? tt::row_of_block<G ? G : 1>() : 0;
   const int packs = (D + n - 1) / n;
-  const bool passing = whole_lines<T>(D);
+  const bool passing = G == 0 || G == kWave || whole_lines<T>(D);
   for (long long row = (long long)blockIdx.x * kRows + sub; row < R; row += (long long)gridDim.x * kRows) {
     const T* __restrict__ p = x + row * (size_t)D;
     P v[NV];
