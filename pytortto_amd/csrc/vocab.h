@@ -210,5 +210,8 @@ constexpr int parts_of(int G, int sums) { return G > kWave ? sums * (G / kWave) 
 
 // log2 of the sum, 0 for an empty row; a NaN stays.
 __device__ __forceinline__ float log_sum(const Stat& a) { return a.s > 0.f ? log2f(a.s) : a.s; }
+// Whether a row has no value above -inf, by its maximum and its sum or the sum's logarithm.  The maximum passes over
+// NaN, so that a row of nothing else has -inf too; its sum is NaN then.
+__device__ __forceinline__ bool is_empty(float m, float s) { return m == -INFINITY && s == s; }
 
 }  // namespace tt

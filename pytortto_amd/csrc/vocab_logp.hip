@@ -540,7 +540,7 @@ __global__ __launch_bounds__(kThreads) void logp_bwd(const T* __restrict__ x, Ba
     const Share s(r, (int)(item % splits), splits);
     const long long t0 = tt::read_index(in.tokens, row, in.wide), t = token_place(t0, V);
     const float2 st = in.stats[row];
-    const bool none = t0 == in.ignored || st.x == -INFINITY, given = in.g_logp && t >= 0;
+    const bool none = t0 == in.ignored || tt::is_empty(st.x, st.y), given = in.g_logp && t >= 0;
     RowGradient<T> g = {st.x, st.y, 0.f, 0.f, 0.f};
     float a = 0.f;
     if (!none) {

@@ -1,0 +1,50 @@
+"""GPU: rows of logits that are NaN throughout, or NaN where they are not -inf: their gradients are NaN, not those of a row
+that a mask has left with nothing.  Sizes for every number of threads that takes a row."""
+import numpy as np
+import pytest
+
+import pytortto_amd as tt
+from pytortto_amd.xparray import hiparray
+from tests import plain64
+
+pytestmark = pytest.mark.gpu
+F = tt.nn.functional
+# (rows, values): a few lanes of a wave, a wave that keeps the row, a wave, blocks that share a row, a block
+SIZES = [(37, 1), (21, 2), (33, 10), (20, 100), (19, 700), (9, 1000), (18, 3000), (9, 9000), (300, 9000)]
+
+
+def _tensor(a, grad=False):
+    return tt.Tensor(hiparray(a), requires_grad=grad, dtype=a.dtype)
+
+
+def _logits(rows, vocab, dtype):
+    """Rows in turn: NaN throughout, NaN and -inf, one NaN, -inf throughout, ordinary ones."""
+    rng = np.random.default_rng(rows * vocab)
+    z = (rng.standard_normal((rows, vocab)) * 2).astype(dtype)
+    z[0::6] = np.nan
+    z[1::6] = -np.inf
+    z[1::6, vocab // 2] = np.nan
+    z[2::6, vocab - 1] = np.nan
+    z[3::6] = -np.inf
+    return z, rng
+
+
+@pytest.mark.parametrize('top', [0, 5, 40])
+@pytest.mark.parametrize('dtype', [np.float32, np.float16])
+@pytest.mark.parametrize('rows,vocab', SIZES)
+def test_token_log_prob(rows, vocab, dtype, top):
+    z, rng = _logits(rows, vocab, dtype)
+    top = min(top, vocab)
+    tokens = rng.integers(0, vocab, rows)
+    g = [rng.standard_normal(s).astype(np.float32) for s in ((rows,), (rows,), (rows, top))]
+    x = _tensor(z, True)
+    got = F.token_log_prob(x, _tensor(tokens), top)
+    with np.errstate(invalid='ignore'):
+        values, bounds = plain64.token_log_prob(z, tokens, top)
+        dz, bound = plain64.token_log_prob_grad(z, tokens, top, g[0], g[1], g[2] if top else None)
+    for y, want, off in zip(got, values, bounds):
+        plain64.check(y.data.get(), want, off)
+    if top:
+        np.testing.assert_array_equal(got[3].data.get(), values[3])
+    tt.backward(got[:3 if top else 2], [_tensor(v) for v in g[:3 if top else 2]])
+    plain64.check(x.grad.get(), dz, plain64.stored(bound, dz, dtype), 'dx')
