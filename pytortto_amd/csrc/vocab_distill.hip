@@ -197,13 +197,14 @@ struct Out {
   int mean;
 };
 
-// A row without a teacher has m = -inf for the backward pass, as one without any possible class: no gradient.
+// A row without a teacher is an empty one for the backward pass, as one without any possible class: no gradient.
 __device__ __forceinline__ double write_row(const Out& o, size_t row, const Stat& a, float log_s, const TeacherSum& te,
                                             float cross, const Scale& sc) {
   const bool none = te.s == 0.f;
   const float loss = none ? 0.f : fmaf(te.q_log_q, tt::kLn2, cross) * (sc.temperature * sc.temperature);
   if (o.loss) o.loss[row] = loss;
-  o.stats[row] = make_float2(none ? -INFINITY : a.m, te.s == te.s ? log_s : te.s);
+  o.stats[row] = none || tt::is_empty(a.m, a.s) ? make_float2(-INFINITY, 0.f)
+                                                : make_float2(a.m, te.s == te.s ? log_s : te.s);
   return loss;
 }
 
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(G < kThreads ? kThreads : G, G == 512 ? 4 : 1) void
     const float log_s = tt::log_sum(a);
     float cross = cross_entropy<T, G>(e, te.K, lane, a, log_s, sc);
     if constexpr (GRAD) {
-      const bool none = ts.s == 0.f || a.m == -INFINITY;
+      const bool none = ts.s == 0.f || tt::is_empty(a.m, a.s);
       const float by = ts.s == ts.s ? scale : ts.s;
       if (!none) queue_entries<T, G>(e, r, all, te.K, lane, a.m, log_s, sc.c, by);
       const Patches<kPatches<G>> patches = take_queued<T, kPatches<G>>(e, r, lane);
@@ -480,7 +481,7 @@ __global__ __launch_bounds__(kThreads) void distill_bwd(const T* __restrict__ x,
     const LogitRow<T> r(x, row, V);
     const Share s(r, (int)(item % splits), splits);
     const float2 st = stats[row];
-    const bool none = st.x == -INFINITY;
+    const bool none = tt::is_empty(st.x, st.y);
     float scale = sc.temperature * (reduction == 0 ? g[row] : g[0]);
     if (reduction == 2) scale /= count[0];
     if (none) {

@@ -48,3 +48,34 @@ def test_token_log_prob(rows, vocab, dtype, top):
         np.testing.assert_array_equal(got[3].data.get(), values[3])
     tt.backward(got[:3 if top else 2], [_tensor(v) for v in g[:3 if top else 2]])
     plain64.check(x.grad.get(), dz, plain64.stored(bound, dz, dtype), 'dx')
+
+
+@pytest.mark.parametrize('reduction', ['none', 'sum', 'mean'])
+@pytest.mark.parametrize('dtype', [np.float32, np.float16])
+@pytest.mark.parametrize('rows,vocab', SIZES)
+def test_distill_loss(rows, vocab, dtype, reduction):
+    z, rng = _logits(rows, vocab, dtype)
+    k = min(vocab, 7)
+    teacher = (rng.standard_normal((rows, k)) * 2).astype(dtype)
+    index = (rng.integers(0, vocab, (rows, 1)) + np.arange(k) * (vocab // k)) % vocab
+    index[(np.arange(rows) // 6) % 3 == 1] = -1             # every kind of row with and without a teacher, and with
+    index[(np.arange(rows) // 6) % 3 == 2, 0] = vocab       # one of another vocabulary
+    g = rng.standard_normal(rows).astype(np.float32) if reduction == 'none' else None
+    with np.errstate(invalid='ignore'):
+        (loss, off), (dz, bound) = plain64.distill(z, teacher, index, 2.0, reduction, g)
+    x = _tensor(z, True)
+    got = F.distill_loss(x, _tensor(teacher), _tensor(index), 2.0, reduction)
+    plain64.check(got.data.get(), loss, off, 'loss')
+    got.backward(None if g is None else _tensor(g))
+    plain64.check(x.grad.get(), dz, plain64.stored(bound, dz, dtype), 'dx')
+
+
+@pytest.mark.parametrize('rows,vocab', SIZES)
+def test_distill_loss_for_another_gradient_than_one(rows, vocab):
+    z, rng = _logits(rows, vocab, np.float32)
+    index, teacher = np.zeros((rows, 1), np.int64), np.zeros((rows, 1), np.float32)
+    with np.errstate(invalid='ignore'):
+        _, (dz, bound) = plain64.distill(z, teacher, index, 1.0, 'sum')
+    x = _tensor(z, True)
+    F.distill_loss(x, _tensor(teacher), _tensor(index), 1.0, 'sum').backward(_tensor(np.asarray(0.5, np.float32)))
+    plain64.check(x.grad.get(), dz * 0.5, bound, 'dx')
