@@ -222,14 +222,38 @@ def build_links(data, grad_fn, copy=False, _output_idx=0):
     return _Tensor(data, dtype=dtype, copy=copy)
 
 
+def _edges_from(nodes):
+    """How many edges lead to each node that ``nodes`` lead to: {node: edges}."""
+    edges, todo, seen = {}, list(nodes), set(nodes)
+    while todo:
+        for fn, _ in todo.pop().next_functions or ():
+            if fn is not None:
+                edges[fn] = edges.get(fn, 0) + 1
+                if fn not in seen:
+                    seen.add(fn)
+                    todo.append(fn)
+    return edges
+
+
 def toposort(*end_nodes):
     """helper.py:53-82: yield nodes so that a node comes after everything that feeds gradient
     into it; nodes whose other consumers are not part of this backward pass are taken from
-    the ``waiting`` set once nothing else is ready.  Of several end nodes, one that others lead to waits for them."""
+    those ``waiting`` once nothing else is ready.  Of several end nodes, one that others lead to waits for them.
+    Where several nodes wait then, one of them may lead to another, so from there on the edges that are left in this pass
+    are counted, and not those of all consumers."""
     ready = [node for node in end_nodes if node.prev_function_counts == 0]
-    waiting = {node for node in end_nodes if node.prev_function_counts}
+    waiting = {node: None for node in end_nodes if node.prev_function_counts}     # (in the order of their arrival)
+    left = None
     while ready or waiting:
-        node = ready.pop() if ready else waiting.pop()
+        if ready:
+            node = ready.pop()
+        elif len(waiting) == 1:
+            node, _ = waiting.popitem()
+        else:
+            left = _edges_from(waiting)
+            ready = [node for node in waiting if node not in left]
+            waiting = {}
+            continue
         yield node
         for fn, _ in node.next_functions or ():
             if fn is None:
@@ -237,8 +261,12 @@ def toposort(*end_nodes):
             fn.prev_function_counts -= 1
             if fn.__class__ is AccumulateGrad and fn.done:
                 fn.done = False
+            elif left is not None:
+                left[fn] -= 1
+                if left[fn] == 0:
+                    ready.append(fn)
             elif fn.prev_function_counts == 0:
                 ready.append(fn)
-                waiting.discard(fn)
+                waiting.pop(fn, None)
             else:
-                waiting.add(fn)
+                waiting[fn] = None
