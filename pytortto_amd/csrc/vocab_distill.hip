@@ -237,17 +237,16 @@ __device__ __forceinline__ void add_up(const Out& o, tt::Ticket* done, unsigned 
   }
 }
 
-// scale p of the values of pack j, and the patches.  FOLD, for scale > 0: halves, whose rounding hides it, take
-// log2(scale) into the exponent.
-template <typename T, bool FOLD, int P>
+// scale p of the values of pack j, and the patches.  (log2(scale) in the exponent would spare halves a product: 1024x131072
+// with 64 entries 109 us where this takes 113.  But a sum of it with m c is rounded at the size of m c, 2e-3 of the
+// gradient in a row of -65504 alone, and added to the difference it is no faster.)
+template <typename T, int P>
 __device__ __forceinline__ Words gradient_pack(const Words& p, const Patches<P>& t, int j, float m, float log_s,
                                                float c, float scale) {
   float z[Pack<T>::n];
   tt::unpack<T>(z, p);
-  const float add = log2f(scale) - log_s - tt::rounded(m, c);
 #pragma unroll
-  for (int i = 0; i < Pack<T>::n; ++i)
-    z[i] = FOLD && sizeof(T) == 2 ? tt::pow2(fmaf(z[i], c, add)) : scale * tt::pow2(tt::bits<T>(z[i], m, c) - log_s);
+  for (int i = 0; i < Pack<T>::n; ++i) z[i] = scale * tt::pow2(tt::bits<T>(z[i], m, c) - log_s);
   patch<T, P>(z, t, j);
   return tt::pack<T>(z);
 }
@@ -390,7 +389,7 @@ __global__ __launch_bounds__(G < kThreads ? kThreads : G, G == 512 ? 4 : 1) void
         asm volatile("" : "+v"(kept[u]));
         const int j = own + u * G;
         if (j < all.p1) {
-          const Words q = none ? Words(0u) : gradient_pack<T, true>(kept[u], patches, j, a.m, log_s, sc.c, by);
+          const Words q = none ? Words(0u) : gradient_pack<T>(kept[u], patches, j, a.m, log_s, sc.c, by);
           tt::write_pack(r, dx, j, q);
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -405,7 +404,7 @@ __global__ __launch_bounds__(G < kThreads ? kThreads : G, G == 512 ? 4 : 1) void
           for (int u = 0; u < kPair; ++u)
             if (j + u * G < rest.p1)
               tt::write_pack(r, dx, j + u * G,
-                             none ? Words(0u) : gradient_pack<T, true>(p[u], patches, j + u * G, a.m, log_s, sc.c, by));
+                             none ? Words(0u) : gradient_pack<T>(p[u], patches, j + u * G, a.m, log_s, sc.c, by));
         }
       write_loose<T, G>(x, dx, r, all, lane, none, a.m, log_s, sc.c, by);
       store_rest(e, dx, r, patches.rest);
@@ -500,7 +499,7 @@ __global__ __launch_bounds__(kThreads) void distill_bwd(const T* __restrict__ x,
       for (int u = 0; u < kUnroll; ++u)
         if (j + u * G < s.p1)
           tt::write_pack(r, dx, j + u * G,
-                         none ? Words(0u) : gradient_pack<T, false>(p[u], patches, j + u * G, st.x, st.y, sc.c, scale));
+                         none ? Words(0u) : gradient_pack<T>(p[u], patches, j + u * G, st.x, st.y, sc.c, scale));
     }
     write_loose<T, G>(x, dx, r, s, lane, none, st.x, st.y, sc.c, scale);
     store_rest(e, dx, r, patches.rest);
