@@ -18,12 +18,14 @@ template <typename T>
 struct Pack;
 template <>
 struct Pack<float> {
+  typedef float value;
   typedef float vector __attribute__((ext_vector_type(4)));
   static constexpr int n = 4;
   static constexpr unsigned lowest = 0xff800000u;      // -inf, as often as a word holds it
 };
 template <>
 struct Pack<_Float16> {
+  typedef _Float16 value;
   typedef _Float16 vector __attribute__((ext_vector_type(8)));
   static constexpr int n = 8;
   static constexpr unsigned lowest = 0xfc00fc00u;
@@ -50,7 +52,7 @@ template <typename T>
 __device__ __forceinline__ Words pack(const float* z) {
   typename Pack<T>::vector v;
 #pragma unroll
-  for (int i = 0; i < Pack<T>::n; ++i) v[i] = (T)z[i];
+  for (int i = 0; i < Pack<T>::n; ++i) v[i] = (typename Pack<T>::value)z[i];
   return __builtin_bit_cast(Words, v);
 }
 

@@ -78,7 +78,12 @@ __device__ __forceinline__ float anchor(float m) { return m == -INFINITY ? 0.f :
 __device__ __forceinline__ float floor_at(float d) { return fmaxf(d, -200.f); }
 
 // d of a value, (z - m) c.  Halves cannot overflow z c, and take one instruction for their widening, the product and
-// the difference; every d of a row has the same rounded m c then, which drops out of all that is made of them.
+// the difference; every d of a row has the same rounded m c then, which drops out of all that is made of them.  (Where c
+// is below 2^14: m c is below 2^30 then, and what it is rounded by below 2^5, a factor of 2^32 for all sums of the row.)
+template <typename T>
+constexpr bool by_product = false;
+template <>
+inline constexpr bool by_product<_Float16> = true;
 __device__ __forceinline__ float rounded(float m, float c) {
 #pragma clang fp contract(off)
   return m * c;
@@ -89,13 +94,13 @@ __device__ __forceinline__ float rounded_between(float m, float to, float c) {
 }
 template <typename T>
 __device__ __forceinline__ float bits(float z, float m, float c) {
-  return sizeof(T) == 2 ? fmaf(z, c, -rounded(m, c)) : (z - m) * c;
+  return by_product<T> ? fmaf(z, c, -rounded(m, c)) : (z - m) * c;
 }
 
 // Moves the sums of `a` to another, larger maximum.
 template <typename T, bool ENTROPY>
 __device__ __forceinline__ void rescale(Stat& a, float m, float c) {
-  const float to = anchor(m), d = sizeof(T) == 2 ? rounded_between(a.m, to, c) : (a.m - to) * c, f = pow2(d);
+  const float to = anchor(m), d = by_product<T> ? rounded_between(a.m, to, c) : (a.m - to) * c, f = pow2(d);
   if (ENTROPY) a.t = f * fmaf(a.s, floor_at(d), a.t);
   a.s *= f;
   a.m = m;
@@ -202,7 +207,7 @@ struct Scale {
 // log p of a value, in nats.  (In bits a float32 that is its type's lowest would overflow.)
 template <typename T>
 __device__ __forceinline__ float log_p(float z, float m, float log_s, const Scale& sc) {
-  return (sizeof(T) == 2 ? bits<T>(z, m, sc.c) * kLn2 : (z - m) * sc.inverse) - log_s * kLn2;
+  return (by_product<T> ? bits<T>(z, m, sc.c) * kLn2 : (z - m) * sc.inverse) - log_s * kLn2;
 }
 
 // LDS floats of `sums` sums over a row.

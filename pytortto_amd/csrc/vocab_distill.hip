@@ -10,6 +10,24 @@
 // with 32 entries: 35 us, 57 with the gradient).
 #include "vocab.h"
 
+namespace tt {
+
+// A half that is divided by a temperature below kCold, where logits times c are too large for the rounded products that
+// halves take as a rule (vocab.h): a row of -65504 alone at 1e-6 would sum to 2^4096.  Its differences are taken first, as
+// float32 does it, which costs the halves of warmer calls up to 18 % (at 1e-4, where both would do, 22369x3000 with 32
+// entries and the gradient take 61.7 us and 54.7 by products, 300x50021 21.8 and 18.5).
+struct ColdHalf {
+  _Float16 v;
+  ColdHalf() = default;
+  __device__ explicit ColdHalf(float z) : v((_Float16)z) {}
+};
+constexpr double kCold = 1.0 / 8192;
+template <>
+struct Pack<ColdHalf> : Pack<_Float16> {};
+__device__ __forceinline__ float widen(ColdHalf z) { return widen(z.v); }
+
+}  // namespace tt
+
 namespace {
 
 using tt::kUnroll;
@@ -690,6 +708,8 @@ int tt_distill_fwd(const void* x, const void* teacher, const void* index, float*
   const Teacher te = {teacher, index, teacher_dtype == TT_F16, index_bits == 64, K};
   if (dtype == TT_F32)
     return forward((const float*)x, te, loss, stats, count, (float*)dx, temperature, reduction, (int)R, V);
+  if (temperature < tt::kCold)
+    return forward((const tt::ColdHalf*)x, te, loss, stats, count, (tt::ColdHalf*)dx, temperature, reduction, (int)R, V);
   return forward((const _Float16*)x, te, loss, stats, count, (_Float16*)dx, temperature, reduction, (int)R, V);
 }
 
@@ -705,6 +725,9 @@ int tt_distill_bwd(const void* x, const void* teacher, const void* index, const 
   const Teacher te = {teacher, index, teacher_dtype == TT_F16, index_bits == 64, K};
   if (dtype == TT_F32)
     return backward((const float*)x, te, stats, count, g, (float*)dx, temperature, reduction, is_ahead, (int)R, V);
+  if (temperature < tt::kCold)
+    return backward((const tt::ColdHalf*)x, te, stats, count, g, (tt::ColdHalf*)dx, temperature, reduction, is_ahead,
+                    (int)R, V);
   return backward((const _Float16*)x, te, stats, count, g, (_Float16*)dx, temperature, reduction, is_ahead, (int)R, V);
 }
 

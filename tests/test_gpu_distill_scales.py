@@ -60,7 +60,7 @@ def _logits(rows, vocab, dtype, size, temperature):
     return z.astype(dtype), (rng.integers(0, 3, (rows, 6)) * temperature).astype(dtype), index
 
 
-SCALES = [(60.0, 1e-3), (20000.0, 0.1), (60000.0, 1e-2), (-60000.0, 1e-4), (30000.0, 1e-5), (3.0, 1e-6), (50.0, 20.0)]
+SCALES = [(60.0, 1e-3), (20000.0, 0.1), (60000.0, 1e-2), (-60000.0, 1e-4), (30000.0, 1e-5), (3.0, 1e-6), (50.0, 20.0), (-65504.0, 1e-6)]
 
 
 @pytest.mark.parametrize('reduction', ['sum', 'mean', 'none'])
