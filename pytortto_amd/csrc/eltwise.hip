@@ -1,5 +1,5 @@
 // Elementwise glue kernels (ReLU, LeakyReLU, residual add, gradient accumulation, fill): HBM-bound,
-// float4 grid-stride loops with a scalar tail.
+// float4 grid-stride loops with a scalar tail; gradients of halves in eights.
 #include "tt_common.h"
 
 namespace {
@@ -71,19 +71,32 @@ __global__ __launch_bounds__(kThreads) void eltwise(const float* __restrict__ a,
   if (t < n) out[t] = apply1<OP>(kUseA ? a[t] : 0.f, kUseB ? b[t] : 0.f, alpha);
 }
 
+unsigned grid_for(size_t packs) {
+  const size_t blocks = (packs + kThreads - 1) / kThreads, cap = (size_t)tt::compute_units() * 16;
+  return (unsigned)(blocks < 1 ? 1 : blocks < cap ? blocks : cap);      // grid-stride beyond 16 blocks per CU
+}
+
 template <int OP>
 int run(const char* fn, const float* a, const float* b, float* out, float alpha, size_t n) {
   TT_REQUIRE_INIT();
   if (n == 0) return 0;
   TT_REQUIRE(out != nullptr, "%s: null output pointer", fn);
   TT_REQUIRE_ALIGNED(fn, a, b, out);
-  size_t blocks = ((n >> 2) + kThreads - 1) / kThreads;
-  const size_t cap = (size_t)tt::compute_units() * 16;   // grid-stride beyond 16 blocks per CU
-  if (blocks < 1) blocks = 1;
-  if (blocks > cap) blocks = cap;
-  eltwise<OP><<<(unsigned)blocks, kThreads, 0, tt::stream()>>>(a, b, out, alpha, n);
+  eltwise<OP><<<grid_for(n >> 2), kThreads, 0, tt::stream()>>>(a, b, out, alpha, n);
   TT_LAUNCH_CHECK();
   return 0;
+}
+
+// Sums of halves, each rounded once.  `out` may be `a` or `b`.  (2^26 values: 78 us to an array of their own, 5.2 TB/s,
+// 59 us into one of the operands, part of which the caches still have.)
+__global__ __launch_bounds__(kThreads) void add_halves(const _Float16* a, const _Float16* b, _Float16* out, size_t n) {
+  typedef _Float16 Halves __attribute__((ext_vector_type(8)));
+  const size_t n8 = n >> 3, stride = (size_t)gridDim.x * kThreads;
+  const Halves *a8 = reinterpret_cast<const Halves*>(a), *b8 = reinterpret_cast<const Halves*>(b);
+  for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < n8; i += stride)
+    reinterpret_cast<Halves*>(out)[i] = a8[i] + b8[i];
+  const size_t t = (n8 << 3) + (size_t)blockIdx.x * kThreads + threadIdx.x;
+  if (t < n) out[t] = a[t] + b[t];
 }
 
 }  // namespace
@@ -109,6 +122,15 @@ int tt_axpy_f32(float alpha, const float* v, float* acc, size_t n) {
 }
 int tt_add_scalar_f32(float* acc, float value, size_t n) {
   return run<kAddScalar>("tt_add_scalar_f32", acc, nullptr, acc, value, n);
+}
+int tt_add_f16(const void* a, const void* b, void* out, size_t n) {
+  TT_REQUIRE_INIT();
+  if (n == 0) return 0;
+  TT_REQUIRE(a && b && out, "tt_add_f16: null pointer");
+  TT_REQUIRE_ALIGNED("tt_add_f16", a, b, out);
+  add_halves<<<grid_for(n >> 3), kThreads, 0, tt::stream()>>>((const _Float16*)a, (const _Float16*)b, (_Float16*)out, n);
+  TT_LAUNCH_CHECK();
+  return 0;
 }
 int tt_fill_f32(float* dst, float value, size_t n) { return run<kFill>("tt_fill_f32", nullptr, nullptr, dst, value, n); }
 

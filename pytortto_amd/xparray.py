@@ -56,7 +56,7 @@ class Device:
         return hash(('hip', self.id))
 
 
-_F32 = np.dtype(np.float32)
+_F32, _F16 = np.dtype(np.float32), np.dtype(np.float16)
 _void_p, _byref = ctypes.c_void_p, ctypes.byref
 _DTYPES = {}            # of array interfaces' type strings
 
@@ -434,14 +434,22 @@ class hiparray:
             _hip.call('tt_fill_f32', self.ptr, float(value), self.size)
 
     def __iadd__(self, other):
-        self._require_f32('+=')
-        self.own()
+        halves = self._dtype == _F16 and isinstance(other, hiparray)
+        if not halves:
+            self._require_f32('+=')
         if isinstance(other, hiparray):
             if other.shape != self._shape or other.dtype != self._dtype:
-                raise ValueError(f'device += needs equal shapes and dtypes, got {self._shape} and {other.shape}')
-            if self.size:
+                raise ValueError(f'device += needs equal shapes and dtypes, got {self._shape} {self._dtype} and '
+                                 f'{other.shape} {other.dtype}')
+            self.own()
+            if not self.size:
+                pass
+            elif halves:
+                _hip.call('tt_add_f16', self.ptr, other.ptr, self.ptr, self.size)
+            else:
                 _hip.call('tt_axpy_f32', 1.0, other.ptr, self.ptr, self.size)
         elif isinstance(other, (int, float, np.floating, np.integer)):
+            self.own()
             if self.size:
                 _hip.call('tt_add_scalar_f32', self.ptr, float(other), self.size)
         else:
