@@ -32,13 +32,15 @@ struct Loose<_Float16> {
   static constexpr int n = 8;
 };
 
-template <typename T>
+// Behind the last column: zeros, or (REPEAT) the pack's first value again, whose normalised value is as finite as the row's.
+template <bool REPEAT = false, typename T>
 __device__ __forceinline__ typename Loose<T>::type read_columns(const T* row, int q, int D) {
   constexpr int n = Loose<T>::n;
   if (q * n + n <= D) return *reinterpret_cast<const typename Loose<T>::type*>(row + (size_t)q * n);
   typename Loose<T>::type p;
+  p[0] = row[(size_t)q * n];
 #pragma unroll
-  for (int i = 0; i < n; ++i) p[i] = q * n + i < D ? row[(size_t)q * n + i] : (T)0.f;
+  for (int i = 1; i < n; ++i) p[i] = q * n + i < D ? row[(size_t)q * n + i] : REPEAT ? p[0] : (T)0.f;
   return p;
 }
 template <typename T>
@@ -202,7 +204,7 @@ __global__ __launch_bounds__(G ? kBwdBlock : kMostBlock) void ln_bwd(const T* __
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       const int q = lane + u * stride;
-      xv[u] = q < packs ? read_columns(x + base, q, D) : P((T)0.f);
+      xv[u] = q < packs ? read_columns<true>(x + base, q, D) : P((T)0.f);
       gv[u] = q < packs ? read_columns(dy + base, q, D) : P((T)0.f);
     }
     const float m = mean[row], r = rstd[row];
@@ -211,7 +213,7 @@ __global__ __launch_bounds__(G ? kBwdBlock : kMostBlock) void ln_bwd(const T* __
     for (int u = 0; u < NV; ++u) {
       if (lane + u * stride >= packs) break;
 #pragma unroll
-      for (int i = 0; i < n; ++i) {       // (behind the last column dy is 0 and adds nothing)
+      for (int i = 0; i < n; ++i) {       // (behind the last column dy is 0 and n finite: nothing is added)
         const float g = tt::widen(gv[u][i]), nn = (tt::widen(xv[u][i]) - m) * r, h = g * wv[u][i];
         of[0] += h;
         of[1] = fmaf(h, nn, of[1]);
@@ -388,7 +390,7 @@ __global__ __launch_bounds__(kLong) void ln_bwd_long(const T* __restrict__ x, co
     const float m = mean[row], r = rstd[row];
     float sh = 0.f, shn = 0.f;
     for (int q = threadIdx.x; q < packs; q += kLong) {
-      const typename Loose<T>::type xv = read_columns(x + base, q, D), gv = read_columns(dy + base, q, D);
+      const typename Loose<T>::type xv = read_columns<true>(x + base, q, D), gv = read_columns(dy + base, q, D);
       float wv[n];
       read_parameters(wv, w, q, D, 1.f);
 #pragma unroll
