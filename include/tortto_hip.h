@@ -478,7 +478,8 @@ int tt_layer_norm_bwd(const void* x, const void* dy, const float* w, const float
  *   - a row of -inf alone: -inf, entropy 0, alternatives -inf, gradient 0;
  *   - a NaN or +inf in a row gives NaN for all its values and -1 for its places.
  * stats [R][2] are kept for the backward pass, or NULL.  The backward adds up the gradients of what the forward returned
- * (each may be NULL) and writes dx [R, V]; entropy and top_index are the forward's. */
+ * (each may be NULL) and writes dx [R, V]; entropy and top_index are the forward's (a place outside the row is passed
+ * over). */
 int tt_token_log_prob_fwd(const void* x, const void* tokens, float* logp, float* entropy, float* top_logp,
                           long long* top_index, float* stats, int dtype, int token_bits, long long ignore_index,
                           long long R, int V, int K);

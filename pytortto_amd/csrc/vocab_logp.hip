@@ -583,7 +583,7 @@ __global__ __launch_bounds__(kThreads) void logp_bwd(const T* __restrict__ x, Ba
       const long long j = given && f == 0 ? t : in.top_index[row * K + f - (given ? 1 : 0)];
       const int pack = (int)((j + r.skip) / n);
       const bool here = j < r.head ? s.head > 0 : j >= r.tail_at ? s.tail > 0 : pack >= s.p0 && pack < s.p1;
-      if (j < 0 || !here) continue;
+      if (j < 0 || j >= V || !here) continue;       // (the places are the caller's memory by now)
       float extra = given && j == t ? a : 0.f;      // summed first: what cancels here leaves no rounding behind
       if (in.g_top)
         for (int k = 0; k < K; ++k)
