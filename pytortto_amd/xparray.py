@@ -298,6 +298,8 @@ class hiparray:
     def __cuda_array_interface__(self):
         """For torch, CuPy and the like to use the memory in place (``torch.as_tensor(array, device='cuda')``); the
         library's stream has to be waited for, or the device, before they read what it computes."""
+        if _hip._pending is not None:       # what is parked may write here, and waiting would not launch it
+            _hip.flush()
         return {'shape': self._shape, 'typestr': self._dtype.str, 'data': (self.ptr, False), 'strides': None,
                 'version': 2}
 
