@@ -65,14 +65,16 @@ class _Buffer:
     """One ``tt_malloc`` allocation; freed (returned to the library's pool) with the last array
     that refers to it.  With ``lazy`` the block is taken on the first use of ``ptr``, and
     ``on_demand`` (a callable receiving the buffer) then fills it: the output of an operation that
-    was absorbed into its successor exists only if somebody else asks for it."""
-    __slots__ = ('_ptr', 'nbytes', 'on_demand', 'deps', '__weakref__')
+    was absorbed into its successor exists only if somebody else asks for it.  ``exported``: others
+    have its address, and may read and write there for as long as they keep the array."""
+    __slots__ = ('_ptr', 'nbytes', 'on_demand', 'deps', 'exported', '__weakref__')
 
     def __init__(self, nbytes, lazy=False):
         self.nbytes = nbytes
         self._ptr = 0
         self.on_demand = None
         self.deps = ()
+        self.exported = False
         if not lazy:
             self._allocate()
 
@@ -161,7 +163,7 @@ class _Borrowed(_Buffer):
     __slots__ = ('owner',)
 
     def __init__(self, ptr, nbytes, owner):
-        self._ptr, self.nbytes, self.owner, self.on_demand, self.deps = ptr, nbytes, owner, None, ()
+        self._ptr, self.nbytes, self.owner, self.on_demand, self.deps, self.exported = ptr, nbytes, owner, None, (), False
 
     def __del__(self):
         pass
@@ -297,11 +299,16 @@ class hiparray:
     @property
     def __cuda_array_interface__(self):
         """For torch, CuPy and the like to use the memory in place (``torch.as_tensor(array, device='cuda')``); the
-        library's stream has to be waited for, or the device, before they read what it computes."""
+        library's stream has to be waited for, or the device, before they read what it computes.  An array that shares
+        its block moves to one of its own, and an array that has been handed out does not share it again: what others
+        write there is seen by the array alone."""
         if _hip._pending is not None:       # what is parked may write here, and waiting would not launch it
             _hip.flush()
-        return {'shape': self._shape, 'typestr': self._dtype.str, 'data': (self.ptr, False), 'strides': None,
-                'version': 2}
+        if self._shared or _unfilled:
+            self.own()
+        at, buf = self.ptr, self._buf
+        buf.exported = True
+        return {'shape': self._shape, 'typestr': self._dtype.str, 'data': (at, False), 'strides': None, 'version': 2}
 
     @property
     def ptr(self):
@@ -363,7 +370,9 @@ class hiparray:
         shared: whoever is about to write one of them in place (``+=``, ``fill``, ``set``, a kernel
         with ``out=``) calls ``own()`` first, which moves that array to a copy.  Gradients handed to
         two operands travel this way: each holder has an array of its own, as the reference's
-        copies give it, and the copy is made only for a holder that writes."""
+        copies give it, and the copy is made only for a holder that writes.  (Of what others may write, at once.)"""
+        if self._buf.exported:
+            return self.copy()
         self._shared = True
         other = hiparray(_buf=self._buf, _shape=self._shape, dtype=self._dtype)
         other._shared = True
@@ -371,7 +380,10 @@ class hiparray:
 
     def lent(self):
         """This array's values as they are now, without a copy: one is made if this block is about to be
-        overwritten while a holder still has them, or if a holder is about to write them."""
+        overwritten while a holder still has them, or if a holder is about to write them.  (Of what others may write, at
+        once.)"""
+        if self._buf.exported:
+            return self.copy()
         other = hiparray.on(_Loan(self._buf), self._shape, self._dtype)
         other._shared = True
         return other

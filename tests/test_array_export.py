@@ -14,13 +14,14 @@ F = tt.nn.functional
 
 class _Library:
     def __init__(self):
-        self.calls = []
+        self.calls, self.blocks = [], 0
 
     def __getattr__(self, name):
         def function(*args):
             self.calls.append(name)
             if name == 'tt_malloc':
-                args[0]._obj.value = 4096 * (1 + len(self.calls))
+                self.blocks += 1
+                args[0]._obj.value = 4096 * self.blocks
             return 0
         return function
 
@@ -53,3 +54,56 @@ def test_what_is_parked_runs_first(library):
     norm.running_mean.data.__cuda_array_interface__
     assert [n for n in library.since() if 'bn' in n], 'the array is handed out before its update was launched'
     del y
+
+
+def _handed_out(array):
+    return array.__cuda_array_interface__['data'][0]
+
+
+def test_a_shared_array_is_handed_out_as_a_copy(library):
+    """Others write past what the library notes of shared memory: neither holder may see the other's values change."""
+    a = hiparray(np.ones(3, np.float32))
+    b, c = a.alias(), a.lent()
+    at = a.ptr
+    library.since()
+    assert _handed_out(b) not in (0, at) and library.since() == ['tt_malloc', 'tt_memcpy_d2d']
+    assert _handed_out(b) == b.ptr and library.since() == []
+    assert a.ptr == at and c.ptr == at
+    assert _handed_out(c) not in (at, b.ptr) and library.since() == ['tt_malloc', 'tt_memcpy_d2d']
+
+
+def test_loans_of_an_array_are_settled_before_it_is_handed_out(library):
+    a = hiparray(np.ones(3, np.float32))
+    loan = a.lent()
+    library.since()
+    at = a.ptr
+    assert _handed_out(a) == at and library.since() == ['tt_malloc', 'tt_memcpy_d2d'] and loan.ptr != at
+
+
+def test_the_ones_of_backward_passes_are_handed_out_as_copies(library):
+    first = xparray.one(0)
+    assert _handed_out(first) != xparray._one.ptr and not xparray.is_one(first) and xparray.is_one(xparray.one(1))
+
+
+@pytest.mark.parametrize('share', ['alias', 'lent'])
+def test_what_was_handed_out_is_not_shared_afterwards(library, share):
+    """... and so never moves: its receiver keeps the array, which keeps the block."""
+    first, _ = hiparray.carve(((3,), np.float32), ((5,), np.float32))
+    for a in (hiparray(np.ones(3, np.float32)), first, hiparray(np.ones((3, 1), np.float32)).reshape(3)):
+        at = _handed_out(a)
+        other = getattr(a, share)()
+        assert other.ptr != at and not a._shared
+        a += other
+        assert a.ptr == at
+        np.testing.assert_array_equal(a.shape, other.shape)
+
+
+def test_a_gradient_that_was_handed_out(library):
+    x = tt.Tensor(hiparray(np.ones(3, np.float32)), requires_grad=True)
+    g = tt.Tensor(hiparray(np.ones(3, np.float32)))
+    at = _handed_out(g.data)
+    x.backward(g)
+    assert x.grad.ptr != at
+    kept = _handed_out(x.grad)
+    x.backward(g)
+    assert x.grad.ptr == kept and g.data.ptr == at
