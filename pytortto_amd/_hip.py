@@ -21,6 +21,7 @@ PROTOTYPES = {
     'tt_device_info': [c_char_p, _I, POINTER(c_int), POINTER(c_int), POINTER(c_int), POINTER(c_size_t)],
     'tt_malloc': [POINTER(c_void_p), c_size_t],
     'tt_free': [_P],
+    'tt_free_exported': [_P],
     'tt_empty_cache': [],
     'tt_mem_stats': [POINTER(c_size_t), POINTER(c_size_t), POINTER(c_size_t)],
     'tt_memcpy_h2d': [_P, _P, c_size_t],

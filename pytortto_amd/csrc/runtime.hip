@@ -23,7 +23,11 @@ struct State {
   std::unordered_map<void*, size_t> live;            // ptr -> rounded size
   std::map<size_t, std::vector<void*>> pool;         // rounded size -> free blocks
   size_t bytes_live = 0;
-  size_t bytes_pooled = 0;
+  size_t bytes_pooled = 0;                           // free ones, those below among them
+  // free blocks whose addresses others had: work that they gave to other streams may still use them
+  std::vector<std::pair<void*, size_t>> exported;
+  size_t bytes_exported = 0;
+  hipEvent_t exported_event = nullptr;
   void* ws = nullptr;
   size_t ws_bytes = 0;
   int conv_math = TT_CONV_MATH_F32;
@@ -51,12 +55,40 @@ size_t round_size(size_t bytes) {
   return (bytes + big - 1) / big * big;
 }
 
+// Free blocks that others have used wait here until there are this many, so that waiting for the others' work costs one
+// event for all of them and not one for each.
+constexpr size_t kMostExported = 64, kMostExportedBytes = (size_t)2 << 30;
+
+// Gives them back to the pool: what the library launches from here on comes after all that the default stream has been
+// given so far (and streams that it waits for).
+int reclaim_exported() {
+  State& s = S();
+  if (s.exported.empty()) return 0;
+  if (!s.exported_event) TT_HIP(hipEventCreateWithFlags(&s.exported_event, hipEventDisableTiming));
+  TT_HIP(hipEventRecord(s.exported_event, nullptr));
+  TT_HIP(hipStreamWaitEvent(s.stream, s.exported_event, 0));
+  for (auto& block : s.exported) s.pool[block.second].push_back(block.first);
+  s.exported.clear();
+  s.bytes_exported = 0;
+  return 0;
+}
+
+void* take_pooled(size_t rounded) {
+  State& s = S();
+  auto it = s.pool.find(rounded);
+  if (it == s.pool.end() || it->second.empty()) return nullptr;
+  void* p = it->second.back();
+  it->second.pop_back();
+  s.bytes_pooled -= rounded;
+  return p;
+}
+
 int release_pool() {
   State& s = S();
   for (auto& kv : s.pool)
     for (void* p : kv.second) TT_HIP(hipFree(p));
   s.pool.clear();
-  s.bytes_pooled = 0;
+  s.bytes_pooled = s.bytes_exported;
   return 0;
 }
 
@@ -199,16 +231,17 @@ int tt_malloc(void** ptr, size_t bytes) {
   TT_REQUIRE(ptr != nullptr, "tt_malloc: null output pointer");
   State& s = S();
   size_t r = round_size(bytes);
-  auto it = s.pool.find(r);
-  void* p = nullptr;
-  if (it != s.pool.end() && !it->second.empty()) {
-    p = it->second.back();
-    it->second.pop_back();
-    s.bytes_pooled -= r;
-  } else {
+  void* p = take_pooled(r);
+  if (!p && (s.exported.size() >= kMostExported || s.bytes_exported >= kMostExportedBytes)) {
+    // (should that fail, as while a stream is captured, they stay where they are)
+    if (reclaim_exported() == 0) p = take_pooled(r);
+    else (void)hipGetLastError();
+  }
+  if (!p) {
     hipError_t e = hipMalloc(&p, r);
     if (e != hipSuccess) {  // out of memory: give pooled blocks back and try once more
       (void)hipGetLastError();
+      if (reclaim_exported() != 0) (void)hipGetLastError();
       TT_HIP(hipStreamSynchronize(s.stream));
       if (release_pool() != 0) return -1;
       TT_HIP(hipMalloc(&p, r));
@@ -220,25 +253,33 @@ int tt_malloc(void** ptr, size_t bytes) {
   return 0;
 }
 
-int tt_free(void* ptr) {
-  if (ptr == nullptr) return 0;
+static int free_block(const char* fn, void* ptr, bool exported) {
   TT_REQUIRE_INIT();
   State& s = S();
   auto it = s.live.find(ptr);
-  TT_REQUIRE(it != s.live.end(), "tt_free: %p was not allocated by tt_malloc (or freed twice)", ptr);
+  TT_REQUIRE(it != s.live.end(), "%s: %p was not allocated by tt_malloc (or freed twice)", fn, ptr);
   size_t r = it->second;
   s.live.erase(it);
   s.bytes_live -= r;
-  // Reuse is safe without waiting: every consumer of the old contents and every producer of
-  // the new ones is ordered on the single library stream.
-  s.pool[r].push_back(ptr);
   s.bytes_pooled += r;
+  if (exported) {
+    s.exported.emplace_back(ptr, r);
+    s.bytes_exported += r;
+  } else {
+    // Reuse is safe without waiting: every consumer of the old contents and every producer of
+    // the new ones is ordered on the single library stream.
+    s.pool[r].push_back(ptr);
+  }
   return 0;
 }
+
+int tt_free(void* ptr) { return ptr == nullptr ? 0 : free_block("tt_free", ptr, false); }
+int tt_free_exported(void* ptr) { return ptr == nullptr ? 0 : free_block("tt_free_exported", ptr, true); }
 
 int tt_empty_cache(void) {
   TT_REQUIRE_INIT();
   State& s = S();
+  if (reclaim_exported() != 0) return -1;
   TT_HIP(hipStreamSynchronize(s.stream));
   if (release_pool() != 0) return -1;
   if (s.ws) TT_HIP(hipFree(s.ws));

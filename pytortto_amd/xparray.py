@@ -117,7 +117,7 @@ class _Buffer:
     def __del__(self):
         try:
             if self._ptr:
-                _hip._lib.tt_free(self._ptr)
+                (_hip._lib.tt_free_exported if self.exported else _hip._lib.tt_free)(self._ptr)
                 self._ptr = 0
         except Exception:   # interpreter shutdown
             pass
@@ -301,13 +301,17 @@ class hiparray:
         """For torch, CuPy and the like to use the memory in place (``torch.as_tensor(array, device='cuda')``); the
         library's stream has to be waited for, or the device, before they read what it computes.  An array that shares
         its block moves to one of its own, and an array that has been handed out does not share it again: what others
-        write there is seen by the array alone."""
+        write there is seen by the array alone.  Once nobody has the array, its block goes to new ones, which wait for the
+        default stream (torch's, as a rule) and the streams that it waits for; who uses the memory on another one
+        keeps the array until that is done."""
         if _hip._pending is not None:       # what is parked may write here, and waiting would not launch it
             _hip.flush()
         if self._shared or _unfilled:
             self.own()
         at, buf = self.ptr, self._buf
         buf.exported = True
+        if buf.__class__ is _Borrowed and isinstance(buf.owner, _Buffer):       # a part of the library's own block
+            buf.owner.exported = True
         return {'shape': self._shape, 'typestr': self._dtype.str, 'data': (at, False), 'strides': None, 'version': 2}
 
     @property

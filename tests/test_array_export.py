@@ -107,3 +107,32 @@ def test_a_gradient_that_was_handed_out(library):
     kept = _handed_out(x.grad)
     x.backward(g)
     assert x.grad.ptr == kept and g.data.ptr == at
+
+
+def test_blocks_of_arrays_that_were_handed_out_wait_for_others(library):
+    """... whoever holds the array last, also where it is a part of a block."""
+    freed = ('tt_malloc', 'tt_memcpy_h2d', 'tt_memcpy_d2d')
+    a, b = hiparray(np.ones(3, np.float32)), hiparray(np.ones(3, np.float32))
+    view = a.reshape(1, 3)
+    view.__cuda_array_interface__
+    del view
+    library.since()
+    del b
+    assert library.since(*freed) == ['tt_free']
+    del a
+    assert library.since(*freed) == ['tt_free_exported']
+    parts = hiparray.carve(((3,), np.float32), ((5,), np.float32))
+    parts[1].__cuda_array_interface__
+    del parts[1]
+    assert library.since(*freed) == []
+    del parts
+    assert library.since(*freed) == ['tt_free_exported']
+
+
+def test_memory_of_others_that_is_handed_out_again(library):
+    class Foreign:
+        __cuda_array_interface__ = {'shape': (3,), 'typestr': '<f4', 'data': (1 << 20, False), 'version': 3}
+    a = hiparray.borrow(Foreign())
+    assert _handed_out(a) == 1 << 20
+    del a
+    assert library.since() == []
