@@ -62,6 +62,8 @@ int tt_sync(void);
 /* What is launched from here on waits for what another stream of the device has been given so far (1: the default
  * stream, 2: the default stream of the calling thread, else a hipStream_t). */
 int tt_wait_stream(unsigned long long stream);
+/* The hipStream_t that everything here is launched on, for others to wait for. */
+int tt_get_stream(unsigned long long* stream);
 
 /* HIP events on the library stream, for timing kernels from the host side. */
 int tt_event_create(void** event);

@@ -30,6 +30,7 @@ PROTOTYPES = {
     'tt_memset': [_P, _I, c_size_t],
     'tt_sync': [],
     'tt_wait_stream': [ctypes.c_ulonglong],
+    'tt_get_stream': [POINTER(ctypes.c_ulonglong)],
     'tt_set_conv_math': [_I],
     'tt_get_conv_math': [POINTER(c_int)],
     'tt_set_conv_dense_cell_min_tiles': [_I],
@@ -350,6 +351,19 @@ def get_conv_math():
     mode = c_int()
     call('tt_get_conv_math', ctypes.byref(mode))
     return {v: k for k, v in CONV_MATH.items()}[mode.value]
+
+
+_stream = None
+
+
+def stream():
+    """The handle of the stream that everything here is launched on; None while nothing has been."""
+    global _stream
+    if _stream is None and _ready:
+        handle = ctypes.c_ulonglong()
+        call('tt_get_stream', ctypes.byref(handle))
+        _stream = handle.value
+    return _stream
 
 
 def synchronize():

@@ -403,6 +403,13 @@ int tt_wait_stream(unsigned long long stream) {
   return 0;
 }
 
+int tt_get_stream(unsigned long long* stream) {
+  TT_REQUIRE_INIT();
+  TT_REQUIRE(stream != nullptr, "tt_get_stream: null output pointer");
+  *stream = (unsigned long long)S().stream;
+  return 0;
+}
+
 int tt_sync(void) {
   TT_REQUIRE_INIT();
   TT_HIP(hipStreamSynchronize(S().stream));

@@ -298,12 +298,12 @@ class hiparray:
     # ---- ndarray-like attributes ----------------------------------------------------------
     @property
     def __cuda_array_interface__(self):
-        """For torch, CuPy and the like to use the memory in place (``torch.as_tensor(array, device='cuda')``); the
-        library's stream has to be waited for, or the device, before they read what it computes.  An array that shares
-        its block moves to one of its own, and an array that has been handed out does not share it again: what others
-        write there is seen by the array alone.  Once nobody has the array, its block goes to new ones, which wait for the
-        default stream (torch's, as a rule) and the streams that it waits for; who uses the memory on another one
-        keeps the array until that is done."""
+        """For torch, CuPy and the like to use the memory in place (``torch.as_tensor(array, device='cuda')``).
+        The interface names the library's stream; for those that do not wait for it (torch), ``tt.cuda.synchronize()``
+        comes before they read what is computed here.  An array that shares its block moves to one of its own, and an
+        array that has been handed out does not share it again: what others write there is seen by the array alone.
+        Once nobody has the array, its block goes to new ones, which wait for the default stream (torch's, as a rule)
+        and the streams that it waits for; who uses the memory on another one keeps the array until that is done."""
         if _hip._pending is not None:       # what is parked may write here, and waiting would not launch it
             _hip.flush()
         if self._shared or _unfilled:
@@ -312,7 +312,8 @@ class hiparray:
         buf.exported = True
         if buf.__class__ is _Borrowed and isinstance(buf.owner, _Buffer):       # a part of the library's own block
             buf.owner.exported = True
-        return {'shape': self._shape, 'typestr': self._dtype.str, 'data': (at, False), 'strides': None, 'version': 2}
+        return {'shape': self._shape, 'typestr': self._dtype.str, 'data': (at, False), 'strides': None, 'version': 3,
+                'stream': _hip.stream()}
 
     @property
     def ptr(self):

@@ -136,3 +136,21 @@ def test_memory_of_others_that_is_handed_out_again(library):
     assert _handed_out(a) == 1 << 20
     del a
     assert library.since() == []
+
+
+def test_the_stream_is_named(library, monkeypatch):
+    monkeypatch.setattr(_hip, '_stream', None)
+
+    def tt_get_stream(handle):
+        handle._obj.value = 77
+        library.calls.append('tt_get_stream')
+        return 0
+
+    library.tt_get_stream = tt_get_stream
+    a = hiparray(np.ones(3, np.float32))
+    about = a.__cuda_array_interface__
+    assert about['stream'] == 77 and about['version'] == 3 and a.__cuda_array_interface__['stream'] == 77
+    assert library.calls.count('tt_get_stream') == 1
+    monkeypatch.setattr(_hip, '_stream', None)
+    monkeypatch.setattr(_hip, '_ready', False)      # nothing has been launched: there is no stream to wait for
+    assert _hip.stream() is None

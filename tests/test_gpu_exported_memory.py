@@ -85,3 +85,23 @@ def test_twice_is_refused():
     with pytest.raises(RuntimeError, match='tt_free_exported: .* freed twice'):
         _hip.call('tt_free_exported', p)
     _hip.call('tt_free_exported', None)
+
+
+def test_the_stream_that_the_interface_names():
+    """Work on the default stream that waits for the named one finds the result, without any other wait."""
+    z = np.random.default_rng(2).standard_normal((4096, 4096)).astype(np.float32)
+    x = tt.Tensor(hiparray(z))
+    theirs = torch.empty((4096, 4096), device='cuda')
+    torch.cuda.synchronize()
+    tt.cuda.synchronize()
+    for _ in range(3):
+        y = x
+        for _ in range(20):
+            y = tt.nn.functional.layer_norm(y, 4096)
+        handle = y.data.__cuda_array_interface__['stream']
+        assert handle == _hip.stream() and handle > 2
+        torch.cuda.default_stream().wait_stream(torch.cuda.ExternalStream(handle))
+        theirs.copy_(_theirs(y.data))
+        want = y.data.get()
+        np.testing.assert_array_equal(theirs.cpu().numpy(), want)
+        theirs.zero_()
