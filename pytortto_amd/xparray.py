@@ -273,7 +273,8 @@ class hiparray:
         CuPy array); nothing is copied and ``source`` is kept alive with the array.  Where the interface names the
         stream of its writers, the library's waits for it; where it does not (torch), they must be done, or be ordered
         in front of the library's stream, before the array is used.  The memory must not be given to others before what
-        reads it here is done, and it is borrowed once, not as two arrays."""
+        reads it here is done, and it is borrowed once, not as two arrays.  Read-only memory is copied before it is
+        written."""
         about = source.__cuda_array_interface__
         shape, kind, get = tuple(about['shape']), about['typestr'], about.get
         known = _DTYPES.get(kind)
@@ -293,7 +294,10 @@ class hiparray:
                 if n != 1 and step != whole:
                     raise ValueError(f'device arrays are C-contiguous, got strides {tuple(strides)} for shape {shape}')
                 whole *= n
-        return cls.on(_Borrowed(about['data'][0] or 0, nbytes, source), shape, dtype)
+        at, read_only = about['data']
+        out = cls.on(_Borrowed(at or 0, nbytes, source), shape, dtype)
+        out._shared = bool(read_only)       # who writes it gets a copy
+        return out
 
     # ---- ndarray-like attributes ----------------------------------------------------------
     @property

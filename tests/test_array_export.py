@@ -154,3 +154,19 @@ def test_the_stream_is_named(library, monkeypatch):
     monkeypatch.setattr(_hip, '_stream', None)
     monkeypatch.setattr(_hip, '_ready', False)      # nothing has been launched: there is no stream to wait for
     assert _hip.stream() is None
+
+
+def test_read_only_memory_of_others_is_not_written(library):
+    class Foreign:
+        def __init__(self, read_only):
+            self.__cuda_array_interface__ = {'shape': (3,), 'typestr': '<f4', 'data': (1 << 20, read_only), 'version': 3}
+
+    for write in (lambda a: a.fill(1.0), lambda a: a.__iadd__(1.0), lambda a: a.set(np.ones(3)), lambda a: a.own(),
+                  lambda a: a.__cuda_array_interface__):
+        a, b = hiparray.borrow(Foreign(True)), hiparray.borrow(Foreign(False))
+        assert a.ptr == b.ptr == 1 << 20
+        library.since()
+        write(a)
+        assert a.ptr != 1 << 20 and library.since()[:2] == ['tt_malloc', 'tt_memcpy_d2d']
+        write(b)
+        assert b.ptr == 1 << 20 and 'tt_memcpy_d2d' not in library.since()
