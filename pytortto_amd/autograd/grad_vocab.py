@@ -71,7 +71,8 @@ class TokenLogProb(Function):
         values = (logp, entropy, top_logp) if top else (logp, entropy)
         outputs = tuple(build_links(y, grad_fn=ctx, _output_idx=i) for i, y in enumerate(values))
         index = Tensor(top_index, dtype=top_index.dtype, copy=False) if top else None
-        ctx.save_for_backward(xt0, tokens, outputs[1], index)
+        # (of the entropy its array alone: the output itself hangs on this node, and the two would keep each other)
+        ctx.save_for_backward(xt0, tokens, Tensor.on(entropy), index)
         ctx.params['stats'] = stats
         return outputs if index is None else outputs + (index,)
 
