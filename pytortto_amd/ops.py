@@ -664,6 +664,7 @@ def nll_loss_bwd(g, logp_shape, target, weight, count, ignore_index, reduction):
 
 _TYPES = {np.dtype(np.float32): 0, np.dtype(np.float16): 1}
 _INDEX_BITS = {np.dtype(np.int64): 64, np.dtype(np.int32): 32}
+_LONGEST_ROW = 1 << 30
 MOST_ALTERNATIVES = 64
 MOST_TEACHER_ENTRIES = 1024
 
@@ -682,12 +683,19 @@ def _index_bits(a, what):
     return bits
 
 
+def _row(fn, n):
+    """The length of a row, checked here: the C ABI takes an int, which ctypes makes of any number."""
+    if n > _LONGEST_ROW:
+        raise RuntimeError(f'{fn}: rows have 2^30 values at most, got {n}')
+    return n
+
+
 def layer_norm_fwd(x, weight, bias, width, eps, keep):
     """(y, stats) over the trailing ``width`` values; the statistics, every row's mean and then every row's reciprocal
     deviation, are None unless ``keep``."""
     kind = _kind(x, 'the input of layer_norm')
     _f32(weight, bias)
-    rows = x.size // width
+    rows = x.size // _row('layer_norm', width)
     y = hiparray.empty(x._shape, x._dtype)
     stats = mean = rstd = None
     if keep:
@@ -724,7 +732,7 @@ def token_log_prob_fwd(x, tokens, top, ignore_index, keep):
     """(logp, entropy, top_logp, top_index, stats); the alternatives are None without ``top``, the statistics unless
     ``keep``."""
     kind, bits = _kind(x, 'logits'), _index_bits(tokens, 'tokens')
-    rows, vocab = tokens.size, x._shape[-1]
+    rows, vocab = tokens.size, _row('token_log_prob', x._shape[-1])
     wanted = [(tokens._shape, _F32), (tokens._shape, _F32)]
     if top:
         wanted += [(tokens._shape + (top,), _F32), (tokens._shape + (top,), np.int64)]
@@ -763,7 +771,7 @@ def distill_fwd(x, teacher, index, temperature, reduction, need_grad):
     has it for one more write of the row; else None."""
     kinds, bits = (_kind(x, 'logits'), _kind(teacher, "the teacher's logits")), _index_bits(index, "the teacher's indexes")
     red = _REDUCTIONS[reduction]
-    vocab, entries = x._shape[-1], index._shape[-1]
+    vocab, entries = _row('distill_loss', x._shape[-1]), index._shape[-1]
     rows = index.size // entries
     loss, stats, count = hiparray.carve((x._shape[:-1] if red == 0 else (), _F32), ((rows, 2), _F32), ((1,), _F32))
     dx = None
