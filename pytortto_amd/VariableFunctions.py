@@ -46,10 +46,14 @@ def tensor(data, requires_grad=False, dtype=None, copy=True, **kwargs):
 
 def as_tensor(data, requires_grad=False):
     """A device tensor on the memory of an object with ``__cuda_array_interface__`` (a torch or CuPy array), without a
-    copy; see ``hiparray.borrow`` for what its owner has to keep to.  Tensors come back as they are."""
+    copy; see ``hiparray.borrow`` for what its owner has to keep to.  Tensors come back as they are, or, where a gradient
+    is asked for that they do not require, as a new leaf on the same memory."""
     if isinstance(data, Tensor):
-        return data
-    out = Tensor.on(hiparray.borrow(data))
+        if data.requires_grad or not requires_grad:
+            return data
+        out = data.detach()
+    else:
+        out = Tensor.on(hiparray.borrow(data))
     if requires_grad:
         out.requires_grad = True
     return out

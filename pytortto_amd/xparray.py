@@ -275,7 +275,11 @@ class hiparray:
         in front of the library's stream, before the array is used.  The memory must not be given to others before what
         reads it here is done, and it is borrowed once, not as two arrays.  Read-only memory is copied before it is
         written."""
-        about = source.__cuda_array_interface__
+        try:
+            about = source.__cuda_array_interface__
+        except AttributeError as exc:
+            raise AttributeError(f'as_tensor takes device memory (an object with __cuda_array_interface__), got '
+                                 f'{source.__class__.__name__}; tt.tensor(...).cuda() copies data from the host') from exc
         shape, kind, get = tuple(about['shape']), about['typestr'], about.get
         known = _DTYPES.get(kind)
         if known is None:
