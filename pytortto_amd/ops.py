@@ -690,12 +690,18 @@ def _row(fn, n):
     return n
 
 
+def _aligned(a):
+    """The array, or a copy where it is a slice of others' memory that begins off the kernels' sixteen bytes."""
+    return a if a is None or a.ptr & 15 == 0 else a.copy()
+
+
 def layer_norm_fwd(x, weight, bias, width, eps, keep):
     """(y, stats) over the trailing ``width`` values; the statistics, every row's mean and then every row's reciprocal
     deviation, are None unless ``keep``."""
     kind = _kind(x, 'the input of layer_norm')
     _f32(weight, bias)
     rows = x.size // _row('layer_norm', width)
+    x, weight, bias = _aligned(x), _aligned(weight), _aligned(bias)
     y = hiparray.empty(x._shape, x._dtype)
     stats = mean = rstd = None
     if keep:
@@ -713,6 +719,7 @@ def layer_norm_bwd(x, dy, weight, stats, shape, need):
         raise TypeError(f'the gradient of layer_norm must be like its output, {x._dtype} {x._shape}, got {dy._dtype} '
                         f'{dy._shape}')
     rows = stats._shape[1]
+    x, dy, weight = _aligned(x), _aligned(dy), _aligned(weight)
     dx = hiparray.empty(x._shape, x._dtype) if need[0] else None
     dw = db = None
     if rows and need[1] and need[2]:
@@ -733,6 +740,7 @@ def token_log_prob_fwd(x, tokens, top, ignore_index, keep):
     ``keep``."""
     kind, bits = _kind(x, 'logits'), _index_bits(tokens, 'tokens')
     rows, vocab = tokens.size, _row('token_log_prob', x._shape[-1])
+    x = _aligned(x)
     wanted = [(tokens._shape, _F32), (tokens._shape, _F32)]
     if top:
         wanted += [(tokens._shape + (top,), _F32), (tokens._shape + (top,), np.int64)]
@@ -751,6 +759,7 @@ def token_log_prob_bwd(x, tokens, stats, entropy, top_index, gradients, top, ign
     """dlogits from the gradients of (logp, entropy, top_logp), each of which may be None."""
     _f32(*gradients)
     rows = tokens.size
+    x = _aligned(x)
     dx = hiparray.empty(x._shape, x._dtype)
     if rows:
         _hip.call('tt_token_log_prob_bwd', x.ptr, tokens.ptr, stats.ptr, entropy.ptr, _ptr(top_index),
@@ -773,6 +782,7 @@ def distill_fwd(x, teacher, index, temperature, reduction, need_grad):
     red = _REDUCTIONS[reduction]
     vocab, entries = _row('distill_loss', x._shape[-1]), index._shape[-1]
     rows = index.size // entries
+    x = _aligned(x)
     loss, stats, count = hiparray.carve((x._shape[:-1] if red == 0 else (), _F32), ((rows, 2), _F32), ((1,), _F32))
     dx = None
     if rows:
@@ -793,6 +803,7 @@ def distill_bwd(x, teacher, index, stats, count, g, dx, temperature, reduction):
         return dx
     entries = index._shape[-1]
     rows = index.size // entries
+    x = _aligned(x)
     if not ahead:
         dx = hiparray.empty(x._shape, x._dtype)
     if rows:
