@@ -49,8 +49,8 @@ int tt_device_info(char* name, int name_len, int* compute_units, int* clock_khz,
 int tt_malloc(void** ptr, size_t bytes);      /* pooled: freed blocks are reused by size class */
 int tt_free(void* ptr);
 /* The same for a block whose address others have had (an exported array): it is not handed out again before what the
- * default stream has been given until then is done.  (A stream that the default stream does not wait for, a non-blocking
- * one, must be done with the block, or the default stream wait for it, before this call.) */
+ * default stream has been given until then is done.  (Work on other streams must be done, or the default stream wait for
+ * it, before this call.) */
 int tt_free_exported(void* ptr);
 int tt_empty_cache(void);                     /* return pooled blocks and the workspace to HIP */
 int tt_mem_stats(size_t* bytes_in_use, size_t* bytes_pooled, size_t* workspace_bytes);

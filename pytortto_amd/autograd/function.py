@@ -241,9 +241,12 @@ def toposort(*end_nodes):
     those ``waiting`` once nothing else is ready.  Of several end nodes, one that others lead to waits for them.
     Where several nodes wait then, one of them may lead to another, so from there on the edges that are left in this pass
     are counted, and not those of all consumers."""
-    ready = [node for node in end_nodes if node.prev_function_counts == 0]
-    waiting = {node: None for node in end_nodes if node.prev_function_counts}     # (in the order of their arrival)
-    left = None
+    ready, waiting, left = [], {}, None         # (``waiting``: in the order of their arrival)
+    for node in end_nodes:
+        if node.prev_function_counts:
+            waiting[node] = None
+        else:
+            ready.append(node)
     while ready or waiting:
         if ready:
             node = ready.pop()

@@ -29,21 +29,22 @@ class LayerNorm(Function):
         w = None if xt1 is None else xt1.data
         b = None if xt2 is None else xt2.data
         _same_device('layer_norm', w, b)
-        if not shape or xd0.shape[-len(shape):] != shape:
+        if not shape or xd0._shape[-len(shape):] != shape:
             raise RuntimeError(f'Given normalized_shape={list(shape)}, expected input with shape '
                                f'[*{"".join(f", {n}" for n in shape)}], but got input of size {list(xd0.shape)}')
         width = prod(shape)
         if width == 0:
             raise RuntimeError(f'layer_norm needs at least one value to normalise over, got {list(shape)}')
-        for name, d in (('weight', w), ('bias', b)):
-            if d is not None and d.shape != shape:
-                raise RuntimeError(f'Expected {name} to be of same shape as normalized_shape, but got {name} of shape '
-                                   f'{list(d.shape)} and normalized_shape = {list(shape)}')
+        if (w is not None and w._shape != shape) or (b is not None and b._shape != shape):
+            name, d = ('weight', w) if w is not None and w._shape != shape else ('bias', b)
+            raise RuntimeError(f'Expected {name} to be of same shape as normalized_shape, but got {name} of shape '
+                               f'{list(d.shape)} and normalized_shape = {list(shape)}')
         keep = ctx.requires_grad and is_grad_enabled()
         yd0, stats = ops.layer_norm_fwd(xd0, w, b, width, eps, keep)
         yt0 = build_links(yd0, grad_fn=ctx)
-        ctx.save_for_backward(xt0, xt1)
-        ctx.params = {'stats': stats, 'shape': shape}
+        if keep:
+            ctx.save_for_backward(xt0, xt1)
+            ctx.params = {'stats': stats, 'shape': shape}
         return yt0
 
     @staticmethod
@@ -70,10 +71,11 @@ class TokenLogProb(Function):
         logp, entropy, top_logp, top_index, stats = ops.token_log_prob_fwd(xd0, td0, top, params['ignore_index'], keep)
         values = (logp, entropy, top_logp) if top else (logp, entropy)
         outputs = tuple(build_links(y, grad_fn=ctx, _output_idx=i) for i, y in enumerate(values))
-        index = Tensor(top_index, dtype=top_index.dtype, copy=False) if top else None
-        # (of the entropy its array alone: the output itself hangs on this node, and the two would keep each other)
-        ctx.save_for_backward(xt0, tokens, Tensor.on(entropy), index)
-        ctx.params['stats'] = stats
+        index = Tensor.on(top_index) if top else None
+        if keep:
+            # (of the entropy its array alone: the output itself hangs on this node, and the two would keep each other)
+            ctx.save_for_backward(xt0, tokens, Tensor.on(entropy), index)
+            ctx.params['stats'] = stats
         return outputs if index is None else outputs + (index,)
 
     @staticmethod
@@ -106,8 +108,9 @@ class DistillLoss(Function):
         keep = ctx.requires_grad and is_grad_enabled()
         yd0, stats, count, dx = ops.distill_fwd(xd0, td0, id0, params['temperature'], params['reduction'], keep)
         yt0 = build_links(yd0, grad_fn=ctx)
-        ctx.save_for_backward(xt0, teacher, index)
-        ctx.params.update(stats=stats, count=count, dx=dx)
+        if keep:
+            ctx.save_for_backward(xt0, teacher, index)
+            ctx.params.update(stats=stats, count=count, dx=dx)
         return yt0
 
     @staticmethod

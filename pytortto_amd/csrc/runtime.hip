@@ -55,18 +55,25 @@ size_t round_size(size_t bytes) {
   return (bytes + big - 1) / big * big;
 }
 
-// Free blocks that others have used wait here until there are this many, so that waiting for the others' work costs one
-// event for all of them and not one for each.
+// Gives the blocks that others have used back to the pool, if the default stream has no work left that may use them.
+// Where it has, `wait` makes the library's stream wait for what the default stream has been given so far.
+// A few small blocks are left alone, so that a call of a few microseconds does not ask for the stream's state each time
+// (0.3 us); larger ones go back as soon as they can, while the caches still have them (38 MB each: 58 us a call of layer
+// normalisation and its gradient in turn over 64 blocks, 54 over as many as there have to be).  The event, too, is for all
+// blocks at once, and left until there are so many of them.
+constexpr size_t kFewExported = 16, kFewExportedBytes = (size_t)16 << 20;
 constexpr size_t kMostExported = 64, kMostExportedBytes = (size_t)2 << 30;
-
-// Gives them back to the pool: what the library launches from here on comes after all that the default stream has been
-// given so far (and streams that it waits for).
-int reclaim_exported() {
+int reclaim_exported(bool wait) {
   State& s = S();
   if (s.exported.empty()) return 0;
-  if (!s.exported_event) TT_HIP(hipEventCreateWithFlags(&s.exported_event, hipEventDisableTiming));
-  TT_HIP(hipEventRecord(s.exported_event, nullptr));
-  TT_HIP(hipStreamWaitEvent(s.stream, s.exported_event, 0));
+  const hipError_t e = hipStreamQuery(nullptr);
+  if (e != hipSuccess) {
+    (void)hipGetLastError();
+    if (!wait) return 0;
+    if (!s.exported_event) TT_HIP(hipEventCreateWithFlags(&s.exported_event, hipEventDisableTiming));
+    TT_HIP(hipEventRecord(s.exported_event, nullptr));
+    TT_HIP(hipStreamWaitEvent(s.stream, s.exported_event, 0));
+  }
   for (auto& block : s.exported) s.pool[block.second].push_back(block.first);
   s.exported.clear();
   s.bytes_exported = 0;
@@ -232,16 +239,17 @@ int tt_malloc(void** ptr, size_t bytes) {
   State& s = S();
   size_t r = round_size(bytes);
   void* p = take_pooled(r);
-  if (!p && (s.exported.size() >= kMostExported || s.bytes_exported >= kMostExportedBytes)) {
+  if (!p && (s.exported.size() >= kFewExported || s.bytes_exported >= kFewExportedBytes)) {
     // (should that fail, as while a stream is captured, they stay where they are)
-    if (reclaim_exported() == 0) p = take_pooled(r);
+    const bool wait = s.exported.size() >= kMostExported || s.bytes_exported >= kMostExportedBytes;
+    if (reclaim_exported(wait) == 0) p = take_pooled(r);
     else (void)hipGetLastError();
   }
   if (!p) {
     hipError_t e = hipMalloc(&p, r);
     if (e != hipSuccess) {  // out of memory: give pooled blocks back and try once more
       (void)hipGetLastError();
-      if (reclaim_exported() != 0) (void)hipGetLastError();
+      if (reclaim_exported(true) != 0) (void)hipGetLastError();
       TT_HIP(hipStreamSynchronize(s.stream));
       if (release_pool() != 0) return -1;
       TT_HIP(hipMalloc(&p, r));
@@ -279,7 +287,7 @@ int tt_free_exported(void* ptr) { return ptr == nullptr ? 0 : free_block("tt_fre
 int tt_empty_cache(void) {
   TT_REQUIRE_INIT();
   State& s = S();
-  if (reclaim_exported() != 0) return -1;
+  if (reclaim_exported(true) != 0) return -1;
   TT_HIP(hipStreamSynchronize(s.stream));
   if (release_pool() != 0) return -1;
   if (s.ws) TT_HIP(hipFree(s.ws));

@@ -16,7 +16,7 @@ from . import _hip
 from .xparray import hiparray, is_one, poison
 
 
-_F32, _F16 = np.dtype(np.float32), np.dtype(np.float16)
+_F32, _F16, _I64 = np.dtype(np.float32), np.dtype(np.float16), np.dtype(np.int64)
 
 
 def _ptr(a):
@@ -683,11 +683,9 @@ def _index_bits(a, what):
     return bits
 
 
-def _row(fn, n):
-    """The length of a row, checked here: the C ABI takes an int, which ctypes makes of any number."""
-    if n > _LONGEST_ROW:
-        raise RuntimeError(f'{fn}: rows have 2^30 values at most, got {n}')
-    return n
+def _refuse_row(fn, n):
+    """(Checked here because the C ABI takes an int, which ctypes makes of any number.)"""
+    raise RuntimeError(f'{fn}: rows have 2^30 values at most, got {n}')
 
 
 def _aligned(a):
@@ -700,8 +698,12 @@ def layer_norm_fwd(x, weight, bias, width, eps, keep):
     deviation, are None unless ``keep``."""
     kind = _kind(x, 'the input of layer_norm')
     _f32(weight, bias)
-    rows = x.size // _row('layer_norm', width)
-    x, weight, bias = _aligned(x), _aligned(weight), _aligned(bias)
+    if width > _LONGEST_ROW:
+        _refuse_row('layer_norm', width)
+    xp, wp, bp = x.ptr, _ptr(weight), _ptr(bias)
+    if (xp | (wp or 0) | (bp or 0)) & 15:
+        return layer_norm_fwd(_aligned(x), _aligned(weight), _aligned(bias), width, eps, keep)
+    rows = x.size // width
     y = hiparray.empty(x._shape, x._dtype)
     stats = mean = rstd = None
     if keep:
@@ -709,7 +711,7 @@ def layer_norm_fwd(x, weight, bias, width, eps, keep):
         mean = stats.ptr
         rstd = mean + 4 * rows
     if rows:
-        _hip.call('tt_layer_norm_fwd', x.ptr, _ptr(weight), _ptr(bias), y.ptr, mean, rstd, eps, kind, rows, width)
+        _hip.call('tt_layer_norm_fwd', xp, wp, bp, y.ptr, mean, rstd, eps, kind, rows, width)
     return y, stats
 
 
@@ -718,8 +720,10 @@ def layer_norm_bwd(x, dy, weight, stats, shape, need):
     if dy._dtype != x._dtype or dy._shape != x._shape:
         raise TypeError(f'the gradient of layer_norm must be like its output, {x._dtype} {x._shape}, got {dy._dtype} '
                         f'{dy._shape}')
+    xp, gp, wp = x.ptr, dy.ptr, _ptr(weight)
+    if (xp | gp | (wp or 0)) & 15:
+        return layer_norm_bwd(_aligned(x), _aligned(dy), _aligned(weight), stats, shape, need)
     rows = stats._shape[1]
-    x, dy, weight = _aligned(x), _aligned(dy), _aligned(weight)
     dx = hiparray.empty(x._shape, x._dtype) if need[0] else None
     dw = db = None
     if rows and need[1] and need[2]:
@@ -730,7 +734,7 @@ def layer_norm_bwd(x, dy, weight, stats, shape, need):
         db = make(shape) if need[2] else None
     if rows:
         mean = stats.ptr
-        _hip.call('tt_layer_norm_bwd', x.ptr, dy.ptr, _ptr(weight), mean, mean + 4 * rows, _ptr(dx), _ptr(dw), _ptr(db),
+        _hip.call('tt_layer_norm_bwd', xp, gp, wp, mean, mean + 4 * rows, _ptr(dx), _ptr(dw), _ptr(db),
                   _TYPES[x._dtype], rows, prod(shape))
     return dx, dw, db
 
@@ -739,18 +743,23 @@ def token_log_prob_fwd(x, tokens, top, ignore_index, keep):
     """(logp, entropy, top_logp, top_index, stats); the alternatives are None without ``top``, the statistics unless
     ``keep``."""
     kind, bits = _kind(x, 'logits'), _index_bits(tokens, 'tokens')
-    rows, vocab = tokens.size, _row('token_log_prob', x._shape[-1])
-    x = _aligned(x)
+    rows, vocab = tokens.size, x._shape[-1]
+    if vocab > _LONGEST_ROW:
+        _refuse_row('token_log_prob', vocab)
+    xp = x.ptr
+    if xp & 15:
+        x = x.copy()
+        xp = x.ptr
     wanted = [(tokens._shape, _F32), (tokens._shape, _F32)]
     if top:
-        wanted += [(tokens._shape + (top,), _F32), (tokens._shape + (top,), np.int64)]
+        wanted += [(tokens._shape + (top,), _F32), (tokens._shape + (top,), _I64)]
     if keep:
         wanted.append(((rows, 2), _F32))
     logp, entropy, *more = hiparray.carve(*wanted)
     stats = more.pop() if keep else None
     top_logp, top_index = more or (None, None)
     if rows:
-        _hip.call('tt_token_log_prob_fwd', x.ptr, tokens.ptr, logp.ptr, entropy.ptr, _ptr(top_logp), _ptr(top_index),
+        _hip.call('tt_token_log_prob_fwd', xp, tokens.ptr, logp.ptr, entropy.ptr, _ptr(top_logp), _ptr(top_index),
                   _ptr(stats), kind, bits, ignore_index, rows, vocab, top)
     return logp, entropy, top_logp, top_index, stats
 
@@ -758,11 +767,13 @@ def token_log_prob_fwd(x, tokens, top, ignore_index, keep):
 def token_log_prob_bwd(x, tokens, stats, entropy, top_index, gradients, top, ignore_index):
     """dlogits from the gradients of (logp, entropy, top_logp), each of which may be None."""
     _f32(*gradients)
-    rows = tokens.size
-    x = _aligned(x)
+    rows, xp = tokens.size, x.ptr
+    if xp & 15:
+        x = x.copy()
+        xp = x.ptr
     dx = hiparray.empty(x._shape, x._dtype)
     if rows:
-        _hip.call('tt_token_log_prob_bwd', x.ptr, tokens.ptr, stats.ptr, entropy.ptr, _ptr(top_index),
+        _hip.call('tt_token_log_prob_bwd', xp, tokens.ptr, stats.ptr, entropy.ptr, _ptr(top_index),
                   *[_ptr(g) for g in gradients], dx.ptr, _TYPES[x._dtype], _INDEX_BITS[tokens._dtype], ignore_index,
                   rows, x._shape[-1], top)
     return dx
@@ -780,15 +791,19 @@ def distill_fwd(x, teacher, index, temperature, reduction, need_grad):
     has it for one more write of the row; else None."""
     kinds, bits = (_kind(x, 'logits'), _kind(teacher, "the teacher's logits")), _index_bits(index, "the teacher's indexes")
     red = _REDUCTIONS[reduction]
-    vocab, entries = _row('distill_loss', x._shape[-1]), index._shape[-1]
-    rows = index.size // entries
-    x = _aligned(x)
+    vocab, entries = x._shape[-1], index._shape[-1]
+    if vocab > _LONGEST_ROW:
+        _refuse_row('distill_loss', vocab)
+    rows, xp = index.size // entries, x.ptr
+    if xp & 15:
+        x = x.copy()
+        xp = x.ptr
     loss, stats, count = hiparray.carve((x._shape[:-1] if red == 0 else (), _F32), ((rows, 2), _F32), ((1,), _F32))
     dx = None
     if rows:
         if need_grad and _distill_ahead(kinds[0], red, rows, vocab):
             dx = hiparray.empty(x._shape, x._dtype)
-        _hip.call('tt_distill_fwd', x.ptr, teacher.ptr, index.ptr, loss.ptr, stats.ptr, count.ptr, _ptr(dx), temperature,
+        _hip.call('tt_distill_fwd', xp, teacher.ptr, index.ptr, loss.ptr, stats.ptr, count.ptr, _ptr(dx), temperature,
                   red, *kinds, bits, rows, vocab, entries)
     elif red:
         loss.fill(0.0 if red == 1 else math.nan)

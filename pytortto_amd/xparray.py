@@ -57,7 +57,7 @@ class Device:
 
 
 _F32, _F16 = np.dtype(np.float32), np.dtype(np.float16)
-_void_p, _byref = ctypes.c_void_p, ctypes.byref
+_void_p, _byref, _new = ctypes.c_void_p, ctypes.byref, object.__new__
 _DTYPES = {}            # of array interfaces' type strings
 
 
@@ -160,10 +160,7 @@ class _Loan(_Buffer):
 class _Borrowed(_Buffer):
     """A block that somebody else allocated, or a part of another one; ``owner`` is kept for as long as an array refers
     to it."""
-    __slots__ = ('owner',)
-
-    def __init__(self, ptr, nbytes, owner):
-        self._ptr, self.nbytes, self.owner, self.on_demand, self.deps, self.exported = ptr, nbytes, owner, None, (), False
+    __slots__ = ('owner',)      # (made without a constructor, by ``carve`` and ``borrow``)
 
     def __del__(self):
         pass
@@ -245,16 +242,21 @@ class hiparray:
     @classmethod
     def carve(cls, *wanted):
         """Arrays of the (shape, dtype) wanted on one block: what one operation returns together, for one allocation."""
-        ends, at = [], 0
+        sizes, at = [], 0
         for shape, dtype in wanted:
-            if dtype.__class__ is type:
-                dtype = np.dtype(dtype)
-            size = prod(shape) * dtype.itemsize
-            ends.append((shape, dtype, size, at))
+            size = prod(shape) * (dtype if dtype.__class__ is not type else np.dtype(dtype)).itemsize
+            sizes.append(size)
             at += (size + 255) & -256
         block = _Buffer(at)
-        first = block._ptr
-        return [cls.on(_Borrowed(first + start, size, block), shape, dtype) for shape, dtype, size, start in ends]
+        at, arrays = block._ptr, []
+        for (shape, dtype), size in zip(wanted, sizes):
+            buf, array = _new(_Borrowed), _new(cls)
+            buf._ptr, buf.nbytes, buf.owner, buf.on_demand, buf.deps, buf.exported = at, size, block, None, (), False
+            array._buf, array._shape, array._version, array._shared = buf, shape, [0], False
+            array._dtype = dtype if dtype.__class__ is not type else np.dtype(dtype)
+            arrays.append(array)
+            at += (size + 255) & -256
+        return arrays
 
     @classmethod
     def zeros(cls, shape, dtype=np.float32):
@@ -299,9 +301,11 @@ class hiparray:
                     raise ValueError(f'device arrays are C-contiguous, got strides {tuple(strides)} for shape {shape}')
                 whole *= n
         at, read_only = about['data']
-        out = cls.on(_Borrowed(at or 0, nbytes, source), shape, dtype)
-        out._shared = bool(read_only)       # who writes it gets a copy
-        return out
+        self, buf = _new(cls), _new(_Borrowed)
+        buf._ptr, buf.nbytes, buf.owner, buf.on_demand, buf.deps, buf.exported = at or 0, nbytes, source, None, (), False
+        self._buf, self._shape, self._dtype, self._version = buf, shape, dtype, [0]
+        self._shared = bool(read_only)      # (who writes it gets a copy)
+        return self
 
     # ---- ndarray-like attributes ----------------------------------------------------------
     @property
@@ -310,18 +314,22 @@ class hiparray:
         The interface names the library's stream; for those that do not wait for it (torch), ``tt.cuda.synchronize()``
         comes before they read what is computed here.  An array that shares its block moves to one of its own, and an
         array that has been handed out does not share it again: what others write there is seen by the array alone.
-        Once nobody has the array, its block goes to new ones, which wait for the default stream (torch's, as a rule)
-        and the streams that it waits for; who uses the memory on another one keeps the array until that is done."""
+        Once nobody has the array, its block goes to new ones when the default stream (torch's, as a rule) is done with
+        it; who uses the memory on another stream keeps the array until that is done."""
+        if not self._buf.exported or self._shared or _hip._pending is not None:
+            self._hand_out()
+        return {'shape': self._shape, 'typestr': self._dtype.str, 'data': (self.ptr, False), 'strides': None, 'version': 3,
+                'stream': _hip._stream or _hip.stream()}
+
+    def _hand_out(self):
         if _hip._pending is not None:       # what is parked may write here, and waiting would not launch it
             _hip.flush()
-        if self._shared or _unfilled:
+        if self._shared or _unfilled.data:
             self.own()
-        at, buf = self.ptr, self._buf
+        buf = self._buf
         buf.exported = True
-        if buf.__class__ is _Borrowed and isinstance(buf.owner, _Buffer):       # a part of the library's own block
+        if buf.__class__ is _Borrowed and buf.owner.__class__ is _Buffer:       # a part of the library's own block
             buf.owner.exported = True
-        return {'shape': self._shape, 'typestr': self._dtype.str, 'data': (at, False), 'strides': None, 'version': 3,
-                'stream': _hip.stream()}
 
     @property
     def ptr(self):
