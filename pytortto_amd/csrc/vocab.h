@@ -70,7 +70,9 @@ struct Stat {
   float m, s, t;
 };
 
-// v_exp_f32: results below 2^-126 are zero, which no sum or gradient of float32 here can tell
+// v_exp_f32: results below 2^-126 are zero, which no sum or gradient of float32 here can tell.  Its argument is a rounded
+// product, so the result is off by up to |d| 2^-24 of itself, which an exponential of z - m would not be: the price of one
+// instruction for it.  It weighs where the result is small: 2e-6 of a probability of 1e-12.
 __device__ __forceinline__ float pow2(float d) { return __builtin_amdgcn_exp2f(d); }
 // Of a row of -inf alone m stays -inf; differences are then taken from zero and every 2^d is zero.
 __device__ __forceinline__ float anchor(float m) { return m == -INFINITY ? 0.f : m; }
