@@ -47,11 +47,12 @@ template <typename T>
 __device__ __forceinline__ bool whole_lines(int D) {
   return D % (128 / (int)sizeof(T)) == 0;
 }
-// `passing`: on its way to memory at once, past the caches, which then hold more of what is read. Float32 rows that end
-// inside a line of memory and have a part of a wave each, so that its pieces come from several instructions, are better
-// left to the cache, which puts them together (forward at 2^27 values: 72 columns 209 us, 394 passing, 264 columns 215
-// and 226; but 2500 columns, a block to a row, 210 and 199). Halves always pass (385 columns at 2^25 values 36 us, 37 if
-// they do not).
+// `passing`: on its way to memory at once, past the caches, which then hold more of what is read. Float32 rows of the
+// forward pass that end inside a line of memory and have a part of a wave each, so that its pieces come from several
+// instructions, are better left to the cache, which puts them together (2^27 values: 72 columns 193 us, 389 passing, 260
+// columns 190 and 235; but 2500 columns, a block to a row, 195 and 185). Halves always pass (385 columns at 2^25 values 36
+// us, 37 if they do not), and so does the backward pass, which has more to read (2^25 values: 60 columns 67 us, 81 left
+// to the cache, 176 columns 69 and 79; 2^27 values: level within 5 %, but 30 columns 418 and 391).
 template <typename T>
 __device__ __forceinline__ void write_columns(T* row, int q, int D, const typename Loose<T>::type& p,
                                               bool passing = true) {
@@ -188,7 +189,6 @@ __global__ __launch_bounds__(G ? kBwdBlock : kMostBlock) void ln_bwd(const T* __
   const int sub = G ? tt::row_of_block<G ? G : 1>() : __builtin_amdgcn_readfirstlane(threadIdx.y);
   const int thread = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
   const int all_packs = (D + n - 1) / n;
-  const bool passing = G == 0 || G > 16 || whole_lines<T>(D);   // (132 columns 91 us, 84 not passing)
   float sums[2][NV][n] = {};        // dw, db
   float wv[NV][n];
 #pragma unroll
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(G ? kBwdBlock : kMostBlock) void ln_bwd(const T* __
         const float nn = (tt::widen(xv[u][i]) - m) * r;
         o[i] = (T)(r * (tt::widen(gv[u][i]) * wv[u][i] - mh - nn * mhn));
       }
-      write_columns(dx + base, q, D, o, passing);
+      write_columns(dx + base, q, D, o);
     }
   }
   if (!dw_out && !db_out) return;
