@@ -50,9 +50,10 @@ __device__ __forceinline__ bool whole_lines(int D) {
 // `passing`: on its way to memory at once, past the caches, which then hold more of what is read. Float32 rows of the
 // forward pass that end inside a line of memory and have a part of a wave each, so that its pieces come from several
 // instructions, are better left to the cache, which puts them together (2^27 values: 72 columns 193 us, 389 passing, 260
-// columns 190 and 235; but 2500 columns, a block to a row, 195 and 185). Halves always pass (385 columns at 2^25 values 36
-// us, 37 if they do not), and so does the backward pass, which has more to read (2^25 values: 60 columns 67 us, 81 left
-// to the cache, 176 columns 69 and 79; 2^27 values: level within 5 %, but 30 columns 418 and 391).
+// columns 190 and 235). Rows that come from one instruction pass (20 columns at 2^27 values 255 us and 249, at 2^25 61 and
+// 46), and so do those of a wave or a block (2500 columns 195 and 185), halves (385 columns at 2^25 values 37 and 36) and the
+// backward pass, which has more to read (2^25 values: 60 columns 81 us and 67, 176 columns 79 and 69; 2^27 values: level
+// within 5 %, but 30 columns 391 and 418).
 template <typename T>
 __device__ __forceinline__ void write_columns(T* row, int q, int D, const typename Loose<T>::type& p,
                                               bool passing = true) {
@@ -127,7 +128,7 @@ __global__ __launch_bounds__(G ? kFwdBlock : kMostBlock) void ln_fwd(const T* __
   const int stride = G ? G : (int)blockDim.x, lane = threadIdx.x % stride;
   const int sub = G ? tt::row_of_block<G ? G : 1>() : 0;
   const int packs = (D + n - 1) / n;
-  const bool passing = G == 0 || G == kWave || whole_lines<T>(D);
+  const bool passing = G == 0 || G == kWave || NV == 1 || whole_lines<T>(D);
   for (long long row = (long long)blockIdx.x * kRows + sub; row < R; row += (long long)gridDim.x * kRows) {
     const T* __restrict__ p = x + row * (size_t)D;
     P v[NV];
