@@ -8,10 +8,11 @@
 // and keeps each thread's columns of dw and db in registers on the way; they are added up over the rows of a block in
 // LDS, and over the blocks by ln_join. Rows longer than the registers hold are read again (the *_long kernels).
 //
-// Memory bounds them: 2^25 float32 values take 45 to 61 us forward and 77 to 85 us backward (4.4 to 6.0 and 4.7 to 5.2
-// TB/s, a large copy 5.0 to 5.6) in rows of 24 to 4096, 1537 columns 65 and 84; float16 23 to 39 us and 42 to 78 us,
-// where rows that begin off sixteen bytes take up to half as much more.  What is left to lose are idle lanes, where a
-// row's packs do not fill its waves, and the blocks' sums.
+// Memory bounds them: 2^25 float32 values take 47 to 57 us forward and 76 to 84 us backward (4.7 to 5.7 and 4.8 to 5.3
+// TB/s, a large copy 5.0 to 5.6) in rows of 24 to 8192; float16 23 to 37 us and 43 to 63 us (3.6 to 5.8 and 3.2 to 4.7
+// TB/s), the longer ones where rows begin off sixteen bytes.  Rows longer than a block holds read twice or three times
+// take 74 and 157 us (20001 columns).  What is left to lose are idle lanes, where a row's packs do not fill its waves, and
+// the blocks' sums.
 #include "rows.h"
 
 namespace {
@@ -49,11 +50,11 @@ __device__ __forceinline__ bool whole_lines(int D) {
 }
 // `passing`: on its way to memory at once, past the caches, which then hold more of what is read. Float32 rows of the
 // forward pass that end inside a line of memory and have a part of a wave each, so that its pieces come from several
-// instructions, are better left to the cache, which puts them together (2^27 values: 72 columns 193 us, 389 passing, 260
-// columns 190 and 235). Rows that come from one instruction pass (20 columns at 2^27 values 255 us and 249, at 2^25 61 and
-// 46), and so do those of a wave or a block (2500 columns 195 and 185), halves (385 columns at 2^25 values 37 and 36) and the
-// backward pass, which has more to read (2^25 values: 60 columns 81 us and 67, 176 columns 79 and 69; 2^27 values: level
-// within 5 %, but 30 columns 391 and 418).
+// instructions, are better left to the cache, which puts them together (2^27 values: 72 columns 199 us, 390 passing, 260
+// columns 191 and 236). Rows that come from one instruction pass (20 columns 256 us and 249), and so do those of a wave or
+// a block (2500 columns 196 and 188), halves (385 columns at 2^25 values 37 and 36) and the backward pass, which has more to
+// read (2^25 values: 60 columns 82 us and 79, 2500 columns 82 and 79; 2^27 values: 319 and 298 at 2500, level within 7 %
+// in shorter rows).
 template <typename T>
 __device__ __forceinline__ void write_columns(T* row, int q, int D, const typename Loose<T>::type& p,
                                               bool passing = true) {
@@ -475,6 +476,11 @@ template <typename T>
 int forward(const T* x, const float* w, const float* b, T* y, float* mean, float* rstd, float eps, int R, int D) {
   const int packs = (D + Loose<T>::n - 1) / Loose<T>::n;
 #define TT_LN_FWD(G, NV) return launch_fwd<T, G, NV>(x, w, b, y, mean, rstd, eps, R, D)
+  // The fewest lanes that hold a row in two or three packs each, which keeps several rows of a wave on their way (2^25
+  // values: 64 columns of float32 48 us, on 32 lanes 77; 256 columns 48, on 64 lanes 50, of halves 24 and 41; 72 columns
+  // with three packs 55, with two 59); a wave alone up to five, before the barriers of a block (1088 columns 52 us, by
+  // blocks 58, of halves 2176 columns 27 and 31); then as few packs a thread as leave waves enough (2304 columns with three
+  // 49 us, with two 64; 3328 with four 49, with three 57; but 2048 with two 48, with one 70).
   if (packs <= 4) TT_LN_FWD(4, 1);
   if (packs <= 8) TT_LN_FWD(8, 1);
   if (packs <= 16) TT_LN_FWD(8, 2);
@@ -486,7 +492,7 @@ int forward(const T* x, const float* w, const float* b, T* y, float* mean, float
   if (packs <= 128) TT_LN_FWD(64, 2);
   if (packs <= 192) TT_LN_FWD(64, 3);
   if (packs <= 256) TT_LN_FWD(64, 4);
-  if (sizeof(T) == 4 && packs <= 320) TT_LN_FWD(64, 5);       // 1025 columns 68 -> 55 us at 2^25 values, 1200: 55 -> 51
+  if (packs <= 320) TT_LN_FWD(64, 5);
   if (packs <= 512) TT_LN_FWD(0, 2);
   if (packs <= 768) TT_LN_FWD(0, 3);
   if (packs <= 4 * kMostBlock) TT_LN_FWD(0, 4);
@@ -507,9 +513,9 @@ int launch_bwd(const T* x, const T* dy, const float* w, const float* mean, const
                float* db, int R, int D) {
   const int packs = (D + Loose<T>::n - 1) / Loose<T>::n;
   // a row's threads, and as many rows as fill the block, which leaves one set of sums. (Long rows of halves, whose sums
-  // weigh as much as a dozen of them: blocks of 1024 threads, 8192 columns 65 -> 55 us at 2^25 values; and rows of
-  // three waves, five of which leave fewer threads idle than two: 1025 columns 93 -> 78 us. Of float32, or of other
-  // short ones, 512: 1024 columns of halves 46 us, 53 with 1024 threads)
+  // weigh as much as a dozen of them: blocks of 1024 threads, 8192 columns 55 us at 2^25 values, 64 with 512; and rows of
+  // three waves, five of which leave fewer threads idle than two: 2100 columns 61 us, 68 with 512. Of float32, or of other
+  // short ones, 512: 1537 columns of halves 59 us, 71 with 1024)
   const int along = G ? kBwdBlock : (packs + NV * kWave - 1) / (NV * kWave) * kWave;
   const int fill = sizeof(T) == 2 && (along > 256 || along == 192) ? kMostBlock : kBwdBlock;
   const int rows = G ? kBwdBlock / (G ? G : 1) : along < fill ? fill / along : 1;
@@ -521,9 +527,8 @@ int launch_bwd(const T* x, const T* dy, const float* w, const float* mean, const
     TT_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_unit, ln_bwd<T, G, NV>, block.x * block.y, 0));
   const unsigned grid = grid_for(R, rows, (long long)tt::compute_units() * (per_unit > 0 ? per_unit : 1));
   const bool sums = dw || db;
-  // the last block joins what takes it a few rounds of loads: that saves the host a launch, 3 us, for a little more of
-  // the device's time (300 rows of 256: 7.0 us, 6.4 with the launch, 5000 of 96: 11.4 and 10.5; 300 of 512, in six
-  // rounds, 10.9 and 6.9)
+  // the last block joins what takes it a few rounds of loads: that saves a launch (1000 rows of 64: 5.2 us, 8.1 with it; 50
+  // of 768, in two rounds, 8.9 and 7.8, where the host is spared its part; 300 of 512, in six rounds, 11.2 and 7.6)
   const int threads = block.x * block.y, ways = 2 * D < threads ? threads / (2 * D) : 1;
   const long long rounds = (2 * (long long)D + threads - 1) / threads * ((grid + kFlight * ways - 1) / (kFlight * ways));
   const bool joins = sums && grid > 1 && rounds <= 3;
@@ -541,20 +546,24 @@ int backward(const T* x, const T* dy, const float* w, const float* mean, const f
   constexpr bool wide = sizeof(T) == 4;
   const int packs = (D + Loose<T>::n - 1) / Loose<T>::n;
 #define TT_LN_BWD(G, NV) return launch_bwd<T, G, NV>(x, dy, w, mean, rstd, dx, dw, db, R, D)
+  // A lane has x, dy and two sums of each column, so fewer packs than forward: one, up to 64 to a row (2^25 values: 40
+  // columns of float32 77 us, with two 100; 72 columns 79, with two 85), but two or three where one would leave a third of
+  // the lanes idle (288 columns with three 78, on 64 lanes with two 82; of halves 576 columns 50, by blocks 60). From 97
+  // packs on a wave with two or three (577 columns of float32 81, by blocks 89, of halves 1025 columns 64, by blocks 81),
+  // then blocks: with one or two packs a thread as long as the row has waves enough for few rows (20 of 1537 columns of
+  // halves 8 us, with two packs 10; many rows are level within 6 %), of float32 three from there on (1088 columns 77, with
+  // two 97), or four where three would leave five waves (3328 columns 81, with three 88), of halves, which are eight to a
+  // pack, two (3200 columns 50, with one 63).
   if (packs <= 4) TT_LN_BWD(4, 1);
   if (packs <= 8) TT_LN_BWD(8, 1);
   if (packs <= 16) TT_LN_BWD(16, 1);
   if (packs <= 32) TT_LN_BWD(32, 1);
-  // (16 lanes with three packs each, whose stores went by the caches, took 81 us at 176 columns of float32 and 2^25 values,
-  // this 69; at 192 columns 67 and 67. Of halves 47.0 and 47.5 at 288 columns, 45.0 and 43.1 at 352)
   if (packs <= 48) TT_LN_BWD(32, 2);
   if (packs <= 64) TT_LN_BWD(64, 1);
-  if (wide && packs <= 96) TT_LN_BWD(32, 3);
-  if (wide && packs <= 128) TT_LN_BWD(64, 2);
-  if (wide && packs <= 192) TT_LN_BWD(64, 3);
+  if (packs <= 96) TT_LN_BWD(32, 3);
+  if (packs <= 128) TT_LN_BWD(64, 2);
+  if (packs <= 192) TT_LN_BWD(64, 3);
   if (packs <= 256) TT_LN_BWD(0, 1);
-  // (float32: three packs to a thread but where they leave an odd number of waves, of which a unit then holds fewer.
-  // 1025 columns 115 us at 2^25 values with two, 85 with three; 3300 columns 101 with three, 86 with four)
   if constexpr (wide) {
     if (packs > 384 && packs <= 512) TT_LN_BWD(0, 2);
     if (packs > 768 && packs <= 960) TT_LN_BWD(0, 4);
