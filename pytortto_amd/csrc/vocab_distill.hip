@@ -8,9 +8,9 @@
 // Memory bounds them, and the fewest bytes are one read and one write of the row: the gradient for an incoming gradient
 // of one is written in the visit that reads the row for the loss (4096x32768 float32 with 32 entries: 1074 MB in 205
 // us, 5.2 TB/s, where a large copy reaches 5.0 to 5.6).  Of rows longer than registers and LDS hold the rest is read
-// twice (1024x131072 float16 with 64 entries: 604 MB instead of 537, in 115 us, 5.2 TB/s; the vector units are busy for
+// twice (1024x131072 float16 with 64 entries: 604 MB instead of 537, in 116 us, 5.2 TB/s; the vector units are busy for
 // 38 % of that).  Short rows are bound by the latency of their teacher: index, then the logit there (131072 rows of 100
-// with 32 entries: 35 us, 57 with the gradient).
+// with 32 entries: 34 us, 58 with the gradient).
 #include "vocab.h"
 
 namespace tt {
@@ -157,7 +157,7 @@ __device__ __forceinline__ void queue_entries(const Entries& e, const LogitRow<T
 }
 // Of its queue a thread takes the first P entries of packs into registers, and into the packs as it writes them; `rest`
 // is stored behind the packs.  (A lone value costs memory a piece of 64 bytes: 131072 rows of 300 with 32 entries take
-// 104 us with P = 4 and 131 us with none.  Of long rows they are few, so P = 0.)
+// 103 us with P = 4 and 137 us with none, 67108 of 1000 with P = 2 118 and 180; but of 100 57 and 54.  Of long rows they are few, so P = 0.)
 template <int G>
 constexpr int kPatches = G < kWave ? 4 : G == kWave ? 2 : 0;
 template <int P>
@@ -259,7 +259,7 @@ __device__ __forceinline__ void add_up(const Out& o, tt::Ticket* done, unsigned 
 }
 
 // scale p of the values of pack j, and the patches.  (log2(scale) in the exponent would spare halves a product: 1024x131072
-// with 64 entries 109 us where this takes 113.  But a sum of it with m c is rounded at the size of m c, 2e-3 of the
+// with 64 entries 106 us where this takes 109.  But a sum of it with m c is rounded at the size of m c, 2e-3 of the
 // gradient in a row of -65504 alone, and added to the difference it is no faster.)
 template <typename T, int P>
 __device__ __forceinline__ Words gradient_pack(const Words& p, const Patches<P>& t, int j, float m, float log_s,
@@ -335,8 +335,8 @@ __global__ __launch_bounds__(kThreads) void distill_count(Teacher te, int* __res
 
 __device__ tt::Ticket distill_done[1 + tt::kBranches], distill_tickets[kMostSplitRows];
 
-// Of a longer row than the registers hold, LDS takes this many packs more of each thread (1024x131072 float16: 143 us
-// without, 124 with them); the loop over them and what is left has few registers.
+// Of a longer row than the registers hold, LDS takes this many packs more of each thread (1024x131072 float16: 126 us
+// without, 117 with them); the loop over them and what is left has few registers.
 constexpr int kShelf = 8, kPair = 2;
 
 // Rows of G threads each: loss, statistics and, with GRAD, the gradient for an incoming gradient of one. For that the
@@ -548,8 +548,8 @@ constexpr long long kMostBlocks = 16;      // of a launch, to a compute unit; th
 unsigned grid_for(long long blocks, long long most) { return (unsigned)(blocks < most ? blocks : most); }
 
 // Rows of up to kWavePacks packs go to a wave each, which keeps them in registers; four of them share a block's LDS,
-// where the teacher's entries have to fit. (22369 rows of 3000 in float32 with 32 entries and their gradient: 113 us,
-// by blocks 190.) Short ones go to kLanes lanes each: 131072 rows of 100 with 32 entries take 57 us, by waves 310.
+// where the teacher's entries have to fit. (22369 rows of 3000 in float32 with 32 entries and their gradient: 114 us,
+// by blocks 134.) Short ones go to kLanes lanes each: 131072 rows of 300 with 32 entries take 101 us, by waves 144.
 constexpr int kWavePacks = 16 * kWave, kWaveEntries = 256;
 bool by_waves(int packs, int K) { return packs <= kWavePacks && K <= kWaveEntries; }
 constexpr int kLanes = 16, kLanesPacks = 8 * kLanes, kLanesEntries = 64;
@@ -558,14 +558,14 @@ bool by_lanes(int packs, int K) { return packs <= kLanesPacks && K <= kLanesEntr
 int packs_for(int V, int dtype) { return dtype == TT_F32 ? (V + 3) / 4 : (V + 7) / 8; }
 
 // Rows shared by blocks, where they are fewer than units: the block that joins a row reads its teacher last. (300 rows
-// of 50021 take 15.8 us whole and 17.8 shared, 512 of 131072 49 and 54; 100 of 131072 25 and 16 us.)
+// of 50021 take 15.6 us whole and 16.7 shared, 512 of 131072 49 and 52; 100 of 131072 25 and 15 us.)
 int forward_splits(long long R, int packs) {
   if (packs <= kWavePacks || R > kMostSplitRows) return 1;
   return tt::splits_for(R, packs, kThreads, 2, kUnroll * kThreads);
 }
 // Where the backward pass has more than those, it has fewer than that of log probabilities, for each block reads the
-// row's teacher (1300 rows of 50021 with 32 entries: 127 -> 115 us; with as many as there 110, but 300 rows of 50021
-// take 27 us instead of 24).
+// row's teacher (1300 rows of 50021 with 32 entries: 120 -> 110 us, with as many as there 103; but of 2047 in float16 96 us,
+// with as many 99).
 int backward_splits(long long R, int packs) {
   const int few = tt::splits_for(R, packs, kThreads, 8, kUnroll * kThreads);
   const int many = tt::splits_for(R, packs, kThreads, 16, 4 * kUnroll * kThreads);
@@ -573,8 +573,8 @@ int backward_splits(long long R, int packs) {
 }
 
 // A row to a block, loss and gradient in one visit: while it fits the registers, which saves two launches (20 rows of
-// 10000: 10 us, 15 us shared by blocks), and longer ones from half as many rows as there are units on (140 rows of
-// 131072 42 and 46 us, 80 rows 35 and 33 us).
+// 10000: 10 us, 13 us shared by blocks), and longer ones from half as many rows as there are units on (140 rows of
+// 131072 42 and 45 us, 80 rows 34 and 32 us).
 bool whole_rows(long long R, int packs) { return packs <= 16 * 512 || 2 * R >= tt::compute_units(); }
 
 // Whether the forward pass writes the gradient too, for an incoming gradient of one: where a row's own block does it
@@ -653,8 +653,8 @@ int forward(const T* x, const Teacher& te, float* loss, float* stats, float* cou
     return 0;
   }
   if (!dx) return launch_rows<T, false>(x, te, o, dx, nullptr, sc, R, V, packs);
-  // each block counts this many rows by itself in the time of a launch (900 rows of 1000: 10.5 and 12.5 us, 1500 rows:
-  // 13.3 and 12.4)
+  // each block counts this many rows by itself in the time of a launch (900 rows of 1000: 9.6 and 10.7 us, 1500 rows
+  // 11.2 and 11.5, 4096 rows 21 and 15)
   const bool counts_itself = R <= 1024;
   if (reduction == 2 && !counts_itself) {
     distill_count<<<kCountBlocks, kThreads, 0, st>>>(te, parts, R, V);

@@ -1,10 +1,10 @@
 // Log probabilities of given tokens, with the entropy and the best alternatives of each row of logits, forward and
 // backward (vocab.h has the formulas).
 //
-// Memory bounds them: the forward pass reads the logits once (4096x32768 float32 in 88 us, 6.1 TB/s, where a plain read
+// Memory bounds them: the forward pass reads the logits once (4096x32768 float32 in 89 us, 6.0 TB/s, where a plain read
 // reaches 6.2), the backward pass reads them once more and writes as much (2047x50021 float32: 819 MB in 136 us, 6.0
 // TB/s). What little there is to do for a row of a decoding step is bound by latency: reading a share, a ticket,
-// joining the shares (1x32768: 7.4 us, 10.5 with five alternatives; 48x131072 float16 with twenty: 17 us, 8 with
+// joining the shares (1x32768: 7 us, 10 with five alternatives; 48x131072 float16 with twenty: 18 us, 8 with
 // none).
 #include "vocab.h"
 
@@ -33,7 +33,7 @@ constexpr int kMostSplitRows = 255;     // rows that may be shared by blocks
 // owners alone are read again, a few thousand values of a row that has just come through the cache, and what reaches
 // the bound (K values and few more, unless the row is laid out against it) is ranked by counting.  Values and places
 // make keys without ties, so the answer does not depend on the order in which candidates arrive.  (512 rows of 131072
-// in float32: 46 us with no alternatives, 55 with five, 73 with twenty.)
+// in float32: 47 us with no alternatives, 56 with five, 73 with twenty.)
 
 typedef unsigned long long Key;
 
@@ -609,11 +609,12 @@ int check(const char* fn, int dtype, int index_bits, long long R, int V, int K) 
 unsigned grid_for(long long blocks) { return (unsigned)(blocks < (1 << 22) ? blocks : (1 << 22)); }
 
 // Rows of up to kWavePacks packs go to a wave each, short ones to some of its lanes, so that a wave has several rows on
-// their way; longer ones go to a block.  131072 rows of float32, a wave against eight lanes: of 10 values 60 and 9 us,
-// of 300 values 58 and 31 us forward; and backward, where more lanes store wider pieces, 8 against 16 lanes: of 37
-// values 17 and 25 us, of 100 values 31 and 29 us, of 300 values 105 and 79 us (a wave: 125 us); 67108 rows of 1000 are
-// level.  With more than kWaveTop alternatives a block, of four times as many threads, has a closer bound (22369 rows
-// of 3000 with 64: 1062 us by waves, 240 us by blocks).
+// their way; longer ones go to a block.  131072 rows of float32, a wave against eight lanes: of 10 values 47 and 8 us,
+// of 300 values 64 and 31 us forward; and backward, where more lanes store wider pieces, 8 against 16 lanes: of 37
+// values 17 and 24 us, of 100 values 31 and 29 us, of 300 values 109 and 80 us (a wave: 120 us); 67108 rows of 1000 take
+// 54 and 52 us forward, 107 by waves and 131 by sixteen lanes backward.  22369 rows of 3000 with five alternatives 64 us by
+// waves and 127 by blocks; with more than kWaveTop a block, of four times as many threads, has a closer bound (with 32 93
+// and 156 us, with 64 428 and 182).
 constexpr int kLanesPacks = 128, kFewPacks = 16, kWavePacks = 1024, kWaveTop = 32;
 template <int G>
 unsigned row_grid(long long R) {
@@ -621,15 +622,17 @@ unsigned row_grid(long long R) {
 }
 
 // Rows shared by blocks, where they are fewer than units: two blocks to a unit, with kUnroll packs to a thread at least
-// (200 rows of 50021 with twenty alternatives take 19 us, with eight blocks to a unit 25; 1000 rows of 9000 with ten 14
-// us whole and 25 shared by two; one row of 32768 is read in 7.6 us, 100 of 131072 in 13, 24 if they stay whole).
+// (200 rows of 50021 with twenty alternatives take 19 us, with eight blocks to a unit 24; 250 of 131072 with five 31, 40 if
+// they stay whole; one row of 32768 4.6 and 6.0). From 256 rows on they stay whole (1000 rows of 9000 with ten 14 us and 22
+// shared by two, 512 of 131072 with five 54 and 57). The join costs few rows of few packs more than it saves (100 rows of
+// 9000 with ten take 10 us, 7 if they stay whole).
 int forward_splits(long long R, int packs) {
   if (packs <= kWavePacks || R > kMostSplitRows) return 1;
   return tt::splits_for(R, packs, kThreads, 2, kUnroll * kThreads);
 }
 // The blocks of the backward pass share nothing, and more of them end more evenly: 32 to a unit, of twice as many
-// packs, where that is more (1300 rows of 50021: 123 -> 98 us; 8000 rows of 8191, which stay whole, take 102 us and
-// would take 107).
+// packs, where that is more (1300 rows of 50021: 118 -> 98 us; 8000 rows of 8191, which stay whole, take 102 us, shared
+// by two 105).
 int backward_splits(long long R, int packs) {
   const int few = tt::splits_for(R, packs, kThreads, 8, kUnroll * kThreads);
   const int many = tt::splits_for(R, packs, kThreads, 32, 2 * kUnroll * kThreads);
