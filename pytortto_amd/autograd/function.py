@@ -66,17 +66,14 @@ class AccumulateGrad(BackwardFunction):
     next_functions = ()
     done = False        # its gradient of this pass is where it belongs
 
-    def accumulate(self, g):
-        self.grad[0] = g
-        self.apply(g)
-        self.grad[0] = None
-        self.done = True
-
     def apply(self, *args):
+        self.accumulate(self.grad[0])
+        self.done = False       # (it was visited in its turn)
+
+    def accumulate(self, g):
         """function.py:70-93: first gradient is stored (contiguous), later ones are added."""
         var = self.variable
         if var.grad is None:
-            g = self.grad[0]
             # a leaf keeps its gradient beyond this pass: it must not stay an alias of another holder's
             if g.__class__ is not xparray.hiparray:
                 g = np.ascontiguousarray(g)
@@ -84,7 +81,8 @@ class AccumulateGrad(BackwardFunction):
                 g.own()
             var.grad = g
         else:
-            var.grad += self.grad[0]
+            var.grad += g
+        self.done = True
 
 
 def _node_class(cls):

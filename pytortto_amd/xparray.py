@@ -76,7 +76,9 @@ class _Buffer:
         self.deps = ()
         self.exported = False
         if not lazy:
-            self._allocate()
+            p = _void_p()
+            _hip.call('tt_malloc', _byref(p), nbytes)
+            self._ptr = p.value or 0
 
     def _allocate(self):
         p = _void_p()
@@ -316,9 +318,11 @@ class hiparray:
         array that has been handed out does not share it again: what others write there is seen by the array alone.
         Once nobody has the array, its block goes to new ones when the default stream (torch's, as a rule) is done with
         it; who uses the memory on another stream keeps the array until that is done."""
-        if not self._buf.exported or self._shared or _hip._pending is not None:
-            self._hand_out()
-        return {'shape': self._shape, 'typestr': self._dtype.str, 'data': (self.ptr, False), 'strides': None, 'version': 3,
+        buf = self._buf
+        if not buf.exported or self._shared or _hip._pending is not None:
+            buf = self._hand_out()
+        at = buf._ptr if buf.on_demand is None else buf.ptr
+        return {'shape': self._shape, 'typestr': self._dtype.str, 'data': (at, False), 'strides': None, 'version': 3,
                 'stream': _hip._stream or _hip.stream()}
 
     def _hand_out(self):
@@ -326,10 +330,12 @@ class hiparray:
             _hip.flush()
         if self._shared or _unfilled.data:
             self.own()
+        self.ptr                            # (a block, with its contents on their way)
         buf = self._buf
         buf.exported = True
         if buf.__class__ is _Borrowed and buf.owner.__class__ is _Buffer:       # a part of the library's own block
             buf.owner.exported = True
+        return buf
 
     @property
     def ptr(self):
