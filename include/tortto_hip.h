@@ -482,7 +482,7 @@ int tt_layer_norm_bwd(const void* x, const void* dy, const float* w, const float
  *   - a row whose token is ignore_index is not read: zeros, places -1, gradient 0;
  *   - a token outside [-V, V) gives NaN for its log probability and its gradient row;
  *   - a row of -inf alone: -inf, entropy 0, alternatives -inf, gradient 0;
- *   - a NaN or +inf in a row gives NaN for all its values and -1 for its places.
+ *   - a NaN or +inf in a row gives NaN for all its values and its gradient, and -1 for its places.
  * stats [R][2] are kept for the backward pass, or NULL.  The backward adds up the gradients of what the forward returned
  * (each may be NULL) and writes dx [R, V]; entropy and top_index are the forward's (a place outside the row is passed
  * over). */

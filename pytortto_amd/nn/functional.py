@@ -96,7 +96,8 @@ def token_log_prob(input, tokens, top=0, ignore_index=-100):
     alternatives, best first and the lowest index first among equals (at most 64).
 
     Negative tokens count from the end.  A position whose token is ``ignore_index`` is not looked at: zeros, and -1 for
-    the indexes.  A token outside the vocabulary gives NaN, and so does a NaN or +inf among the logits (indexes -1).
+    the indexes.  A token outside the vocabulary gives NaN, and so does a NaN or +inf among the logits (indexes -1),
+    for the gradient too.
     Logits of -inf alone leave log probabilities of -inf, entropy 0 and no gradient.  ``tt.backward`` takes gradients of
     several of the outputs in one pass."""
     return TokenLogProb.apply(input, tokens=tokens, top=top, ignore_index=ignore_index)
@@ -108,5 +109,6 @@ def distill_loss(input, teacher, index, temperature=1.0, reduction='mean'):
     ``index`` [..., K] their classes, int64 or int32, and -1 where there is no entry.
 
     Entries of one class add up.  Positions without an entry, or with -inf alone, have loss and gradient 0 and are not
-    counted by 'mean'; an index of V or more gives NaN.  Gradients flow to ``input`` only."""
+    counted by 'mean'; an index of V or more gives NaN, and so does a NaN or +inf among a position's logits, for its
+    gradient too.  Logits of -inf alone have no gradient.  Gradients flow to ``input`` only."""
     return DistillLoss.apply(input, teacher=teacher, index=index, temperature=float(temperature), reduction=reduction)
