@@ -510,6 +510,21 @@ int tt_distill_bwd(const void* x, const void* teacher, const void* index, const 
                    const float* g, void* dx, double temperature, int reduction, int is_ahead, int dtype,
                    int teacher_dtype, int index_bits, long long R, int V, int K);
 
+/* Softmax cross entropy of N positions over V classes straight from features x [N, H] and the head's weight w [V, H] (both
+ * float32, dtype 0, or float16, 1), with the logits z = x w^T only in scratch memory, a chunk of positions at a time:
+ *   loss_i = log sum_v exp z_iv - z_i,target(i),  G_iv = g_i (softmax(z_i)_v - [v = target(i)]),  dx = G w,  dw = G^T x.
+ * target: int64 or int32 as index_bits says; negative ones count from the end, one outside [-V, V) makes the loss and both
+ * gradients NaN.  A position whose target is ignore_index has loss 0 and no gradient, whatever its features hold.  reduction: 0 none
+ * (loss [N]), 1 sum, 2 mean over the positions that are not ignored (NaN, with gradients of zeros, if there are none); the
+ * gradients have the reduction's scale.  g [N] or NULL: 1.  loss, dx and dw may each be NULL.  dx [N, H] and dw [V, H] are
+ * float32, or float16 where half_gradients says so.  Products of float32 are of two float16 terms a value, scaled by powers
+ * of two; an infinity among them gives NaN.  No counterpart in the reference. */
+int tt_linear_cross_entropy(const void* x, const void* w, const void* target, const float* g, float* loss, void* dx,
+                            void* dw, int dtype, int half_gradients, int index_bits, long long ignore_index,
+                            int reduction, long long N, int H, int V);
+/* to = g[0] from, n values, as float32 or float16. */
+int tt_scaled_gradient(const float* from, const float* g, void* to, int dtype, size_t n);
+
 /* ---- optimiser steps (optim/_functional.py:4-119) ---------------------------------------------- */
 
 /* One SGD update of a parameter in place (_functional.py:4-22): d = grad (+ weight_decay * param);
@@ -537,6 +552,19 @@ int tt_adam_step_multi_f32(int count, float* const* params, const float* const* 
                            float* const* exp_avg_sqs, float* const* max_exp_avg_sqs, const size_t* sizes,
                            const int* steps, double lr, double beta1, double beta2, double eps, double weight_decay,
                            int amsgrad, int decoupled_weight_decay);
+
+/* One step of Muon in place, for `count` matrices [rows, columns] of one group: momentum <- momentum + (1 - mu)(grad -
+ * momentum); u = the momentum, or with nesterov grad + mu (momentum - grad); param <- param (1 - lr weight_decay) - lr
+ * scale O(u), O as tt_orthogonalize has it.  No counterpart in the reference. */
+int tt_muon_step_multi_f32(int count, float* const* params, const float* const* grads, float* const* momenta,
+                           const int* rows, const int* columns, const double* scales, double lr, double momentum,
+                           double weight_decay, int nesterov, int steps, double a, double b, double c, double eps);
+/* Newton-Schulz orthogonalisation of x [rows, columns], float32 (dtype 0) or float16 (1): out has x's singular vectors, and
+ * of every singular value s / max(|x|_F, eps) what `steps` (1 to 100) times s <- a s + b s^3 + c s^5 make of it.  All
+ * inside runs in two float16 terms of every value and float32 sums.  Coefficients that let a value of [0, 1] grow past 1.9 are
+ * refused.  out may be x.  No counterpart in the reference. */
+int tt_orthogonalize(const void* x, void* out, int dtype, int rows, int columns, int steps, double a, double b, double c,
+                     double eps);
 
 /* ---- elementwise glue so whole stacks stay on the device ----------------------------------- */
 

@@ -3,7 +3,8 @@
 Mirrors the names of samrere/pytortto that the path sits behind: ``tensor``, ``Tensor``,
 ``manual_seed``, ``randn``/``zeros``/``ones``, ``no_grad``, ``nn.Conv2d``, ``nn.ConvTranspose2d``,
 ``nn.BatchNorm2d``, ``nn.functional.conv2d`` / ``conv_transpose2d`` / ``batch_norm``; and, for models over a
-vocabulary, ``nn.LayerNorm``, ``nn.functional.token_log_prob`` and ``nn.DistillLoss``.
+vocabulary, ``nn.LayerNorm``, ``nn.functional.token_log_prob``, ``nn.DistillLoss``,
+``nn.functional.linear_cross_entropy`` and ``optim.Muon``.
 ``.cuda()`` moves data into device arrays owned through ``libtortto_hip.so``; every computation
 on them runs in hand-written HIP kernels.  Importing this package does not touch the GPU.
 """
@@ -17,7 +18,7 @@ from .VariableFunctions import (manual_seed, empty, zeros, ones, randn, tensor, 
                                 mean, flatten, mm, matmul)
 from .autograd import (no_grad, enable_grad, set_grad_enabled, is_grad_enabled, Function, AccumulateGrad,
                        ToCopy, Add, Convolution, TransposedConvolution, BatchNorm, Relu, LeakyRelu,
-                       MaxPool2DWithIndices, LogSoftmax, NllLoss, LayerNorm, TokenLogProb, DistillLoss,
+                       MaxPool2DWithIndices, LogSoftmax, NllLoss, LayerNorm, TokenLogProb, DistillLoss, LinearCrossEntropy,
                        View, Transpose, Mm, Mean)
 from .serialization import save, load
 from . import nn

@@ -105,10 +105,14 @@ PROTOTYPES = {
     'tt_distill_ahead': [POINTER(c_int), _I, _I, _L, _I],
     'tt_distill_fwd': [_P] * 7 + [c_double] + [_I] * 4 + [_L, _I, _I],
     'tt_distill_bwd': [_P] * 7 + [c_double] + [_I] * 5 + [_L, _I, _I],
+    'tt_linear_cross_entropy': [_P] * 7 + [_I] * 3 + [_L, _I, _L, _I, _I],
+    'tt_scaled_gradient': [_P, _P, _P, _I, c_size_t],
     'tt_sgd_step_f32': [_P, _P, _P, c_size_t, c_double, c_double, c_double, c_double, _I, _I],
     'tt_sgd_step_multi_f32': [_I, _P, _P, _P, _P, _P, c_double, c_double, c_double, c_double, _I],
     'tt_adam_step_f32': [_P, _P, _P, _P, _P, c_size_t, _I, c_double, c_double, c_double, c_double, c_double, _I, _I],
     'tt_adam_step_multi_f32': [_I, _P, _P, _P, _P, _P, _P, _P, c_double, c_double, c_double, c_double, c_double, _I, _I],
+    'tt_muon_step_multi_f32': [_I] + [_P] * 6 + [c_double] * 3 + [_I, _I] + [c_double] * 4,
+    'tt_orthogonalize': [_P, _P, _I, _I, _I, _I] + [c_double] * 4,
     'tt_add_f32': [_P, _P, _P, c_size_t],
     'tt_add_f16': [_P, _P, _P, c_size_t],
     'tt_add_relu_f32': [_P, _P, _P, c_size_t],

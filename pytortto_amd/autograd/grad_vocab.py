@@ -1,5 +1,5 @@
 """Autograd functions of models over a vocabulary: ``LayerNorm`` (interface of ``src/tortto/autograd/grad_nn.py:993-1052``),
-``TokenLogProb`` and ``DistillLoss`` (not in the reference).  Device tensors only, float32 or float16; parameters,
+``TokenLogProb``, ``DistillLoss`` and ``LinearCrossEntropy`` (not in the reference).  Device tensors only, float32 or float16; parameters,
 losses and all statistics are float32."""
 import math
 from math import prod
@@ -119,3 +119,40 @@ class DistillLoss(Function):
         x, teacher, index = ctx.saved_tensors
         p = ctx.params
         return ops.distill_bwd(x, teacher, index, p['stats'], p['count'], gd0, p['dx'], p['temperature'], p['reduction'])
+
+
+class LinearCrossEntropy(Function):
+    """The gradients of a scalar loss are made with it, while the logits are there: a backward pass would have to make those
+    again, a third of its products more."""
+
+    @staticmethod
+    def forward(ctx, *inputs, **params):
+        xt0, xt1 = inputs   # input, weight
+        xd0, wd0, target, reduction = xt0.data, xt1.data, params['target'], params['reduction']
+        _device_only('linear_cross_entropy', xd0)
+        td0 = target.data
+        _same_device('linear_cross_entropy', wd0, td0)
+        if xd0.ndim == 0 or wd0.ndim != 2 or td0.shape != xd0.shape[:-1] or xd0.shape[-1] != wd0.shape[1] or 0 in wd0.shape:
+            raise RuntimeError(f'linear_cross_entropy takes input [..., H], weight [V, H] and target [...], got {xd0.shape}, '
+                               f'{wd0.shape} and {td0.shape}')
+        if wd0.dtype != xd0.dtype:
+            raise TypeError(f'linear_cross_entropy takes input and weight of one type, got {xd0.dtype} and {wd0.dtype}')
+        if reduction not in ('none', 'sum', 'mean'):
+            raise ValueError(f'{reduction} is not a valid value for reduction')
+        keep = ctx.requires_grad and is_grad_enabled()
+        need = ctx.needs_input_grad if keep else (False, False)
+        yd0, dx, dw = ops.linear_cross_entropy_fwd(xd0, wd0, td0, params['ignore_index'], reduction, need)
+        yt0 = build_links(yd0, grad_fn=ctx)
+        if keep:
+            ctx.save_for_backward(xt0, xt1, target)
+            ctx.params.update(dx=dx, dw=dw)
+        return yt0
+
+    @staticmethod
+    def backward(ctx, *grad_outputs):
+        gd0, = grad_outputs
+        x, w, target = ctx.saved_tensors
+        p = ctx.params
+        if p['reduction'] == 'none':
+            return ops.linear_cross_entropy_bwd(x, w, target, gd0, p['ignore_index'], ctx.needs_input_grad)
+        return tuple(None if a is None else ops.scaled_gradient(a, gd0, x.dtype) for a in (p['dx'], p['dw']))

@@ -4,7 +4,7 @@
 from ..autograd.grad_fcn import Squeeze, Unsqueeze
 from ..autograd.grad_nn import (BatchNorm, Convolution, LeakyRelu, LogSoftmax, MaxPool2DWithIndices, NllLoss, Relu,
                                 TransposedConvolution)
-from ..autograd.grad_vocab import DistillLoss, LayerNorm, TokenLogProb
+from ..autograd.grad_vocab import DistillLoss, LayerNorm, LinearCrossEntropy, TokenLogProb
 
 
 def pad(input, pad, mode='constant', value=0.0):
@@ -112,3 +112,17 @@ def distill_loss(input, teacher, index, temperature=1.0, reduction='mean'):
     counted by 'mean'; an index of V or more gives NaN, and so does a NaN or +inf among a position's logits, for its
     gradient too.  Logits of -inf alone have no gradient.  Gradients flow to ``input`` only."""
     return DistillLoss.apply(input, teacher=teacher, index=index, temperature=float(temperature), reduction=reduction)
+
+
+def linear_cross_entropy(input, weight, target, ignore_index=-100, reduction='mean'):
+    """Softmax cross entropy of the logits ``input @ weight.T`` with classes ``target``, without keeping the logits: a chunk
+    of positions at a time has them in scratch memory (2 GiB at most, as a rule).  ``input`` [..., H] and ``weight`` [V, H] are both
+    float32 or both float16, ``target`` [...] is int64 or int32; the loss is float32, in nats.
+
+    Negative targets count from the end.  A position whose target is ``ignore_index`` has loss 0 and no gradient, whatever its
+    features hold, and is not counted by 'mean' (NaN, with gradients of zeros, where none is left).  A target outside the
+    vocabulary gives NaN, for its loss and the gradients.  Gradients flow to ``input`` and ``weight``.
+
+    float32 products are computed from two float16 terms of every value (22 bits of it, or 2^-40 of the largest value of its row, and
+    of the largest gradient of a logit), with float32 sums."""
+    return LinearCrossEntropy.apply(input, weight, target=target, ignore_index=ignore_index, reduction=reduction)

@@ -87,6 +87,27 @@ class DistillLoss(Module):
         return F.distill_loss(inpt, teacher, index, self.temperature, self.reduction)
 
 
+class LinearCrossEntropy(Module):
+    """``F.linear_cross_entropy`` with the head's weight [num_classes, in_features], initialised as ``Linear``'s."""
+
+    def __init__(self, in_features, num_classes, ignore_index=-100, reduction='mean'):
+        super().__init__()
+        self.in_features, self.num_classes = in_features, num_classes
+        self.ignore_index, self.reduction = ignore_index, reduction
+        self.weight = Parameter(_vf.zeros((num_classes, in_features)))
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        init.kaiming_uniform_(self.weight, a=math.sqrt(5))
+
+    def extra_repr(self):
+        return (f'in_features={self.in_features}, num_classes={self.num_classes}, ignore_index={self.ignore_index}, '
+                f'reduction={self.reduction}')
+
+    def forward(self, inpt, target):
+        return F.linear_cross_entropy(inpt, self.weight, target, self.ignore_index, self.reduction)
+
+
 class NLLLoss(Module):
     def __init__(self, weight=None, ignore_index=-100, reduction='mean'):
         super().__init__()

@@ -826,3 +826,69 @@ def distill_bwd(x, teacher, index, stats, count, g, dx, temperature, reduction):
                   _REDUCTIONS[reduction], ahead, _TYPES[x._dtype], _TYPES[teacher._dtype], _INDEX_BITS[index._dtype],
                   rows, x._shape[-1], entries)
     return dx
+
+
+_MOST_POSITIONS, _MOST_CLASSES, _MOST_FEATURES = 1 << 30, 1 << 20, 1 << 20
+MOST_ROWS = 1 << 20         # of a matrix that is orthogonalised, and columns
+
+
+def _check_products(fn, *sizes):
+    """(Here because the C ABI takes ints, see ``_refuse_row``.)"""
+    for n, most, what in sizes:
+        if n > most:
+            raise RuntimeError(f'{fn}: {most} {what} at most, got {n}')
+
+
+def linear_cross_entropy_fwd(x, w, target, ignore_index, reduction, need):
+    """(loss, dx, dw): for a scalar loss the gradients needed are made here, for an incoming one of 1 and in float32; without
+    a reduction, and where none is needed, they are None."""
+    kind, bits = _kind(x, 'the input of linear_cross_entropy'), _index_bits(target, 'the target of linear_cross_entropy')
+    red = _REDUCTIONS[reduction]
+    _check_products('linear_cross_entropy', (target.size, _MOST_POSITIONS, 'positions'), (w._shape[0], _MOST_CLASSES, 'classes'),
+                    (w._shape[1], _MOST_FEATURES, 'features'))
+    x, w = _aligned(x), _aligned(w)
+    loss = hiparray.empty(target._shape if red == 0 else ())
+    dx = hiparray.empty(x._shape) if need[0] and red else None
+    dw = hiparray.empty(w._shape) if need[1] and red else None
+    if target.size:
+        _hip.call('tt_linear_cross_entropy', x.ptr, w.ptr, target.ptr, None, loss.ptr, _ptr(dx), _ptr(dw), kind, 0, bits,
+                  ignore_index, red, target.size, w._shape[1], w._shape[0])
+    elif red:
+        loss.fill(0.0 if red == 1 else math.nan)
+        dw = hiparray.zeros(w._shape) if dw is not None else None
+    return loss, dx, dw
+
+
+def linear_cross_entropy_bwd(x, w, target, g, ignore_index, need):
+    """(dx, dw) of the losses of all positions, each None unless needed."""
+    _f32(g)
+    x, w, g = _aligned(x), _aligned(w), _aligned(g)
+    dx = hiparray.empty(x._shape, x._dtype) if need[0] else None
+    dw = (hiparray.empty if target.size else hiparray.zeros)(w._shape, w._dtype) if need[1] else None
+    kind = _TYPES[x._dtype]
+    if target.size:
+        _hip.call('tt_linear_cross_entropy', x.ptr, w.ptr, target.ptr, g.ptr, None, _ptr(dx), _ptr(dw), kind, kind,
+                  _INDEX_BITS[target._dtype], ignore_index, 0, target.size, w._shape[1], w._shape[0])
+    return dx, dw
+
+
+def scaled_gradient(ahead, g, dtype):
+    """g (one value) times a float32 gradient that a forward pass has made, as ``dtype``; the same array where that changes
+    nothing."""
+    _f32(g)
+    if dtype == _F32 and is_one(g):
+        return ahead
+    out = hiparray.empty(ahead._shape, dtype)
+    if out.size:
+        _hip.call('tt_scaled_gradient', ahead.ptr, g.ptr, out.ptr, _TYPES[dtype], out.size)
+    return out
+
+
+def orthogonalize(x, steps, coefficients, eps):
+    _check_products('orthogonalize', *((n, MOST_ROWS, 'rows and columns') for n in x._shape))
+    kind = _kind(x, 'the matrix')
+    x = _aligned(x)
+    out = hiparray.empty(x._shape, x._dtype)
+    if x.size:
+        _hip.call('tt_orthogonalize', x.ptr, out.ptr, kind, *x._shape, steps, *coefficients, eps)
+    return out

@@ -4,7 +4,7 @@ import ctypes
 
 import numpy as np
 
-from .. import _hip
+from .. import _hip, ops
 from ..xparray import hiparray
 
 
@@ -65,3 +65,37 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, max_exp_avg_sqs, state_steps, am
     """_functional.py:68-119."""
     _adam(params, grads, exp_avgs, exp_avg_sqs, max_exp_avg_sqs, state_steps, amsgrad, beta1, beta2, lr,
           weight_decay, eps, True)
+
+
+def muon(params, grads, momenta, lr, momentum, weight_decay, nesterov, steps, coefficients, eps, adjust):
+    """The matrices of a group share their launches.  Parameters of more than two dimensions are matrices of their first and the
+    others (a convolution's output channels and its taps)."""
+    while params:
+        for param, g, m in zip(params, grads, momenta):
+            _device(param, g, m)
+            if g.shape != param.data.shape or m.shape != param.data.shape:
+                raise RuntimeError(f'a gradient and a momentum are of their parameter\'s shape {param.data.shape}, got {g.shape} '
+                                   f'and {m.shape}')
+        # (one that comes twice is stepped twice, one after the other)
+        seen, now, later = set(), [], []
+        for i, param in enumerate(params):
+            (later if id(param) in seen else now).append(i)
+            seen.add(id(param))
+        for i in now:               # written in place: nothing may still depend on the old values
+            params[i].data.own()
+            momenta[i].own()
+        count = len(now)
+        rows = [params[i].data.shape[0] for i in now]
+        columns = [params[i].data.size // r if r else 0 for i, r in zip(now, rows)]
+        for r, c in zip(rows, columns):
+            ops._check_products('muon', (r, ops.MOST_ROWS, 'rows'), (c, ops.MOST_ROWS, 'columns'))
+        whole = [k for k in range(count) if rows[k] and columns[k]]
+        count, now = len(whole), [now[k] for k in whole]
+        rows, columns = [rows[k] for k in whole], [columns[k] for k in whole]
+        if count:
+            pointers, ints = ctypes.c_void_p * count, ctypes.c_int * count
+            _hip.call('tt_muon_step_multi_f32', count, pointers(*[params[i].data.ptr for i in now]),
+                      pointers(*[grads[i].ptr for i in now]), pointers(*[momenta[i].ptr for i in now]), ints(*rows),
+                      ints(*columns), (ctypes.c_double * count)(*[adjust(r, c) for r, c in zip(rows, columns)]), lr, momentum,
+                      weight_decay, int(bool(nesterov)), steps, *coefficients, eps)
+        params, grads, momenta = ([some[i] for i in later] for some in (params, grads, momenta))

@@ -1,6 +1,10 @@
 """``SGD`` (``src/tortto/optim/sgd.py``), ``Adam`` and ``AdamW`` (``adam.py``, ``adamw.py``): argument
 checks and per-parameter state of the reference; the arithmetic is one kernel launch per parameter
-(``_functional.py`` here)."""
+(``_functional.py`` here).  ``Muon`` and ``orthogonalize`` are not in the reference."""
+import math
+
+from .. import ops
+from ..tensor import Tensor
 from ..xparray import hiparray
 from . import _functional as F
 from .optimizer import Optimizer, required
@@ -77,3 +81,73 @@ class AdamW(Adam):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, amsgrad=False):
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=amsgrad)
+
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def _coefficients(values):
+    values = tuple(float(v) for v in values)
+    if len(values) != 3 or not all(math.isfinite(v) for v in values):
+        raise ValueError(f'Newton-Schulz takes three coefficients, got {values}')
+    return values
+
+
+def orthogonalize(matrix, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
+    """The nearest semi-orthogonal matrix, roughly: X / max(|X|, eps) (Frobenius norm), then ``steps`` times
+    X <- a X + b (X X^T) X + c (X X^T)^2 X, which brings singular values to about 1 and leaves the singular vectors.  ``matrix`` [rows,
+    columns] is a float32 or float16 device tensor, the result a new one of its type, without a graph.  Coefficients that let a
+    singular value out of [0, 1] grow past 1.9 are refused."""
+    if not isinstance(matrix, Tensor) or matrix.data.__class__ is not hiparray:
+        raise RuntimeError('orthogonalize: device (HIP) path only; move the matrix with .cuda() first')
+    if matrix.ndim != 2:
+        raise RuntimeError(f'orthogonalize takes a matrix, got shape {matrix.shape}')
+    if steps.__class__ is not int or not 1 <= steps <= 100:
+        raise ValueError(f'orthogonalize takes 1 to 100 steps, got {steps}')
+    _check(0.0 < eps <= 1e30, 'Invalid epsilon value: {}', eps)
+    return Tensor.on(ops.orthogonalize(matrix.data, steps, _coefficients(coefficients), float(eps)))
+
+
+_ADJUST = {'original': lambda rows, columns: math.sqrt(max(1.0, rows / columns)),
+           'match_rms_adamw': lambda rows, columns: 0.2 * math.sqrt(max(rows, columns))}
+
+
+class Muon(Optimizer):
+    """Momentum, orthogonalised by Newton-Schulz products, for matrices:
+
+        m <- m + (1 - momentum) (g - m)        u = g + momentum (m - g) with ``nesterov``, else m
+        p <- p (1 - lr weight_decay) - lr scale orthogonalize(u)
+
+    ``adjust_lr_fn`` names the scale: 'original' sqrt(max(1, rows / columns)), 'match_rms_adamw' 0.2 sqrt(max(rows, columns)).
+    Parameters of more than two dimensions are matrices of their first and the others; those of one belong to another
+    optimiser."""
+
+    def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_coefficients=COEFFICIENTS, eps=1e-7,
+                 ns_steps=5, adjust_lr_fn='original'):
+        _check(lr >= 0.0, 'Invalid learning rate: {}', lr)
+        _check(0.0 <= momentum < 1.0, 'Invalid momentum value: {}', momentum)
+        _check(weight_decay >= 0.0, 'Invalid weight_decay value: {}', weight_decay)
+        _check(0.0 < eps <= 1e30, 'Invalid epsilon value: {}', eps)
+        _check(ns_steps.__class__ is int and 1 <= ns_steps <= 100, 'Invalid number of steps: {}', ns_steps)
+        _check(adjust_lr_fn in _ADJUST, 'Invalid adjust_lr_fn: {}', adjust_lr_fn)
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov,
+                                      ns_coefficients=_coefficients(ns_coefficients), eps=eps, ns_steps=ns_steps,
+                                      adjust_lr_fn=adjust_lr_fn))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]['params']:
+            if p.ndim < 2:
+                self.param_groups.pop()
+                raise ValueError(f'Muon takes matrices, got a parameter of shape {p.shape}')
+
+    def step(self):
+        for group, members in self._with_grad():
+            states = [self.state[p] for p in members]
+            for p, state in zip(members, states):
+                if 'momentum_buffer' not in state:
+                    F._device(p)
+                    state['momentum_buffer'] = hiparray.zeros(p.data.shape)
+            F.muon(members, [p.grad for p in members], [s['momentum_buffer'] for s in states], group['lr'], group['momentum'],
+                   group['weight_decay'], group['nesterov'], group['ns_steps'], group['ns_coefficients'], group['eps'],
+                   _ADJUST[group['adjust_lr_fn']])
