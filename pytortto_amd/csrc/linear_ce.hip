@@ -4,7 +4,7 @@
 //   G_iv = g_i (e^(z_iv - M_i) / S_i - [v = t(i)])        dX = G W        dW = G^T x
 //
 // Rows are worked on in chunks.  The first product leaves a chunk's logits in scratch memory (none without gradients)
-// and, with the tile still in registers, every row's maximum and sum over 64 columns; these are joined, and one pass turns the logits
+// and, with the tile still in registers, every row's maximum and sum over a tile's columns; these are joined, and one pass turns the logits
 // into G where they stand.  The two other products read it there: G^T needs no copy, see product.h.  So a training step
 // has three products and not a fourth for logits that it forgot, and the scratch memory is bounded whatever the batch.
 //
@@ -21,7 +21,7 @@ namespace {
 
 using namespace tt;
 
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kLog2e = 1.44269504088896340736f;
 constexpr size_t kMostLogits = (size_t)2 << 30;     // bytes of a chunk's logits
 constexpr size_t kMostStats = (size_t)256 << 20;
 constexpr int kTop = 14;                            // scaled values are below 2^(kTop + 1)
@@ -69,114 +69,155 @@ __global__ __launch_bounds__(1024) void lce_begin(Targets t, long long rows, int
 }
 
 // Rows of x or W as the products' operands: two terms of float32, or a copy of float16.  Rows without a target are
-// zeros, whatever they hold.  A wave has a row.
-template <typename T>
+// zeros, whatever they hold.  G threads have a row; of 16 G columns they keep it between its largest value and its terms.
+template <typename T, int G>
 __global__ __launch_bounds__(256) void lce_rows(const T* __restrict__ from, char* __restrict__ to, int* __restrict__ exponents,
                                                 const float* __restrict__ g, long long rows, int columns, int ld, Targets t,
                                                 int* most) {
-  const long long row = (long long)blockIdx.x * 4 + row_of_block<kWave>();
+  __shared__ float part[256 / kWave];
+  constexpr int kKept = 4;
+  const long long row = (long long)blockIdx.x * (256 / G) + row_of_block<G>();
   if (row >= rows) return;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x % G, quads = (columns + 63) / 64 * 16;
   const T* x = from + (size_t)row * columns;
   char* y = to + (size_t)row * ld;
-  const bool kept = !t.at || class_of(t, row) != kIgnored;
+  const bool kept = !t.at || class_of(t, row) != kIgnored, whole = columns % 4 == 0;
+  const auto four = [&](int q) {
+    typedef T Four __attribute__((ext_vector_type(4)));
+    floatx4 v = {};
+    if (!kept) return v;
+    if (whole && q * 4 < columns) {
+      const Four p = *reinterpret_cast<const Four*>(x + q * 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = widen(p[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (q * 4 + i < columns) v[i] = widen(x[q * 4 + i]);
+    }
+    return v;
+  };
+  floatx4 own[kKept];
+#pragma unroll
+  for (int k = 0; k < kKept; ++k) own[k] = lane + k * G < quads ? four(lane + k * G) : floatx4{};
   int e = 0;
   bool counts = kept;       // among the largest exponents
   if (sizeof(T) == 4) {
     float m = 0.f;
-    if (kept)
-      for (int c = lane; c < columns; c += 64) m = fmaxf(m, fabsf(widen(x[c])));
-    m = lanes_reduce<64>(m, Larger());
+    const auto look = [&](const floatx4& v) { m = fmaxf(m, fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])))); };
+#pragma unroll
+    for (int k = 0; k < kKept; ++k) look(own[k]);
+    for (int q = lane + kKept * G; q < quads; q += G) look(four(q));
+    m = row_max<G>(m, part);
     counts = m > 0.f && __builtin_isfinite(m);
     e = counts ? exponent(m) - kTop - 1 : 0;
-    for (int c = lane; c < (columns + 63) / 64 * 64; c += 64) {
-      _Float16 hi, lo;
-      split(kept && c < columns ? ldexpf(widen(x[c]), -e) : 0.f, &hi, &lo);
-      char* p = y + at_column(c);
-      *reinterpret_cast<_Float16*>(p) = hi;
-      *reinterpret_cast<_Float16*>(p + kTermBytes) = lo;
-    }
     if (lane == 0) exponents[row] = counts ? e : kAny;
-  } else {
-    for (int c = lane; c < (columns + 63) / 64 * 64; c += 64)
-      *reinterpret_cast<_Float16*>(y + c * 2) = kept && c < columns ? (_Float16)x[c] : (_Float16)0.f;
   }
-  if (most && lane == 0 && counts) {
-    if (!g) atomicMax(most, e);
-    else if (g[row] != 0.f) atomicMax(most, e + exponent(g[row]));
+  const auto put = [&](int q, const floatx4& v) {
+    if (sizeof(T) == 4) {
+      store_terms(y, q * 4, floatx4{ldexpf(v[0], -e), ldexpf(v[1], -e), ldexpf(v[2], -e), ldexpf(v[3], -e)});
+    } else {
+      *reinterpret_cast<half4*>(y + q * 8) = half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < kKept; ++k)
+    if (lane + k * G < quads) put(lane + k * G, own[k]);
+  for (int q = lane + kKept * G; q < quads; q += G) put(q, four(q));
+  if (most && lane == 0 && counts && (!g || g[row] != 0.f)) {
+    // (looked at first: it rises a few times, and an atomic operation of every row costs 9 ns of all the others)
+    const int it = g ? e + exponent(g[row]) : e;
+    if (shared(most) < it) atomicMax(most, it);
   }
 }
 
-struct LogitsEpilogue {
+struct Logits {
   const int* f;         // exponents of x's rows and W's, of float32
   const int* e;
   Targets t;
   long long first;      // row of the chunk's first
   float* z;             // [rows][ld] or none
   long long ld;
-  float2* stats;        // [rows][blocks of 64 columns]
+  float2* stats;        // [rows][blocks]: of a tile's columns the largest logit, and the sum of e^(z - it) without its 1
   float* own;           // [rows] the target's logit
   int blocks;
-
-  template <int TERMS, typename G>
-  __device__ __forceinline__ void apply(G& p, int m0, int n0, int rows, int V) const {
-    constexpr int MT = sizeof(p.acc) / sizeof(p.acc[0]);
-    const int c0 = n0 + G::column(), lane = threadIdx.x & 63;
-    int scale[16];
-    if (TERMS == 2) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int c = c0 + (j >> 2) * 16 + (j & 3);
-        scale[j] = c < V ? e[c] : 0;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int r = m0 + G::row() + 16 * i;
-      const bool in = r < rows;
-      const int fi = TERMS == 2 && in ? f[r] : 0, target = in ? class_of(t, first + r) : kIgnored;
-      float v[16], most = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int c = c0 + (j >> 2) * 16 + (j & 3);
-        v[j] = p.acc[i][j >> 2][j & 3];
-        if (TERMS == 2) v[j] = ldexpf(v[j], scale[j] + fi);
-        if (c == target) own[r] = v[j];
-        if (c < V) most = fmaxf(most, v[j]);
-      }
-      if (z && in) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c0 + 16 * j < ld) *reinterpret_cast<floatx4*>(z + (size_t)r * ld + c0 + 16 * j) = floatx4{v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]};
-      }
-      most = fmaxf(most, __shfl_xor(most, 16, kWave));
-      most = fmaxf(most, __shfl_xor(most, 32, kWave));
-      const float from = most == -INFINITY ? 0.f : most;
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (c0 + (j >> 2) * 16 + (j & 3) < V) sum += __builtin_amdgcn_exp2f((v[j] - from) * kLog2e);
-      sum += __shfl_xor(sum, 16, kWave);
-      sum += __shfl_xor(sum, 32, kWave);
-      const int block = (c0 - (lane >> 4) * 4) >> 6;
-      if (in && lane < 16 && block < blocks) stats[(size_t)r * blocks + block] = make_float2(most, sum);
-    }
-  }
 };
 
 template <int TERMS, int SIZE>
-__global__ __launch_bounds__((Sized<TERMS, false, false, SIZE>::kThreads)) void lce_logits(Operand x, Operand w, int rows, int V,
-                                                                                          int stages, LogitsEpilogue epilogue) {
+__global__ __launch_bounds__(256) void lce_logits(Operand x, Operand w, int rows, int V, int pairs, Logits q) {
   typedef Sized<TERMS, false, false, SIZE> G;
   extern __shared__ __align__(16) char lds[];
   int m, n;
   tile_of(blockIdx.x, gridDim.x, (rows + G::kM - 1) / G::kM, (V + G::kN - 1) / G::kN, &m, &n);
+  const int m0 = m * G::kM, n0 = n * G::kN;
   G p;
-  p.run(x, w, m * G::kM, n * G::kN, 0, stages, lds);
-  epilogue.template apply<TERMS>(p, m * G::kM, n * G::kN, rows, V);
+  p.run(x, w, m0, n0, 0, pairs, lds);
+  // the rows' targets and exponents, and the columns' exponents
+  int2* about = reinterpret_cast<int2*>(lds + G::kExtra);
+  for (int r = threadIdx.x; r < G::kM; r += 256)
+    if (m0 + r < rows) about[r] = make_int2(class_of(q.t, q.first + m0 + r), TERMS == 2 ? q.f[m0 + r] : 0);
+  const int at = threadIdx.x & 63, c0 = n0 + at % G::kLanes * 4;
+  int4 scale = {};
+  if (TERMS == 2) scale = *reinterpret_cast<const int4*>(q.e + c0);        // (padded to a whole tile)
+  __syncthreads();
+  constexpr int U = G::kAhead;
+  p.rows(lds, [](int, int) { return 0; }, [&](int r, int, floatx4 (&v)[U], int (&)[U]) {
+    int target[U];
+    float most[U], sum[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int2 mine = about[r + u * G::kStep];
+      target[u] = mine.x;
+      if (TERMS == 2) {
+        v[u][0] = ldexpf(v[u][0], scale.x + mine.y);
+        v[u][1] = ldexpf(v[u][1], scale.y + mine.y);
+        v[u][2] = ldexpf(v[u][2], scale.z + mine.y);
+        v[u][3] = ldexpf(v[u][3], scale.w + mine.y);
+      }
+    }
+    if (q.z && c0 < q.ld) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (m0 + r + u * G::kStep < rows) *reinterpret_cast<floatx4*>(q.z + (size_t)(m0 + r + u * G::kStep) * q.ld + c0) = v[u];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c0 + i >= V) v[u][i] = -INFINITY;
+      most[u] = fmaxf(fmaxf(v[u][0], v[u][1]), fmaxf(v[u][2], v[u][3]));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) most[u] = lanes_reduce<G::kLanes>(most[u], Larger());
+    int largest[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      // (the largest values apart, in whole units: one of them is left out)
+      const float from = most[u] == -INFINITY ? 0.f : most[u];
+      sum[u] = 0.f;
+      largest[u] = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool it = v[u][i] == most[u];
+        const unsigned long long those = __ballot(it && c0 + i < V);
+        largest[u] += __popcll(G::kLanes == 64 ? those : (those >> (at / G::kLanes * G::kLanes)) & ((1ull << (G::kLanes % 64)) - 1));
+        sum[u] += it ? 0.f : __builtin_amdgcn_exp2f((v[u][i] - from) * kLog2e);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) sum[u] = lanes_reduce<G::kLanes>(sum[u], Plus());
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int row = m0 + r + u * G::kStep, here = target[u] - c0;
+      if (row >= rows) continue;
+      if (here >= 0 && here < 4) q.own[row] = here == 0 ? v[u][0] : here == 1 ? v[u][1] : here == 2 ? v[u][2] : v[u][3];
+      if (at % G::kLanes == 0) q.stats[(size_t)row * q.blocks + n] = make_float2(most[u], sum[u] + (float)(largest[u] - 1));
+    }
+  });
 }
 
-// A row's maximum and log2 of its sum from those of its blocks, and its loss.  A wave has a row.
+// A row's maximum and log2 of its sum from those of its blocks, and its loss.  A wave has a row.  The sum is kept without the
+// largest term, which is 1: of a target that has nearly all of the probability, the loss is what is left, and keeps its digits.
 __global__ __launch_bounds__(256) void lce_join(const float2* __restrict__ stats, const float* __restrict__ own, float2* __restrict__ of,
                                                 float* __restrict__ loss, Targets t, long long first, int rows, int blocks) {
   const int r = blockIdx.x * 4 + row_of_block<kWave>();
@@ -191,23 +232,26 @@ __global__ __launch_bounds__(256) void lce_join(const float2* __restrict__ stats
   for (int b = lane; b < blocks; b += 64) most = fmaxf(most, s[b].x);
   most = lanes_reduce<64>(most, Larger());
   const float from = most == -INFINITY ? 0.f : most;
-  float sum = 0.f;
+  float rest = 0.f;
+  int largest = 0;
   for (int b = lane; b < blocks; b += 64) {
     const float2 v = s[b];
-    sum += v.y * __builtin_amdgcn_exp2f(((v.x == -INFINITY ? from : v.x) - from) * kLog2e);
+    const bool it = v.x == most;
+    largest += it;
+    rest += it ? v.y : (1.f + v.y) * __builtin_amdgcn_exp2f((v.x - from) * kLog2e);
   }
-  sum = lanes_reduce<64>(sum, Plus());
+  rest = lanes_reduce<64>(rest, Plus()) + (float)(lanes_reduce<64>(largest, Plus()) - 1);
   if (lane == 0) {
-    const float log_sum = log2f(sum);
-    of[r] = make_float2(from, log_sum);
-    loss[r] = target == kInvalid ? NAN : log_sum * kLn2 + (from - own[r]);
+    const float log_sum = log1pf(rest);
+    of[r] = make_float2(from, log_sum * kLog2e);
+    loss[r] = target == kInvalid ? NAN : log_sum + (from - own[r]);
   }
 }
 
 // With the exponent of a row of zeros, it is the largest that leaves the row's G (times its g) in range.
 __device__ __forceinline__ int exponent_of_row(int e, int top, float g) { return e == kAny ? top - exponent(g) + 1 : e; }
 
-// The logits of a chunk become G, where they stand: 64 floats are the 64 first and 64 second terms.
+// The logits of a chunk become G, where they stand: 32 floats are their first and second terms, or 64 their values as halves and a gap.
 template <int TERMS>
 __global__ __launch_bounds__(256) void lce_gradient(float* __restrict__ z, long long ld, const float2* __restrict__ of,
                                                     const float* __restrict__ loss, const float* __restrict__ g,
@@ -239,7 +283,7 @@ __global__ __launch_bounds__(256) void lce_gradient(float* __restrict__ z, long 
   if (TERMS == 2) {
     store_terms(row, c, v);
   } else {
-    *reinterpret_cast<half4*>(row + at_column(c)) = half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+    *reinterpret_cast<half4*>(row + (c >> 6) * (2 * kLine) + (c & 63) * 2) = half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
   }
 }
 
@@ -253,61 +297,85 @@ struct GradientOut {
   const Control* control;
   int half, add;
   int columns;
-  __device__ __forceinline__ void store(int row, int c, floatx4 v) const {
-    const float s = control->scale;
+  // What a row's sums are multiplied with besides the scale: a power of two.
+  __device__ __forceinline__ int exponent_for(int row) const {
     const int top = top_f ? control->top_f() : control->top_e();
-    const int e = control->top_e() + control->top_f() - kTop - (exponents ? exponent_of_row(exponents[row], top, g ? g[row] : 1.f) : 0);
+    return control->top_e() + control->top_f() - kTop - (exponents ? exponent_of_row(exponents[row], top, g ? g[row] : 1.f) : 0);
+  }
+  // What stands there, to be added to.
+  __device__ __forceinline__ floatx4 before(int row, int c) const {
+    const size_t at = (size_t)row * columns + c;
+    const float* p = reinterpret_cast<const float*>(to) + at;
+    floatx4 v = {};
+    if (columns - c >= 4 && (at & 3) == 0) return *reinterpret_cast<const floatx4*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < columns - c) v[i] = p[i];
+    return v;
+  }
+  __device__ __forceinline__ void store(int row, int c, floatx4 v, float s, int e, const floatx4& old) const {
     const size_t at = (size_t)row * columns + c;
     const int n = columns - c;
+    const bool whole = n >= 4 && (at & 3) == 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = ldexpf(v[i] * s, e);
+    v += old;
     if (half) {
       _Float16* p = reinterpret_cast<_Float16*>(to) + at;
-      if (n >= 4 && (at & 3) == 0) {
+      if (whole) {
         *reinterpret_cast<half4*>(p) = half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
       } else {
-        for (int i = 0; i < 4 && i < n; ++i) p[i] = (_Float16)v[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < n) p[i] = (_Float16)v[i];
       }
     } else {
       float* p = reinterpret_cast<float*>(to) + at;
-      if (n >= 4 && (at & 3) == 0) {
-        floatx4* q = reinterpret_cast<floatx4*>(p);
-        *q = add ? *q + v : v;
+      if (whole) {
+        *reinterpret_cast<floatx4*>(p) = v;
       } else {
-        for (int i = 0; i < 4 && i < n; ++i) p[i] = add ? p[i] + v[i] : v[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < n) p[i] = v[i];
       }
     }
   }
 };
 
 template <int TERMS, bool A_ACROSS, int SIZE>
-__global__ __launch_bounds__((Sized<TERMS, A_ACROSS, true, SIZE>::kThreads)) void lce_product(Operand a, Operand b, int M, int N, int stages,
-                                                                                            int per, int splits, float* partial, GradientOut out) {
+__global__ __launch_bounds__(256) void lce_product(Operand a, Operand b, int M, int N, int pairs, int per, int splits, float* partial,
+                                                   GradientOut out) {
   typedef Sized<TERMS, A_ACROSS, true, SIZE> G;
   extern __shared__ __align__(16) char lds[];
   const int blocks = gridDim.x / splits, split = blockIdx.x / blocks;
   int m, n;
   tile_of(blockIdx.x % blocks, blocks, (M + G::kM - 1) / G::kM, (N + G::kN - 1) / G::kN, &m, &n);
-  const int first = split * per, count = min(per, stages - first);
+  const int first = split * per, count = min(per, pairs - first), m0 = m * G::kM, n0 = n * G::kN;
   G p;
-  p.run(a, b, m * G::kM, n * G::kN, first, count, lds);
-  constexpr int MT = sizeof(p.acc) / sizeof(p.acc[0]), NT = sizeof(p.acc[0]) / sizeof(p.acc[0][0]);
+  p.run(a, b, m0, n0, first, count, lds);
+  if (splits > 1) {
+    const long long ld = (N + 3) / 4 * 4;
+    float* to = partial + ((size_t)split * M + m0) * ld + n0;
+    p.rows(lds, [](int, int) { return 0; }, [&](int r, int c, const floatx4 (&v)[G::kAhead], int (&)[G::kAhead]) {
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int row = m * G::kM + G::row() + 16 * i;
-    if (row >= M) continue;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int c = n * G::kN + G::column() + 16 * j;
-      if (c >= N) continue;
-      if (splits > 1) {
-        const long long ld = (N + 3) / 4 * 4;
-        *reinterpret_cast<floatx4*>(partial + ((size_t)split * M + row) * ld + c) = p.acc[i][j];
-      } else {
-        out.store(row, c, p.acc[i][j]);
-      }
-    }
+      for (int u = 0; u < G::kAhead; ++u)
+        if (m0 + r + u * G::kStep < M && n0 + c < N) *reinterpret_cast<floatx4*>(to + (r + u * G::kStep) * ld + c) = v[u];
+    });
+    return;
   }
+  int* about = reinterpret_cast<int*>(lds + G::kExtra);
+  for (int r = threadIdx.x; r < G::kM; r += 256)
+    if (m0 + r < M) about[r] = out.exponent_for(m0 + r);
+  const float scale = out.control->scale;
+  __syncthreads();
+  p.rows(lds, [&](int r, int c) { return out.add && m0 + r < M && n0 + c < N ? out.before(m0 + r, n0 + c) : floatx4{}; },
+         [&](int r, int c, const floatx4 (&v)[G::kAhead], const floatx4 (&old)[G::kAhead]) {
+#pragma unroll
+           for (int u = 0; u < G::kAhead; ++u) {
+             const int k = r + u * G::kStep;
+             if (m0 + k < M && n0 + c < N) out.store(m0 + k, n0 + c, v[u], scale, about[k], old[u]);
+           }
+         });
 }
 
 __global__ __launch_bounds__(256) void lce_sum(const float* __restrict__ partial, int splits, int M, int N, GradientOut out) {
@@ -316,7 +384,8 @@ __global__ __launch_bounds__(256) void lce_sum(const float* __restrict__ partial
   if (at >= (long long)M * quads) return;
   floatx4 v = {};
   for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const floatx4*>(partial + ((size_t)s * M * quads + at) * 4);
-  out.store((int)(at / quads), (int)(at % quads) * 4, v);
+  const int row = (int)(at / quads);
+  out.store(row, (int)(at % quads) * 4, v, out.control->scale, out.exponent_for(row), floatx4{});
 }
 
 __global__ __launch_bounds__(1024) void lce_loss(const float* __restrict__ loss, long long rows, int mean, Targets t, const Control* control,
@@ -350,48 +419,54 @@ int launch_scale(const float* from, const float* g, T* to, size_t n) {
   return 0;
 }
 
+template <typename T>
+void launch_rows(const T* from, char* to, int* exponents, const float* g, long long rows, int columns, int ld, const Targets& t, int* most) {
+  if (columns <= 1024) lce_rows<T, 64><<<(unsigned)((rows + 3) / 4), 256, 0, stream()>>>(from, to, exponents, g, rows, columns, ld, t, most);
+  else lce_rows<T, 256><<<(unsigned)rows, 256, 0, stream()>>>(from, to, exponents, g, rows, columns, ld, t, most);
+}
+
 template <int TERMS, int SIZE>
-int launch_logits(const Operand& x, const Operand& w, int rows, int V, int H, const LogitsEpilogue& epilogue) {
+int launch_logits(const Operand& x, const Operand& w, int rows, int V, int H, const Logits& q) {
   typedef Sized<TERMS, false, false, SIZE> G;
   TT_ALLOW_LDS((lce_logits<TERMS, SIZE>), G::kLds);
   lce_logits<TERMS, SIZE><<<(unsigned)tiles_of(rows, V, SIZE), G::kThreads, G::kLds, stream()>>>(
-      x, w, rows, V, (int)(padded(H) / G::kDepth), epilogue);
+      x, w, rows, V, (int)(padded(H) / (64 / TERMS)), q);
   TT_LAUNCH_CHECK();
   return 0;
 }
 template <int TERMS>
-int launch_logits(const Operand& x, const Operand& w, int rows, int V, int H, const LogitsEpilogue& epilogue) {
-  switch (tile_size(rows, V)) {
-    case 2: return launch_logits<TERMS, 2>(x, w, rows, V, H, epilogue);
-    case 1: return launch_logits<TERMS, 1>(x, w, rows, V, H, epilogue);
-    default: return launch_logits<TERMS, 0>(x, w, rows, V, H, epilogue);
+int launch_logits(int size, const Operand& x, const Operand& w, int rows, int V, int H, const Logits& q) {
+  switch (size) {
+    case 2: return launch_logits<TERMS, 2>(x, w, rows, V, H, q);
+    case 1: return launch_logits<TERMS, 1>(x, w, rows, V, H, q);
+    default: return launch_logits<TERMS, 0>(x, w, rows, V, H, q);
   }
 }
 
-// How a gradient's product [m, n] over `stages` is cut: the size of its tiles, and how many blocks share one.
+// How a gradient's product [m, n] over `pairs` is cut: the size of its tiles, and how many blocks share one.
 struct Plan {
-  int size, per, splits;      // stages for each block, blocks
+  int size, per, splits;      // pairs for each block, blocks
 };
-Plan plan_product(long long m, long long n, long long stages) {
+Plan plan_product(long long m, long long n, long long pairs) {
   Plan p;
   p.size = tile_size(m, n);
   // few tiles and a long reduction: large tiles shared by several blocks
-  while (p.size < 2 && stages >= 64 && tiles_of(m, n, p.size + 1) * (stages / 16) >= compute_units() && m > kTileSide[p.size] && n > kTileSide[p.size]) ++p.size;
+  while (p.size < 2 && pairs >= 64 && tiles_of(m, n, p.size + 1) * (pairs / 16) >= compute_units() && m > kTileSide[p.size] && n > kTileSide[p.size]) ++p.size;
   const long long tiles = tiles_of(m, n, p.size);
   long long splits = compute_units() / tiles;
-  splits = std::max(1LL, std::min(splits, stages / 8));
-  p.per = (int)((stages + splits - 1) / splits);
-  p.splits = (int)((stages + p.per - 1) / p.per);
+  splits = std::max(1LL, std::min(splits, pairs / 8));
+  p.per = (int)((pairs + splits - 1) / splits);
+  p.splits = (int)((pairs + p.per - 1) / p.per);
   return p;
 }
 
 template <int TERMS, bool A_ACROSS, int SIZE>
-int launch_product(const Operand& a, const Operand& b, int M, int N, int stages, int per, float* partial, const GradientOut& out) {
+int launch_product(const Operand& a, const Operand& b, int M, int N, int pairs, int per, float* partial, const GradientOut& out) {
   typedef Sized<TERMS, A_ACROSS, true, SIZE> G;
   TT_ALLOW_LDS((lce_product<TERMS, A_ACROSS, SIZE>), G::kLds);
-  const int splits = (stages + per - 1) / per;      // (fewer for a chunk that is not whole)
+  const int splits = (pairs + per - 1) / per;      // (fewer for a chunk that is not whole)
   lce_product<TERMS, A_ACROSS, SIZE><<<(unsigned)(tiles_of(M, N, SIZE) * splits), G::kThreads, G::kLds, stream()>>>(
-      a, b, M, N, stages, per, splits, partial, out);
+      a, b, M, N, pairs, per, splits, partial, out);
   TT_LAUNCH_CHECK();
   if (splits > 1) {
     const long long quads = (long long)M * ((N + 3) / 4);
@@ -401,11 +476,11 @@ int launch_product(const Operand& a, const Operand& b, int M, int N, int stages,
   return 0;
 }
 template <int TERMS, bool A_ACROSS>
-int launch_product(const Plan& plan, const Operand& a, const Operand& b, int M, int N, int stages, float* partial, const GradientOut& out) {
+int launch_product(const Plan& plan, const Operand& a, const Operand& b, int M, int N, int pairs, float* partial, const GradientOut& out) {
   switch (plan.size) {
-    case 2: return launch_product<TERMS, A_ACROSS, 2>(a, b, M, N, stages, plan.per, partial, out);
-    case 1: return launch_product<TERMS, A_ACROSS, 1>(a, b, M, N, stages, plan.per, partial, out);
-    default: return launch_product<TERMS, A_ACROSS, 0>(a, b, M, N, stages, plan.per, partial, out);
+    case 2: return launch_product<TERMS, A_ACROSS, 2>(a, b, M, N, pairs, plan.per, partial, out);
+    case 1: return launch_product<TERMS, A_ACROSS, 1>(a, b, M, N, pairs, plan.per, partial, out);
+    default: return launch_product<TERMS, A_ACROSS, 0>(a, b, M, N, pairs, plan.per, partial, out);
   }
 }
 
@@ -434,16 +509,17 @@ int run(const Call& q) {
   const int V = q.t.V, H = q.H, mean = q.reduction == 2;
   const long long N = q.N, Hp = padded(H), Vp = padded(V);
   const bool grad = q.dx || q.dw, copy_w = TERMS == 2 || H % 8 != 0;
-  const int blocks = (int)(Vp / 64), depth = TERMS == 1 ? 64 : 32;
+  const int depth = 64 / TERMS;
   long long chunk = (long long)((grad ? kMostLogits : kMostStats) / ((size_t)Vp * (grad ? 4 : 8) / (grad ? 1 : 64)));
   chunk = std::max(256LL, chunk / 256 * 256);
   chunk = std::min(chunk, N);
   const bool several = chunk < N;
-  const int stagesV = (int)(Vp / depth), stagesN = (int)((chunk + depth - 1) / depth);
-  const Plan plan_x = plan_product(chunk, H, stagesV), plan_w = plan_product(V, H, stagesN);
+  const int pairsV = (int)(Vp / depth), pairsN = (int)((chunk + depth - 1) / depth);
+  const int size = tile_size(chunk, V), blocks = (V + kTileSide[size] - 1) / kTileSide[size];
+  const Plan plan_x = plan_product(chunk, H, pairsV), plan_w = plan_product(V, H, pairsN);
 
   Carve c;
-  const size_t at_control = c.take(sizeof(Control)), at_f = c.take(TERMS == 2 ? 4 * N : 0), at_e = c.take(TERMS == 2 ? 4 * (size_t)V : 0);
+  const size_t at_control = c.take(sizeof(Control)), at_f = c.take(TERMS == 2 ? 4 * N : 0), at_e = c.take(TERMS == 2 ? 4 * (size_t)(V + 256) : 0);
   const size_t at_x = c.take((size_t)N * Hp * 2 * TERMS), at_w = c.take(copy_w ? (size_t)V * Hp * 2 * TERMS : 0);
   const size_t at_stats = c.take((size_t)chunk * blocks * 8), at_own = c.take(4 * chunk), at_of = c.take(8 * chunk);
   const size_t at_loss = c.take(4 * N), at_z = c.take(grad ? (size_t)chunk * Vp * 4 : 0);
@@ -464,21 +540,21 @@ int run(const Call& q) {
   lce_begin<<<1, 1024, 0, stream()>>>(q.t, N, mean, TERMS == 2 ? kLowest : 0, TERMS == 2 || q.g ? kLowest : 0, control);
   TT_LAUNCH_CHECK();
   const int ldx = (int)(Hp * 2 * TERMS);
-  lce_rows<T><<<(unsigned)((N + 3) / 4), 256, 0, stream()>>>((const T*)q.x, base + at_x, f, q.g, N, H, ldx, q.t,
+  launch_rows<T>((const T*)q.x, base + at_x, f, q.g, N, H, ldx, q.t,
                                                              TERMS == 2 || q.g ? &control->most_f : nullptr);
   TT_LAUNCH_CHECK();
-  Operand w = {(const char*)q.w, (long long)V * H * 2, H * 2, kTermBytes};
+  Operand w = {(const char*)q.w, (long long)V * H * 2, H * 2, kLine};
   if (copy_w) {
-    lce_rows<T><<<(unsigned)((V + 3) / 4), 256, 0, stream()>>>((const T*)q.w, base + at_w, e, nullptr, V, H, ldx, Targets{nullptr, 0, 0, 0},
+    launch_rows<T>((const T*)q.w, base + at_w, e, nullptr, V, H, ldx, Targets{nullptr, 0, 0, 0},
                                                                TERMS == 2 ? &control->most_e : nullptr);
     TT_LAUNCH_CHECK();
-    w = Operand{base + at_w, (long long)V * ldx, ldx, kTermBytes * TERMS};
+    w = Operand{base + at_w, (long long)V * ldx, ldx, kLine};
   }
   for (long long first = 0; first < N; first += chunk) {
     const int rows = (int)std::min(chunk, N - first);
-    const Operand x = {base + at_x + (size_t)first * ldx, (long long)rows * ldx, ldx, kTermBytes * TERMS};
-    const LogitsEpilogue epilogue = {f ? f + first : nullptr, e, q.t, first, z, Vp, stats, own, blocks};
-    if (launch_logits<TERMS>(x, w, rows, V, H, epilogue)) return -1;
+    const Operand x = {base + at_x + (size_t)first * ldx, (long long)rows * ldx, ldx, kLine};
+    const Logits logits = {f ? f + first : nullptr, e, q.t, first, z, Vp, stats, own, blocks};
+    if (launch_logits<TERMS>(size, x, w, rows, V, H, logits)) return -1;
     lce_join<<<(unsigned)((rows + 3) / 4), 256, 0, stream()>>>(stats, own, of, losses + first, q.t, first, rows, blocks);
     TT_LAUNCH_CHECK();
     if (!grad) continue;
@@ -488,11 +564,11 @@ int run(const Call& q) {
           z + (size_t)r * Vp, Vp, of + r, losses + first + r, q.g, f ? f + first + r : nullptr, e, q.t, first + r, V, control);
       TT_LAUNCH_CHECK();
     }
-    const Operand gradient = {(const char*)z, (long long)rows * Vp * 4, (int)(Vp * 4), 2 * kTermBytes};
+    const Operand gradient = {(const char*)z, (long long)rows * Vp * 4, (int)(Vp * 4), TERMS == 1 ? 2 * kLine : kLine};
     if (q.dx) {
       const GradientOut out = {(char*)q.dx + (size_t)first * H * (q.half_out ? 2 : 4), f ? f + first : nullptr, 1, q.g ? q.g + first : nullptr, control,
                                q.half_out, 0, H};
-      if (launch_product<TERMS, false>(plan_x, gradient, w, rows, H, stagesV, partial, out)) return -1;
+      if (launch_product<TERMS, false>(plan_x, gradient, w, rows, H, pairsV, partial, out)) return -1;
     }
     if (q.dw) {
       const GradientOut out = {several && q.half_out ? (void*)(base + at_sum) : q.dw, e, 0, nullptr, control, several ? 0 : q.half_out, first > 0, H};

@@ -43,8 +43,8 @@ struct Place {
   __host__ __device__ Place(int rows, int columns) {
     tall = rows > columns;
     m = tall ? columns : rows;
-    ldx = (long long)((columns + 63) / 64) * 256;
-    lda = (long long)((m + 63) / 64) * 256;
+    ldx = padded(columns) * 4;
+    lda = padded(m) * 4;
     x = ldx * rows;
     a = lda * m;
   }
@@ -124,18 +124,6 @@ __global__ __launch_bounds__(256) void muon_scale(Batch b, Rule q) {
   }
 }
 
-template <typename G, typename F>
-__device__ __forceinline__ void each(const G& p, int m0, int n0, int M, F f) {
-  constexpr int MT = sizeof(p.acc) / sizeof(p.acc[0]), NT = sizeof(p.acc[0]) / sizeof(p.acc[0][0]);
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int row = m0 + G::row() + 16 * i;
-    if (row >= M) continue;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) f(row, n0 + G::column() + 16 * j, p.acc[i][j]);
-  }
-}
-
 constexpr int kGram = 0, kPolynomial = 1, kUpdate = 2;
 
 // One product of a step for a tile of one matrix.
@@ -147,54 +135,93 @@ __device__ __forceinline__ void muon_tile(const Matrix& x, const Rule& q, bool l
   char* x0 = x.scratch + (q.step & 1 ? p.x : 0);
   char* x1 = x.scratch + (q.step & 1 ? 0 : p.x);
   char *a = x.scratch + 2 * p.x, *s = a + p.a;
-  const Operand X = {x0, p.x, (int)p.ldx, 2 * kTermBytes}, A = {a, p.a, (int)p.lda, 2 * kTermBytes}, S = {s, p.a, (int)p.lda, 2 * kTermBytes};
+  const Operand X = {x0, p.x, (int)p.ldx, kLine}, A = {a, p.a, (int)p.lda, kLine}, S = {s, p.a, (int)p.lda, kLine};
   const int M = WHAT == kUpdate ? x.rows : p.m, N = WHAT == kUpdate ? x.columns : p.m;
   int m, n;
   tile_of((int)block, (int)blocks, (M + G::kM - 1) / G::kM, (N + G::kN - 1) / G::kN, &m, &n);
   G g;
   const int m0 = m * G::kM, n0 = n * G::kN, edge = (N + 63) / 64 * 64;
+  constexpr int U = G::kAhead;
+  const auto each = [&](int r, int c, int edge, auto f) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (m0 + r + u * G::kStep < M && n0 + c < edge) f(u, m0 + r + u * G::kStep, n0 + c);
+  };
   if (WHAT == kGram) {
     const int k = ACROSS ? x.rows : x.columns;
     g.run(X, X, m0, n0, 0, (k + 31) / 32, lds);
-    each(g, m0, n0, M, [&](int row, int c, const floatx4& v) {
-      if (c < edge) store_terms(a + row * p.lda, c, v * (1.f / kUp));
+    g.rows(lds, [](int, int) { return 0; }, [&](int r, int c, const floatx4 (&v)[U], int (&)[U]) {
+      each(r, c, edge, [&](int u, int row, int column) { store_terms(a + row * p.lda, column, v[u] * (1.f / kUp)); });
     });
   } else if (WHAT == kPolynomial) {
     g.run(A, A, m0, n0, 0, (p.m + 31) / 32, lds);
-    each(g, m0, n0, M, [&](int row, int c, const floatx4& v) {
-      if (c < edge) store_terms(s + row * p.lda, c, load_terms(a + row * p.lda, c) * (q.b * 0.25f) + v * (q.c * (0.25f / kUp)));
-    });
+    g.rows(lds, [&](int r, int c) { return m0 + r < M && n0 + c < edge ? load_terms(a + (m0 + r) * p.lda, n0 + c) : floatx4{}; },
+           [&](int r, int c, const floatx4 (&v)[U], const floatx4 (&old)[U]) {
+             each(r, c, edge, [&](int u, int row, int column) {
+               store_terms(s + row * p.lda, column, old[u] * (q.b * 0.25f) + v[u] * (q.c * (0.25f / kUp)));
+             });
+           });
   } else {
     // wide: S X with X's rows as k;  tall: X S, S being symmetric
     if (ACROSS) g.run(S, X, m0, n0, 0, (p.m + 31) / 32, lds);
     else g.run(X, S, m0, n0, 0, (p.m + 31) / 32, lds);
-    each(g, m0, n0, M, [&](int row, int c, const floatx4& v) {
-      if (c >= edge) return;
-      const floatx4 y = load_terms(x0 + row * p.ldx, c) * q.a + v * (1.f / 4096.f);
-      if (!last) {
-        store_terms(x1 + row * p.ldx, c, y);
-        return;
-      }
-      const size_t at = (size_t)row * x.columns + c;
+    const auto old = [&](int r, int c) { return m0 + r < M && n0 + c < edge ? load_terms(x0 + (m0 + r) * p.ldx, n0 + c) : floatx4{}; };
+    if (!last) {
+      g.rows(lds, old, [&](int r, int c, const floatx4 (&v)[U], const floatx4 (&o)[U]) {
+        each(r, c, edge, [&](int u, int row, int column) { store_terms(x1 + row * p.ldx, column, o[u] * q.a + v[u] * (1.f / 4096.f)); });
+      });
+      return;
+    }
+    const int columns = x.columns;
+    const bool whole = columns % 4 == 0 && (reinterpret_cast<uintptr_t>(x.to) & 15) == 0;
+    const auto put = [&](auto* to, int column, const floatx4& y) {
+      typedef __typeof__(*to) T;
+      typedef T Four __attribute__((ext_vector_type(4)));
+      if (whole) {
+        *reinterpret_cast<Four*>(to) = Four{(T)y[0], (T)y[1], (T)y[2], (T)y[3]};
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (c + i >= x.columns) break;
-        const float o = y[i] * (1.f / kUp);
-        if (x.momentum) {
-          float* w = reinterpret_cast<float*>(x.to) + at + i;
-          *w = *w * q.keep - x.rate * o;
-        } else if (q.half) {
-          reinterpret_cast<_Float16*>(x.to)[at + i] = (_Float16)o;
-        } else {
-          reinterpret_cast<float*>(x.to)[at + i] = o;
-        }
+        for (int i = 0; i < 4; ++i)
+          if (column + i < columns) to[i] = (T)y[i];
       }
-    });
+    };
+    if (x.momentum) {
+      float* w = reinterpret_cast<float*>(x.to);
+      const float rate = x.rate;
+      g.rows(lds,
+             [&](int r, int c) {
+               floatx4 v = {};
+               if (m0 + r >= M || n0 + c >= columns) return v;
+               const float* from = w + (size_t)(m0 + r) * columns + n0 + c;
+               if (whole) {
+                 v = *reinterpret_cast<const floatx4*>(from);
+               } else {
+#pragma unroll
+                 for (int i = 0; i < 4; ++i)
+                   if (n0 + c + i < columns) v[i] = from[i];
+               }
+               return v * q.keep - old(r, c) * (q.a * rate * (1.f / kUp));
+             },
+             [&](int r, int c, const floatx4 (&v)[U], const floatx4 (&o)[U]) {
+               each(r, c, columns, [&](int u, int row, int column) {
+                 put(w + (size_t)row * columns + column, column, o[u] - v[u] * (rate * (1.f / 4096.f / kUp)));
+               });
+             });
+    } else {
+      g.rows(lds, old, [&](int r, int c, const floatx4 (&v)[U], const floatx4 (&o)[U]) {
+        each(r, c, columns, [&](int u, int row, int column) {
+          const floatx4 y = (o[u] * q.a + v[u] * (1.f / 4096.f)) * (1.f / kUp);
+          const size_t at = (size_t)row * columns + column;
+          if (q.half) put(reinterpret_cast<_Float16*>(x.to) + at, column, y);
+          else put(reinterpret_cast<float*>(x.to) + at, column, y);
+        });
+      });
+    }
   }
 }
 
 template <int WHAT, int SIZE>
-__global__ __launch_bounds__((Sized<2, false, false, SIZE>::kThreads)) void muon_product(Batch b, Rule q, int last) {
+__global__ __launch_bounds__(256) void muon_product(Batch b, Rule q, int last) {
   extern __shared__ __align__(16) char lds[];
   const int at = matrix_of(b);
   const Matrix& x = b.of[at];

@@ -3,21 +3,26 @@
 //
 //   D[m, n] = sum_k A(m, k) B(n, k),  float32 accumulators
 //
-// Operands are rows of float16 terms.  A row's columns stand in blocks of 64: 128 bytes of the values themselves (TERMS = 1),
-// or of the leading terms with the 128 bytes of the second terms behind them (TERMS = 2).  Two terms hold x = hi + lo with
-// hi = f16(x) and lo = f16(x - hi), x scaled by a power of two so that neither leaves the type's range: 22 bits and
-// more of the value, or 2^-25 of the scaled unit.  Three products then stand for one of float32,
-//   lo_a hi_b + hi_a lo_b + hi_a hi_b,
+// Operands are rows of float16 terms.  Of one term (TERMS = 1) a row is its values, 64 columns of 128 bytes after the other (with a
+// distance between them, if need be); of two it is, for every 32 columns, 64 bytes of leading terms and 64 bytes of second ones.
+// Two terms hold x = hi + lo with hi = f16(x) and lo = f16(x - hi), x scaled by a power of two so that neither leaves the
+// type's range: 22 bits and more of the value, or 2^-25 of the scaled unit.  Three products then stand for one of float32,
+//   hi_a hi_b + hi_a lo_b + lo_a hi_b,
 // and what is left out, lo_a lo_b, is below 2^-22 of the term.  Where a product comes from float16 tensors TERMS = 1 has all of it.
 //
 // Either operand may be stored with k along its rows (the usual form: a row is one m, or one n) or with k across them
 // (X^T X, G^T X: a row is one k, columns are m or n).  The first is read from LDS sixteen bytes a lane, the second by
 // ds_read_b64_tr_b16, which hands sixteen lanes the columns of a 4 x 16 piece; so nothing is ever transposed in memory.
 //
-// A stage is 128 bytes of every row and column of the tile (64 k of one term, 32 of two) and goes from memory straight
-// to LDS, past the registers, into one of two buffers while the other is worked on.  Lanes fetch from permuted addresses, so that what
-// lanes read together later stands in different banks.  Buffer loads check the offset: rows behind the last come as zeros.
+// A pair is what 128 bytes of every row hold: two parts of 32 k of one term, or both terms of 32 k.  It comes to LDS as two
+// units, each half of the tile's rows and half of its columns, straight from memory, past the registers and by whole cache lines, into a
+// ring of five units.  A step works on the fragments of one part while those of the next are read and one unit of the
+// pair after the next is loaded, all three taking turns; so there is one barrier for two steps, and loads have a step and more to arrive.  Lanes
+// fetch from permuted addresses, so that what lanes read together later stands in different banks.  Buffer loads check the
+// offset: rows behind the last, and all that is behind the last k, come as zeros.
 #pragma once
+#include <utility>
+
 #include "tt_common.h"
 
 namespace tt {
@@ -27,11 +32,11 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
 
-constexpr int kBlockColumns = 64;               // columns of a block of a row
-constexpr int kTermBytes = 128;                 // of one term of a block
+constexpr int kLine = 128;                      // bytes of 64 columns of one term, or 32 of two
+constexpr int kTermBytes = 64;                  // of one term of 32 columns
 
-// `bytes` from `at` to the end of the last row; `ld` bytes from row to row, `block` from one block of 64 columns to the
-// next.  All are multiples of sixteen, and a tile's rows times ld stay below 2^31 (checked on the host).
+// `bytes` from `at` to the end of the last row; `ld` bytes from row to row, `block` from one line of 128 bytes to the next.
+// All are multiples of sixteen, and a tile's rows times ld stay below 2^31 (checked on the host).
 struct Operand {
   const char* at;
   long long bytes;
@@ -41,168 +46,299 @@ struct Operand {
 template <typename T>
 using lds_ptr = __attribute__((address_space(3))) T*;
 
-// Brings a tile's share of one operand, ROWS rows (or columns) of 128 bytes a stage, to LDS.
+// Brings a tile's share of one operand to LDS: of a pair, ROWS / 2 rows (or, where k goes across, columns) a unit.
 template <int TERMS, bool ACROSS, int ROWS, int THREADS>
 struct Fetch {
-  static constexpr int kDepth = TERMS == 1 ? 64 : 32;
-  static constexpr int kLoads = ROWS * 8 / THREADS;
-  static_assert(kLoads * THREADS == ROWS * 8, "whole loads");
+  static constexpr int kHalf = ROWS / 2, kLoads = kHalf * 8 / THREADS;
+  static_assert(kLoads * THREADS == kHalf * 8, "whole loads");
+  static constexpr int kColumns = kLine / 2 / TERMS;            // of a line
+  static constexpr int kRowBytes = kHalf * 2 * TERMS;           // of a row of k in a unit
   unsigned offset[kLoads];
+  unsigned half;            // from a pair's first unit to its second
   const char* at;
   long long left;
   int ld, block;
 
-  // Which 32-byte unit of a row of k the unit u stands in: rows that sixteen lanes read together differ in it.
-  static __device__ __forceinline__ int unit_mask(int k) {
-    constexpr int most = ROWS / 16 - 1;
+  // A unit holds its rows of 128 bytes one after the other, with the sixteen bytes c of row r at place c ^ (r % 8); or its rows of k, with
+  // the 32-byte piece u (sixteen columns of a term) at place u ^ piece_mask(k), which differs among the rows that sixteen lanes read together.
+  static __device__ __forceinline__ int piece_mask(int k) {
+    constexpr int most = kHalf / 16 - 1;
     return ((k & 3) | ((k >> 1) & 4)) & most;
   }
 
-  // Rows (or columns) from `first` on, a multiple of 64 or of ROWS; from stage `stage` on.
-  __device__ __forceinline__ void begin(const Operand& o, int first, int stage) {
-    const long long skip =
-        ACROSS ? (long long)(first / kBlockColumns) * o.block + (first % kBlockColumns) * 2 + (long long)stage * kDepth * o.ld
-               : (long long)first * o.ld + (TERMS == 1 ? (long long)stage * o.block : (long long)(stage >> 1) * o.block + (stage & 1) * 64);
+  // Rows (or columns) from `first` on, a multiple of the tile's; pairs from `pair` on.
+  __device__ __forceinline__ void begin(const Operand& o, int first, int pair) {
+    const long long skip = ACROSS ? (long long)(first / kColumns) * o.block + (long long)pair * (64 / TERMS) * o.ld
+                                  : (long long)first * o.ld + (long long)pair * o.block;
     at = o.at + skip;
     left = o.bytes - skip;
     ld = o.ld;
     block = o.block;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    half = ACROSS ? (unsigned)(kHalf / kColumns * block) : (unsigned)(kHalf * ld);
+    if (ACROSS && kHalf < kColumns) half = kHalf * 2;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int q = (wave * kLoads + i) * 64 + lane;      // the sixteen bytes of LDS that this lane fills
+      const int q = (wave * kLoads + i) * 64 + lane;      // the sixteen bytes of a unit that this lane fills
       if (ACROSS) {
-        constexpr int per = ROWS / 8;
-        const int line = q / per, pos = q % per, k = line % kDepth, term = line / kDepth;
-        const int column = (((pos >> 1) ^ unit_mask(k)) << 4) + ((pos & 1) << 3);
-        offset[i] = (unsigned)(k * ld + term * kTermBytes + (column / kBlockColumns) * block + (column % kBlockColumns) * 2);
+        constexpr int per = kRowBytes / 16, pieces = kHalf / 16;
+        const int k = q / per, pos = q % per, piece = (pos >> 1) ^ piece_mask(k);
+        const int column = piece % pieces * 16 + (pos & 1) * 8, term = piece / pieces;
+        offset[i] = (unsigned)(k * ld + (column / kColumns) * block + (column % kColumns) * 2 + term * kTermBytes);
       } else {
         const int row = q >> 3, c = (q & 7) ^ (row & 7);
-        offset[i] = (unsigned)(row * ld + (TERMS == 1 ? c * 16 : (c >> 2) * kTermBytes + (c & 3) * 16));
+        offset[i] = (unsigned)(row * ld + c * 16);
       }
     }
   }
 
-  __device__ __forceinline__ void load(char* lds) const {
+  // Load `i` of a pair's unit 0 or 1.
+  __device__ __forceinline__ void load_part(char* lds, int i, int unit) const {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int records = left > 0x7fffffffLL ? 0x7fffffff : left < 0 ? 0 : (int)left;
-    const __amdgpu_buffer_rsrc_t srd = __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, records, 0x00020000);
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(srd, (lds_ptr<void>)(lds + (wave * kLoads + i) * 1024), 16, offset[i], 0, 0, 0);
+    const long long rest = unit ? left - half : left;
+    const int records = rest > 0x7fffffffLL ? 0x7fffffff : rest < 0 ? 0 : (int)rest;
+    const auto srd = __builtin_amdgcn_make_buffer_rsrc((void*)(unit ? at + half : at), 0, records, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(srd, (lds_ptr<void>)(lds + (wave * kLoads + i) * 1024), 16, offset[i], 0, 0, 0);
   }
 
-  // to stage `next`
-  __device__ __forceinline__ void advance(int next) {
-    const int step = ACROSS ? kDepth * ld : TERMS == 1 ? block : (next & 1) ? 64 : block - 64;
+  // To the next pair; where there is none, loads from then on bring zeros.
+  __device__ __forceinline__ void advance(bool more) {
+    const int step = ACROSS ? 64 / TERMS * ld : block;
     at += step;
-    left -= step;
+    left = more ? left - step : 0;
   }
 };
 
 // Fragments of 16 rows and 32 k: lane l has row l % 16 and k = 8 (l / 16) .. + 7.
 template <int TERMS, bool ACROSS, int ROWS, int TILES>
 struct Fragments {
-  static constexpr int kDepth = TERMS == 1 ? 64 : 32;
+  typedef Fetch<TERMS, ACROSS, ROWS, 64> Unit;
   int at[ACROSS ? TILES : 2];
 
+  // `first`: the wave's first row of its unit
   __device__ __forceinline__ void begin(int first) {
     const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
     if (ACROSS) {
       const int k = g * 8 + (j >> 2);
-      const int mask = Fetch<TERMS, true, ROWS, 64>::unit_mask(k);
+      const int mask = Unit::piece_mask(k);
 #pragma unroll
-      for (int i = 0; i < TILES; ++i) at[i] = k * (ROWS * 2) + ((((first >> 4) + i) ^ mask) << 5) + ((j & 3) << 3);
+      for (int i = 0; i < TILES; ++i) at[i] = k * Unit::kRowBytes + ((((first >> 4) + i) ^ mask) << 5) + ((j & 3) << 3);
     } else {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) at[s] = (first + j) * 128 + (((s * 4 + g) ^ (j & 7)) << 4);
+      for (int part = 0; part < 2; ++part) at[part] = (first + j) * 128 + (((part * 4 + g) ^ (j & 7)) << 4);
     }
   }
-  // Fragment `tile` of part s: of one term the stage's k 32 s .. 32 s + 31, of two terms the term s.
-  __device__ __forceinline__ half8 read(const char* lds, int tile, int s) const {
+  __device__ __forceinline__ half8 read(const char* unit, int tile, int part) const {
     if (ACROSS) {
-      const char* p = lds + at[tile] + s * (32 * ROWS * 2);
+      const char* p = unit + at[tile] + part * (TERMS == 1 ? 32 * Unit::kRowBytes : Unit::kHalf * 2);
       const shortx4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr<shortx4>)p);
-      const shortx4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr<shortx4>)(p + 4 * ROWS * 2));
+      const shortx4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr<shortx4>)(p + 4 * Unit::kRowBytes));
       return __builtin_bit_cast(half8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
-    return *reinterpret_cast<const half8*>(lds + at[s] + tile * (16 * 128));
+    return *reinterpret_cast<const half8*>(unit + at[part] + tile * (16 * 128));
   }
 };
 
-// A tile of WM x WN waves, each with MT x NT fragments of 16 x 16.
-template <int TERMS, bool A_ACROSS, bool B_ACROSS, int WM, int WN, int MT, int NT>
+// A tile of 2 x 2 waves, each with MT x NT fragments of 16 x 16.
+template <int TERMS, bool A_ACROSS, bool B_ACROSS, int MT, int NT>
 struct Product {
-  static constexpr int kM = WM * MT * 16, kN = WN * NT * 16, kThreads = 64 * WM * WN;
-  static constexpr int kDepth = TERMS == 1 ? 64 : 32;
-  static constexpr int kStage = (kM + kN) * 128, kLds = 2 * kStage;
+  static constexpr int kM = 2 * MT * 16, kN = 2 * NT * 16, kThreads = 256;
+  static constexpr int kUnits = 5, kUnit = (kM + kN) * 64, kLds = kUnits * kUnit;
   typedef Fetch<TERMS, A_ACROSS, kM, kThreads> FetchA;
   typedef Fetch<TERMS, B_ACROSS, kN, kThreads> FetchB;
+  static constexpr int kReads = MT + NT, kAll = MT * NT, kLoads = FetchA::kLoads + FetchB::kLoads;
 
   // Lane l's acc[i][j] are D[row() + 16 i][column() + 16 j + 0 .. 3].  (The fragments change places in the instruction:
   // a lane then holds neighbours of one row.)
   floatx4 acc[MT][NT];
 
   static __device__ __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
-  static __device__ __forceinline__ int row() { return (wave() / WN) * (MT * 16) + (threadIdx.x & 15); }
-  static __device__ __forceinline__ int column() { return (wave() % WN) * (NT * 16) + ((threadIdx.x & 63) >> 4) * 4; }
+  static __device__ __forceinline__ int row() { return (wave() >> 1) * (MT * 16) + (threadIdx.x & 15); }
+  static __device__ __forceinline__ int column() { return (wave() & 1) * (NT * 16) + ((threadIdx.x & 63) >> 4) * 4; }
 
-  struct Reads {
-    Fragments<TERMS, A_ACROSS, kM, MT> a;
-    Fragments<TERMS, B_ACROSS, kN, NT> b;
+  // One instruction.  With 64 accumulators a wave has no registers to spare, and the compiler moves results from one to
+  // another; written out, each stays where it is.
+  static constexpr bool kPinned = MT * NT == 64;
+  __device__ __forceinline__ void multiply(int i, int j, const half8& a, const half8& b) {
+    if (kPinned) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(b), "v"(a));
+    else acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, a, acc[i][j], 0, 0, 0);
+  }
+
+  // What a step works on: products of the fragments (a, b), while those of the next part come to (to_a, to_b).
+  struct Step {
+    const half8 (&a)[MT];
+    const half8 (&b)[NT];
+    half8 (&to_a)[MT];
+    half8 (&to_b)[NT];
+    const Fragments<TERMS, A_ACROSS, kM, MT>& ra;
+    const Fragments<TERMS, B_ACROSS, kN, NT>& rb;
+    const FetchA& fa;
+    const FetchB& fb;
   };
-
-  __device__ __forceinline__ void stage(const char* __restrict from, char* __restrict to, const Reads& r, const FetchA& fa,
-                                        const FetchB& fb, bool more) {
-    if (more) {
-      fa.load(to);
-      fb.load(to + kM * 128);
-    }
-    const char* fromB = from + kM * 128;
-    half8 a[2][MT], b[2][NT];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-#pragma unroll
-      for (int i = 0; i < MT; ++i) a[s][i] = r.a.read(from, i, s);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) b[s][j] = r.b.read(fromB, j, s);
-    }
-    if (TERMS == 1) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) multiply(a[s], b[s]);
-    } else {
-      multiply(a[1], b[0]);
-      multiply(a[0], b[1]);
-      multiply(a[0], b[0]);
-    }
+  template <int K, int PART>
+  static __device__ __forceinline__ void read_one(Step& w, const char* __restrict unit_a, const char* __restrict unit_b) {
+    if constexpr (K < NT) w.to_b[K] = w.rb.read(unit_b + kM * 64, K, PART);
+    else if constexpr (K < kReads) w.to_a[K - NT] = w.ra.read(unit_a, K - NT, PART);
   }
-  __device__ __forceinline__ void multiply(const half8 (&a)[MT], const half8 (&b)[NT]) {
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[j], a[i], acc[i][j], 0, 0, 0);
+  template <int K, int UNIT>
+  static __device__ __forceinline__ void load_one(const Step& w, char* __restrict to) {
+    if constexpr (K < FetchA::kLoads) w.fa.load_part(to, K, UNIT);
+    else if constexpr (K < kLoads) w.fb.load_part(to + kM * 64, K - FetchA::kLoads, UNIT);
+  }
+  // Product Q of a step, and in front of it the reads and loads whose turn it is; both in the first three quarters, so that no
+  // read is waited for at the end and loads have more time.
+  template <int Q, int PART, int UNIT>
+  __device__ __forceinline__ void one(Step& w, const char* __restrict unit_a, const char* __restrict unit_b, char* __restrict to) {
+    constexpr int early = kAll * 3 / 4 > kReads ? kAll * 3 / 4 : kAll;
+    constexpr int r0 = Q < early ? Q * kReads / early : kReads, r1 = Q + 1 < early ? (Q + 1) * kReads / early : kReads;
+    constexpr int l0 = Q < early ? Q * kLoads / early : kLoads, l1 = Q + 1 < early ? (Q + 1) * kLoads / early : kLoads;
+    if constexpr (r1 > r0) read_one<r0, PART>(w, unit_a, unit_b);
+    if constexpr (r1 > r0 + 1) read_one<r0 + 1, PART>(w, unit_a, unit_b);
+    if constexpr (l1 > l0) load_one<l0, UNIT>(w, to);
+    if constexpr (l1 > l0 + 1) load_one<l0 + 1, UNIT>(w, to);
+    static_assert(r1 <= r0 + 2 && l1 <= l0 + 2, "reads and loads");
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(Q / NT, Q % NT, w.a[Q / NT], w.b[Q % NT]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  template <int PART, int UNIT, int... Q>
+  __device__ __forceinline__ void all(Step& w, const char* __restrict unit_a, const char* __restrict unit_b, char* __restrict to,
+                                      std::integer_sequence<int, Q...>) {
+    (one<Q, PART, UNIT>(w, unit_a, unit_b, to), ...);
+  }
+  template <int... Q>
+  __device__ __forceinline__ void plain(const half8 (&a)[MT], const half8 (&b)[NT], std::integer_sequence<int, Q...>) {
+    (multiply(Q / NT, Q % NT, a[Q / NT], b[Q % NT]), ...);
+  }
+  // Reads of part PART of a pair, loads of unit UNIT.  (A function of its own so that the compiler takes the units for
+  // different memory, and does not wait for the loads on their way before it reads.)
+  template <int PART, int UNIT>
+  __device__ __forceinline__ void step(Step w, const char* __restrict unit_a, const char* __restrict unit_b, char* __restrict to) {
+    all<PART, UNIT>(w, unit_a, unit_b, to, std::make_integer_sequence<int, kAll>());
   }
 
-  // `stages` of the reduction from stage `first` on; lds: kLds bytes.
-  __device__ __forceinline__ void run(const Operand& A, const Operand& B, int m0, int n0, int first, int stages, char* lds) {
+  // Everybody has read what the next loads overwrite, and all loads but those of the last step have arrived.
+  static __device__ __forceinline__ void meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads) : "memory");
+  }
+
+  // `pairs` from pair `first` on (of 64 k of one term, 32 of two); lds: kLds bytes.
+  __device__ __forceinline__ void run(const Operand& A, const Operand& B, int m0, int n0, int first, int pairs, char* lds) {
     FetchA fa;
     FetchB fb;
     fa.begin(A, m0, first);
     fb.begin(B, n0, first);
-    Reads r;
-    r.a.begin((wave() / WN) * (MT * 16));
-    r.b.begin((wave() % WN) * (NT * 16));
+    Fragments<TERMS, A_ACROSS, kM, MT> ra;
+    Fragments<TERMS, B_ACROSS, kN, NT> rb;
+    ra.begin(0);
+    rb.begin(0);
+    int loaded = 0;
+    const auto next_pair = [&]() {
+      ++loaded;
+      fa.advance(loaded < pairs);
+      fb.advance(loaded < pairs);
+    };
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      char* to = lds + 2 * p * kUnit;
+#pragma unroll
+      for (int i = 0; i < FetchA::kLoads; ++i) fa.load_part(to, i, 0);
+#pragma unroll
+      for (int i = 0; i < FetchB::kLoads; ++i) fb.load_part(to + kM * 64, i, 0);
+#pragma unroll
+      for (int i = 0; i < FetchA::kLoads; ++i) fa.load_part(to + kUnit, i, 1);
+#pragma unroll
+      for (int i = 0; i < FetchB::kLoads; ++i) fb.load_part(to + kUnit + kM * 64, i, 1);
+      next_pair();
+    }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = floatx4{};
-    fa.load(lds);
-    fb.load(lds + kM * 128);
-    for (int t = 0; t < stages; ++t) {
-      fa.advance(first + t + 1);
-      fb.advance(first + t + 1);
-      __syncthreads();              // (waits for this stage's loads, too)
-      stage(lds + (t & 1) * kStage, lds + ((t + 1) & 1) * kStage, r, fa, fb, t + 1 < stages);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * kLoads) : "memory");
+    const int half_a = (wave() >> 1) * kUnit, half_b = (wave() & 1) * kUnit;      // this wave's units of a pair
+    half8 a[MT], b[NT], a1[MT], b1[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) b[j] = rb.read(lds + half_b + kM * 64, j, 0);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) a[i] = ra.read(lds + half_a, i, 0);
+    int at = 0;                           // where the pair's first unit stands in the ring
+    const auto around = [](int offset) { return offset >= kLds ? offset - kLds : offset; };
+    // One pair more: its first part's fragments are in (a, y), its second's come to (a1, b1), and the next one's first to (a, z).
+    const auto go = [&](half8(&y)[NT], half8(&z)[NT]) {
+      step<1, 0>(Step{a, y, a1, b1, ra, rb, fa, fb}, lds + around(at + half_a), lds + around(at + half_b), lds + around(at + 4 * kUnit));
+      if (TERMS == 2) plain(a, b1, std::make_integer_sequence<int, kAll>());
+      meet();
+      const int next = around(at + 2 * kUnit);
+      if (TERMS == 1) step<0, 1>(Step{a1, b1, a, z, ra, rb, fa, fb}, lds + around(next + half_a), lds + around(next + half_b), lds + at);
+      else step<0, 1>(Step{a1, y, a, z, ra, rb, fa, fb}, lds + around(next + half_a), lds + around(next + half_b), lds + at);
+      at = next;
+      next_pair();
+    };
+    if (TERMS == 1) {
+#pragma unroll 1
+      for (int p = 0; p < pairs; ++p) go(b, b);
+    } else {
+      // two at a time, so that no fragment has to be moved; one too many is zeros
+      half8 b2[NT];
+#pragma unroll 1
+      for (int p = 0; p < pairs; p += 2) {
+        go(b, b2);
+        go(b2, b);
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");       // (nothing is on its way to LDS any more)
+    if (kPinned) {
+      // the last results may be read eighteen cycles after their instruction
+      asm volatile("s_nop 15\n\ts_nop 7" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) asm volatile("" : "+a"(acc[i][j]));
+    }
+  }
+
+  // The sums, row by row, for what is done with them: kLanes lanes have four neighbours each of a row, a wave kRows rows.
+  // They change places through LDS, half of the tile's rows at a time, so that the code behind is a short loop over whole rows (written out
+  // for every accumulator it did not fit the instruction cache) and what it reads and writes comes by whole lines.
+  // `before(row, c)` reads what a row needs, kAhead turns early: a load that is waited for waits for all stores in front of it.
+  // `f(row of the tile, column of the tile, sums, what was read)` is called for kAhead rows at a time, kStep apart, also
+  // behind the last.
+  static constexpr int kLanes = kN / 4, kRows = 64 / kLanes, kTurns = kM / 2 / (4 * kRows), kAhead = kTurns < 4 ? kTurns : 4;
+  static constexpr int kStep = 4 * kRows;
+  static constexpr int kRowFloats = kN + 4, kExtra = kM / 2 * kRowFloats * 4;       // (behind it LDS is free for the caller)
+  static_assert(kTurns % kAhead == 0 && kExtra + kM * 8 <= kLds, "rows");
+  template <typename R, typename F>
+  __device__ __forceinline__ void rows(char* lds, R before, F f) {
+    float* at = reinterpret_cast<float*>(lds);
+    const int lane = threadIdx.x & 63, first = wave() * kRows + lane / kLanes, c = lane % kLanes * 4;
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+      decltype(before(0, 0)) old[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) old[u] = before(h * (kM / 2) + first + u * kStep, c);
+      if (wave() >> 1 == h) {
+        float* to = at + (threadIdx.x & 15) * kRowFloats + column();
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) *reinterpret_cast<floatx4*>(to + i * 16 * kRowFloats + j * 16) = acc[i][j];
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int t = 0; t < kTurns; t += kAhead) {
+        const int r = first + t * kStep;
+        floatx4 v[kAhead];
+        decltype(before(0, 0)) was[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          v[u] = *reinterpret_cast<const floatx4*>(at + (r + u * kStep) * kRowFloats + c);
+          was[u] = old[u];
+          if (t + kAhead < kTurns) old[u] = before(h * (kM / 2) + r + (u + kAhead) * kStep, c);
+        }
+        f(h * (kM / 2) + r, c, v, was);
+      }
+      __syncthreads();
     }
   }
 };
@@ -224,7 +360,7 @@ __device__ __forceinline__ void split(float v, _Float16* hi, _Float16* lo) {
   *lo = __builtin_isfinite(rest) ? (_Float16)rest : (_Float16)0.f;
 }
 // Where column c of a row of blocks with two terms stands, in bytes (of the first term).
-__device__ __forceinline__ int at_column(int c) { return (c >> 6) * (2 * kTermBytes) + (c & 63) * 2; }
+__device__ __forceinline__ int at_column(int c) { return (c >> 5) * kLine + (c & 31) * 2; }
 __device__ __forceinline__ void store_terms(char* row, int c, const floatx4& v) {
   half4 hi, lo;
 #pragma unroll
@@ -247,17 +383,18 @@ __device__ __forceinline__ floatx4 load_terms(const char* row, int c) {
   return v;
 }
 
-inline long long padded(long long columns) { return (columns + kBlockColumns - 1) / kBlockColumns * kBlockColumns; }
+// Columns of a row with its padding, which is zeros.
+__host__ __device__ inline long long padded(long long columns) { return (columns + 63) / 64 * 64; }
 
 // The three sizes of tiles.
 template <int TERMS, bool A_ACROSS, bool B_ACROSS, int SIZE>
 struct Sized;
 template <int TERMS, bool A, bool B>
-struct Sized<TERMS, A, B, 0> : Product<TERMS, A, B, 4, 1, 1, 4> {};     // 64 x 64
+struct Sized<TERMS, A, B, 0> : Product<TERMS, A, B, 2, 2> {};     // 64 x 64
 template <int TERMS, bool A, bool B>
-struct Sized<TERMS, A, B, 1> : Product<TERMS, A, B, 2, 2, 4, 4> {};     // 128 x 128
+struct Sized<TERMS, A, B, 1> : Product<TERMS, A, B, 4, 4> {};     // 128 x 128
 template <int TERMS, bool A, bool B>
-struct Sized<TERMS, A, B, 2> : Product<TERMS, A, B, 2, 4, 8, 4> {};     // 256 x 256
+struct Sized<TERMS, A, B, 2> : Product<TERMS, A, B, 8, 8> {};     // 256 x 256
 constexpr int kTileSide[3] = {64, 128, 256};
 inline long long tiles_of(long long m, long long n, int size) {
   const int side = kTileSide[size];
