@@ -511,7 +511,7 @@ int run(const Call& q) {
   const bool grad = q.dx || q.dw, copy_w = TERMS == 2 || H % 8 != 0;
   const int depth = 64 / TERMS;
   long long chunk = (long long)((grad ? kMostLogits : kMostStats) / ((size_t)Vp * (grad ? 4 : 8) / (grad ? 1 : 64)));
-  chunk = std::max(256LL, chunk / 256 * 256);
+  chunk = std::max(256LL, std::min(chunk, (1LL << 34) / (Hp * 2 * TERMS)) / 256 * 256);
   chunk = std::min(chunk, N);
   const bool several = chunk < N;
   const int pairsV = (int)(Vp / depth), pairsN = (int)((chunk + depth - 1) / depth);
@@ -600,6 +600,7 @@ int tt_linear_cross_entropy(const void* x, const void* w, const void* target, co
   TT_REQUIRE(N >= 1 && N <= (1LL << 30), "%s: 1 to 2^30 positions, got %lld", fn, N);
   TT_REQUIRE(H >= 1 && H <= 1 << 20, "%s: 1 to 2^20 features, got %d", fn, H);
   TT_REQUIRE(V >= 1 && V <= 1 << 20, "%s: 1 to 2^20 classes, got %d", fn, V);
+  TT_REQUIRE((long long)H * V <= 1LL << 32, "%s: a weight of 2^32 values at most, got %d x %d", fn, V, H);
   TT_REQUIRE(x && w && target && (loss || dx || dw), "%s: null pointer", fn);
   TT_REQUIRE(!half_gradients || kind == 1, "%s: gradients of float32 tensors are float32", fn);
   TT_REQUIRE_ALIGNED(fn, x, w, g, loss, dx, dw);

@@ -307,6 +307,7 @@ bool in_range(double a, double b, double c, int steps) {
 int check(const char* fn, int rows, int columns) {
   TT_REQUIRE(rows >= 1 && columns >= 1 && rows <= 1 << 20 && columns <= 1 << 20, "%s: matrices of 1 to 2^20 rows and columns, got %d x %d", fn,
              rows, columns);
+  TT_REQUIRE((long long)rows * columns <= 1LL << 32, "%s: matrices of 2^32 values at most, got %d x %d", fn, rows, columns);
   return 0;
 }
 int check(const char* fn, double a, double b, double c, double eps, int steps) {

@@ -16,7 +16,7 @@
 //
 // A pair is what 128 bytes of every row hold: two parts of 32 k of one term, or both terms of 32 k.  It comes to LDS as two
 // units, each half of the tile's rows and half of its columns, straight from memory, past the registers and by whole cache lines, into a
-// ring of five units.  A step works on the fragments of one part while those of the next are read and one unit of the
+// ring of units, five for the largest tiles.  A step works on the fragments of one part while those of the next are read and one unit of the
 // pair after the next is loaded, all three taking turns; so there is one barrier for two steps, and loads have a step and more to arrive.  Lanes
 // fetch from permuted addresses, so that what lanes read together later stands in different banks.  Buffer loads check the
 // offset: rows behind the last, and all that is behind the last k, come as zeros.
@@ -54,10 +54,10 @@ struct Fetch {
   static constexpr int kColumns = kLine / 2 / TERMS;            // of a line
   static constexpr int kRowBytes = kHalf * 2 * TERMS;           // of a row of k in a unit
   unsigned offset[kLoads];
-  unsigned half;            // from a pair's first unit to its second
+  unsigned half, step;      // from a pair's first unit to its second, from a pair to the next
   const char* at;
-  long long left;
-  int ld, block;
+  int left;                 // from there to the end, by sixteen bytes: 2^35 bytes at most (checked on the host)
+  int bytes[2];             // what may be read of either unit
 
   // A unit holds its rows of 128 bytes one after the other, with the sixteen bytes c of row r at place c ^ (r % 8); or its rows of k, with
   // the 32-byte piece u (sixteen columns of a term) at place u ^ piece_mask(k), which differs among the rows that sixteen lanes read together.
@@ -71,12 +71,13 @@ struct Fetch {
     const long long skip = ACROSS ? (long long)(first / kColumns) * o.block + (long long)pair * (64 / TERMS) * o.ld
                                   : (long long)first * o.ld + (long long)pair * o.block;
     at = o.at + skip;
-    left = o.bytes - skip;
-    ld = o.ld;
-    block = o.block;
+    left = (int)((o.bytes - skip) >> 4);
+    const int ld = o.ld, block = o.block;
+    step = ACROSS ? (unsigned)(64 / TERMS * ld) : (unsigned)block;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     half = ACROSS ? (unsigned)(kHalf / kColumns * block) : (unsigned)(kHalf * ld);
     if (ACROSS && kHalf < kColumns) half = kHalf * 2;
+    measure();
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int q = (wave * kLoads + i) * 64 + lane;      // the sixteen bytes of a unit that this lane fills
@@ -92,20 +93,27 @@ struct Fetch {
     }
   }
 
+  __device__ __forceinline__ void measure() {
+#pragma unroll
+    for (int unit = 0; unit < 2; ++unit) {
+      int rest = left - (unit ? (int)(half >> 4) : 0);
+      rest = rest < 0 ? 0 : rest;
+      // (the compiler has a vector instruction for the two limits, and is told that it may come back from there)
+      bytes[unit] = __builtin_amdgcn_readfirstlane(rest < 0x7ffffff ? rest : 0x7ffffff) << 4;
+    }
+  }
   // Load `i` of a pair's unit 0 or 1.
   __device__ __forceinline__ void load_part(char* lds, int i, int unit) const {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long rest = unit ? left - half : left;
-    const int records = rest > 0x7fffffffLL ? 0x7fffffff : rest < 0 ? 0 : (int)rest;
-    const auto srd = __builtin_amdgcn_make_buffer_rsrc((void*)(unit ? at + half : at), 0, records, 0x00020000);
+    const auto srd = __builtin_amdgcn_make_buffer_rsrc((void*)(unit ? at + half : at), 0, bytes[unit], 0x00020000);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(srd, (lds_ptr<void>)(lds + (wave * kLoads + i) * 1024), 16, offset[i], 0, 0, 0);
   }
 
   // To the next pair; where there is none, loads from then on bring zeros.
   __device__ __forceinline__ void advance(bool more) {
-    const int step = ACROSS ? 64 / TERMS * ld : block;
     at += step;
-    left = more ? left - step : 0;
+    left = more ? left - (int)(step >> 4) : 0;
+    measure();
   }
 };
 
@@ -139,11 +147,11 @@ struct Fragments {
   }
 };
 
-// A tile of 2 x 2 waves, each with MT x NT fragments of 16 x 16.
-template <int TERMS, bool A_ACROSS, bool B_ACROSS, int MT, int NT>
+// A tile of 2 x 2 waves, each with MT x NT fragments of 16 x 16; AHEAD pairs are on their way or there.
+template <int TERMS, bool A_ACROSS, bool B_ACROSS, int MT, int NT, int AHEAD>
 struct Product {
   static constexpr int kM = 2 * MT * 16, kN = 2 * NT * 16, kThreads = 256;
-  static constexpr int kUnits = 5, kUnit = (kM + kN) * 64, kLds = kUnits * kUnit;
+  static constexpr int kUnits = 2 * AHEAD + 1, kUnit = (kM + kN) * 64, kLds = kUnits * kUnit;
   typedef Fetch<TERMS, A_ACROSS, kM, kThreads> FetchA;
   typedef Fetch<TERMS, B_ACROSS, kN, kThreads> FetchB;
   static constexpr int kReads = MT + NT, kAll = MT * NT, kLoads = FetchA::kLoads + FetchB::kLoads;
@@ -217,9 +225,12 @@ struct Product {
     all<PART, UNIT>(w, unit_a, unit_b, to, std::make_integer_sequence<int, kAll>());
   }
 
-  // Everybody has read what the next loads overwrite, and all loads but those of the last step have arrived.
+  // Everybody has read what the next loads overwrite, and the next pair's loads have arrived: all but those of the pairs
+  // behind it and of the last step.
+  static constexpr int kMayWait = (2 * (AHEAD - 2) + 1) * kLoads;
+  static_assert(kMayWait + kLoads <= 63, "the counter of loads");
   static __device__ __forceinline__ void meet() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kMayWait) : "memory");
   }
 
   // `pairs` from pair `first` on (of 64 k of one term, 32 of two); lds: kLds bytes.
@@ -239,7 +250,7 @@ struct Product {
       fb.advance(loaded < pairs);
     };
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
+    for (int p = 0; p < AHEAD; ++p) {
       char* to = lds + 2 * p * kUnit;
 #pragma unroll
       for (int i = 0; i < FetchA::kLoads; ++i) fa.load_part(to, i, 0);
@@ -255,7 +266,7 @@ struct Product {
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = floatx4{};
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * kLoads) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * (AHEAD - 1) * kLoads) : "memory");
     const int half_a = (wave() >> 1) * kUnit, half_b = (wave() & 1) * kUnit;      // this wave's units of a pair
     half8 a[MT], b[NT], a1[MT], b1[NT];
 #pragma unroll
@@ -266,7 +277,7 @@ struct Product {
     const auto around = [](int offset) { return offset >= kLds ? offset - kLds : offset; };
     // One pair more: its first part's fragments are in (a, y), its second's come to (a1, b1), and the next one's first to (a, z).
     const auto go = [&](half8(&y)[NT], half8(&z)[NT]) {
-      step<1, 0>(Step{a, y, a1, b1, ra, rb, fa, fb}, lds + around(at + half_a), lds + around(at + half_b), lds + around(at + 4 * kUnit));
+      step<1, 0>(Step{a, y, a1, b1, ra, rb, fa, fb}, lds + around(at + half_a), lds + around(at + half_b), lds + around(at + 2 * AHEAD * kUnit));
       if (TERMS == 2) plain(a, b1, std::make_integer_sequence<int, kAll>());
       meet();
       const int next = around(at + 2 * kUnit);
@@ -390,11 +401,11 @@ __host__ __device__ inline long long padded(long long columns) { return (columns
 template <int TERMS, bool A_ACROSS, bool B_ACROSS, int SIZE>
 struct Sized;
 template <int TERMS, bool A, bool B>
-struct Sized<TERMS, A, B, 0> : Product<TERMS, A, B, 2, 2> {};     // 64 x 64
+struct Sized<TERMS, A, B, 0> : Product<TERMS, A, B, 2, 2, 6> {};     // 64 x 64
 template <int TERMS, bool A, bool B>
-struct Sized<TERMS, A, B, 1> : Product<TERMS, A, B, 4, 4> {};     // 128 x 128
+struct Sized<TERMS, A, B, 1> : Product<TERMS, A, B, 4, 4, 4> {};     // 128 x 128
 template <int TERMS, bool A, bool B>
-struct Sized<TERMS, A, B, 2> : Product<TERMS, A, B, 8, 8> {};     // 256 x 256
+struct Sized<TERMS, A, B, 2> : Product<TERMS, A, B, 8, 8, 2> {};     // 256 x 256
 constexpr int kTileSide[3] = {64, 128, 256};
 inline long long tiles_of(long long m, long long n, int size) {
   const int side = kTileSide[size];
