@@ -364,8 +364,11 @@ __device__ __forceinline__ void tile_of(int block, int blocks, int tilesM, int t
   *n = at % run / high;
 }
 
-// Two terms of a value that a power of two has brought into range.  What is not finite has no second term.
+// Two terms of a value that a power of two has brought into range.  What is not finite has no second term.  (The value is a
+// float32 in a register first: rounded to float16 straight from the product in front, as one instruction can do it, the
+// first term could be another in one place than in the other, one unit of its last place off in one of a thousand.)
 __device__ __forceinline__ void split(float v, _Float16* hi, _Float16* lo) {
+  asm("" : "+v"(v));
   *hi = (_Float16)v;
   const float rest = v - (float)*hi;
   *lo = __builtin_isfinite(rest) ? (_Float16)rest : (_Float16)0.f;
