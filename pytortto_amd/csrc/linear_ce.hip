@@ -139,9 +139,32 @@ struct Logits {
   float* z;             // [rows][ld] or none
   long long ld;
   float2* stats;        // [rows][blocks]: of a tile's columns the largest logit, and the sum of e^(z - it) without its 1
-  float* own;           // [rows] the target's logit
+  float* own;           // [rows] the target's logit, without z
   int blocks;
 };
+
+// One instruction each (fmaxf and fminf first quiet their arguments); the larger of a NaN and a number is the NaN.
+__device__ __forceinline__ float larger(float a, float b) {
+  float r;
+  asm("v_maximum3_f32 %0, %1, %2, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+__device__ __forceinline__ float smaller(float a, float b) {
+  float r;
+  asm("v_min_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+// What a lane and the one 16 (32) lanes away have, in the same order in both.
+struct Pair {
+  float a, b;
+};
+template <int APART>
+__device__ __forceinline__ Pair with_lane(float v) {
+  const unsigned x = __builtin_bit_cast(unsigned, v);
+  const auto both = APART == 16 ? __builtin_amdgcn_permlane16_swap(x, x, false, false) : __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  const unsigned a = both[0], b = both[1];      // (a cast of an element itself is one of the first element)
+  return {__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
+}
 
 template <int TERMS, int SIZE>
 __global__ __launch_bounds__(256) void lce_logits(Operand x, Operand w, int rows, int V, int pairs, Logits q) {
@@ -149,77 +172,102 @@ __global__ __launch_bounds__(256) void lce_logits(Operand x, Operand w, int rows
   extern __shared__ __align__(16) char lds[];
   int m, n;
   tile_of(blockIdx.x, gridDim.x, (rows + G::kM - 1) / G::kM, (V + G::kN - 1) / G::kN, &m, &n);
-  const int m0 = m * G::kM, n0 = n * G::kN;
+  const int m0 = m * G::kM, n0 = n * G::kN, at = threadIdx.x;
+  // the rows' targets and exponents, and the columns' exponents
+  int2 mine = make_int2(kInvalid, 0);
+  int column_e = 0;
+  if (at < G::kM && m0 + at < rows) mine = make_int2(class_of(q.t, q.first + m0 + at), TERMS == 2 ? q.f[m0 + at] : 0);
+  if (TERMS == 2 && at < G::kN) column_e = q.e[n0 + at];      // (padded to a whole tile)
   G p;
   p.run(x, w, m0, n0, 0, pairs, lds);
-  // the rows' targets and exponents, and the columns' exponents
   int2* about = reinterpret_cast<int2*>(lds + G::kExtra);
-  for (int r = threadIdx.x; r < G::kM; r += 256)
-    if (m0 + r < rows) about[r] = make_int2(class_of(q.t, q.first + m0 + r), TERMS == 2 ? q.f[m0 + r] : 0);
-  const int at = threadIdx.x & 63, c0 = n0 + at % G::kLanes * 4;
-  int4 scale = {};
-  if (TERMS == 2) scale = *reinterpret_cast<const int4*>(q.e + c0);        // (padded to a whole tile)
+  int* scales = reinterpret_cast<int*>(about + G::kM);
+  float2* halves = reinterpret_cast<float2*>(scales + G::kN);     // [2][kM] of a row's two waves
+  if (at < G::kM) about[at] = mine;
+  if (TERMS == 2 && at < G::kN) scales[at] = column_e;
   __syncthreads();
-  constexpr int U = G::kAhead;
-  p.rows(lds, [](int, int) { return 0; }, [&](int r, int, floatx4 (&v)[U], int (&)[U]) {
-    int target[U];
-    float most[U], sum[U];
+  const int c0 = G::column();
+  int4 scale[G::kAcross];
+  if (TERMS == 2) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int2 mine = about[r + u * G::kStep];
-      target[u] = mine.x;
+    for (int j = 0; j < G::kAcross; ++j) scale[j] = *reinterpret_cast<const int4*>(scales + c0 + j * 16);
+  }
+  // A row's columns in this wave are in four lanes, 4 NT of them in a thread: little is left between lanes.  (Row by row, with the row
+  // across a wave, the reductions were most of 12 us that a tile of 256 x 256 took behind its product.)
+#pragma unroll
+  for (int i = 0; i < G::kDown; ++i) {
+    const int r = G::row() + i * 16;
+    const int2 it = about[r];
+    float v[G::kAcross * 4];
+#pragma unroll
+    for (int j = 0; j < G::kAcross; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[j * 4 + e] = p.acc[i][j][e];
+        if (TERMS == 2) v[j * 4 + e] = ldexpf(v[j * 4 + e], (&scale[j].x)[e] + it.y);
+      }
+    const int here = it.x - n0 - c0;
+    if (!q.z && here >= 0 && here < G::kAcross * 16 && (here & 12) == 0) {
+      float own = 0.f;
+#pragma unroll
+      for (int k = 0; k < G::kAcross * 4; ++k)
+        if (here == (k >> 2) * 16 + (k & 3)) own = v[k];
+      q.own[m0 + r] = own;
+    }
+    if (n0 + G::kN > V) {
+#pragma unroll
+      for (int k = 0; k < G::kAcross * 4; ++k)
+        if (n0 + c0 + (k >> 2) * 16 + (k & 3) >= V) v[k] = -INFINITY;
+    }
+    // the largest goes up, and all others stay: the sum is over these
+    float top = v[0];
+#pragma unroll
+    for (int k = 1; k < G::kAcross * 4; ++k) {
+      const float other = smaller(top, v[k]);
+      top = larger(top, v[k]);
+      v[k] = other;
+    }
+    const Pair one = with_lane<16>(top), two = with_lane<32>(larger(one.a, one.b));
+    const float most = larger(two.a, two.b), from = most == -INFINITY ? 0.f : most;
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 1; k < G::kAcross * 4; ++k) sum += __builtin_amdgcn_exp2f((v[k] - from) * kLog2e);
+    const Pair four = with_lane<16>(sum);
+    sum = four.a + four.b + __builtin_amdgcn_exp2f((smaller(one.a, one.b) - from) * kLog2e);
+    const Pair all = with_lane<32>(sum);
+    sum = all.a + all.b + __builtin_amdgcn_exp2f((smaller(two.a, two.b) - from) * kLog2e);
+    if ((at & 48) == 0) halves[(at >> 6 & 1) * G::kM + r] = make_float2(most, sum);
+  }
+  __syncthreads();
+  if (at < G::kM && m0 + at < rows) {
+    const float2 a = halves[at], b = halves[G::kM + at];
+    const float2 more = a.x < b.x ? b : a, less = a.x < b.x ? a : b;
+    const float rest = more.y + (1.f + less.y) * (a.x == b.x ? 1.f : __builtin_amdgcn_exp2f((less.x - more.x) * kLog2e));
+    q.stats[(size_t)(m0 + at) * q.blocks + n] = make_float2(more.x, rest);
+  }
+  if (!q.z) return;
+  float* z = q.z + (size_t)m0 * q.ld + n0;
+  const int ld = (int)q.ld;
+  const int4 mine4 = TERMS == 2 ? *reinterpret_cast<const int4*>(scales + (at & 63) % G::kLanes * 4) : int4{};
+  p.rows(lds, [](int, int) { return 0; }, [&](int r, int c, floatx4 (&v)[G::kAhead], int (&)[G::kAhead]) {
+#pragma unroll
+    for (int u = 0; u < G::kAhead; ++u) {
+      const int k = r + u * G::kStep;
       if (TERMS == 2) {
-        v[u][0] = ldexpf(v[u][0], scale.x + mine.y);
-        v[u][1] = ldexpf(v[u][1], scale.y + mine.y);
-        v[u][2] = ldexpf(v[u][2], scale.z + mine.y);
-        v[u][3] = ldexpf(v[u][3], scale.w + mine.y);
+        // (again: written back to the accumulators, they would need as many registers more)
+        const int e = about[k].y;
+        v[u] = floatx4{ldexpf(v[u][0], mine4.x + e), ldexpf(v[u][1], mine4.y + e), ldexpf(v[u][2], mine4.z + e), ldexpf(v[u][3], mine4.w + e)};
       }
-    }
-    if (q.z && c0 < q.ld) {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (m0 + r + u * G::kStep < rows) *reinterpret_cast<floatx4*>(q.z + (size_t)(m0 + r + u * G::kStep) * q.ld + c0) = v[u];
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (c0 + i >= V) v[u][i] = -INFINITY;
-      most[u] = fmaxf(fmaxf(v[u][0], v[u][1]), fmaxf(v[u][2], v[u][3]));
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) most[u] = lanes_reduce<G::kLanes>(most[u], Larger());
-    int largest[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      // (the largest values apart, in whole units: one of them is left out)
-      const float from = most[u] == -INFINITY ? 0.f : most[u];
-      sum[u] = 0.f;
-      largest[u] = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool it = v[u][i] == most[u];
-        const unsigned long long those = __ballot(it && c0 + i < V);
-        largest[u] += __popcll(G::kLanes == 64 ? those : (those >> (at / G::kLanes * G::kLanes)) & ((1ull << (G::kLanes % 64)) - 1));
-        sum[u] += it ? 0.f : __builtin_amdgcn_exp2f((v[u][i] - from) * kLog2e);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) sum[u] = lanes_reduce<G::kLanes>(sum[u], Plus());
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int row = m0 + r + u * G::kStep, here = target[u] - c0;
-      if (row >= rows) continue;
-      if (here >= 0 && here < 4) q.own[row] = here == 0 ? v[u][0] : here == 1 ? v[u][1] : here == 2 ? v[u][2] : v[u][3];
-      if (at % G::kLanes == 0) q.stats[(size_t)row * q.blocks + n] = make_float2(most[u], sum[u] + (float)(largest[u] - 1));
+      if (m0 + k < rows && n0 + c < ld) *reinterpret_cast<floatx4*>(z + (unsigned)(k * ld + c)) = v[u];
     }
   });
 }
 
 // A row's maximum and log2 of its sum from those of its blocks, and its loss.  A wave has a row.  The sum is kept without the
 // largest term, which is 1: of a target that has nearly all of the probability, the loss is what is left, and keeps its digits.
-__global__ __launch_bounds__(256) void lce_join(const float2* __restrict__ stats, const float* __restrict__ own, float2* __restrict__ of,
-                                                float* __restrict__ loss, Targets t, long long first, int rows, int blocks) {
+__global__ __launch_bounds__(256) void lce_join(const float2* __restrict__ stats, const float* __restrict__ own, const float* __restrict__ z,
+                                                long long ld, float2* __restrict__ of, float* __restrict__ loss, Targets t, long long first,
+                                                int rows, int blocks) {
   const int r = blockIdx.x * 4 + row_of_block<kWave>();
   if (r >= rows) return;
   const int lane = threadIdx.x & 63, target = class_of(t, first + r);
@@ -244,7 +292,7 @@ __global__ __launch_bounds__(256) void lce_join(const float2* __restrict__ stats
   if (lane == 0) {
     const float log_sum = log1pf(rest);
     of[r] = make_float2(from, log_sum * kLog2e);
-    loss[r] = target == kInvalid ? NAN : log_sum + (from - own[r]);
+    loss[r] = target == kInvalid ? NAN : log_sum + (from - (z ? z[(size_t)r * ld + target] : own[r]));
   }
 }
 
@@ -351,6 +399,8 @@ __global__ __launch_bounds__(256) void lce_product(Operand a, Operand b, int M, 
   int m, n;
   tile_of(blockIdx.x % blocks, blocks, (M + G::kM - 1) / G::kM, (N + G::kN - 1) / G::kN, &m, &n);
   const int first = split * per, count = min(per, pairs - first), m0 = m * G::kM, n0 = n * G::kN;
+  const int mine = splits == 1 && threadIdx.x < G::kM && m0 + (int)threadIdx.x < M ? out.exponent_for(m0 + threadIdx.x) : 0;
+  const float scale = out.control->scale;
   G p;
   p.run(a, b, m0, n0, first, count, lds);
   if (splits > 1) {
@@ -364,18 +414,64 @@ __global__ __launch_bounds__(256) void lce_product(Operand a, Operand b, int M, 
     return;
   }
   int* about = reinterpret_cast<int*>(lds + G::kExtra);
-  for (int r = threadIdx.x; r < G::kM; r += 256)
-    if (m0 + r < M) about[r] = out.exponent_for(m0 + r);
-  const float scale = out.control->scale;
+  if (threadIdx.x < G::kM) about[threadIdx.x] = mine;
   __syncthreads();
-  p.rows(lds, [&](int r, int c) { return out.add && m0 + r < M && n0 + c < N ? out.before(m0 + r, n0 + c) : floatx4{}; },
-         [&](int r, int c, const floatx4 (&v)[G::kAhead], const floatx4 (&old)[G::kAhead]) {
+  const auto none = [](int, int) { return 0; };
+  if (out.columns % 4) {
+    // rows of any alignment
+    p.rows(lds, [&](int r, int c) { return out.add && m0 + r < M && n0 + c < N ? out.before(m0 + r, n0 + c) : floatx4{}; },
+           [&](int r, int c, const floatx4 (&v)[G::kAhead], const floatx4 (&old)[G::kAhead]) {
 #pragma unroll
-           for (int u = 0; u < G::kAhead; ++u) {
-             const int k = r + u * G::kStep;
-             if (m0 + k < M && n0 + c < N) out.store(m0 + k, n0 + c, v[u], scale, about[k], old[u]);
-           }
-         });
+             for (int u = 0; u < G::kAhead; ++u) {
+               const int k = r + u * G::kStep;
+               if (m0 + k < M && n0 + c < N) out.store(m0 + k, n0 + c, v[u], scale, about[k], old[u]);
+             }
+           });
+    return;
+  }
+  // of four columns all are there or none, and every four can be stored at once
+  const auto scaled = [&](const floatx4& v, int k) {
+    const int e = about[k];
+    return floatx4{ldexpf(v[0] * scale, e), ldexpf(v[1] * scale, e), ldexpf(v[2] * scale, e), ldexpf(v[3] * scale, e)};
+  };
+  const size_t corner = (size_t)m0 * out.columns + n0;
+  if (out.half) {
+    _Float16* to = reinterpret_cast<_Float16*>(out.to) + corner;
+    p.rows(lds, none, [&](int r, int c, const floatx4 (&v)[G::kAhead], const int (&)[G::kAhead]) {
+#pragma unroll
+      for (int u = 0; u < G::kAhead; ++u) {
+        const int k = r + u * G::kStep;
+        const floatx4 s = scaled(v[u], k);
+        if (m0 + k < M && n0 + c < N)
+          *reinterpret_cast<half4*>(to + (unsigned)(k * out.columns + c)) = half4{(_Float16)s[0], (_Float16)s[1], (_Float16)s[2], (_Float16)s[3]};
+      }
+    });
+    return;
+  }
+  float* to = reinterpret_cast<float*>(out.to) + corner;
+  if (out.add) {
+    p.rows(lds,
+           [&](int r, int c) {
+             return m0 + r < M && n0 + c < N ? *reinterpret_cast<const floatx4*>(to + (unsigned)(r * out.columns + c)) : floatx4{};
+           },
+           [&](int r, int c, const floatx4 (&v)[G::kAhead], const floatx4 (&old)[G::kAhead]) {
+#pragma unroll
+             for (int u = 0; u < G::kAhead; ++u) {
+               const int k = r + u * G::kStep;
+               const floatx4 s = scaled(v[u], k) + old[u];
+               if (m0 + k < M && n0 + c < N) *reinterpret_cast<floatx4*>(to + (unsigned)(k * out.columns + c)) = s;
+             }
+           });
+    return;
+  }
+  p.rows(lds, none, [&](int r, int c, const floatx4 (&v)[G::kAhead], const int (&)[G::kAhead]) {
+#pragma unroll
+    for (int u = 0; u < G::kAhead; ++u) {
+      const int k = r + u * G::kStep;
+      const floatx4 s = scaled(v[u], k);
+      if (m0 + k < M && n0 + c < N) *reinterpret_cast<floatx4*>(to + (unsigned)(k * out.columns + c)) = s;
+    }
+  });
 }
 
 __global__ __launch_bounds__(256) void lce_sum(const float* __restrict__ partial, int splits, int M, int N, GradientOut out) {
@@ -555,7 +651,7 @@ int run(const Call& q) {
     const Operand x = {base + at_x + (size_t)first * ldx, (long long)rows * ldx, ldx, kLine};
     const Logits logits = {f ? f + first : nullptr, e, q.t, first, z, Vp, stats, own, blocks};
     if (launch_logits<TERMS>(size, x, w, rows, V, H, logits)) return -1;
-    lce_join<<<(unsigned)((rows + 3) / 4), 256, 0, stream()>>>(stats, own, of, losses + first, q.t, first, rows, blocks);
+    lce_join<<<(unsigned)((rows + 3) / 4), 256, 0, stream()>>>(stats, own, z, Vp, of, losses + first, q.t, first, rows, blocks);
     TT_LAUNCH_CHECK();
     if (!grad) continue;
     for (int r = 0; r < rows; r += 65535) {

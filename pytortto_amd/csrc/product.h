@@ -316,9 +316,9 @@ struct Product {
   // `f(row of the tile, column of the tile, sums, what was read)` is called for kAhead rows at a time, kStep apart, also
   // behind the last.
   static constexpr int kLanes = kN / 4, kRows = 64 / kLanes, kTurns = kM / 2 / (4 * kRows), kAhead = kTurns < 4 ? kTurns : 4;
-  static constexpr int kStep = 4 * kRows;
+  static constexpr int kStep = 4 * kRows, kDown = MT, kAcross = NT;
   static constexpr int kRowFloats = kN + 4, kExtra = kM / 2 * kRowFloats * 4;       // (behind it LDS is free for the caller)
-  static_assert(kTurns % kAhead == 0 && kExtra + kM * 8 <= kLds, "rows");
+  static_assert(kTurns % kAhead == 0 && kExtra + kM * 24 + kN * 4 <= kLds, "rows");
   template <typename R, typename F>
   __device__ __forceinline__ void rows(char* lds, R before, F f) {
     float* at = reinterpret_cast<float*>(lds);
