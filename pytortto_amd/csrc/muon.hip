@@ -228,10 +228,10 @@ __device__ __forceinline__ void muon_tile(const Matrix& x, const Rule& q, bool l
   // wide: S X with X's rows as k;  tall: X S, S being symmetric
   if (ACROSS) g.run(S, X, m0, n0, 0, (p.m + 31) / 32, lds);
   else g.run(X, S, m0, n0, 0, (p.m + 31) / 32, lds);
-  const auto old = [&](int r, int c) { return m0 + r < M && n0 + c < edge ? load_terms(x0 + (m0 + r) * p.ldx, n0 + c) : floatx4{}; };
+  const auto none = [](int, int) { return 0; };
   if (!last) {
-    g.rows(lds, old, [&](int r, int c, const floatx4 (&v)[U], const floatx4 (&o)[U]) {
-      each(r, c, edge, [&](int u, int row, int column) { store_terms(x1 + row * p.ldx, column, o[u] * q.a + v[u] * (1.f / 4096.f)); });
+    g.rows(lds, none, [&](int r, int c, const floatx4 (&v)[U], const int (&)[U]) {
+      each(r, c, edge, [&](int u, int row, int column) { store_terms(x1 + row * p.ldx, column, v[u] * (1.f / 4096.f)); });
     });
     return;
   }
@@ -254,7 +254,7 @@ __device__ __forceinline__ void muon_tile(const Matrix& x, const Rule& q, bool l
            [&](int r, int c) {
              if (m0 + r >= M || n0 + c >= columns) return floatx4{};
              const size_t at = (size_t)(m0 + r) * columns + n0 + c;
-             return read_four(w, at, columns - n0 - c, whole) * q.keep - old(r, c) * (q.a * rate * (1.f / kUp));
+             return read_four(w, at, columns - n0 - c, whole) * q.keep;
            },
            [&](int r, int c, const floatx4 (&v)[U], const floatx4 (&o)[U]) {
              each(r, c, columns, [&](int u, int row, int column) {
@@ -262,9 +262,9 @@ __device__ __forceinline__ void muon_tile(const Matrix& x, const Rule& q, bool l
              });
            });
   } else {
-    g.rows(lds, old, [&](int r, int c, const floatx4 (&v)[U], const floatx4 (&o)[U]) {
+    g.rows(lds, none, [&](int r, int c, const floatx4 (&v)[U], const int (&)[U]) {
       each(r, c, columns, [&](int u, int row, int column) {
-        const floatx4 y = (o[u] * q.a + v[u] * (1.f / 4096.f)) * (1.f / kUp);
+        const floatx4 y = v[u] * (1.f / 4096.f / kUp);
         const size_t at = (size_t)row * columns + column;
         if (q.half) put(reinterpret_cast<_Float16*>(x.to) + at, column, y);
         else put(reinterpret_cast<float*>(x.to) + at, column, y);
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(256) void muon_product(Batch b, Rule q, int last) {
   }
 }
 
-// A = X X^T, or b A + c A A, from the partial sums of the upper tiles: 64 x 64 of it, and the same on the other side of the diagonal.
+// A = X X^T, or a I + b A + c A A, from the partial sums of the upper tiles: 64 x 64 of it, and the same on the other side of the diagonal.
 template <int WHAT>
 __global__ __launch_bounds__(256) void muon_join(Batch b, Rule q) {
   __shared__ float turned[kJoin][kJoin + 1];
@@ -309,6 +309,10 @@ __global__ __launch_bounds__(256) void muon_join(Batch b, Rule q) {
       for (int s = 0; s < x.splits; ++s) v += *reinterpret_cast<const floatx4*>(from + s * p.square());
       if (WHAT == kGram) v *= 1.f / kUp;
       else v = load_terms(a + row * p.lda, c) * (q.b * 0.25f) + v * (q.c * (0.25f / kUp));
+      if (WHAT == kPolynomial) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += row == c + e ? q.a * 4096.f : 0.f;
+      }
       store_terms(to + row * p.lda, c, v);
     }
     if (m != n) {
@@ -627,13 +631,13 @@ int run(Batch& gram, Rule q, int steps) {
   return 0;
 }
 
-// Whether singular values in [0, 1] keep every entry of X, A and b A + c A A inside its range.
+// Whether singular values in [0, 1] keep every entry of X, A and the polynomial of A inside its range.
 bool in_range(double a, double b, double c, int steps) {
   for (int i = 0; i <= 4096; ++i) {
     double s = i / 4096.0;
     for (int k = 0; k < steps; ++k) {
       const double s2 = s * s, p = b * s2 + c * s2 * s2;
-      if (!(fabs(p) <= 15.0)) return false;
+      if (!(fabs(p) <= 15.0 && fabs(a + p) <= 15.0)) return false;
       s *= a + p;
       if (!(fabs(s) <= 1.9)) return false;
     }
