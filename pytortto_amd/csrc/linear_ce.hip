@@ -26,7 +26,7 @@ constexpr size_t kMostLogits = (size_t)2 << 30;     // bytes of a chunk's logits
 constexpr size_t kMostStats = (size_t)256 << 20;
 constexpr int kTop = 14;                            // scaled values are below 2^(kTop + 1)
 constexpr int kLowest = -1000;                      // an exponent below all
-constexpr int kAny = -2000;                         // that of a row of zeros: whatever suits the others
+constexpr int kAny = -2000;                         // that of a row of zeros, below that: whatever suits the others
 
 // Set at the start of a call, read by all that follows.
 struct Control {
@@ -56,31 +56,60 @@ __device__ __forceinline__ int exponent(float v) {
   return e;
 }
 
-__global__ __launch_bounds__(1024) void lce_begin(Targets t, long long rows, int mean, int lowest_e, int lowest_f, Control* c) {
+// Of float32, e and f are the exponents of W's rows and x's.  (One block, with every row's behind each other: an atomic operation of each row
+// where it is found took 9 ns of all the others, 10 us of 1064 rows.)
+__global__ __launch_bounds__(1024) void lce_begin(Targets t, long long rows, int mean, const int* __restrict__ e, const int* __restrict__ f,
+                                                  const float* __restrict__ g, Control* c) {
   __shared__ long long part[16];
+  __shared__ int part_e[16], part_f[16];
   long long n = 0;
-  for (long long i = threadIdx.x; i < rows; i += 1024) n += read_index(t.at, (size_t)i, t.wide) != t.ignore;
+  int most_e = e ? kLowest : 0, most_f = f || g ? kLowest : 0;
+#pragma unroll 4
+  for (long long i = threadIdx.x; i < rows; i += 1024) {
+    const bool kept = read_index(t.at, (size_t)i, t.wide) != t.ignore;
+    const int own = f ? f[i] : 0;
+    const float weight = g ? g[i] : 1.f;
+    n += kept;
+    if (kept && own != kAny && weight != 0.f) most_f = max(most_f, g ? own + exponent(weight) : own);
+  }
+  if (e) {
+#pragma unroll 8
+    for (int i = threadIdx.x; i < t.V; i += 1024) most_e = max(most_e, e[i]);
+  }
   n = row_sum<1024>(n, part);
+  const auto larger_int = [](int a, int b) { return max(a, b); };
+  most_e = row_reduce<1024>(most_e, part_e, larger_int);
+  most_f = row_reduce<1024>(most_f, part_f, larger_int);
   if (threadIdx.x == 0) {
     c->scale = !mean ? 1.f : n ? 1.f / (float)n : 0.f;
-    c->most_e = lowest_e;
-    c->most_f = lowest_f;
+    c->most_e = most_e;
+    c->most_f = most_f;
   }
 }
 
 // Rows of x or W as the products' operands: two terms of float32, or a copy of float16.  Rows without a target are
 // zeros, whatever they hold.  G threads have a row; of 16 G columns they keep it between its largest value and its terms.
+// Both matrices share a launch: the first blocks have x's rows.
+template <typename T>
+struct Rows {
+  const T* from;
+  char* to;
+  int* exponents;
+  long long rows;
+  Targets t;
+};
 template <typename T, int G>
-__global__ __launch_bounds__(256) void lce_rows(const T* __restrict__ from, char* __restrict__ to, int* __restrict__ exponents,
-                                                const float* __restrict__ g, long long rows, int columns, int ld, Targets t,
-                                                int* most) {
+__global__ __launch_bounds__(256) void lce_rows(Rows<T> of_x, Rows<T> of_w, unsigned blocks_x, int columns, int ld) {
   __shared__ float part[256 / kWave];
   constexpr int kKept = 4;
-  const long long row = (long long)blockIdx.x * (256 / G) + row_of_block<G>();
-  if (row >= rows) return;
+  const bool second = blockIdx.x >= blocks_x;
+  const Rows<T>& q = second ? of_w : of_x;
+  const Targets t = q.t;
+  const long long row = (long long)(blockIdx.x - (second ? blocks_x : 0)) * (256 / G) + row_of_block<G>();
+  if (row >= q.rows) return;
   const int lane = threadIdx.x % G, quads = (columns + 63) / 64 * 16;
-  const T* x = from + (size_t)row * columns;
-  char* y = to + (size_t)row * ld;
+  const T* x = q.from + (size_t)row * columns;
+  char* y = q.to + (size_t)row * ld;
   const bool kept = !t.at || class_of(t, row) != kIgnored, whole = columns % 4 == 0;
   const auto four = [&](int q) {
     typedef T Four __attribute__((ext_vector_type(4)));
@@ -101,7 +130,6 @@ __global__ __launch_bounds__(256) void lce_rows(const T* __restrict__ from, char
 #pragma unroll
   for (int k = 0; k < kKept; ++k) own[k] = lane + k * G < quads ? four(lane + k * G) : floatx4{};
   int e = 0;
-  bool counts = kept;       // among the largest exponents
   if (sizeof(T) == 4) {
     float m = 0.f;
     const auto look = [&](const floatx4& v) { m = fmaxf(m, fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])))); };
@@ -109,9 +137,9 @@ __global__ __launch_bounds__(256) void lce_rows(const T* __restrict__ from, char
     for (int k = 0; k < kKept; ++k) look(own[k]);
     for (int q = lane + kKept * G; q < quads; q += G) look(four(q));
     m = row_max<G>(m, part);
-    counts = m > 0.f && __builtin_isfinite(m);
+    const bool counts = m > 0.f && __builtin_isfinite(m);
     e = counts ? exponent(m) - kTop - 1 : 0;
-    if (lane == 0) exponents[row] = counts ? e : kAny;
+    if (lane == 0) q.exponents[row] = counts ? e : kAny;
   }
   const auto put = [&](int q, const floatx4& v) {
     if (sizeof(T) == 4) {
@@ -124,11 +152,6 @@ __global__ __launch_bounds__(256) void lce_rows(const T* __restrict__ from, char
   for (int k = 0; k < kKept; ++k)
     if (lane + k * G < quads) put(lane + k * G, own[k]);
   for (int q = lane + kKept * G; q < quads; q += G) put(q, four(q));
-  if (most && lane == 0 && counts && (!g || g[row] != 0.f)) {
-    // (looked at first: it rises a few times, and an atomic operation of every row costs 9 ns of all the others)
-    const int it = g ? e + exponent(g[row]) : e;
-    if (shared(most) < it) atomicMax(most, it);
-  }
 }
 
 struct Logits {
@@ -141,6 +164,8 @@ struct Logits {
   float2* stats;        // [rows][blocks]: of a tile's columns the largest logit, and the sum of e^(z - it) without its 1
   float* own;           // [rows] the target's logit, without z
   int blocks;
+  float* partial;       // [splits][rows][ld] or none: the blocks that share a tile leave their sums here, for lce_few
+  int per, splits;      // pairs for each
 };
 
 // One instruction each (fmaxf and fminf first quiet their arguments); the larger of a NaN and a number is the NaN.
@@ -171,8 +196,21 @@ __global__ __launch_bounds__(256) void lce_logits(Operand x, Operand w, int rows
   typedef Sized<TERMS, false, false, SIZE> G;
   extern __shared__ __align__(16) char lds[];
   int m, n;
-  tile_of(blockIdx.x, gridDim.x, (rows + G::kM - 1) / G::kM, (V + G::kN - 1) / G::kN, &m, &n);
+  const int blocks = gridDim.x / q.splits, split = blockIdx.x / blocks;
+  tile_of(blockIdx.x % blocks, blocks, (rows + G::kM - 1) / G::kM, (V + G::kN - 1) / G::kN, &m, &n);
   const int m0 = m * G::kM, n0 = n * G::kN, at = threadIdx.x;
+  if (SIZE == 0 && q.splits > 1) {
+    const int first = split * q.per;
+    float* to = q.partial + ((size_t)split * rows + m0) * q.ld + n0;
+    G p;
+    p.run(x, w, m0, n0, first, min(q.per, pairs - first), lds);
+    p.rows(lds, [](int, int) { return 0; }, [&](int r, int c, const floatx4 (&v)[G::kAhead], int (&)[G::kAhead]) {
+#pragma unroll
+      for (int u = 0; u < G::kAhead; ++u)
+        if (m0 + r + u * G::kStep < rows && n0 + c < q.ld) *reinterpret_cast<floatx4*>(to + (r + u * G::kStep) * q.ld + c) = v[u];
+    });
+    return;
+  }
   // the rows' targets and exponents, and the columns' exponents
   int2 mine = make_int2(kInvalid, 0);
   int column_e = 0;
@@ -299,7 +337,31 @@ __global__ __launch_bounds__(256) void lce_join(const float2* __restrict__ stats
 // With the exponent of a row of zeros, it is the largest that leaves the row's G (times its g) in range.
 __device__ __forceinline__ int exponent_of_row(int e, int top, float g) { return e == kAny ? top - exponent(g) + 1 : e; }
 
-// The logits of a chunk become G, where they stand: 32 floats are their first and second terms, or 64 their values as halves and a gap.
+// A row of G: 32 floats of the logits' row are first and second terms, or 64 are values as halves and a gap.
+template <int TERMS>
+__device__ __forceinline__ void store_gradient(const floatx4& v, float* z, int c) {
+  char* row = reinterpret_cast<char*>(z);
+  if (TERMS == 2) store_terms(row, c, v);
+  else *reinterpret_cast<half4*>(row + (c >> 6) * (2 * kLine) + (c & 63) * 2) = half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+}
+// Four logits of a row, from column c on, become G.
+template <int TERMS>
+__device__ __forceinline__ void put_gradient(floatx4 v, float* z, int c, int V, int target, float most, float log_sum, float loss, float weight,
+                                             int shift, int top_e, const int* __restrict__ e) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int column = c + i;
+    float p = __builtin_amdgcn_exp2f((v[i] - most) * kLog2e - log_sum);
+    if (column == target) p = expm1f(-loss);
+    if (target == kInvalid) p = NAN;
+    if (TERMS == 2 && column < V) p = ldexpf(p * weight, shift + exponent_of_row(e[column], top_e, 1.f));
+    else p = ldexpf(p * weight, shift);
+    v[i] = column < V ? p : 0.f;
+  }
+  store_gradient<TERMS>(v, z, c);
+}
+
+// The logits of a chunk become G, where they stand.
 template <int TERMS>
 __global__ __launch_bounds__(256) void lce_gradient(float* __restrict__ z, long long ld, const float2* __restrict__ of,
                                                     const float* __restrict__ loss, const float* __restrict__ g,
@@ -309,30 +371,83 @@ __global__ __launch_bounds__(256) void lce_gradient(float* __restrict__ z, long 
   if (c >= ld) return;
   float* at = z + (size_t)r * ld;
   const int target = class_of(t, first + r);
-  floatx4 v = {};
-  if (target != kIgnored) {
-    v = *reinterpret_cast<const floatx4*>(at + c);
-    const float2 s = of[r];
-    const float weight = g ? g[first + r] : 1.f, mine = loss[r];
-    const int top_e = control->top_e();
-    const int shift = kTop - top_e - control->top_f() + (TERMS == 2 ? exponent_of_row(f[r], control->top_f(), weight) : 0);
+  if (target == kIgnored) {
+    store_gradient<TERMS>(floatx4{}, at, c);
+    return;
+  }
+  const floatx4 v = *reinterpret_cast<const floatx4*>(at + c);
+  const float2 s = of[r];
+  const float weight = g ? g[first + r] : 1.f;
+  const int top_e = control->top_e();
+  const int shift = kTop - top_e - control->top_f() + (TERMS == 2 ? exponent_of_row(f[r], control->top_f(), weight) : 0);
+  put_gradient<TERMS>(v, at, c, V, target, s.x, s.y, loss[r], weight, shift, top_e, e);
+}
+
+// What lce_join and lce_gradient do, and the logits from the sums of the blocks that shared their tiles: of few rows over few classes, where
+// the reduction is what there is to share out (64 x 2048 x 1000 float32: 16 tiles of 64 x 64 and the two kernels took 32 us, 128 shares and this 15).  A
+// block has a row; of 4096 columns it keeps the logits in registers.
+template <int TERMS>
+__global__ __launch_bounds__(256) void lce_few(Logits q, int rows, int V, const float* __restrict__ g, float* __restrict__ loss,
+                                               const Control* __restrict__ control) {
+  __shared__ float part[3][256 / kWave];
+  __shared__ float own;
+  constexpr int kKept = 4;
+  const int r = blockIdx.x, target = class_of(q.t, r), quads = (int)(q.ld / 4);
+  float* z = q.z ? q.z + (size_t)r * q.ld : nullptr;
+  const float weight = g ? g[r] : 1.f;
+  const int f = TERMS == 2 ? q.f[r] : 0;
+  const auto logits = [&](int k) {
+    floatx4 v = {};
+    for (int s = 0; s < q.splits; ++s) v += *reinterpret_cast<const floatx4*>(q.partial + ((size_t)s * rows + r) * q.ld + k * 4);
+    const int4 e = TERMS == 2 ? *reinterpret_cast<const int4*>(q.e + k * 4) : int4{};
+    if (TERMS == 2) v = floatx4{ldexpf(v[0], e.x + f), ldexpf(v[1], e.y + f), ldexpf(v[2], e.z + f), ldexpf(v[3], e.w + f)};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int column = c + i;
-      float p = __builtin_amdgcn_exp2f((v[i] - s.x) * kLog2e - s.y);
-      if (column == target) p = expm1f(-mine);
-      if (target == kInvalid) p = NAN;
-      if (TERMS == 2 && column < V) p = ldexpf(p * weight, shift + exponent_of_row(e[column], top_e, 1.f));
-      else p = ldexpf(p * weight, shift);
-      v[i] = column < V ? p : 0.f;
+      if (k * 4 + i >= V) v[i] = -INFINITY;
+      if (k * 4 + i == target) own = v[i];
     }
+    return v;
+  };
+  floatx4 kept[kKept];
+  if (target != kIgnored) {
+    float most = -INFINITY, sum = 0.f;
+    int largest = 0;
+    const auto look = [&](const floatx4& v) { most = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), most); };
+#pragma unroll
+    for (int k = 0; k < kKept; ++k) {
+      kept[k] = (int)threadIdx.x + k * 256 < quads ? logits(threadIdx.x + k * 256) : floatx4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      look(kept[k]);
+    }
+    for (int k = threadIdx.x + kKept * 256; k < quads; k += 256) look(logits(k));
+    most = row_max<256>(most, part[0]);
+    const float from = most == -INFINITY ? 0.f : most;
+    const auto add = [&](const floatx4& v, int k) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool it = v[i] == most;
+        largest += it && k * 4 + i < V;
+        sum += it ? 0.f : __builtin_amdgcn_exp2f((v[i] - from) * kLog2e);
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < kKept; ++k) add(kept[k], threadIdx.x + k * 256);
+    for (int k = threadIdx.x + kKept * 256; k < quads; k += 256) add(logits(k), k);
+    const float rest = row_sum<256>(sum, part[1]) + (float)(row_sum<256>(largest, reinterpret_cast<int*>(part[2])) - 1);
+    const float log_sum = log1pf(rest), mine = target == kInvalid ? NAN : log_sum + (from - own);
+    if (threadIdx.x == 0) loss[r] = mine;
+    if (!z) return;
+    const int top_e = control->top_e();
+    const int shift = kTop - top_e - control->top_f() + (TERMS == 2 ? exponent_of_row(f, control->top_f(), weight) : 0);
+    const auto put = [&](const floatx4& v, int k) { put_gradient<TERMS>(v, z, k * 4, V, target, from, log_sum * kLog2e, mine, weight, shift, top_e, q.e); };
+#pragma unroll
+    for (int k = 0; k < kKept; ++k)
+      if ((int)threadIdx.x + k * 256 < quads) put(kept[k], threadIdx.x + k * 256);
+    for (int k = threadIdx.x + kKept * 256; k < quads; k += 256) put(logits(k), k);
+    return;
   }
-  char* row = reinterpret_cast<char*>(at);
-  if (TERMS == 2) {
-    store_terms(row, c, v);
-  } else {
-    *reinterpret_cast<half4*>(row + (c >> 6) * (2 * kLine) + (c & 63) * 2) = half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
-  }
+  if (threadIdx.x == 0) loss[r] = 0.f;
+  if (!z) return;
+  for (int k = threadIdx.x; k < quads; k += 256) store_gradient<TERMS>(floatx4{}, z, k * 4);
 }
 
 // What the two gradients' products do with their sums: take the scales back, and store them as float32 (to or on top of what is there)
@@ -516,16 +631,18 @@ int launch_scale(const float* from, const float* g, T* to, size_t n) {
 }
 
 template <typename T>
-void launch_rows(const T* from, char* to, int* exponents, const float* g, long long rows, int columns, int ld, const Targets& t, int* most) {
-  if (columns <= 1024) lce_rows<T, 64><<<(unsigned)((rows + 3) / 4), 256, 0, stream()>>>(from, to, exponents, g, rows, columns, ld, t, most);
-  else lce_rows<T, 256><<<(unsigned)rows, 256, 0, stream()>>>(from, to, exponents, g, rows, columns, ld, t, most);
+void launch_rows(const Rows<T>& x, const Rows<T>& w, int columns, int ld) {
+  const int side = columns <= 1024 ? 4 : 1;
+  const unsigned blocks_x = (unsigned)((x.rows + side - 1) / side), blocks = blocks_x + (unsigned)((w.rows + side - 1) / side);
+  if (side == 4) lce_rows<T, 64><<<blocks, 256, 0, stream()>>>(x, w, blocks_x, columns, ld);
+  else lce_rows<T, 256><<<blocks, 256, 0, stream()>>>(x, w, blocks_x, columns, ld);
 }
 
 template <int TERMS, int SIZE>
 int launch_logits(const Operand& x, const Operand& w, int rows, int V, int H, const Logits& q) {
   typedef Sized<TERMS, false, false, SIZE> G;
   TT_ALLOW_LDS((lce_logits<TERMS, SIZE>), G::kLds);
-  lce_logits<TERMS, SIZE><<<(unsigned)tiles_of(rows, V, SIZE), G::kThreads, G::kLds, stream()>>>(
+  lce_logits<TERMS, SIZE><<<(unsigned)(tiles_of(rows, V, SIZE) * q.splits), G::kThreads, G::kLds, stream()>>>(
       x, w, rows, V, (int)(padded(H) / (64 / TERMS)), q);
   TT_LAUNCH_CHECK();
   return 0;
@@ -612,6 +729,11 @@ int run(const Call& q) {
   const bool several = chunk < N;
   const int pairsV = (int)(Vp / depth), pairsN = (int)((chunk + depth - 1) / depth);
   const int size = tile_size(chunk, V), blocks = (V + kTileSide[size] - 1) / kTileSide[size];
+  // (the reduction of few small tiles is shared out)
+  const int pairsH = (int)(Hp / depth);
+  int splits = size || several ? 1 : (int)std::max(1LL, std::min(compute_units() / tiles_of(chunk, V, 0), (long long)pairsH / 8));
+  const int per = (pairsH + splits - 1) / splits;
+  splits = (pairsH + per - 1) / per;
   const Plan plan_x = plan_product(chunk, H, pairsV), plan_w = plan_product(V, H, pairsN);
 
   Carve c;
@@ -621,7 +743,8 @@ int run(const Call& q) {
   const size_t at_loss = c.take(4 * N), at_z = c.take(grad ? (size_t)chunk * Vp * 4 : 0);
   const size_t part_x = q.dx && plan_x.splits > 1 ? (size_t)plan_x.splits * chunk * ((H + 3) / 4) * 16 : 0;
   const size_t part_w = q.dw && plan_w.splits > 1 ? (size_t)plan_w.splits * V * ((H + 3) / 4) * 16 : 0;
-  const size_t at_part = c.take(std::max(part_x, part_w));
+  const size_t part_z = splits > 1 ? (size_t)splits * chunk * Vp * 4 : 0;
+  const size_t at_part = c.take(std::max({part_x, part_w, part_z}));
   const size_t at_sum = c.take(several && q.half_out && q.dw ? (size_t)V * H * 4 : 0);
   void* ws;
   if (tt::workspace(c.bytes, &ws)) return -1;
@@ -633,28 +756,24 @@ int run(const Call& q) {
   float2 *stats = (float2*)(base + at_stats), *of = (float2*)(base + at_of);
   float* own = (float*)(base + at_own);
 
-  lce_begin<<<1, 1024, 0, stream()>>>(q.t, N, mean, TERMS == 2 ? kLowest : 0, TERMS == 2 || q.g ? kLowest : 0, control);
-  TT_LAUNCH_CHECK();
   const int ldx = (int)(Hp * 2 * TERMS);
-  launch_rows<T>((const T*)q.x, base + at_x, f, q.g, N, H, ldx, q.t,
-                                                             TERMS == 2 || q.g ? &control->most_f : nullptr);
+  const Rows<T> of_x = {(const T*)q.x, base + at_x, f, N, q.t};
+  const Rows<T> of_w = {(const T*)q.w, base + at_w, e, copy_w ? V : 0, Targets{nullptr, 0, 0, 0}};
+  launch_rows<T>(of_x, of_w, H, ldx);
   TT_LAUNCH_CHECK();
-  Operand w = {(const char*)q.w, (long long)V * H * 2, H * 2, kLine};
-  if (copy_w) {
-    launch_rows<T>((const T*)q.w, base + at_w, e, nullptr, V, H, ldx, Targets{nullptr, 0, 0, 0},
-                                                               TERMS == 2 ? &control->most_e : nullptr);
-    TT_LAUNCH_CHECK();
-    w = Operand{base + at_w, (long long)V * ldx, ldx, kLine};
-  }
+  lce_begin<<<1, 1024, 0, stream()>>>(q.t, N, mean, e, f, q.g, control);
+  TT_LAUNCH_CHECK();
+  const Operand w = copy_w ? Operand{base + at_w, (long long)V * ldx, ldx, kLine} : Operand{(const char*)q.w, (long long)V * H * 2, H * 2, kLine};
   for (long long first = 0; first < N; first += chunk) {
     const int rows = (int)std::min(chunk, N - first);
     const Operand x = {base + at_x + (size_t)first * ldx, (long long)rows * ldx, ldx, kLine};
-    const Logits logits = {f ? f + first : nullptr, e, q.t, first, z, Vp, stats, own, blocks};
+    const Logits logits = {f ? f + first : nullptr, e, q.t, first, z, Vp, stats, own, blocks, partial, per, splits};
     if (launch_logits<TERMS>(size, x, w, rows, V, H, logits)) return -1;
-    lce_join<<<(unsigned)((rows + 3) / 4), 256, 0, stream()>>>(stats, own, z, Vp, of, losses + first, q.t, first, rows, blocks);
+    if (splits > 1) lce_few<TERMS><<<(unsigned)rows, 256, 0, stream()>>>(logits, rows, V, q.g, losses, control);
+    else lce_join<<<(unsigned)((rows + 3) / 4), 256, 0, stream()>>>(stats, own, z, Vp, of, losses + first, q.t, first, rows, blocks);
     TT_LAUNCH_CHECK();
     if (!grad) continue;
-    for (int r = 0; r < rows; r += 65535) {
+    for (int r = splits > 1 ? rows : 0; r < rows; r += 65535) {
       const int some = std::min(rows - r, 65535);
       lce_gradient<TERMS><<<dim3((unsigned)((Vp / 4 + 255) / 256), some), 256, 0, stream()>>>(
           z + (size_t)r * Vp, Vp, of + r, losses + first + r, q.g, f ? f + first + r : nullptr, e, q.t, first + r, V, control);
