@@ -32,6 +32,7 @@ constexpr int kAny = -2000;                         // that of a row of zeros, b
 struct Control {
   float scale;          // of the loss and its gradients: 1 / positions for 'mean'
   int most_e, most_f;   // the largest exponents of W's rows, and of x's rows with their g
+  Ticket done;
   __device__ __forceinline__ int top_e() const { return most_e == kLowest ? 0 : most_e; }
   __device__ __forceinline__ int top_f() const { return most_f == kLowest ? 0 : most_f; }
 };
@@ -84,6 +85,7 @@ __global__ __launch_bounds__(1024) void lce_begin(Targets t, long long rows, int
     c->scale = !mean ? 1.f : n ? 1.f / (float)n : 0.f;
     c->most_e = most_e;
     c->most_f = most_f;
+    c->done.n = 0;
   }
 }
 
@@ -284,6 +286,7 @@ __global__ __launch_bounds__(256) void lce_logits(Operand x, Operand w, int rows
     q.stats[(size_t)(m0 + at) * q.blocks + n] = make_float2(more.x, rest);
   }
   if (!q.z) return;
+  // (past the caches, here and in lce_product: 2047 x 1000 x 50021 float16 with gradients 1086 -> 1061 us)
   float* z = q.z + (size_t)m0 * q.ld + n0;
   const int ld = (int)q.ld;
   const int4 mine4 = TERMS == 2 ? *reinterpret_cast<const int4*>(scales + (at & 63) % G::kLanes * 4) : int4{};
@@ -296,21 +299,43 @@ __global__ __launch_bounds__(256) void lce_logits(Operand x, Operand w, int rows
         const int e = about[k].y;
         v[u] = floatx4{ldexpf(v[u][0], mine4.x + e), ldexpf(v[u][1], mine4.y + e), ldexpf(v[u][2], mine4.z + e), ldexpf(v[u][3], mine4.w + e)};
       }
-      if (m0 + k < rows && n0 + c < ld) *reinterpret_cast<floatx4*>(z + (unsigned)(k * ld + c)) = v[u];
+      if (m0 + k < rows && n0 + c < ld) __builtin_nontemporal_store(v[u], reinterpret_cast<floatx4*>(z + (unsigned)(k * ld + c)));
     }
   });
 }
 
+// The loss of all positions, in the order of the positions.
+struct Total {
+  float* to;            // or none
+  long long n;
+  int mean;
+  const Control* control;
+};
+template <int THREADS, typename L>
+__device__ __forceinline__ void total(const Total& q, L loss) {
+  __shared__ double part[THREADS / kWave];
+  double s = 0.0;
+  for (long long i = threadIdx.x; i < q.n; i += THREADS) s += (double)loss(i);
+  s = row_sum<THREADS>(s, part);
+  if (threadIdx.x == 0) *q.to = q.mean && q.control->scale == 0.f ? NAN : (float)(s * (double)q.control->scale);
+}
+// The same by the last of `blocks` blocks, each of which has shared some.  (Of few: a launch less.)
+__device__ __forceinline__ void total_by_last(const Total& q, const float* loss, unsigned blocks) {
+  __shared__ bool last;
+  stores_done();
+  __syncthreads();
+  if (threadIdx.x == 0) last = last_ticket(const_cast<Ticket*>(&q.control->done), blocks);
+  __syncthreads();
+  if (last) total<256>(q, [&](long long i) { return shared(loss + i); });
+}
+
 // A row's maximum and log2 of its sum from those of its blocks, and its loss.  A wave has a row.  The sum is kept without the
 // largest term, which is 1: of a target that has nearly all of the probability, the loss is what is left, and keeps its digits.
-__global__ __launch_bounds__(256) void lce_join(const float2* __restrict__ stats, const float* __restrict__ own, const float* __restrict__ z,
-                                                long long ld, float2* __restrict__ of, float* __restrict__ loss, Targets t, long long first,
-                                                int rows, int blocks) {
-  const int r = blockIdx.x * 4 + row_of_block<kWave>();
-  if (r >= rows) return;
+__device__ __forceinline__ void join_row(const float2* __restrict__ stats, const float* __restrict__ own, const float* __restrict__ z, long long ld,
+                                         float2* __restrict__ of, float* __restrict__ loss, const Targets& t, long long first, int r, int blocks) {
   const int lane = threadIdx.x & 63, target = class_of(t, first + r);
   if (target == kIgnored) {
-    if (lane == 0) loss[r] = 0.f;
+    if (lane == 0) share(loss + r, 0.f);
     return;
   }
   const float2* s = stats + (size_t)r * blocks;
@@ -330,10 +355,16 @@ __global__ __launch_bounds__(256) void lce_join(const float2* __restrict__ stats
   if (lane == 0) {
     const float log_sum = log1pf(rest);
     of[r] = make_float2(from, log_sum * kLog2e);
-    loss[r] = target == kInvalid ? NAN : log_sum + (from - (z ? z[(size_t)r * ld + target] : own[r]));
+    share(loss + r, target == kInvalid ? NAN : log_sum + (from - (z ? z[(size_t)r * ld + target] : own[r])));
   }
 }
-
+__global__ __launch_bounds__(256) void lce_join(const float2* __restrict__ stats, const float* __restrict__ own, const float* __restrict__ z,
+                                                long long ld, float2* __restrict__ of, float* __restrict__ loss, Targets t, long long first,
+                                                int rows, int blocks, Total all) {
+  const int r = blockIdx.x * 4 + row_of_block<kWave>();
+  if (r < rows) join_row(stats, own, z, ld, of, loss, t, first, r, blocks);
+  if (all.to) total_by_last(all, loss, gridDim.x);
+}
 // With the exponent of a row of zeros, it is the largest that leaves the row's G (times its g) in range.
 __device__ __forceinline__ int exponent_of_row(int e, int top, float g) { return e == kAny ? top - exponent(g) + 1 : e; }
 
@@ -387,8 +418,8 @@ __global__ __launch_bounds__(256) void lce_gradient(float* __restrict__ z, long 
 // the reduction is what there is to share out (64 x 2048 x 1000 float32: 16 tiles of 64 x 64 and the two kernels took 32 us, 128 shares and this 15).  A
 // block has a row; of 4096 columns it keeps the logits in registers.
 template <int TERMS>
-__global__ __launch_bounds__(256) void lce_few(Logits q, int rows, int V, const float* __restrict__ g, float* __restrict__ loss,
-                                               const Control* __restrict__ control) {
+__device__ __forceinline__ void few_row(const Logits& q, int rows, int V, const float* __restrict__ g, float* __restrict__ loss,
+                                        const Control* __restrict__ control) {
   __shared__ float part[3][256 / kWave];
   __shared__ float own;
   constexpr int kKept = 4;
@@ -434,7 +465,7 @@ __global__ __launch_bounds__(256) void lce_few(Logits q, int rows, int V, const 
     for (int k = threadIdx.x + kKept * 256; k < quads; k += 256) add(logits(k), k);
     const float rest = row_sum<256>(sum, part[1]) + (float)(row_sum<256>(largest, reinterpret_cast<int*>(part[2])) - 1);
     const float log_sum = log1pf(rest), mine = target == kInvalid ? NAN : log_sum + (from - own);
-    if (threadIdx.x == 0) loss[r] = mine;
+    if (threadIdx.x == 0) share(loss + r, mine);
     if (!z) return;
     const int top_e = control->top_e();
     const int shift = kTop - top_e - control->top_f() + (TERMS == 2 ? exponent_of_row(f, control->top_f(), weight) : 0);
@@ -445,9 +476,15 @@ __global__ __launch_bounds__(256) void lce_few(Logits q, int rows, int V, const 
     for (int k = threadIdx.x + kKept * 256; k < quads; k += 256) put(logits(k), k);
     return;
   }
-  if (threadIdx.x == 0) loss[r] = 0.f;
+  if (threadIdx.x == 0) share(loss + r, 0.f);
   if (!z) return;
   for (int k = threadIdx.x; k < quads; k += 256) store_gradient<TERMS>(floatx4{}, z, k * 4);
+}
+template <int TERMS>
+__global__ __launch_bounds__(256) void lce_few(Logits q, int rows, int V, const float* __restrict__ g, float* __restrict__ loss,
+                                               const Control* __restrict__ control, Total all) {
+  few_row<TERMS>(q, rows, V, g, loss, control);
+  if (all.to) total_by_last(all, loss, gridDim.x);
 }
 
 // What the two gradients' products do with their sums: take the scales back, and store them as float32 (to or on top of what is there)
@@ -574,7 +611,7 @@ __global__ __launch_bounds__(256) void lce_product(Operand a, Operand b, int M, 
              for (int u = 0; u < G::kAhead; ++u) {
                const int k = r + u * G::kStep;
                const floatx4 s = scaled(v[u], k) + old[u];
-               if (m0 + k < M && n0 + c < N) *reinterpret_cast<floatx4*>(to + (unsigned)(k * out.columns + c)) = s;
+               if (m0 + k < M && n0 + c < N) __builtin_nontemporal_store(s, reinterpret_cast<floatx4*>(to + (unsigned)(k * out.columns + c)));
              }
            });
     return;
@@ -584,7 +621,7 @@ __global__ __launch_bounds__(256) void lce_product(Operand a, Operand b, int M, 
     for (int u = 0; u < G::kAhead; ++u) {
       const int k = r + u * G::kStep;
       const floatx4 s = scaled(v[u], k);
-      if (m0 + k < M && n0 + c < N) *reinterpret_cast<floatx4*>(to + (unsigned)(k * out.columns + c)) = s;
+      if (m0 + k < M && n0 + c < N) __builtin_nontemporal_store(s, reinterpret_cast<floatx4*>(to + (unsigned)(k * out.columns + c)));
     }
   });
 }
@@ -599,13 +636,8 @@ __global__ __launch_bounds__(256) void lce_sum(const float* __restrict__ partial
   out.store(row, (int)(at % quads) * 4, v, out.control->scale, out.exponent_for(row), floatx4{});
 }
 
-__global__ __launch_bounds__(1024) void lce_loss(const float* __restrict__ loss, long long rows, int mean, Targets t, const Control* control,
-                                                 float* __restrict__ out) {
-  __shared__ double part[16];
-  double s = 0.0;
-  for (long long i = threadIdx.x; i < rows; i += 1024) s += (double)loss[i];
-  s = row_sum<1024>(s, part);
-  if (threadIdx.x == 0) *out = mean && control->scale == 0.f ? NAN : (float)(s * (double)control->scale);
+__global__ __launch_bounds__(1024) void lce_loss(const float* __restrict__ loss, Total all) {
+  total<1024>(all, [&](long long i) { return loss[i]; });
 }
 
 // g (none: 1) times a float32 gradient, as float32 or float16.
@@ -764,13 +796,16 @@ int run(const Call& q) {
   lce_begin<<<1, 1024, 0, stream()>>>(q.t, N, mean, e, f, q.g, control);
   TT_LAUNCH_CHECK();
   const Operand w = copy_w ? Operand{base + at_w, (long long)V * ldx, ldx, kLine} : Operand{(const char*)q.w, (long long)V * H * 2, H * 2, kLine};
+  const Total all = {q.reduction ? q.loss : nullptr, N, mean, control};
+  const bool at_once = !several && (splits > 1 ? N : (N + 3) / 4) <= 256;
+  const Total by_last = at_once ? all : Total{};
   for (long long first = 0; first < N; first += chunk) {
     const int rows = (int)std::min(chunk, N - first);
     const Operand x = {base + at_x + (size_t)first * ldx, (long long)rows * ldx, ldx, kLine};
     const Logits logits = {f ? f + first : nullptr, e, q.t, first, z, Vp, stats, own, blocks, partial, per, splits};
     if (launch_logits<TERMS>(size, x, w, rows, V, H, logits)) return -1;
-    if (splits > 1) lce_few<TERMS><<<(unsigned)rows, 256, 0, stream()>>>(logits, rows, V, q.g, losses, control);
-    else lce_join<<<(unsigned)((rows + 3) / 4), 256, 0, stream()>>>(stats, own, z, Vp, of, losses + first, q.t, first, rows, blocks);
+    if (splits > 1) lce_few<TERMS><<<(unsigned)rows, 256, 0, stream()>>>(logits, rows, V, q.g, losses, control, by_last);
+    else lce_join<<<(unsigned)((rows + 3) / 4), 256, 0, stream()>>>(stats, own, z, Vp, of, losses + first, q.t, first, rows, blocks, by_last);
     TT_LAUNCH_CHECK();
     if (!grad) continue;
     for (int r = splits > 1 ? rows : 0; r < rows; r += 65535) {
@@ -793,8 +828,8 @@ int run(const Call& q) {
   if (several && q.half_out && q.dw) {
     if (launch_scale((float*)(base + at_sum), nullptr, (_Float16*)q.dw, (size_t)V * H)) return -1;
   }
-  if (q.loss && q.reduction) {
-    lce_loss<<<1, 1024, 0, stream()>>>(losses, N, mean, q.t, control, q.loss);
+  if (all.to && !at_once) {
+    lce_loss<<<1, 1024, 0, stream()>>>(losses, all);
     TT_LAUNCH_CHECK();
   }
   return 0;
