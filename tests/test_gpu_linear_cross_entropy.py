@@ -60,6 +60,77 @@ def test_sizes(rows, width, vocab, dtype):
 
 
 @pytest.mark.parametrize('dtype', [np.float32, np.float16])
+@pytest.mark.parametrize('rows,width,vocab', [(1, 4096, 64), (3, 2048, 63), (7, 1100, 7003), (33, 2048, 4097), (64, 2048, 1000), (65, 1025, 130),
+                                              (1, 2049, 8190), (128, 1500, 1), (256, 1024, 200), (257, 1536, 77), (500, 1040, 500)])
+def test_few_positions_and_wide_features(rows, width, vocab, dtype):
+    """Few small tiles, whose reduction several blocks share."""
+    x, w, target = _inputs(rows, width, vocab, dtype, rows + vocab, padded=0.2)
+    _compare(x, w, target)
+    _compare(x, w, target, 'sum', scale=0.25, need=(False, True))
+    g = np.random.default_rng(rows).standard_normal(rows).astype(np.float32)
+    g[::3] = 0.0
+    _compare(x, w, target, 'none', g)
+
+
+@pytest.mark.parametrize('dtype', [np.float32, np.float16])
+def test_few_positions_with_what_is_not_finite_or_not_there(dtype):
+    """The rows of the test before: NaN stays in its row's loss, a class outside is NaN, and so is a class whose logits are."""
+    x, w, target = _inputs(40, 2000, 300, dtype, 5)
+    x[3, 7] = np.nan
+    target[5], target[9] = 300, -301
+    target[11:14] = -100
+    x[12] = np.inf
+    loss = F.linear_cross_entropy(_tensor(x), _tensor(w), _tensor(target), reduction='none').data.get()
+    assert np.isnan(loss[[3, 5, 9]]).all() and (loss[11:14] == 0).all()
+    assert np.isfinite(np.delete(loss, [3, 5, 9])).all()
+    w[17, 0] = np.nan
+    loss = F.linear_cross_entropy(_tensor(x), _tensor(w), _tensor(target), reduction='none').data.get()
+    assert np.isnan(np.delete(loss, [11, 12, 13])).all() and (loss[11:14] == 0).all()
+    # a row and a matrix of zeros: ln of the classes, and gradients that are the others' alone
+    x, w, target = _inputs(40, 2000, 300, dtype, 6)
+    x[4] = 0
+    w[8] = 0
+    _compare(x, w, target)
+    _compare(np.zeros_like(x), w, target)
+    _compare(x, np.zeros_like(w), target)
+
+
+@pytest.mark.parametrize('dtype', [np.float32, np.float16])
+def test_a_weight_past_32_bits(dtype):
+    """2^20 classes of 2176 features, 4.6 GB or twice that; all but five rows are zeros, so that the sums are known."""
+    vocab, width = 1 << 20, 2176
+    rng = np.random.default_rng(14)
+    hit = np.array([0, 1, vocab // 2, vocab - 2, vocab - 1])
+    rows = (rng.standard_normal((5, width)) * width ** -0.5 * 4).astype(dtype)
+    x = rng.standard_normal((3, width)).astype(dtype)
+    target = np.array([vocab - 1, 0, vocab // 2])
+    weight = torch.zeros((vocab, width), dtype=torch.float32 if dtype == np.float32 else torch.float16, device='cuda')
+    weight[torch.from_numpy(hit).cuda()] = torch.from_numpy(rows).cuda()
+    torch.cuda.synchronize()
+    xt, wt = _tensor(x, True), tt.as_tensor(weight, True)
+    loss = F.linear_cross_entropy(xt, wt, _tensor(target), reduction='sum')
+    loss.backward()
+    z = x.astype(np.float64) @ rows.astype(np.float64).T
+    lse = np.log(np.exp(z).sum(1) + (vocab - 5))
+    own = z[np.arange(3), [4, 0, 2]]
+    assert abs(loss.data.get().item() - (lse - own).sum()) <= 2e-6 * np.abs(lse).sum()
+    g = np.exp(z - lse[:, None])
+    g[np.arange(3), [4, 0, 2]] -= 1.0
+    # G is held to 2^-11 (2^-19: 2^-22 and what the logits are off by) of itself, and so is what is stored
+    step, least = (2.0 ** -11, 2.0 ** -25) if dtype == np.float16 else (2.0 ** -19, 0.0)
+    want, size = g @ rows.astype(np.float64), np.abs(g) @ np.abs(rows.astype(np.float64))
+    assert (np.abs(xt.grad.get() - want) <= 3 * step * size + least).all()
+    dw = torch.as_tensor(wt.grad, device='cuda')
+    got = dw[torch.from_numpy(hit).cuda()].double().cpu().numpy()
+    want, size = g.T @ x.astype(np.float64), np.abs(g).T @ np.abs(x.astype(np.float64))
+    assert (np.abs(got - want) <= 3 * step * size + least).all()
+    rest = np.exp(-lse) @ x.astype(np.float64)
+    size = np.exp(-lse) @ np.abs(x.astype(np.float64))
+    for v in (2, vocab // 2 - 1, vocab // 2 + 1, vocab - 3):
+        assert (np.abs(dw[v].double().cpu().numpy() - rest) <= 3 * step * size + least).all()
+
+
+@pytest.mark.parametrize('dtype', [np.float32, np.float16])
 @pytest.mark.parametrize('rows,width,vocab', [(1024, 96, 3500), (2100, 256, 1100), (900, 1000, 4000), (4000, 70, 777)])
 def test_larger(rows, width, vocab, dtype):
     """Every size of tile, for every product."""

@@ -40,6 +40,19 @@ def test_sizes(rows, columns, dtype):
     _compare(_matrix(rows, columns, dtype))
 
 
+@pytest.mark.parametrize('rows,columns', [(64, 384), (64, 385), (65, 384), (384, 64), (385, 64), (63, 192), (192, 64), (60, 193), (193, 33),
+                                          (1, 384), (384, 1), (17, 383)])
+def test_around_what_one_block_takes(rows, columns):
+    _compare(_matrix(rows, columns))
+    _compare(_matrix(rows, columns, np.float16), 2)
+
+
+@pytest.mark.parametrize('rows,columns', [(1, 70000), (70000, 1), (40, 60001), (60001, 40), (130, 20000)])
+def test_long_reductions(rows, columns):
+    """Many blocks share a tile."""
+    _compare(_matrix(rows, columns))
+
+
 @pytest.mark.parametrize('rows,columns', [(1300, 1300), (1025, 2100), (2300, 900)])
 def test_larger(rows, columns):
     _compare(_matrix(rows, columns), 3)
