@@ -429,6 +429,7 @@ __device__ __forceinline__ void few_row(const Logits& q, int rows, int V, const 
   const int f = TERMS == 2 ? q.f[r] : 0;
   const auto logits = [&](int k) {
     floatx4 v = {};
+#pragma unroll 4
     for (int s = 0; s < q.splits; ++s) v += *reinterpret_cast<const floatx4*>(q.partial + ((size_t)s * rows + r) * q.ld + k * 4);
     const int4 e = TERMS == 2 ? *reinterpret_cast<const int4*>(q.e + k * 4) : int4{};
     if (TERMS == 2) v = floatx4{ldexpf(v[0], e.x + f), ldexpf(v[1], e.y + f), ldexpf(v[2], e.z + f), ldexpf(v[3], e.w + f)};
@@ -631,6 +632,7 @@ __global__ __launch_bounds__(256) void lce_sum(const float* __restrict__ partial
   const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
   if (at >= (long long)M * quads) return;
   floatx4 v = {};
+#pragma unroll 4
   for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const floatx4*>(partial + ((size_t)s * M * quads + at) * 4);
   const int row = (int)(at / quads);
   out.store(row, (int)(at % quads) * 4, v, out.control->scale, out.exponent_for(row), floatx4{});

@@ -27,7 +27,7 @@ constexpr size_t kMostScratch = (size_t)4 << 30;
 constexpr size_t kMostPartial = (size_t)1 << 30;
 constexpr float kUp = 16384.f;              // the scale of X and A
 constexpr int kParts = 1024;                // partial sums of a matrix's squares, at most
-constexpr int kJoin = 64;                   // side of what a block of muon_join works on
+constexpr int kJoin = 64;                   // columns of what a block of muon_join works on
 
 struct Matrix {
   const void* from;         // the gradient, or the matrix itself (float32 or float16)
@@ -288,44 +288,53 @@ __global__ __launch_bounds__(256) void muon_product(Batch b, Rule q, int last) {
   }
 }
 
-// A = X X^T, or a I + b A + c A A, from the partial sums of the upper tiles: 64 x 64 of it, and the same on the other side of the diagonal.
-template <int WHAT>
+// A = X X^T, or a I + b A + c A A, from the partial sums of the upper tiles: STRIP x 64 of it, and the same on the other side of the
+// diagonal.  The sums come from other dies' blocks, and what bounds few blocks is how many loads are on their way: 9 sums of 777 x 777 took 91
+// blocks with 64 rows 13.7 us, and 364 with 16 rows 5.1.  Many are bound by memory, and better with whole lines on the other
+// side, too: the polynomials of 6 matrices of 2048 x 2048, 3168 blocks, take 32 us with 64 rows and 38 with 16.
+template <int WHAT, int STRIP>
 __global__ __launch_bounds__(256) void muon_join(Batch b, Rule q) {
-  __shared__ float turned[kJoin][kJoin + 1];
+  __shared__ float turned[kJoin][STRIP + 1];
+  constexpr int kStrips = kJoin / STRIP, kHigh = STRIP / 16, kAtOnce = 8 / kHigh;
   const int at = matrix_of(b);
   const Matrix& x = b.of[at];
   const Place p(x.rows, x.columns);
-  const int edge = (int)padded(p.m);
+  const int edge = (int)padded(p.m), block = (int)(blockIdx.x - b.first[at]), strip = block % kStrips * STRIP;
   int m, n;
-  upper_tile((int)(blockIdx.x - b.first[at]), edge / kJoin, &m, &n);
+  upper_tile(block / kStrips, edge / kJoin, &m, &n);
   char *a = x.scratch + 2 * p.x, *to = WHAT == kGram ? a : a + p.a;
-  const int r0 = m * kJoin + (threadIdx.x >> 4), c = n * kJoin + (threadIdx.x & 15) * 4;
+  const int r = threadIdx.x >> 4, r0 = m * kJoin + strip + r, c = n * kJoin + (threadIdx.x & 15) * 4;
+  floatx4 v[kHigh] = {};
+  const float* from[kHigh];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kHigh; ++i) from[i] = x.partial + (long long)min(r0 + 16 * i, p.m - 1) * edge + c;
+#pragma unroll kAtOnce
+  for (int s = 0; s < x.splits; ++s) {
+#pragma unroll
+    for (int i = 0; i < kHigh; ++i) v[i] += *reinterpret_cast<const floatx4*>(from[i] + s * p.square());
+  }
+#pragma unroll
+  for (int i = 0; i < kHigh; ++i) {
     const int row = r0 + 16 * i;
-    floatx4 v = {};
     if (row < p.m) {
-      const float* from = x.partial + (long long)row * edge + c;
-      for (int s = 0; s < x.splits; ++s) v += *reinterpret_cast<const floatx4*>(from + s * p.square());
-      if (WHAT == kGram) v *= 1.f / kUp;
-      else v = load_terms(a + row * p.lda, c) * (q.b * 0.25f) + v * (q.c * (0.25f / kUp));
-      if (WHAT == kPolynomial) {
+      if (WHAT == kGram) {
+        v[i] *= 1.f / kUp;
+      } else {
+        v[i] = load_terms(a + row * p.lda, c) * (q.b * 0.25f) + v[i] * (q.c * (0.25f / kUp));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += row == c + e ? q.a * 4096.f : 0.f;
+        for (int e = 0; e < 4; ++e) v[i][e] += row == c + e ? q.a * 4096.f : 0.f;
       }
-      store_terms(to + row * p.lda, c, v);
+      store_terms(to + row * p.lda, c, v[i]);
     }
-    if (m != n) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) turned[(threadIdx.x & 15) * 4 + e][(threadIdx.x >> 4) + 16 * i] = v[e];
-    }
+    for (int e = 0; e < 4; ++e) turned[(threadIdx.x & 15) * 4 + e][r + 16 * i] = row < p.m ? v[i][e] : 0.f;
   }
   if (m == n) return;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int k = (threadIdx.x >> 4) + 16 * i, row = n * kJoin + k, j = (threadIdx.x & 15) * 4;
-    if (row < p.m) store_terms(to + row * p.lda, m * kJoin + j, floatx4{turned[k][j], turned[k][j + 1], turned[k][j + 2], turned[k][j + 3]});
+  for (int i = 0; i < kHigh; ++i) {
+    const int k = (threadIdx.x + i * 256) / (STRIP / 4), j = threadIdx.x % (STRIP / 4) * 4, other = n * kJoin + k;
+    if (other < p.m) store_terms(to + other * p.lda, m * kJoin + strip + j, floatx4{turned[k][j], turned[k][j + 1], turned[k][j + 2], turned[k][j + 3]});
   }
 }
 
@@ -586,6 +595,14 @@ int run_small(const Batch& b, const Rule& q, int steps) {
   return most <= 64 ? launch_small<64>(b, q, steps) : most <= 192 ? launch_small<192>(b, q, steps) : launch_small<kLong>(b, q, steps);
 }
 
+template <int WHAT>
+int launch_join(bool strips, const Batch& b, const Rule& q) {
+  if (strips) muon_join<WHAT, 16><<<b.first[b.count], 256, 0, stream()>>>(b, q);
+  else muon_join<WHAT, 64><<<b.first[b.count], 256, 0, stream()>>>(b, q);
+  TT_LAUNCH_CHECK();
+  return 0;
+}
+
 // ---- batches ---------------------------------------------------------------------------------------
 // The matrices of one batch, all steps.
 int run(Batch& gram, Rule q, int steps) {
@@ -615,17 +632,17 @@ int run(Batch& gram, Rule q, int steps) {
     rows.first[i + 1] = rows.first[i] + scale_blocks(r, c);
     gram_join.first[i + 1] = polynomial_join.first[i + 1] = gram_join.first[i] + (unsigned)upper(padded(std::min(r, c)) / kJoin);
   }
+  const bool strips = gram_join.first[gram.count] < (unsigned)compute_units();
+  for (int i = 1; strips && i <= gram.count; ++i) gram_join.first[i] = polynomial_join.first[i] = 4 * gram_join.first[i];
   muon_begin<<<begin.first[begin.count], 256, 0, stream()>>>(begin, q);
   TT_LAUNCH_CHECK();
   muon_scale<<<rows.first[rows.count], 256, 0, stream()>>>(rows, q);
   TT_LAUNCH_CHECK();
   for (q.step = 0; q.step < steps; ++q.step) {
     if (launch<kGram>(gram_size, gram, q, 0)) return -1;
-    muon_join<kGram><<<gram_join.first[gram.count], 256, 0, stream()>>>(gram_join, q);
-    TT_LAUNCH_CHECK();
+    if (launch_join<kGram>(strips, gram_join, q)) return -1;
     if (launch<kPolynomial>(polynomial_size, polynomial, q, 0)) return -1;
-    muon_join<kPolynomial><<<polynomial_join.first[gram.count], 256, 0, stream()>>>(polynomial_join, q);
-    TT_LAUNCH_CHECK();
+    if (launch_join<kPolynomial>(strips, polynomial_join, q)) return -1;
     if (launch<kUpdate>(update_size, update, q, q.step == steps - 1)) return -1;
   }
   return 0;
