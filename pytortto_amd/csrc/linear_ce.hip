@@ -156,6 +156,11 @@ __global__ __launch_bounds__(256) void lce_rows(Rows<T> of_x, Rows<T> of_w, unsi
   for (int q = lane + kKept * G; q < quads; q += G) put(q, four(q));
 }
 
+// Columns of the logits, or rows of a gradient, that a launch has, and how many blocks of columns are in front of it.
+struct Part {
+  int first, end, blocks;
+};
+
 struct Logits {
   const int* f;         // exponents of x's rows and W's, of float32
   const int* e;
@@ -194,13 +199,13 @@ __device__ __forceinline__ Pair with_lane(float v) {
 }
 
 template <int TERMS, int SIZE>
-__global__ __launch_bounds__(256) void lce_logits(Operand x, Operand w, int rows, int V, int pairs, Logits q) {
+__global__ __launch_bounds__(256) void lce_logits(Operand x, Operand w, int rows, int V, int pairs, Logits q, Part part) {
   typedef Sized<TERMS, false, false, SIZE> G;
   extern __shared__ __align__(16) char lds[];
   int m, n;
-  const int blocks = gridDim.x / q.splits, split = blockIdx.x / blocks;
-  tile_of(blockIdx.x % blocks, blocks, (rows + G::kM - 1) / G::kM, (V + G::kN - 1) / G::kN, &m, &n);
-  const int m0 = m * G::kM, n0 = n * G::kN, at = threadIdx.x;
+  const int tile = xcd_remap(blockIdx.x, gridDim.x), blocks = gridDim.x / q.splits, split = tile / blocks;
+  tile_at(tile % blocks, (rows + G::kM - 1) / G::kM, (part.end - part.first + G::kN - 1) / G::kN, &m, &n);
+  const int m0 = m * G::kM, n0 = part.first + n * G::kN, at = threadIdx.x;
   if (SIZE == 0 && q.splits > 1) {
     const int first = split * q.per;
     float* to = q.partial + ((size_t)split * rows + m0) * q.ld + n0;
@@ -283,7 +288,7 @@ __global__ __launch_bounds__(256) void lce_logits(Operand x, Operand w, int rows
     const float2 a = halves[at], b = halves[G::kM + at];
     const float2 more = a.x < b.x ? b : a, less = a.x < b.x ? a : b;
     const float rest = more.y + (1.f + less.y) * (a.x == b.x ? 1.f : __builtin_amdgcn_exp2f((less.x - more.x) * kLog2e));
-    q.stats[(size_t)(m0 + at) * q.blocks + n] = make_float2(more.x, rest);
+    q.stats[(size_t)(m0 + at) * q.blocks + part.blocks + n] = make_float2(more.x, rest);
   }
   if (!q.z) return;
   // (past the caches, here and in lce_product: 2047 x 1000 x 50021 float16 with gradients 1086 -> 1061 us)
@@ -545,13 +550,13 @@ struct GradientOut {
 
 template <int TERMS, bool A_ACROSS, int SIZE>
 __global__ __launch_bounds__(256) void lce_product(Operand a, Operand b, int M, int N, int pairs, int per, int splits, float* partial,
-                                                   GradientOut out) {
+                                                   GradientOut out, Part part) {
   typedef Sized<TERMS, A_ACROSS, true, SIZE> G;
   extern __shared__ __align__(16) char lds[];
-  const int blocks = gridDim.x / splits, split = blockIdx.x / blocks;
+  const int tile = xcd_remap(blockIdx.x, gridDim.x), blocks = gridDim.x / splits, split = tile / blocks;
   int m, n;
-  tile_of(blockIdx.x % blocks, blocks, (M + G::kM - 1) / G::kM, (N + G::kN - 1) / G::kN, &m, &n);
-  const int first = split * per, count = min(per, pairs - first), m0 = m * G::kM, n0 = n * G::kN;
+  tile_at(tile % blocks, (part.end - part.first + G::kM - 1) / G::kM, (N + G::kN - 1) / G::kN, &m, &n);
+  const int first = split * per, count = min(per, pairs - first), m0 = part.first + m * G::kM, n0 = n * G::kN;
   const int mine = splits == 1 && threadIdx.x < G::kM && m0 + (int)threadIdx.x < M ? out.exponent_for(m0 + threadIdx.x) : 0;
   const float scale = out.control->scale;
   G p;
@@ -672,21 +677,33 @@ void launch_rows(const Rows<T>& x, const Rows<T>& w, int columns, int ld) {
   else lce_rows<T, 256><<<blocks, 256, 0, stream()>>>(x, w, blocks_x, columns, ld);
 }
 
+// Where the tiles are not whole rounds over the compute units and few are left for the last one, the last columns (of n, m the other side)
+// are left to smaller tiles, in a launch behind the others': the first of these columns.  (777 x 1024 x 50021 float32, 784 tiles of 256 x 256:
+// the logits took 283 us; 768 of them take 232 and 208 of 64 x 64 behind them 16.)
+long long first_left(long long m, long long n, int size) {
+  const long long side = kTileSide[size], high = (m + side - 1) / side, wide = (n + side - 1) / side, units = compute_units();
+  const long long rounds = high * wide / units, rest = high * wide % units;
+  if (size == 0 || rounds == 0 || rest == 0 || rest > units / 4) return n;
+  const long long kept = rounds * units / high;
+  return kept > 0 && (wide - kept) * high <= units / 2 ? kept * side : n;
+}
+int size_left(long long m, long long n, int size) { return std::min(tile_size(m, n), size - 1); }
+
 template <int TERMS, int SIZE>
-int launch_logits(const Operand& x, const Operand& w, int rows, int V, int H, const Logits& q) {
+int launch_logits(const Operand& x, const Operand& w, int rows, int V, int H, const Logits& q, const Part& part) {
   typedef Sized<TERMS, false, false, SIZE> G;
   TT_ALLOW_LDS((lce_logits<TERMS, SIZE>), G::kLds);
-  lce_logits<TERMS, SIZE><<<(unsigned)(tiles_of(rows, V, SIZE) * q.splits), G::kThreads, G::kLds, stream()>>>(
-      x, w, rows, V, (int)(padded(H) / (64 / TERMS)), q);
+  lce_logits<TERMS, SIZE><<<(unsigned)(tiles_of(rows, part.end - part.first, SIZE) * q.splits), G::kThreads, G::kLds, stream()>>>(
+      x, w, rows, V, (int)(padded(H) / (64 / TERMS)), q, part);
   TT_LAUNCH_CHECK();
   return 0;
 }
 template <int TERMS>
-int launch_logits(int size, const Operand& x, const Operand& w, int rows, int V, int H, const Logits& q) {
+int launch_logits(int size, const Operand& x, const Operand& w, int rows, int V, int H, const Logits& q, const Part& part) {
   switch (size) {
-    case 2: return launch_logits<TERMS, 2>(x, w, rows, V, H, q);
-    case 1: return launch_logits<TERMS, 1>(x, w, rows, V, H, q);
-    default: return launch_logits<TERMS, 0>(x, w, rows, V, H, q);
+    case 2: return launch_logits<TERMS, 2>(x, w, rows, V, H, q, part);
+    case 1: return launch_logits<TERMS, 1>(x, w, rows, V, H, q, part);
+    default: return launch_logits<TERMS, 0>(x, w, rows, V, H, q, part);
   }
 }
 
@@ -708,12 +725,12 @@ Plan plan_product(long long m, long long n, long long pairs) {
 }
 
 template <int TERMS, bool A_ACROSS, int SIZE>
-int launch_product(const Operand& a, const Operand& b, int M, int N, int pairs, int per, float* partial, const GradientOut& out) {
+int launch_product(const Operand& a, const Operand& b, int M, int N, int pairs, int per, float* partial, const GradientOut& out, const Part& part) {
   typedef Sized<TERMS, A_ACROSS, true, SIZE> G;
   TT_ALLOW_LDS((lce_product<TERMS, A_ACROSS, SIZE>), G::kLds);
   const int splits = (pairs + per - 1) / per;      // (fewer for a chunk that is not whole)
-  lce_product<TERMS, A_ACROSS, SIZE><<<(unsigned)(tiles_of(M, N, SIZE) * splits), G::kThreads, G::kLds, stream()>>>(
-      a, b, M, N, pairs, per, splits, partial, out);
+  lce_product<TERMS, A_ACROSS, SIZE><<<(unsigned)(tiles_of(part.end - part.first, N, SIZE) * splits), G::kThreads, G::kLds, stream()>>>(
+      a, b, M, N, pairs, per, splits, partial, out, part);
   TT_LAUNCH_CHECK();
   if (splits > 1) {
     const long long quads = (long long)M * ((N + 3) / 4);
@@ -723,12 +740,20 @@ int launch_product(const Operand& a, const Operand& b, int M, int N, int pairs, 
   return 0;
 }
 template <int TERMS, bool A_ACROSS>
-int launch_product(const Plan& plan, const Operand& a, const Operand& b, int M, int N, int pairs, float* partial, const GradientOut& out) {
-  switch (plan.size) {
-    case 2: return launch_product<TERMS, A_ACROSS, 2>(a, b, M, N, pairs, plan.per, partial, out);
-    case 1: return launch_product<TERMS, A_ACROSS, 1>(a, b, M, N, pairs, plan.per, partial, out);
-    default: return launch_product<TERMS, A_ACROSS, 0>(a, b, M, N, pairs, plan.per, partial, out);
+int launch_product(int size, const Operand& a, const Operand& b, int M, int N, int pairs, int per, float* partial, const GradientOut& out,
+                   const Part& part) {
+  switch (size) {
+    case 2: return launch_product<TERMS, A_ACROSS, 2>(a, b, M, N, pairs, per, partial, out, part);
+    case 1: return launch_product<TERMS, A_ACROSS, 1>(a, b, M, N, pairs, per, partial, out, part);
+    default: return launch_product<TERMS, A_ACROSS, 0>(a, b, M, N, pairs, per, partial, out, part);
   }
+}
+template <int TERMS, bool A_ACROSS>
+int launch_product(const Plan& plan, const Operand& a, const Operand& b, int M, int N, int pairs, float* partial, const GradientOut& out) {
+  const int end = plan.splits > 1 ? M : (int)first_left(N, M, plan.size);
+  if (launch_product<TERMS, A_ACROSS>(plan.size, a, b, M, N, pairs, plan.per, partial, out, Part{0, end, 0})) return -1;
+  if (end == M) return 0;
+  return launch_product<TERMS, A_ACROSS>(size_left(N, M - end, plan.size), a, b, M, N, pairs, plan.per, partial, out, Part{end, M, 0});
 }
 
 // Parts of the workspace, one behind the other.
@@ -762,7 +787,8 @@ int run(const Call& q) {
   chunk = std::min(chunk, N);
   const bool several = chunk < N;
   const int pairsV = (int)(Vp / depth), pairsN = (int)((chunk + depth - 1) / depth);
-  const int size = tile_size(chunk, V), blocks = (V + kTileSide[size] - 1) / kTileSide[size];
+  const int size = tile_size(chunk, V), V1 = (int)first_left(chunk, V, size), left = V1 < V ? size_left(chunk, V - V1, size) : size;
+  const int blocks1 = (V1 + kTileSide[size] - 1) / kTileSide[size], blocks = blocks1 + (V - V1 + kTileSide[left] - 1) / kTileSide[left];
   // (the reduction of few small tiles is shared out)
   const int pairsH = (int)(Hp / depth);
   int splits = size || several ? 1 : (int)std::max(1LL, std::min(compute_units() / tiles_of(chunk, V, 0), (long long)pairsH / 8));
@@ -805,7 +831,8 @@ int run(const Call& q) {
     const int rows = (int)std::min(chunk, N - first);
     const Operand x = {base + at_x + (size_t)first * ldx, (long long)rows * ldx, ldx, kLine};
     const Logits logits = {f ? f + first : nullptr, e, q.t, first, z, Vp, stats, own, blocks, partial, per, splits};
-    if (launch_logits<TERMS>(size, x, w, rows, V, H, logits)) return -1;
+    if (launch_logits<TERMS>(size, x, w, rows, V, H, logits, Part{0, V1, 0})) return -1;
+    if (V1 < V && launch_logits<TERMS>(left, x, w, rows, V, H, logits, Part{V1, V, blocks1})) return -1;
     if (splits > 1) lce_few<TERMS><<<(unsigned)rows, 256, 0, stream()>>>(logits, rows, V, q.g, losses, control, by_last);
     else lce_join<<<(unsigned)((rows + 3) / 4), 256, 0, stream()>>>(stats, own, z, Vp, of, losses + first, q.t, first, rows, blocks, by_last);
     TT_LAUNCH_CHECK();

@@ -200,8 +200,8 @@ __device__ __forceinline__ void muon_tile(const Matrix& x, const Rule& q, bool l
   G g;
   if (WHAT != kUpdate) {
     // sums of a part of the reduction, for muon_join
-    const int side = (p.m + G::kM - 1) / G::kM, tiles = (int)upper(side), split = (int)block / tiles;
-    upper_tile((int)block % tiles, side, &m, &n);
+    const int side = (p.m + G::kM - 1) / G::kM, tiles = (int)upper(side), at = xcd_remap(block, blocks), split = at / tiles;
+    upper_tile(at % tiles, side, &m, &n);
     const int pairs = ((WHAT == kGram ? ACROSS ? x.rows : x.columns : p.m) + 31) / 32, per = (pairs + x.splits - 1) / x.splits;
     const int first = split * per, count = first + per < pairs ? per : pairs - first;
     const int m0 = m * G::kM, n0 = n * G::kN, edge = (int)padded(p.m);
@@ -218,7 +218,7 @@ __device__ __forceinline__ void muon_tile(const Matrix& x, const Rule& q, bool l
     return;
   }
   const int M = x.rows, columns = x.columns, edge = (int)padded(columns);
-  tile_of((int)block, (int)blocks, (M + G::kM - 1) / G::kM, (columns + G::kN - 1) / G::kN, &m, &n);
+  tile_at(xcd_remap(block, blocks), (M + G::kM - 1) / G::kM, (columns + G::kN - 1) / G::kN, &m, &n);
   const int m0 = m * G::kM, n0 = n * G::kN;
   const auto each = [&](int r, int c, int end, auto f) {
 #pragma unroll

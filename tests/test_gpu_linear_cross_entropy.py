@@ -60,6 +60,15 @@ def test_sizes(rows, width, vocab, dtype):
 
 
 @pytest.mark.parametrize('dtype', [np.float32, np.float16])
+@pytest.mark.parametrize('rows,width,vocab', [(1000, 1000, 4300), (777, 800, 17001)])
+def test_rounds_that_are_not_whole(rows, width, vocab, dtype):
+    """A few tiles more than the compute units can take at once: the last classes are left to smaller tiles."""
+    x, w, target = _inputs(rows, width, vocab, dtype, 3, padded=0.1)
+    target[:40] = vocab - 1 - np.arange(40) * 13
+    _compare(x, w, target, 'sum')
+
+
+@pytest.mark.parametrize('dtype', [np.float32, np.float16])
 @pytest.mark.parametrize('rows,width,vocab', [(1, 4096, 64), (3, 2048, 63), (7, 1100, 7003), (33, 2048, 4097), (64, 2048, 1000), (65, 1025, 130),
                                               (1, 2049, 8190), (128, 1500, 1), (256, 1024, 200), (257, 1536, 77), (500, 1040, 500)])
 def test_few_positions_and_wide_features(rows, width, vocab, dtype):
