@@ -91,7 +91,7 @@ __global__ __launch_bounds__(1024) void lce_begin(Targets t, long long rows, int
 
 // Rows of x or W as the products' operands: two terms of float32, or a copy of float16.  Rows without a target are
 // zeros, whatever they hold.  G threads have a row; of 16 G columns they keep it between its largest value and its terms.
-// Both matrices share a launch: the first blocks have x's rows.
+// Both matrices share a launch: the first blocks have x's rows.  Bound by memory: 50021 + 777 rows of 1024 float32 72 us, 5.8 TB/s.
 template <typename T>
 struct Rows {
   const T* from;
@@ -198,6 +198,10 @@ __device__ __forceinline__ Pair with_lane(float v) {
   return {__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
 }
 
+// A tile of logits, and its rows' maxima and sums.  Bound by the matrix instructions under the power limit, and by the logits it stores, which
+// all blocks do at about the same time: 4096 x 2048 x 131072 float16 2.08 ms (1060 TFLOP/s), without a gradient to come 1.67 (1310);
+// 4096 x 1024 x 32768 float32 664 us (three products counted 1240).  Dies that begin at different times, so that they store at
+// different times, were 3 % slower.
 template <int TERMS, int SIZE>
 __global__ __launch_bounds__(256) void lce_logits(Operand x, Operand w, int rows, int V, int pairs, Logits q, Part part) {
   typedef Sized<TERMS, false, false, SIZE> G;
@@ -397,7 +401,8 @@ __device__ __forceinline__ void put_gradient(floatx4 v, float* z, int c, int V, 
   store_gradient<TERMS>(v, z, c);
 }
 
-// The logits of a chunk become G, where they stand.
+// The logits of a chunk become G, where they stand.  Bound by memory: 4096 x 131072, float16 530 us (6.1 TB/s: half of G's line stays as it is),
+// 4096 x 32768 float32 247 us (4.3 TB/s).
 template <int TERMS>
 __global__ __launch_bounds__(256) void lce_gradient(float* __restrict__ z, long long ld, const float2* __restrict__ of,
                                                     const float* __restrict__ loss, const float* __restrict__ g,
@@ -548,6 +553,8 @@ struct GradientOut {
   }
 };
 
+// A tile of dX = G W or dW = G^T x.  Bound as lce_logits is: of 4096 x 2048 x 131072 float16 1.56 ms (dX, 1410 TFLOP/s) and 1.95 (dW, 1130: a
+// reduction of 64 pairs, and 1.1 GB of sums to store), of 4096 x 1024 x 32768 float32 535 and 563 us (1540 and 1460).
 template <int TERMS, bool A_ACROSS, int SIZE>
 __global__ __launch_bounds__(256) void lce_product(Operand a, Operand b, int M, int N, int pairs, int per, int splits, float* partial,
                                                    GradientOut out, Part part) {
@@ -647,7 +654,7 @@ __global__ __launch_bounds__(1024) void lce_loss(const float* __restrict__ loss,
   total<1024>(all, [&](long long i) { return loss[i]; });
 }
 
-// g (none: 1) times a float32 gradient, as float32 or float16.
+// g (none: 1) times a float32 gradient, as float32 or float16.  Bound by memory: 131072 x 2048 to float16 5.1 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void lce_scale(const float* __restrict__ from, const float* __restrict__ g, T* __restrict__ to, size_t n) {
   const float s = g ? *g : 1.f;
@@ -789,7 +796,7 @@ int run(const Call& q) {
   const int pairsV = (int)(Vp / depth), pairsN = (int)((chunk + depth - 1) / depth);
   const int size = tile_size(chunk, V), V1 = (int)first_left(chunk, V, size), left = V1 < V ? size_left(chunk, V - V1, size) : size;
   const int blocks1 = (V1 + kTileSide[size] - 1) / kTileSide[size], blocks = blocks1 + (V - V1 + kTileSide[left] - 1) / kTileSide[left];
-  // (the reduction of few small tiles is shared out)
+  // (the reduction of few small tiles is shared out, eight pairs or more to a block: fewer would be loads on their way and little else)
   const int pairsH = (int)(Hp / depth);
   int splits = size || several ? 1 : (int)std::max(1LL, std::min(compute_units() / tiles_of(chunk, V, 0), (long long)pairsH / 8));
   const int per = (pairsH + splits - 1) / splits;
@@ -825,6 +832,7 @@ int run(const Call& q) {
   TT_LAUNCH_CHECK();
   const Operand w = copy_w ? Operand{base + at_w, (long long)V * ldx, ldx, kLine} : Operand{(const char*)q.w, (long long)V * H * 2, H * 2, kLine};
   const Total all = {q.reduction ? q.loss : nullptr, N, mean, control};
+  // (of at most as many blocks as there are at one time: each counts itself, 9 ns of the others' time)
   const bool at_once = !several && (splits > 1 ? N : (N + 3) / 4) <= 256;
   const Total by_last = at_once ? all : Total{};
   for (long long first = 0; first < N; first += chunk) {
