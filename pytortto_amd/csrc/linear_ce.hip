@@ -424,9 +424,9 @@ __global__ __launch_bounds__(256) void lce_gradient(float* __restrict__ z, long 
   put_gradient<TERMS>(v, at, c, V, target, s.x, s.y, loss[r], weight, shift, top_e, e);
 }
 
-// What lce_join and lce_gradient do, and the logits from the sums of the blocks that shared their tiles: of few rows over few classes, where
-// the reduction is what there is to share out (64 x 2048 x 1000 float32: 16 tiles of 64 x 64 and the two kernels took 32 us, 128 shares and this 15).  A
-// block has a row; of 4096 columns it keeps the logits in registers.
+// What lce_join and lce_gradient do, and the logits from the sums of the blocks that shared their tiles: of few rows over few classes,
+// where the reduction is what there is to share out (64 x 2048 x 1000 float32: 16 tiles of 64 x 64 and the two kernels took 32 us, 128 shares
+// and this 15).  A block has a row; of 4096 columns it keeps the logits in registers.
 template <int TERMS>
 __device__ __forceinline__ void few_row(const Logits& q, int rows, int V, const float* __restrict__ g, float* __restrict__ loss,
                                         const Control* __restrict__ control) {
@@ -480,7 +480,9 @@ __device__ __forceinline__ void few_row(const Logits& q, int rows, int V, const 
     if (!z) return;
     const int top_e = control->top_e();
     const int shift = kTop - top_e - control->top_f() + (TERMS == 2 ? exponent_of_row(f, control->top_f(), weight) : 0);
-    const auto put = [&](const floatx4& v, int k) { put_gradient<TERMS>(v, z, k * 4, V, target, from, log_sum * kLog2e, mine, weight, shift, top_e, q.e); };
+    const auto put = [&](const floatx4& v, int k) {
+      put_gradient<TERMS>(v, z, k * 4, V, target, from, log_sum * kLog2e, mine, weight, shift, top_e, q.e);
+    };
 #pragma unroll
     for (int k = 0; k < kKept; ++k)
       if ((int)threadIdx.x + k * 256 < quads) put(kept[k], threadIdx.x + k * 256);
@@ -722,7 +724,7 @@ Plan plan_product(long long m, long long n, long long pairs) {
   Plan p;
   p.size = tile_size(m, n);
   // few tiles and a long reduction: large tiles shared by several blocks
-  while (p.size < 2 && pairs >= 64 && tiles_of(m, n, p.size + 1) * (pairs / 16) >= compute_units() && m > kTileSide[p.size] && n > kTileSide[p.size]) ++p.size;
+  while (p.size < 2 && pairs >= 64 && tiles_of(m, n, p.size + 1) * (pairs / 16) >= compute_units() && std::min(m, n) > kTileSide[p.size]) ++p.size;
   const long long tiles = tiles_of(m, n, p.size);
   long long splits = compute_units() / tiles;
   splits = std::max(1LL, std::min(splits, pairs / 8));
