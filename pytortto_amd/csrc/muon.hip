@@ -7,7 +7,8 @@
 // reads either operand along or across its rows).
 //
 // All products are of two float16 terms an operand, X and A scaled by 2^14 and a I + b A + c A A (in muon_small without a I) by 2^12: with
-// singular values up to 1.9, and a and the polynomial up to 15, which calls are checked for, no entry leaves float16's range, and one is held to 2^-22 of itself or 2^-39 of the unit.
+// singular values up to 1.9, and a and the polynomial up to 15, which calls are checked for, no entry
+// leaves float16's range, and one is held to 2^-22 of itself or 2^-39 of the unit.
 // The two symmetric products are made of the tiles on and above the diagonal; several blocks may share one along the reduction, and
 // leave sums that muon_join adds up, in order, and mirrors.  The matrices of a step share the launches, five for each of its
 // Newton-Schulz steps and two in front: a network has tens of them, most too small to fill the device.
