@@ -641,6 +641,7 @@ __global__ __launch_bounds__(256) void lce_product(Operand a, Operand b, int M, 
   });
 }
 
+// The sums of the blocks that shared a reduction.  (A later chunk's are added to what the chunks in front of it have left, as lce_product's are.)
 __global__ __launch_bounds__(256) void lce_sum(const float* __restrict__ partial, int splits, int M, int N, GradientOut out) {
   const int quads = (N + 3) / 4;
   const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -648,8 +649,8 @@ __global__ __launch_bounds__(256) void lce_sum(const float* __restrict__ partial
   floatx4 v = {};
 #pragma unroll 4
   for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const floatx4*>(partial + ((size_t)s * M * quads + at) * 4);
-  const int row = (int)(at / quads);
-  out.store(row, (int)(at % quads) * 4, v, out.control->scale, out.exponent_for(row), floatx4{});
+  const int row = (int)(at / quads), c = (int)(at % quads) * 4;
+  out.store(row, c, v, out.control->scale, out.exponent_for(row), out.add ? out.before(row, c) : floatx4{});
 }
 
 __global__ __launch_bounds__(1024) void lce_loss(const float* __restrict__ loss, Total all) {
