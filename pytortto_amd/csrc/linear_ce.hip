@@ -9,9 +9,10 @@
 // has three products and not a fourth for logits that it forgot, and the scratch memory is bounded whatever the batch.
 //
 // float16: the tensors are the products' operands as they are; G is rounded to float16 once, scaled by 2^14.
-// float32: operands have two float16 terms.  Row i of x and row v of W are scaled by powers of two 2^-f_i and 2^-e_v to below
-// 2^15; G, which meets W's rows and x's rows as k, carries 2^(e_v + f_i), and all of it a common 2^c that brings the largest
-// to 2^15: G's entries are held to 2^-22 of themselves, and to 2^-40 of the largest.
+// float32: operands have two float16 terms.  For the logits row i of x and row v of W are scaled by powers of two 2^-f_i and 2^-e_v to below
+// 2^15, so that every position and every class has the digits that it would have alone.  In the gradients' products, where these rows are k, a
+// scale of each row's own would have to be G's, and small rows' G would fall out of its range; there W and g x are scaled by one
+// power of two each, and G is the bare softmax(z) - [v = t], times 2^15: its entries are held to 2^-22 of themselves and to 2^-40, whatever the rows they meet.
 #include "product.h"
 #include "rows.h"
 
@@ -26,12 +27,13 @@ constexpr size_t kMostLogits = (size_t)2 << 30;     // bytes of a chunk's logits
 constexpr size_t kMostStats = (size_t)256 << 20;
 constexpr int kTop = 14;                            // scaled values are below 2^(kTop + 1)
 constexpr int kLowest = -1000;                      // an exponent below all
-constexpr int kAny = -2000;                         // that of a row of zeros, below that: whatever suits the others
+constexpr int kAny = -2000;                         // that of a row of zeros, or with what is not finite
+constexpr int kTopGradient = 15;                    // the scale of G of float32
 
 // Set at the start of a call, read by all that follows.
 struct Control {
   float scale;          // of the loss and its gradients: 1 / positions for 'mean'
-  int most_e, most_f;   // the largest exponents of W's rows, and of x's rows with their g
+  int most_e, most_f;   // the largest exponents of W's rows, and of x's rows with their g (float16: of g)
   Ticket done;
   __device__ __forceinline__ int top_e() const { return most_e == kLowest ? 0 : most_e; }
   __device__ __forceinline__ int top_f() const { return most_f == kLowest ? 0 : most_f; }
@@ -154,6 +156,49 @@ __global__ __launch_bounds__(256) void lce_rows(Rows<T> of_x, Rows<T> of_w, unsi
   for (int k = 0; k < kKept; ++k)
     if (lane + k * G < quads) put(lane + k * G, own[k]);
   for (int q = lane + kKept * G; q < quads; q += G) put(q, four(q));
+}
+
+// x times g, and W, as operands of the gradients' products: float32 with one scale for the whole matrix.  G threads have a row.  Bound
+// by memory: 32768 + 4096 rows of 1024 53 us, 5.7 TB/s.
+template <int G>
+__global__ __launch_bounds__(256) void lce_again(Rows<float> of_x, Rows<float> of_w, const float* __restrict__ g, unsigned blocks_x, int columns,
+                                                 int ld, const Control* __restrict__ control) {
+  const bool second = blockIdx.x >= blocks_x;
+  const Rows<float>& q = second ? of_w : of_x;
+  const long long row = (long long)(blockIdx.x - (second ? blocks_x : 0)) * (256 / G) + row_of_block<G>();
+  if (row >= q.rows) return;
+  const int quads = (columns + 63) / 64 * 16;
+  const float* x = q.from + (size_t)row * columns;
+  char* y = q.to + (size_t)row * ld;
+  const bool kept = !q.t.at || class_of(q.t, row) != kIgnored, whole = columns % 4 == 0;
+  // v 2^-first m 2^then: g's exponent is not multiplied with, so that nothing leaves the range on the way
+  float m = 1.f;
+  int first = 0, then = 0;
+  if (second) {
+    first = control->top_e();
+  } else {
+    first = q.exponents[row] == kAny ? 0 : q.exponents[row];
+    then = first - control->top_f();
+    if (g && kept) {
+      m = g[row];
+      const int e = exponent(m);
+      m = ldexpf(m, -e);
+      then += e;
+    }
+  }
+  for (int k = threadIdx.x % G; k < quads; k += G) {
+    floatx4 v = {};
+    if (kept && whole && k * 4 < columns) {
+      v = *reinterpret_cast<const floatx4*>(x + k * 4);
+    } else if (kept) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (k * 4 + i < columns) v[i] = x[k * 4 + i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = ldexpf(ldexpf(v[i], -first) * m, then);
+    store_terms(y, k * 4, v);
+  }
 }
 
 // Columns of the logits, or rows of a gradient, that a launch has, and how many blocks of columns are in front of it.
@@ -374,8 +419,11 @@ __global__ __launch_bounds__(256) void lce_join(const float2* __restrict__ stats
   if (r < rows) join_row(stats, own, z, ld, of, loss, t, first, r, blocks);
   if (all.to) total_by_last(all, loss, gridDim.x);
 }
-// With the exponent of a row of zeros, it is the largest that leaves the row's G (times its g) in range.
-__device__ __forceinline__ int exponent_of_row(int e, int top, float g) { return e == kAny ? top - exponent(g) + 1 : e; }
+// What a row's G is multiplied with: float32's weight of the position comes in with x, or behind the product.
+template <int TERMS>
+__device__ __forceinline__ float factor_of(const Control* control, const float* g, long long i) {
+  return TERMS == 2 ? (float)(1 << kTopGradient) : ldexpf(g ? g[i] : 1.f, kTop - control->top_f());
+}
 
 // A row of G: 32 floats of the logits' row are first and second terms, or 64 are values as halves and a gap.
 template <int TERMS>
@@ -386,27 +434,23 @@ __device__ __forceinline__ void store_gradient(const floatx4& v, float* z, int c
 }
 // Four logits of a row, from column c on, become G.
 template <int TERMS>
-__device__ __forceinline__ void put_gradient(floatx4 v, float* z, int c, int V, int target, float most, float log_sum, float loss, float weight,
-                                             int shift, int top_e, const int* __restrict__ e) {
+__device__ __forceinline__ void put_gradient(floatx4 v, float* z, int c, int V, int target, float most, float log_sum, float loss, float factor) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int column = c + i;
     float p = __builtin_amdgcn_exp2f((v[i] - most) * kLog2e - log_sum);
     if (column == target) p = expm1f(-loss);
     if (target == kInvalid) p = NAN;
-    if (TERMS == 2 && column < V) p = ldexpf(p * weight, shift + exponent_of_row(e[column], top_e, 1.f));
-    else p = ldexpf(p * weight, shift);
-    v[i] = column < V ? p : 0.f;
+    v[i] = column < V ? p * factor : 0.f;
   }
   store_gradient<TERMS>(v, z, c);
 }
 
 // The logits of a chunk become G, where they stand.  Bound by memory: 4096 x 131072, float16 530 us (6.1 TB/s: half of G's line stays as it is),
-// 4096 x 32768 float32 247 us (4.3 TB/s).
+// 4096 x 32768 float32 165 us (6.5 TB/s).
 template <int TERMS>
 __global__ __launch_bounds__(256) void lce_gradient(float* __restrict__ z, long long ld, const float2* __restrict__ of,
-                                                    const float* __restrict__ loss, const float* __restrict__ g,
-                                                    const int* __restrict__ f, const int* __restrict__ e, Targets t,
+                                                    const float* __restrict__ loss, const float* __restrict__ g, Targets t,
                                                     long long first, int V, const Control* __restrict__ control) {
   const int r = blockIdx.y, c = (blockIdx.x * 256 + threadIdx.x) * 4;
   if (c >= ld) return;
@@ -418,10 +462,7 @@ __global__ __launch_bounds__(256) void lce_gradient(float* __restrict__ z, long 
   }
   const floatx4 v = *reinterpret_cast<const floatx4*>(at + c);
   const float2 s = of[r];
-  const float weight = g ? g[first + r] : 1.f;
-  const int top_e = control->top_e();
-  const int shift = kTop - top_e - control->top_f() + (TERMS == 2 ? exponent_of_row(f[r], control->top_f(), weight) : 0);
-  put_gradient<TERMS>(v, at, c, V, target, s.x, s.y, loss[r], weight, shift, top_e, e);
+  put_gradient<TERMS>(v, at, c, V, target, s.x, s.y, loss[r], factor_of<TERMS>(control, g, first + r));
 }
 
 // What lce_join and lce_gradient do, and the logits from the sums of the blocks that shared their tiles: of few rows over few classes,
@@ -435,7 +476,6 @@ __device__ __forceinline__ void few_row(const Logits& q, int rows, int V, const 
   constexpr int kKept = 4;
   const int r = blockIdx.x, target = class_of(q.t, r), quads = (int)(q.ld / 4);
   float* z = q.z ? q.z + (size_t)r * q.ld : nullptr;
-  const float weight = g ? g[r] : 1.f;
   const int f = TERMS == 2 ? q.f[r] : 0;
   const auto logits = [&](int k) {
     floatx4 v = {};
@@ -478,11 +518,8 @@ __device__ __forceinline__ void few_row(const Logits& q, int rows, int V, const 
     const float log_sum = log1pf(rest), mine = target == kInvalid ? NAN : log_sum + (from - own);
     if (threadIdx.x == 0) share(loss + r, mine);
     if (!z) return;
-    const int top_e = control->top_e();
-    const int shift = kTop - top_e - control->top_f() + (TERMS == 2 ? exponent_of_row(f, control->top_f(), weight) : 0);
-    const auto put = [&](const floatx4& v, int k) {
-      put_gradient<TERMS>(v, z, k * 4, V, target, from, log_sum * kLog2e, mine, weight, shift, top_e, q.e);
-    };
+    const float factor = factor_of<TERMS>(control, g, r);
+    const auto put = [&](const floatx4& v, int k) { put_gradient<TERMS>(v, z, k * 4, V, target, from, log_sum * kLog2e, mine, factor); };
 #pragma unroll
     for (int k = 0; k < kKept; ++k)
       if ((int)threadIdx.x + k * 256 < quads) put(kept[k], threadIdx.x + k * 256);
@@ -502,18 +539,29 @@ __global__ __launch_bounds__(256) void lce_few(Logits q, int rows, int V, const 
 
 // What the two gradients' products do with their sums: take the scales back, and store them as float32 (to or on top of what is there)
 // or float16; or leave partial sums for lce_sum.
+enum Of { kHalf, kPositions, kClasses };      // float16 operands; rows of float32's dX; rows of its dW
+struct Scale {
+  float s;
+  int e;
+};
 struct GradientOut {
   void* to;
-  const int* exponents;     // of the rows, of float32
-  int top_f;                // they are x's, not W's
-  const float* g;           // of the rows, if they are x's
+  Of of;
+  const float* g;           // of the rows, if they are positions
+  Targets t;
+  long long first;          // row of the first position
   const Control* control;
   int half, add;
   int columns;
-  // What a row's sums are multiplied with besides the scale: a power of two.
-  __device__ __forceinline__ int exponent_for(int row) const {
-    const int top = top_f ? control->top_f() : control->top_e();
-    return control->top_e() + control->top_f() - kTop - (exponents ? exponent_of_row(exponents[row], top, g ? g[row] : 1.f) : 0);
+  // What a row's sums are multiplied with: s 2^e.
+  __device__ __forceinline__ Scale scale_of(int row) const {
+    const float s = control->scale;
+    if (of == kHalf) return {s, control->top_f() - kTop};
+    if (of == kClasses) return {s, control->top_f() - kTopGradient};
+    if (!g || class_of(t, first + row) == kIgnored) return {s, control->top_e() - kTopGradient};
+    const float weight = g[row];
+    const int e = exponent(weight);
+    return {s * ldexpf(weight, -e), control->top_e() - kTopGradient + e};
   }
   // What stands there, to be added to.
   __device__ __forceinline__ floatx4 before(int row, int c) const {
@@ -526,12 +574,12 @@ struct GradientOut {
       if (i < columns - c) v[i] = p[i];
     return v;
   }
-  __device__ __forceinline__ void store(int row, int c, floatx4 v, float s, int e, const floatx4& old) const {
+  __device__ __forceinline__ void store(int row, int c, floatx4 v, const Scale& q, const floatx4& old) const {
     const size_t at = (size_t)row * columns + c;
     const int n = columns - c;
     const bool whole = n >= 4 && (at & 3) == 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = ldexpf(v[i] * s, e);
+    for (int i = 0; i < 4; ++i) v[i] = ldexpf(v[i] * q.s, q.e);
     v += old;
     if (half) {
       _Float16* p = reinterpret_cast<_Float16*>(to) + at;
@@ -566,8 +614,7 @@ __global__ __launch_bounds__(256) void lce_product(Operand a, Operand b, int M, 
   int m, n;
   tile_at(tile % blocks, (part.end - part.first + G::kM - 1) / G::kM, (N + G::kN - 1) / G::kN, &m, &n);
   const int first = split * per, count = min(per, pairs - first), m0 = part.first + m * G::kM, n0 = n * G::kN;
-  const int mine = splits == 1 && threadIdx.x < G::kM && m0 + (int)threadIdx.x < M ? out.exponent_for(m0 + threadIdx.x) : 0;
-  const float scale = out.control->scale;
+  const Scale mine = splits == 1 && threadIdx.x < G::kM && m0 + (int)threadIdx.x < M ? out.scale_of(m0 + threadIdx.x) : Scale{};
   G p;
   p.run(a, b, m0, n0, first, count, lds);
   if (splits > 1) {
@@ -580,7 +627,7 @@ __global__ __launch_bounds__(256) void lce_product(Operand a, Operand b, int M, 
     });
     return;
   }
-  int* about = reinterpret_cast<int*>(lds + G::kExtra);
+  Scale* about = reinterpret_cast<Scale*>(lds + G::kExtra);
   if (threadIdx.x < G::kM) about[threadIdx.x] = mine;
   __syncthreads();
   const auto none = [](int, int) { return 0; };
@@ -591,15 +638,15 @@ __global__ __launch_bounds__(256) void lce_product(Operand a, Operand b, int M, 
 #pragma unroll
              for (int u = 0; u < G::kAhead; ++u) {
                const int k = r + u * G::kStep;
-               if (m0 + k < M && n0 + c < N) out.store(m0 + k, n0 + c, v[u], scale, about[k], old[u]);
+               if (m0 + k < M && n0 + c < N) out.store(m0 + k, n0 + c, v[u], about[k], old[u]);
              }
            });
     return;
   }
   // of four columns all are there or none, and every four can be stored at once
   const auto scaled = [&](const floatx4& v, int k) {
-    const int e = about[k];
-    return floatx4{ldexpf(v[0] * scale, e), ldexpf(v[1] * scale, e), ldexpf(v[2] * scale, e), ldexpf(v[3] * scale, e)};
+    const Scale q = about[k];
+    return floatx4{ldexpf(v[0] * q.s, q.e), ldexpf(v[1] * q.s, q.e), ldexpf(v[2] * q.s, q.e), ldexpf(v[3] * q.s, q.e)};
   };
   const size_t corner = (size_t)m0 * out.columns + n0;
   if (out.half) {
@@ -650,7 +697,7 @@ __global__ __launch_bounds__(256) void lce_sum(const float* __restrict__ partial
 #pragma unroll 4
   for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const floatx4*>(partial + ((size_t)s * M * quads + at) * 4);
   const int row = (int)(at / quads), c = (int)(at % quads) * 4;
-  out.store(row, c, v, out.control->scale, out.exponent_for(row), out.add ? out.before(row, c) : floatx4{});
+  out.store(row, c, v, out.scale_of(row), out.add ? out.before(row, c) : floatx4{});
 }
 
 __global__ __launch_bounds__(1024) void lce_loss(const float* __restrict__ loss, Total all) {
@@ -685,6 +732,15 @@ void launch_rows(const Rows<T>& x, const Rows<T>& w, int columns, int ld) {
   const unsigned blocks_x = (unsigned)((x.rows + side - 1) / side), blocks = blocks_x + (unsigned)((w.rows + side - 1) / side);
   if (side == 4) lce_rows<T, 64><<<blocks, 256, 0, stream()>>>(x, w, blocks_x, columns, ld);
   else lce_rows<T, 256><<<blocks, 256, 0, stream()>>>(x, w, blocks_x, columns, ld);
+}
+
+int launch_again(const Rows<float>& x, const Rows<float>& w, const float* g, int columns, int ld, const Control* control) {
+  const int side = columns <= 1024 ? 4 : 1;
+  const unsigned blocks_x = (unsigned)((x.rows + side - 1) / side), blocks = blocks_x + (unsigned)((w.rows + side - 1) / side);
+  if (side == 4) lce_again<64><<<blocks, 256, 0, stream()>>>(x, w, g, blocks_x, columns, ld, control);
+  else lce_again<256><<<blocks, 256, 0, stream()>>>(x, w, g, blocks_x, columns, ld, control);
+  TT_LAUNCH_CHECK();
+  return 0;
 }
 
 // Where the tiles are not whole rounds over the compute units and few are left for the last one, the last columns (of n, m the other side)
@@ -809,6 +865,7 @@ int run(const Call& q) {
   Carve c;
   const size_t at_control = c.take(sizeof(Control)), at_f = c.take(TERMS == 2 ? 4 * N : 0), at_e = c.take(TERMS == 2 ? 4 * (size_t)(V + 256) : 0);
   const size_t at_x = c.take((size_t)N * Hp * 2 * TERMS), at_w = c.take(copy_w ? (size_t)V * Hp * 2 * TERMS : 0);
+  const size_t at_x2 = c.take(TERMS == 2 && q.dw ? (size_t)N * Hp * 4 : 0), at_w2 = c.take(TERMS == 2 && q.dx ? (size_t)V * Hp * 4 : 0);
   const size_t at_stats = c.take((size_t)chunk * blocks * 8), at_own = c.take(4 * chunk), at_of = c.take(8 * chunk);
   const size_t at_loss = c.take(4 * N), at_z = c.take(grad ? (size_t)chunk * Vp * 4 : 0);
   const size_t part_x = q.dx && plan_x.splits > 1 ? (size_t)plan_x.splits * chunk * ((H + 3) / 4) * 16 : 0;
@@ -834,6 +891,15 @@ int run(const Call& q) {
   lce_begin<<<1, 1024, 0, stream()>>>(q.t, N, mean, e, f, q.g, control);
   TT_LAUNCH_CHECK();
   const Operand w = copy_w ? Operand{base + at_w, (long long)V * ldx, ldx, kLine} : Operand{(const char*)q.w, (long long)V * H * 2, H * 2, kLine};
+  Operand w_gradient = w;
+  if constexpr (TERMS == 2) {
+    if (grad) {
+      const Rows<float> again_x = {(const float*)q.x, base + at_x2, f, q.dw ? N : 0, q.t};
+      const Rows<float> again_w = {(const float*)q.w, base + at_w2, nullptr, q.dx ? V : 0, Targets{nullptr, 0, 0, 0}};
+      if (launch_again(again_x, again_w, q.g, H, ldx, control)) return -1;
+      w_gradient.at = base + at_w2;
+    }
+  }
   const Total all = {q.reduction ? q.loss : nullptr, N, mean, control};
   // (of at most as many blocks as there are at one time: each counts itself, 9 ns of the others' time)
   const bool at_once = !several && (splits > 1 ? N : (N + 3) / 4) <= 256;
@@ -851,18 +917,21 @@ int run(const Call& q) {
     for (int r = splits > 1 ? rows : 0; r < rows; r += 65535) {
       const int some = std::min(rows - r, 65535);
       lce_gradient<TERMS><<<dim3((unsigned)((Vp / 4 + 255) / 256), some), 256, 0, stream()>>>(
-          z + (size_t)r * Vp, Vp, of + r, losses + first + r, q.g, f ? f + first + r : nullptr, e, q.t, first + r, V, control);
+          z + (size_t)r * Vp, Vp, of + r, losses + first + r, q.g, q.t, first + r, V, control);
       TT_LAUNCH_CHECK();
     }
     const Operand gradient = {(const char*)z, (long long)rows * Vp * 4, (int)(Vp * 4), TERMS == 1 ? 2 * kLine : kLine};
     if (q.dx) {
-      const GradientOut out = {(char*)q.dx + (size_t)first * H * (q.half_out ? 2 : 4), f ? f + first : nullptr, 1, q.g ? q.g + first : nullptr, control,
-                               q.half_out, 0, H};
-      if (launch_product<TERMS, false>(plan_x, gradient, w, rows, H, pairsV, partial, out)) return -1;
+      const GradientOut out = {(char*)q.dx + (size_t)first * H * (q.half_out ? 2 : 4), TERMS == 2 ? kPositions : kHalf, q.g ? q.g + first : nullptr,
+                               q.t, first, control, q.half_out, 0, H};
+      if (launch_product<TERMS, false>(plan_x, gradient, w_gradient, rows, H, pairsV, partial, out)) return -1;
     }
     if (q.dw) {
-      const GradientOut out = {several && q.half_out ? (void*)(base + at_sum) : q.dw, e, 0, nullptr, control, several ? 0 : q.half_out, first > 0, H};
-      if (launch_product<TERMS, true>(plan_w, gradient, x, V, H, (rows + depth - 1) / depth, partial, out)) return -1;
+      const GradientOut out = {several && q.half_out ? (void*)(base + at_sum) : q.dw, TERMS == 2 ? kClasses : kHalf, nullptr, q.t, first, control,
+                               several ? 0 : q.half_out, first > 0, H};
+      Operand x_gradient = x;
+      if (TERMS == 2) x_gradient.at = base + at_x2 + (size_t)first * ldx;
+      if (launch_product<TERMS, true>(plan_w, gradient, x_gradient, V, H, (rows + depth - 1) / depth, partial, out)) return -1;
     }
   }
   if (several && q.half_out && q.dw) {

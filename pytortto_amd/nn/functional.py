@@ -123,6 +123,7 @@ def linear_cross_entropy(input, weight, target, ignore_index=-100, reduction='me
     features hold, and is not counted by 'mean' (NaN, with gradients of zeros, where none is left).  A target outside the
     vocabulary gives NaN, for its loss and the gradients.  Gradients flow to ``input`` and ``weight``.
 
-    float32 products are computed from two float16 terms of every value (22 bits of it, or 2^-40 of the largest value of its row, and
-    of the largest gradient of a logit), with float32 sums."""
+    float32 products are computed from two float16 terms of every value, with float32 sums: 22 bits of it, or 2^-40 of the largest
+    value of its row (for the logits) or of its matrix (for the gradients; there ``input`` has its losses' weights on it).  softmax(z) - [v =
+    target] is held to 22 bits, or 2^-40."""
     return LinearCrossEntropy.apply(input, weight, target=target, ignore_index=ignore_index, reduction=reduction)
