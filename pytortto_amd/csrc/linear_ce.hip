@@ -3,10 +3,11 @@
 //   z = x W^T     M_i = max_v z_iv     S_i = sum_v e^(z_iv - M_i)     loss_i = ln S_i + M_i - z_i,t(i)
 //   G_iv = g_i (e^(z_iv - M_i) / S_i - [v = t(i)])        dX = G W        dW = G^T x
 //
-// Rows are worked on in chunks.  The first product leaves a chunk's logits in scratch memory (none without gradients)
+// Positions are worked on in chunks.  Their rows come into the products' form; the first product leaves a chunk's logits in scratch memory (none without gradients)
 // and, with the tile still in registers, every row's maximum and sum over a tile's columns; these are joined, and one pass turns the logits
 // into G where they stand.  The two other products read it there: G^T needs no copy, see product.h.  So a training step
-// has three products and not a fourth for logits that it forgot, and the scratch memory is bounded whatever the batch.
+// has three products and not a fourth for logits that it forgot, and the scratch memory has a bound that the batch does not move: 2 GiB of logits,
+// 2 GiB of features (twice that with gradients of float32), the weight's terms once or twice, and partial sums.
 //
 // float16: the tensors are the products' operands as they are; G is rounded to float16 once, scaled by 2^14.
 // float32: operands have two float16 terms.  For the logits row i of x and row v of W are scaled by powers of two 2^-f_i and 2^-e_v to below
@@ -25,13 +26,15 @@ using namespace tt;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr size_t kMostLogits = (size_t)2 << 30;     // bytes of a chunk's logits
 constexpr size_t kMostStats = (size_t)256 << 20;
+constexpr size_t kMostRows = (size_t)2 << 30;       // of a chunk's features in the products' form
 constexpr int kTop = 14;                            // scaled values are below 2^(kTop + 1)
 constexpr int kLowest = -1000;                      // an exponent below all
 constexpr int kAny = -2000;                         // that of a row of zeros, or with what is not finite
 constexpr int kTopGradient = 15;                    // the scale of G of float32
 
-// Set at the start of a call, read by all that follows.
+// Set at the start of a call, and most_f at that of a chunk, read by all that follows.
 struct Control {
+  double sum;           // of the losses of the chunks so far
   float scale;          // of the loss and its gradients: 1 / positions for 'mean'
   int most_e, most_f;   // the largest exponents of W's rows, and of x's rows with their g (float16: of g)
   Ticket done;
@@ -59,31 +62,38 @@ __device__ __forceinline__ int exponent(float v) {
   return e;
 }
 
-// Of float32, e and f are the exponents of W's rows and x's.  (One block, with every row's behind each other: an atomic operation of each row
-// where it is found took 9 ns of all the others, 10 us of 1064 rows.)
-__global__ __launch_bounds__(1024) void lce_begin(Targets t, long long rows, int mean, const int* __restrict__ e, const int* __restrict__ f,
-                                                  const float* __restrict__ g, Control* c) {
+// Of float32, e and f are the exponents of W's rows and of those of x in the chunk.  (One block, with every row's behind each other: an atomic
+// operation of each row where it is found took 9 ns of all the others, 10 us of 1064 rows.)
+__global__ __launch_bounds__(1024) void lce_begin(Targets t, long long positions, long long first, long long rows, int mean, const int* __restrict__ e,
+                                                  const int* __restrict__ f, const float* __restrict__ g, Control* c) {
   __shared__ long long part[16];
   __shared__ int part_e[16], part_f[16];
   long long n = 0;
   int most_e = e ? kLowest : 0, most_f = f || g ? kLowest : 0;
+  const long long end = first ? first + rows : positions;
 #pragma unroll 4
-  for (long long i = threadIdx.x; i < rows; i += 1024) {
+  for (long long i = first + threadIdx.x; i < end; i += 1024) {
     const bool kept = read_index(t.at, (size_t)i, t.wide) != t.ignore;
-    const int own = f ? f[i] : 0;
-    const float weight = g ? g[i] : 1.f;
     n += kept;
+    if (i >= first + rows) continue;
+    const int own = f ? f[i - first] : 0;
+    const float weight = g ? g[i] : 1.f;
     if (kept && own != kAny && weight != 0.f) most_f = max(most_f, g ? own + exponent(weight) : own);
+  }
+  const auto larger_int = [](int a, int b) { return max(a, b); };
+  most_f = row_reduce<1024>(most_f, part_f, larger_int);
+  if (first) {
+    if (threadIdx.x == 0) c->most_f = most_f;
+    return;
   }
   if (e) {
 #pragma unroll 8
     for (int i = threadIdx.x; i < t.V; i += 1024) most_e = max(most_e, e[i]);
   }
   n = row_sum<1024>(n, part);
-  const auto larger_int = [](int a, int b) { return max(a, b); };
   most_e = row_reduce<1024>(most_e, part_e, larger_int);
-  most_f = row_reduce<1024>(most_f, part_f, larger_int);
   if (threadIdx.x == 0) {
+    c->sum = 0.0;
     c->scale = !mean ? 1.f : n ? 1.f / (float)n : 0.f;
     c->most_e = most_e;
     c->most_f = most_f;
@@ -101,6 +111,7 @@ struct Rows {
   int* exponents;
   long long rows;
   Targets t;
+  long long first;      // target of the first row
 };
 template <typename T, int G>
 __global__ __launch_bounds__(256) void lce_rows(Rows<T> of_x, Rows<T> of_w, unsigned blocks_x, int columns, int ld) {
@@ -114,7 +125,7 @@ __global__ __launch_bounds__(256) void lce_rows(Rows<T> of_x, Rows<T> of_w, unsi
   const int lane = threadIdx.x % G, quads = (columns + 63) / 64 * 16;
   const T* x = q.from + (size_t)row * columns;
   char* y = q.to + (size_t)row * ld;
-  const bool kept = !t.at || class_of(t, row) != kIgnored, whole = columns % 4 == 0;
+  const bool kept = !t.at || class_of(t, q.first + row) != kIgnored, whole = columns % 4 == 0;
   const auto four = [&](int q) {
     typedef T Four __attribute__((ext_vector_type(4)));
     floatx4 v = {};
@@ -170,7 +181,7 @@ __global__ __launch_bounds__(256) void lce_again(Rows<float> of_x, Rows<float> o
   const int quads = (columns + 63) / 64 * 16;
   const float* x = q.from + (size_t)row * columns;
   char* y = q.to + (size_t)row * ld;
-  const bool kept = !q.t.at || class_of(q.t, row) != kIgnored, whole = columns % 4 == 0;
+  const bool kept = !q.t.at || class_of(q.t, q.first + row) != kIgnored, whole = columns % 4 == 0;
   // v 2^-first m 2^then: g's exponent is not multiplied with, so that nothing leaves the range on the way
   float m = 1.f;
   int first = 0, then = 0;
@@ -358,12 +369,12 @@ __global__ __launch_bounds__(256) void lce_logits(Operand x, Operand w, int rows
   });
 }
 
-// The loss of all positions, in the order of the positions.
+// The loss of all positions, in the order of the positions: those of a chunk are added to what the chunks in front of it have left.
 struct Total {
   float* to;            // or none
   long long n;
-  int mean;
-  const Control* control;
+  int mean, last;       // the last chunk's
+  Control* control;
 };
 template <int THREADS, typename L>
 __device__ __forceinline__ void total(const Total& q, L loss) {
@@ -371,14 +382,17 @@ __device__ __forceinline__ void total(const Total& q, L loss) {
   double s = 0.0;
   for (long long i = threadIdx.x; i < q.n; i += THREADS) s += (double)loss(i);
   s = row_sum<THREADS>(s, part);
-  if (threadIdx.x == 0) *q.to = q.mean && q.control->scale == 0.f ? NAN : (float)(s * (double)q.control->scale);
+  if (threadIdx.x) return;
+  s += q.control->sum;
+  if (!q.last) q.control->sum = s;
+  else *q.to = q.mean && q.control->scale == 0.f ? NAN : (float)(s * (double)q.control->scale);
 }
 // The same by the last of `blocks` blocks, each of which has shared some.  (Of few: a launch less.)
 __device__ __forceinline__ void total_by_last(const Total& q, const float* loss, unsigned blocks) {
   __shared__ bool last;
   stores_done();
   __syncthreads();
-  if (threadIdx.x == 0) last = last_ticket(const_cast<Ticket*>(&q.control->done), blocks);
+  if (threadIdx.x == 0) last = last_ticket(&q.control->done, blocks);
   __syncthreads();
   if (last) total<256>(q, [&](long long i) { return shared(loss + i); });
 }
@@ -728,6 +742,7 @@ int launch_scale(const float* from, const float* g, T* to, size_t n) {
 
 template <typename T>
 void launch_rows(const Rows<T>& x, const Rows<T>& w, int columns, int ld) {
+  // (of kMostRows bytes of rows and 2^20 classes: below 2^32 threads, which is all that a launch can have)
   const int side = columns <= 1024 ? 4 : 1;
   const unsigned blocks_x = (unsigned)((x.rows + side - 1) / side), blocks = blocks_x + (unsigned)((w.rows + side - 1) / side);
   if (side == 4) lce_rows<T, 64><<<blocks, 256, 0, stream()>>>(x, w, blocks_x, columns, ld);
@@ -848,9 +863,8 @@ int run(const Call& q) {
   const long long N = q.N, Hp = padded(H), Vp = padded(V);
   const bool grad = q.dx || q.dw, copy_w = TERMS == 2 || H % 8 != 0;
   const int depth = 64 / TERMS;
-  long long chunk = (long long)((grad ? kMostLogits : kMostStats) / ((size_t)Vp * (grad ? 4 : 8) / (grad ? 1 : 64)));
-  chunk = std::max(256LL, std::min(chunk, (1LL << 34) / (Hp * 2 * TERMS)) / 256 * 256);
-  chunk = std::min(chunk, N);
+  const size_t most = std::min(grad ? kMostLogits / ((size_t)Vp * 4) : kMostStats / ((size_t)Vp / 8), kMostRows / ((size_t)Hp * 2 * TERMS));
+  const long long chunk = std::min(N, std::max(256LL, (long long)most / 256 * 256));
   const bool several = chunk < N;
   const int pairsV = (int)(Vp / depth), pairsN = (int)((chunk + depth - 1) / depth);
   const int size = tile_size(chunk, V), V1 = (int)first_left(chunk, V, size), left = V1 < V ? size_left(chunk, V - V1, size) : size;
@@ -863,11 +877,11 @@ int run(const Call& q) {
   const Plan plan_x = plan_product(chunk, H, pairsV), plan_w = plan_product(V, H, pairsN);
 
   Carve c;
-  const size_t at_control = c.take(sizeof(Control)), at_f = c.take(TERMS == 2 ? 4 * N : 0), at_e = c.take(TERMS == 2 ? 4 * (size_t)(V + 256) : 0);
-  const size_t at_x = c.take((size_t)N * Hp * 2 * TERMS), at_w = c.take(copy_w ? (size_t)V * Hp * 2 * TERMS : 0);
-  const size_t at_x2 = c.take(TERMS == 2 && q.dw ? (size_t)N * Hp * 4 : 0), at_w2 = c.take(TERMS == 2 && q.dx ? (size_t)V * Hp * 4 : 0);
+  const size_t at_control = c.take(sizeof(Control)), at_f = c.take(TERMS == 2 ? 4 * chunk : 0), at_e = c.take(TERMS == 2 ? 4 * (size_t)(V + 256) : 0);
+  const size_t at_x = c.take((size_t)chunk * Hp * 2 * TERMS), at_w = c.take(copy_w ? (size_t)V * Hp * 2 * TERMS : 0);
+  const size_t at_x2 = c.take(TERMS == 2 && q.dw ? (size_t)chunk * Hp * 4 : 0), at_w2 = c.take(TERMS == 2 && q.dx ? (size_t)V * Hp * 4 : 0);
   const size_t at_stats = c.take((size_t)chunk * blocks * 8), at_own = c.take(4 * chunk), at_of = c.take(8 * chunk);
-  const size_t at_loss = c.take(4 * N), at_z = c.take(grad ? (size_t)chunk * Vp * 4 : 0);
+  const size_t at_loss = c.take(4 * chunk), at_z = c.take(grad ? (size_t)chunk * Vp * 4 : 0);
   const size_t part_x = q.dx && plan_x.splits > 1 ? (size_t)plan_x.splits * chunk * ((H + 3) / 4) * 16 : 0;
   const size_t part_w = q.dw && plan_w.splits > 1 ? (size_t)plan_w.splits * V * ((H + 3) / 4) * 16 : 0;
   const size_t part_z = splits > 1 ? (size_t)splits * chunk * Vp * 4 : 0;
@@ -879,45 +893,48 @@ int run(const Call& q) {
   Control* control = (Control*)(base + at_control);
   int *f = TERMS == 2 ? (int*)(base + at_f) : nullptr, *e = TERMS == 2 ? (int*)(base + at_e) : nullptr;
   float *z = grad ? (float*)(base + at_z) : nullptr, *partial = (float*)(base + at_part);
-  float* losses = q.reduction == 0 && q.loss ? q.loss : (float*)(base + at_loss);
   float2 *stats = (float2*)(base + at_stats), *of = (float2*)(base + at_of);
   float* own = (float*)(base + at_own);
 
   const int ldx = (int)(Hp * 2 * TERMS);
-  const Rows<T> of_x = {(const T*)q.x, base + at_x, f, N, q.t};
-  const Rows<T> of_w = {(const T*)q.w, base + at_w, e, copy_w ? V : 0, Targets{nullptr, 0, 0, 0}};
-  launch_rows<T>(of_x, of_w, H, ldx);
-  TT_LAUNCH_CHECK();
-  lce_begin<<<1, 1024, 0, stream()>>>(q.t, N, mean, e, f, q.g, control);
-  TT_LAUNCH_CHECK();
   const Operand w = copy_w ? Operand{base + at_w, (long long)V * ldx, ldx, kLine} : Operand{(const char*)q.w, (long long)V * H * 2, H * 2, kLine};
   Operand w_gradient = w;
-  if constexpr (TERMS == 2) {
-    if (grad) {
-      const Rows<float> again_x = {(const float*)q.x, base + at_x2, f, q.dw ? N : 0, q.t};
-      const Rows<float> again_w = {(const float*)q.w, base + at_w2, nullptr, q.dx ? V : 0, Targets{nullptr, 0, 0, 0}};
-      if (launch_again(again_x, again_w, q.g, H, ldx, control)) return -1;
-      w_gradient.at = base + at_w2;
-    }
-  }
-  const Total all = {q.reduction ? q.loss : nullptr, N, mean, control};
+  if (TERMS == 2) w_gradient.at = base + at_w2;
   // (of at most as many blocks as there are at one time: each counts itself, 9 ns of the others' time)
   const bool at_once = !several && (splits > 1 ? N : (N + 3) / 4) <= 256;
-  const Total by_last = at_once ? all : Total{};
   for (long long first = 0; first < N; first += chunk) {
     const int rows = (int)std::min(chunk, N - first);
-    const Operand x = {base + at_x + (size_t)first * ldx, (long long)rows * ldx, ldx, kLine};
-    const Logits logits = {f ? f + first : nullptr, e, q.t, first, z, Vp, stats, own, blocks, partial, per, splits};
+    const T* from = (const T*)q.x + (size_t)first * H;
+    const Targets none = {nullptr, 0, 0, 0};
+    launch_rows<T>({from, base + at_x, f, rows, q.t, first}, {(const T*)q.w, base + at_w, e, copy_w && first == 0 ? V : 0, none, 0}, H, ldx);
+    TT_LAUNCH_CHECK();
+    if (first == 0 || (grad && (f || q.g))) {
+      lce_begin<<<1, 1024, 0, stream()>>>(q.t, N, first, rows, mean, e, f, q.g, control);
+      TT_LAUNCH_CHECK();
+    }
+    if constexpr (TERMS == 2) {
+      const Rows<float> again_x = {from, base + at_x2, f, q.dw ? rows : 0, q.t, first};
+      const Rows<float> again_w = {(const float*)q.w, base + at_w2, nullptr, q.dx && first == 0 ? V : 0, none, 0};
+      if (again_x.rows + again_w.rows > 0 && launch_again(again_x, again_w, q.g ? q.g + first : nullptr, H, ldx, control)) return -1;
+    }
+    const Operand x = {base + at_x, (long long)rows * ldx, ldx, kLine};
+    float* losses = q.reduction == 0 && q.loss ? q.loss + first : (float*)(base + at_loss);
+    const Total all = {q.reduction ? q.loss : nullptr, rows, mean, first + rows == N, control}, by_last = at_once ? all : Total{};
+    const Logits logits = {f, e, q.t, first, z, Vp, stats, own, blocks, partial, per, splits};
     if (launch_logits<TERMS>(size, x, w, rows, V, H, logits, Part{0, V1, 0})) return -1;
     if (V1 < V && launch_logits<TERMS>(left, x, w, rows, V, H, logits, Part{V1, V, blocks1})) return -1;
     if (splits > 1) lce_few<TERMS><<<(unsigned)rows, 256, 0, stream()>>>(logits, rows, V, q.g, losses, control, by_last);
-    else lce_join<<<(unsigned)((rows + 3) / 4), 256, 0, stream()>>>(stats, own, z, Vp, of, losses + first, q.t, first, rows, blocks, by_last);
+    else lce_join<<<(unsigned)((rows + 3) / 4), 256, 0, stream()>>>(stats, own, z, Vp, of, losses, q.t, first, rows, blocks, by_last);
     TT_LAUNCH_CHECK();
+    if (all.to && !at_once) {
+      lce_loss<<<1, 1024, 0, stream()>>>(losses, all);
+      TT_LAUNCH_CHECK();
+    }
     if (!grad) continue;
     for (int r = splits > 1 ? rows : 0; r < rows; r += 65535) {
       const int some = std::min(rows - r, 65535);
       lce_gradient<TERMS><<<dim3((unsigned)((Vp / 4 + 255) / 256), some), 256, 0, stream()>>>(
-          z + (size_t)r * Vp, Vp, of + r, losses + first + r, q.g, q.t, first + r, V, control);
+          z + (size_t)r * Vp, Vp, of + r, losses + r, q.g, q.t, first + r, V, control);
       TT_LAUNCH_CHECK();
     }
     const Operand gradient = {(const char*)z, (long long)rows * Vp * 4, (int)(Vp * 4), TERMS == 1 ? 2 * kLine : kLine};
@@ -930,16 +947,12 @@ int run(const Call& q) {
       const GradientOut out = {several && q.half_out ? (void*)(base + at_sum) : q.dw, TERMS == 2 ? kClasses : kHalf, nullptr, q.t, first, control,
                                several ? 0 : q.half_out, first > 0, H};
       Operand x_gradient = x;
-      if (TERMS == 2) x_gradient.at = base + at_x2 + (size_t)first * ldx;
+      if (TERMS == 2) x_gradient.at = base + at_x2;
       if (launch_product<TERMS, true>(plan_w, gradient, x_gradient, V, H, (rows + depth - 1) / depth, partial, out)) return -1;
     }
   }
   if (several && q.half_out && q.dw) {
     if (launch_scale((float*)(base + at_sum), nullptr, (_Float16*)q.dw, (size_t)V * H)) return -1;
-  }
-  if (all.to && !at_once) {
-    lce_loss<<<1, 1024, 0, stream()>>>(losses, all);
-    TT_LAUNCH_CHECK();
   }
   return 0;
 }
