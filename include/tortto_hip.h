@@ -517,8 +517,9 @@ int tt_distill_bwd(const void* x, const void* teacher, const void* index, const 
  * gradients NaN.  A position whose target is ignore_index has loss 0 and no gradient, whatever its features hold.  reduction: 0 none
  * (loss [N]), 1 sum, 2 mean over the positions that are not ignored (NaN, with gradients of zeros, if there are none); the
  * gradients have the reduction's scale.  g [N] or NULL: 1.  loss, dx and dw may each be NULL.  dx [N, H] and dw [V, H] are
- * float32, or float16 where half_gradients says so.  Products of float32 are of two float16 terms a value, scaled by powers
- * of two; an infinity among them gives NaN.  No counterpart in the reference. */
+ * float32, or float16 where half_gradients says so.  A position with a logit of NaN or +inf, or with none but -inf, has a loss and
+ * gradients of NaN.  Products of float32 are of two float16 terms a value, scaled by powers of two; an infinity among them
+ * gives NaN.  No counterpart in the reference. */
 int tt_linear_cross_entropy(const void* x, const void* w, const void* target, const float* g, float* loss, void* dx,
                             void* dw, int dtype, int half_gradients, int index_bits, long long ignore_index,
                             int reduction, long long N, int H, int V);

@@ -397,6 +397,9 @@ __device__ __forceinline__ void total_by_last(const Total& q, const float* loss,
   if (last) total<256>(q, [&](long long i) { return shared(loss + i); });
 }
 
+// The logarithm of a row's sum, without its largest term in `rest`.  With a logit of +inf, or none but -inf, there is none: inf - inf.
+__device__ __forceinline__ float log_of_sum(float most, float rest) { return __builtin_isinf(most) ? NAN : log1pf(rest); }
+
 // A row's maximum and log2 of its sum from those of its blocks, and its loss.  A wave has a row.  The sum is kept without the
 // largest term, which is 1: of a target that has nearly all of the probability, the loss is what is left, and keeps its digits.
 __device__ __forceinline__ void join_row(const float2* __restrict__ stats, const float* __restrict__ own, const float* __restrict__ z, long long ld,
@@ -421,7 +424,7 @@ __device__ __forceinline__ void join_row(const float2* __restrict__ stats, const
   }
   rest = lanes_reduce<64>(rest, Plus()) + (float)(lanes_reduce<64>(largest, Plus()) - 1);
   if (lane == 0) {
-    const float log_sum = log1pf(rest);
+    const float log_sum = log_of_sum(most, rest);
     of[r] = make_float2(from, log_sum * kLog2e);
     share(loss + r, target == kInvalid ? NAN : log_sum + (from - (z ? z[(size_t)r * ld + target] : own[r])));
   }
@@ -529,7 +532,7 @@ __device__ __forceinline__ void few_row(const Logits& q, int rows, int V, const 
     for (int k = 0; k < kKept; ++k) add(kept[k], threadIdx.x + k * 256);
     for (int k = threadIdx.x + kKept * 256; k < quads; k += 256) add(logits(k), k);
     const float rest = row_sum<256>(sum, part[1]) + (float)(row_sum<256>(largest, reinterpret_cast<int*>(part[2])) - 1);
-    const float log_sum = log1pf(rest), mine = target == kInvalid ? NAN : log_sum + (from - own);
+    const float log_sum = log_of_sum(most, rest), mine = target == kInvalid ? NAN : log_sum + (from - own);
     if (threadIdx.x == 0) share(loss + r, mine);
     if (!z) return;
     const float factor = factor_of<TERMS>(control, g, r);

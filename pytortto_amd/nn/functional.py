@@ -121,7 +121,8 @@ def linear_cross_entropy(input, weight, target, ignore_index=-100, reduction='me
 
     Negative targets count from the end.  A position whose target is ``ignore_index`` has loss 0 and no gradient, whatever its
     features hold, and is not counted by 'mean' (NaN, with gradients of zeros, where none is left).  A target outside the
-    vocabulary gives NaN, for its loss and the gradients.  Gradients flow to ``input`` and ``weight``.
+    vocabulary gives NaN, for its loss and the gradients, and so does a NaN among a position's logits, one of +inf, or none but -inf; a
+    class at -inf has no probability.  Gradients flow to ``input`` and ``weight``.
 
     float32 products are computed from two float16 terms of every value, with float32 sums: 22 bits of it, or 2^-40 of the largest
     value of its row (for the logits) or of its matrix (for the gradients; there ``input`` has its losses' weights on it).  softmax(z) - [v =
