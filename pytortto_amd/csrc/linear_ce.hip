@@ -900,7 +900,8 @@ int run(const Call& q) {
   float* own = (float*)(base + at_own);
 
   const int ldx = (int)(Hp * 2 * TERMS);
-  const Operand w = copy_w ? Operand{base + at_w, (long long)V * ldx, ldx, kLine} : Operand{(const char*)q.w, (long long)V * H * 2, H * 2, kLine};
+  const Operand w = copy_w ? Operand{base + at_w, (long long)V * ldx, ldx, kLine}
+                           : Operand{(const char*)q.w, (long long)V * H * 2, H * 2, kLine, H % 64 ? H / 64 : -1, H % 64 / 8};
   Operand w_gradient = w;
   if (TERMS == 2) w_gradient.at = base + at_w2;
   // (of at most as many blocks as there are at one time: each counts itself, 9 ns of the others' time)

@@ -40,19 +40,24 @@ constexpr int kLine = 128;                      // bytes of 64 columns of one te
 constexpr int kTermBytes = 64;                  // of one term of 32 columns
 
 // `bytes` from `at` to the end of the last row; `ld` bytes from row to row, `block` from one line of 128 bytes to the next.
-// All are multiples of sixteen, and a tile's rows times ld stay below 2^31 (checked on the host).
+// All are multiples of sixteen, and a tile's rows times ld stay below 2^31 (checked on the host).  Rows end in zeros up to a whole line, or, of the
+// second operand of a product of one term with k along both, in the next row: of their line number `cut` the first `kept` pieces of sixteen bytes
+// are theirs, and the others are not read.
 struct Operand {
   const char* at;
   long long bytes;
   int ld, block;
+  int cut = -1, kept = 0;
 };
 
 template <typename T>
 using lds_ptr = __attribute__((address_space(3))) T*;
 
-// Brings a tile's share of one operand to LDS: of a pair, ROWS / 2 rows (or, where k goes across, columns) a unit.
-template <int TERMS, bool ACROSS, int ROWS, int THREADS>
+// Brings a tile's share of one operand to LDS: of a pair, ROWS / 2 rows (or, where k goes across, columns) a unit.  CUT: its rows may end in
+// the next (read against zeros of the other operand, a value that is not finite there would make NaN of this row).
+template <int TERMS, bool ACROSS, int ROWS, int THREADS, bool CUT = false>
 struct Fetch {
+  static_assert(!CUT || (TERMS == 1 && !ACROSS), "rows of one term");
   static constexpr int kHalf = ROWS / 2, kLoads = kHalf * 8 / THREADS;
   static_assert(kLoads * THREADS == kHalf * 8, "whole loads");
   static constexpr int kColumns = kLine / 2 / TERMS;            // of a line
@@ -62,6 +67,7 @@ struct Fetch {
   const char* at;
   int left;                 // from there to the end, by sixteen bytes: 2^35 bytes at most (checked on the host)
   int bytes[2];             // what may be read of either unit
+  int until, kept;          // CUT: pairs to the last of the row, and what it has of it
 
   // A unit holds its rows of 128 bytes one after the other, with the sixteen bytes c of row r at place c ^ (r % 8); or its rows of k, with
   // the 32-byte piece u (sixteen columns of a term) at place u ^ piece_mask(k), which differs among the rows that sixteen lanes read together.
@@ -95,6 +101,18 @@ struct Fetch {
         offset[i] = (unsigned)(row * ld + c * 16);
       }
     }
+    if (CUT) {
+      until = o.cut - pair;
+      kept = o.kept;
+      if (until == 0) cut();
+    }
+  }
+  // What is behind the row is out of what may be read.  (A lane has the same sixteen bytes of a line in all of its loads.)
+  __device__ __forceinline__ void cut() {
+    const int lane = threadIdx.x & 63;
+    if (((lane & 7) ^ (lane >> 3)) < kept) return;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) offset[i] = 0x80000000u;
   }
 
   __device__ __forceinline__ void measure() {
@@ -118,6 +136,7 @@ struct Fetch {
     at += step;
     left = more ? left - (int)(step >> 4) : 0;
     measure();
+    if (CUT && --until == 0) cut();
   }
 };
 
@@ -157,7 +176,7 @@ struct Product {
   static constexpr int kM = 2 * MT * 16, kN = 2 * NT * 16, kThreads = 256;
   static constexpr int kUnits = 2 * AHEAD + 1, kUnit = (kM + kN) * 64, kLds = kUnits * kUnit;
   typedef Fetch<TERMS, A_ACROSS, kM, kThreads> FetchA;
-  typedef Fetch<TERMS, B_ACROSS, kN, kThreads> FetchB;
+  typedef Fetch<TERMS, B_ACROSS, kN, kThreads, TERMS == 1 && !A_ACROSS && !B_ACROSS> FetchB;
   static constexpr int kReads = MT + NT, kAll = MT * NT, kLoads = FetchA::kLoads + FetchB::kLoads;
 
   // Lane l's acc[i][j] are D[row() + 16 i][column() + 16 j + 0 .. 3].  (The fragments change places in the instruction:

@@ -95,3 +95,26 @@ def test_no_class_at_all(rows, width, vocab):
     w[:, 0] = -np.inf
     x[:, 0] = 1.0
     assert np.isnan(_losses(x, w, target)).all()
+
+
+@pytest.mark.parametrize('rows,width,vocab', [(1, 8, 5), (3, 72, 70), (40, 2056, 300), (9, 1000, 33000), (300, 200, 4100), (1100, 56, 9000),
+                                              (2048, 72, 4200), (2048, 184, 4321), (513, 248, 30000)])
+def test_rows_of_float16_that_end_inside_a_line(rows, width, vocab):
+    """A weight's row ends where the next begins, which may begin with what is not finite: the same bits as of rows with zeros behind them."""
+    x, w, target = _inputs(rows, width, vocab, np.float16)
+    x[:, 0] = 1.0
+    w[2::5, 0] = -np.inf
+    target[target % 5 == 2] -= 1
+    more = (0, -width % 64)
+    got, want = _losses(x, w, target), _losses(np.pad(x, ((0, 0), more)), np.pad(w, ((0, 0), more)), target)
+    assert np.isfinite(want).all()
+    np.testing.assert_array_equal(got, want)
+    # a finite weight's gradients, too
+    w[2::5, 0] = 0.5
+    results = []
+    for a, b in ((x, w), (np.pad(x, ((0, 0), more)), np.pad(w, ((0, 0), more)))):
+        xt, wt = _tensor(a, True), _tensor(b, True)
+        F.linear_cross_entropy(xt, wt, _tensor(target)).backward()
+        results.append((xt.grad.get()[:, :width].astype(np.float64), wt.grad.get()[:, :width].astype(np.float64)))
+    for one, other in zip(*results):
+        assert np.abs(one - other).max() <= 2.0 ** -10 * np.abs(other).max() + 2.0 ** -24
