@@ -26,7 +26,8 @@ using namespace tt;
 constexpr int kMost = 48;                   // matrices of a launch (their table is a kernel's argument)
 constexpr size_t kMostScratch = (size_t)4 << 30;
 constexpr size_t kMostPartial = (size_t)1 << 30;
-constexpr float kUp = 16384.f;              // the scale of X and A
+constexpr int kUpBits = 14;
+constexpr float kUp = 1 << kUpBits;         // the scale of X and A
 constexpr int kParts = 1024;                // partial sums of a matrix's squares, at most
 constexpr int kJoin = 64;                   // columns of what a block of muon_join works on
 
@@ -76,13 +77,28 @@ __host__ __device__ inline int parts_of(size_t n) { return n > (size_t)kParts * 
 
 struct Rule {
   float a, b, c;
-  float eps;
+  double eps;
   float mix;                        // 1 - momentum
   float keep;                       // 1 - learning rate times weight decay
   int nesterov, half, step;
 };
 
 __device__ __forceinline__ float update_of(const Rule& q, float g, float m) { return q.nesterov ? m - q.mix * (m - g) : m; }
+
+// kUp / max(|u|_F, eps) for a sum of squares, as 2^e m with m in (1, 2]: the quotient itself would leave float32's range for norms below 5e-35, and
+// lose digits above 8e37.
+struct Inverse {
+  int e;
+  float m;
+  __device__ __forceinline__ Inverse(double squares, double eps) {
+    const double norm = sqrt(squares), by = norm > eps || norm != norm ? norm : eps;
+    int k = 0;
+    const double part = __builtin_isfinite(by) ? frexp(by, &k) : by;
+    e = kUpBits - k;
+    m = (float)(1.0 / part);
+  }
+  __device__ __forceinline__ float operator()(float u) const { return ldexpf(u, e) * m; }
+};
 
 // n values of an array from value i on, n = 4 where the array and i allow it.
 template <typename T>
@@ -154,8 +170,7 @@ __global__ __launch_bounds__(256) void muon_scale(Batch b, Rule q) {
   double s = 0.0;
   for (int i = threadIdx.x; i < parts; i += 256) s += p.parts(x.scratch)[i];
   s = row_sum<256>(s, part);
-  const double norm = sqrt(s);
-  const float inverse = (float)(1.0 / (norm > (double)q.eps || norm != norm ? norm : (double)q.eps)) * kUp;
+  const Inverse inverse(s, q.eps);
   const size_t quads = padded(x.columns) / 4, all = (size_t)x.rows * quads;
   const bool aligned = all_aligned(x) && x.columns % 4 == 0;
   size_t k = (size_t)(blockIdx.x - b.first[at]) * kScaled + threadIdx.x;
@@ -172,7 +187,7 @@ __global__ __launch_bounds__(256) void muon_scale(Batch b, Rule q) {
         for (int e = 0; e < 4; ++e) u[e] = update_of(q, u[e], m[e]);
       }
     }
-    store_terms(x.scratch + row * p.ldx, c, u * inverse);
+    store_terms(x.scratch + row * p.ldx, c, floatx4{inverse(u[0]), inverse(u[1]), inverse(u[2]), inverse(u[3])});
   }
 }
 
@@ -494,8 +509,7 @@ __global__ __launch_bounds__(256) void muon_small(Batch b, Rule q, int steps) {
     s += (double)u * (double)u;
   }
   s = row_sum<256>(s, part);
-  const double norm = sqrt(s);
-  const float inverse = (float)(1.0 / (norm > (double)q.eps || norm != norm ? norm : (double)q.eps)) * kUp;
+  const Inverse inverse(s, q.eps);
   for (int i = threadIdx.x; i < kShort * (ld / 16); i += 256) reinterpret_cast<floatx4*>(X)[i] = floatx4{};
   __syncthreads();
   for (int i = threadIdx.x; i < size; i += 256) {
@@ -503,7 +517,7 @@ __global__ __launch_bounds__(256) void muon_small(Batch b, Rule q, int steps) {
     int row, column;
     place(i, &row, &column);
     _Float16 hi, lo;
-    split(u * inverse, &hi, &lo);
+    split(inverse(u), &hi, &lo);
     char* p = X + row * ld + at_column(column);
     *reinterpret_cast<_Float16*>(p) = hi;
     *reinterpret_cast<_Float16*>(p + kTermBytes) = lo;
@@ -705,7 +719,7 @@ int tt_orthogonalize(const void* x, void* out, int kind, int rows, int columns, 
   Batch batch = {};
   batch.count = 1;
   batch.of[0] = Matrix{x, nullptr, out, nullptr, nullptr, 0.f, rows, columns, 1};
-  const Rule q = {(float)a, (float)b, (float)c, (float)eps, 0.f, 0.f, 0, kind, 0};
+  const Rule q = {(float)a, (float)b, (float)c, eps, 0.f, 0.f, 0, kind, 0};
   return is_small(rows, columns) ? run_small(batch, q, steps) : run(batch, q, steps);
 } catch (const std::exception& e) {
   return tt::fail(-1, "orthogonalize: %s", e.what());
@@ -731,7 +745,7 @@ int tt_muon_step_multi_f32(int count, float* const* params, const float* const* 
     const bool first = is_small(rows[i], columns[i]), second = is_small(rows[j], columns[j]);
     return first != second ? second : (long long)rows[i] * columns[i] > (long long)rows[j] * columns[j];
   });
-  const Rule q = {(float)a, (float)b, (float)c, (float)eps, (float)(1.0 - momentum), (float)(1.0 - lr * weight_decay), nesterov, 0, 0};
+  const Rule q = {(float)a, (float)b, (float)c, eps, (float)(1.0 - momentum), (float)(1.0 - lr * weight_decay), nesterov, 0, 0};
   for (size_t done = 0; done < order.size();) {
     Batch batch = {};
     size_t bytes = 0;

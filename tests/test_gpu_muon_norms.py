@@ -1,0 +1,52 @@
+"""GPU: ``optim.orthogonalize`` and ``optim.Muon`` where a matrix's norm, or eps, is near the ends of float32's range or past them."""
+import numpy as np
+import pytest
+
+import pytortto_amd as tt
+from pytortto_amd.xparray import hiparray
+from tests.test_gpu_muon import _compare, _matrix, _tensor
+
+pytestmark = pytest.mark.gpu
+# one block's LDS, and several blocks
+SIZES = [(20, 30), (64, 384), (70, 70), (300, 130)]
+
+
+@pytest.mark.parametrize('rows,columns', SIZES)
+@pytest.mark.parametrize('scale', [1e-44, 1e-40, 1e-38, 1e-35, 1e-33, 1e33, 1e36, 1e38])
+def test_any_norm(scale, rows, columns):
+    """(Values of 1e-44 are a few units of the smallest float32.)"""
+    x = np.clip(_matrix(rows, columns, np.float64, scale=1.0) * scale, -3e38, 3e38).astype(np.float32)
+    assert x.any() and np.isfinite(x).all()
+    _compare(x, eps=1e-300)
+    if scale < 1e-30:
+        _compare(x, eps=1e-33)
+
+
+@pytest.mark.parametrize('rows,columns', SIZES)
+@pytest.mark.parametrize('eps', [5e-324, 1e-300, 1e-46, 1e-45, 1e-40, 1e-36, 1e-20, 1e30])
+def test_zeros_stay_zeros(eps, rows, columns):
+    for dtype in (np.float32, np.float16):
+        got = tt.optim.orthogonalize(_tensor(np.zeros((rows, columns), dtype)), eps=eps).data.get()
+        assert not got.any()
+
+
+@pytest.mark.parametrize('eps', [5e-324, 1e-40, 1e-36, 1e-7])
+def test_a_parameter_without_a_gradient_keeps_its_values(eps):
+    """All gradients are zeros, as those of a part that is not used: the decay is all that a step does."""
+    values = [np.random.default_rng(i).standard_normal(s).astype(np.float32) for i, s in enumerate(SIZES)]
+    leaves = [_tensor(v, True) for v in values]
+    opt = tt.optim.Muon(leaves, lr=0.5, weight_decay=0.125, eps=eps)
+    for leaf in leaves:
+        leaf.grad = hiparray(np.zeros(leaf.shape, np.float32))
+    opt.step()
+    for leaf, v in zip(leaves, values):
+        np.testing.assert_array_equal(leaf.data.get(), v * np.float32(1 - 0.5 * 0.125))
+
+
+@pytest.mark.parametrize('rows,columns', SIZES)
+def test_what_is_not_finite_is_nan_for_any_eps(rows, columns):
+    for value in (np.nan, np.inf, -np.inf):
+        for eps in (5e-324, 1e-7, 1e30):
+            x = _matrix(rows, columns)
+            x[3, 4] = value
+            assert np.isnan(tt.optim.orthogonalize(_tensor(x), eps=eps).data.get()).all()
