@@ -556,7 +556,9 @@ int tt_adam_step_multi_f32(int count, float* const* params, const float* const* 
 
 /* One step of Muon in place, for `count` matrices [rows, columns] of one group: momentum <- momentum + (1 - mu)(grad -
  * momentum); u = the momentum, or with nesterov grad + mu (momentum - grad); param <- param (1 - lr weight_decay) - lr
- * scale O(u), O as tt_orthogonalize has it.  No counterpart in the reference. */
+ * scale O(u), O as tt_orthogonalize has it.  All that may be refused, and the scratch memory, comes before the first launch;
+ * with params NULL (grads and momenta are not read then) that is all that happens, so that a step of several calls can ask for
+ * everything first.  No counterpart in the reference. */
 int tt_muon_step_multi_f32(int count, float* const* params, const float* const* grads, float* const* momenta,
                            const int* rows, const int* columns, const double* scales, double lr, double momentum,
                            double weight_decay, int nesterov, int steps, double a, double b, double c, double eps);

@@ -624,25 +624,40 @@ int launch_join(bool strips, const Batch& b, const Rule& q) {
 }
 
 // ---- batches ---------------------------------------------------------------------------------------
-// The matrices of one batch, all steps.
-int run(Batch& gram, Rule q, int steps) {
-  Batch polynomial = gram, update = gram;
-  const int gram_size = plan<kGram>(gram), polynomial_size = plan<kPolynomial>(polynomial), update_size = plan<kUpdate>(update);
-  const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  size_t bytes = 0;
-  for (int i = 0; i < gram.count; ++i) {
-    const Place p(gram.of[i].rows, gram.of[i].columns);
-    bytes += up(p.bytes()) + up((size_t)std::max(gram.of[i].splits, polynomial.of[i].splits) * p.square() * 4);
-  }
+// The matrices of one batch, with the plans of their products.
+struct Work {
+  Batch gram, polynomial, update;       // (of small ones the first alone)
+  int gram_size, polynomial_size, update_size;
+  bool small;
+  size_t bytes;                         // of scratch memory
+};
+size_t up(size_t n) { return (n + 255) / 256 * 256; }
+size_t partial_bytes(const Work& w, int i) {
+  const Matrix& x = w.gram.of[i];
+  return up((size_t)std::max(x.splits, w.polynomial.of[i].splits) * Place(x.rows, x.columns).square() * 4);
+}
+Work prepare(const Batch& batch, bool small) {
+  Work w = {batch, batch, batch, 0, 0, 0, small, 0};
+  if (small) return w;
+  w.gram_size = plan<kGram>(w.gram);
+  w.polynomial_size = plan<kPolynomial>(w.polynomial);
+  w.update_size = plan<kUpdate>(w.update);
+  for (int i = 0; i < batch.count; ++i) w.bytes += up(Place(batch.of[i].rows, batch.of[i].columns).bytes()) + partial_bytes(w, i);
+  return w;
+}
+
+// All steps of a batch.
+int run(Work& w, Rule q, int steps) {
+  if (w.small) return run_small(w.gram, q, steps);
+  Batch &gram = w.gram, &polynomial = w.polynomial, &update = w.update;
   void* ws;
-  if (tt::workspace(bytes, &ws)) return -1;
+  if (tt::workspace(w.bytes, &ws)) return -1;
   char* at = (char*)ws;
   for (int i = 0; i < gram.count; ++i) {
-    const Place p(gram.of[i].rows, gram.of[i].columns);
     gram.of[i].scratch = polynomial.of[i].scratch = update.of[i].scratch = at;
-    at += up(p.bytes());
+    at += up(Place(gram.of[i].rows, gram.of[i].columns).bytes());
     gram.of[i].partial = polynomial.of[i].partial = (float*)at;
-    at += up((size_t)std::max(gram.of[i].splits, polynomial.of[i].splits) * p.square() * 4);
+    at += partial_bytes(w, i);
   }
   Batch begin = gram, rows = gram, gram_join = gram, polynomial_join = polynomial;
   begin.first[0] = rows.first[0] = gram_join.first[0] = polynomial_join.first[0] = 0;
@@ -659,11 +674,11 @@ int run(Batch& gram, Rule q, int steps) {
   muon_scale<<<rows.first[rows.count], 256, 0, stream()>>>(rows, q);
   TT_LAUNCH_CHECK();
   for (q.step = 0; q.step < steps; ++q.step) {
-    if (launch<kGram>(gram_size, gram, q, 0)) return -1;
+    if (launch<kGram>(w.gram_size, gram, q, 0)) return -1;
     if (launch_join<kGram>(strips, gram_join, q)) return -1;
-    if (launch<kPolynomial>(polynomial_size, polynomial, q, 0)) return -1;
+    if (launch<kPolynomial>(w.polynomial_size, polynomial, q, 0)) return -1;
     if (launch_join<kPolynomial>(strips, polynomial_join, q)) return -1;
-    if (launch<kUpdate>(update_size, update, q, q.step == steps - 1)) return -1;
+    if (launch<kUpdate>(w.update_size, update, q, q.step == steps - 1)) return -1;
   }
   return 0;
 }
@@ -720,7 +735,8 @@ int tt_orthogonalize(const void* x, void* out, int kind, int rows, int columns, 
   batch.count = 1;
   batch.of[0] = Matrix{x, nullptr, out, nullptr, nullptr, 0.f, rows, columns, 1};
   const Rule q = {(float)a, (float)b, (float)c, eps, 0.f, 0.f, 0, kind, 0};
-  return is_small(rows, columns) ? run_small(batch, q, steps) : run(batch, q, steps);
+  Work work = prepare(batch, is_small(rows, columns));
+  return run(work, q, steps);
 } catch (const std::exception& e) {
   return tt::fail(-1, "orthogonalize: %s", e.what());
 }
@@ -732,12 +748,12 @@ int tt_muon_step_multi_f32(int count, float* const* params, const float* const* 
   const char* fn = "muon_step";
   TT_REQUIRE(count >= 0, "%s: negative count", fn);
   if (count == 0) return 0;
-  TT_REQUIRE(params && grads && momenta && rows && columns && scales, "%s: null table", fn);
+  TT_REQUIRE((!params || (grads && momenta)) && rows && columns && scales, "%s: null table", fn);
   if (check(fn, a, b, c, eps, steps)) return -1;
   std::vector<int> order;
   for (int i = 0; i < count; ++i) {
     if (check(fn, rows[i], columns[i])) return -1;
-    TT_REQUIRE(params[i] && grads[i] && momenta[i], "%s: null pointer for matrix %d", fn, i);
+    TT_REQUIRE(!params || (params[i] && grads[i] && momenta[i]), "%s: null pointer for matrix %d", fn, i);
     order.push_back(i);
   }
   // (large ones first: the last blocks of a launch are then small ones', and those of one block each come last)
@@ -746,6 +762,8 @@ int tt_muon_step_multi_f32(int count, float* const* params, const float* const* 
     return first != second ? second : (long long)rows[i] * columns[i] > (long long)rows[j] * columns[j];
   });
   const Rule q = {(float)a, (float)b, (float)c, eps, (float)(1.0 - momentum), (float)(1.0 - lr * weight_decay), nesterov, 0, 0};
+  std::vector<Work> works;
+  size_t most = 0;
   for (size_t done = 0; done < order.size();) {
     Batch batch = {};
     size_t bytes = 0;
@@ -756,9 +774,18 @@ int tt_muon_step_multi_f32(int count, float* const* params, const float* const* 
       const size_t more = (size_t)Place(rows[i], columns[i]).bytes();
       if (batch.count && bytes + more > kMostScratch) break;
       bytes += more;
-      batch.of[batch.count++] = Matrix{grads[i], momenta[i], params[i], nullptr, nullptr, (float)(lr * scales[i]), rows[i], columns[i], 1};
+      batch.of[batch.count++] = params ? Matrix{grads[i], momenta[i], params[i], nullptr, nullptr, (float)(lr * scales[i]), rows[i], columns[i], 1}
+                                       : Matrix{nullptr, nullptr, nullptr, nullptr, nullptr, 0.f, rows[i], columns[i], 1};
     }
-    if (small ? run_small(batch, q, steps) : run(batch, q, steps)) return -1;
+    works.push_back(prepare(batch, small));
+    most = std::max(most, works.back().bytes);
+  }
+  // (the largest batch's memory before the first batch moves anything)
+  void* ws;
+  if (most && tt::workspace(most, &ws)) return -1;
+  if (!params) return 0;
+  for (Work& work : works) {
+    if (run(work, q, steps)) return -1;
   }
   return 0;
 } catch (const std::exception& e) {

@@ -1,16 +1,19 @@
 """The update rules (``src/tortto/optim/_functional.py``) as fused kernels, a group's parameters in a few launches.
 Device parameters only: host tensors belong to tortto's NumPy path and are refused."""
 import ctypes
+from math import prod
 
 import numpy as np
 
 from .. import _hip, ops
 from ..xparray import hiparray
 
+_F32 = np.dtype(np.float32)
+
 
 def _device(param, *arrays):
     for a in (param.data,) + arrays:
-        if a is not None and (a.__class__ is not hiparray or a.dtype != np.float32):
+        if a is not None and (a.__class__ is not hiparray or a._dtype != _F32):
             raise RuntimeError('the optimisers of pytortto_amd update float32 device parameters only; move the model '
                                'with .cuda() first')
 
@@ -67,35 +70,48 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, max_exp_avg_sqs, state_steps, am
           weight_decay, eps, True)
 
 
-def muon(params, grads, momenta, lr, momentum, weight_decay, nesterov, steps, coefficients, eps, adjust):
-    """The matrices of a group share their launches.  Parameters of more than two dimensions are matrices of their first and the
-    others (a convolution's output channels and its taps)."""
-    while params:
-        for param, g, m in zip(params, grads, momenta):
-            _device(param, g, m)
-            if g.shape != param.data.shape or m.shape != param.data.shape:
-                raise RuntimeError(f'a gradient and a momentum are of their parameter\'s shape {param.data.shape}, got {g.shape} '
-                                   f'and {m.shape}')
-        # (one that comes twice is stepped twice, one after the other)
-        seen, now, later = set(), [], []
-        for i, param in enumerate(params):
-            (later if id(param) in seen else now).append(i)
-            seen.add(id(param))
-        for i in now:               # written in place: nothing may still depend on the old values
-            params[i].data.own()
-            momenta[i].own()
-        count = len(now)
-        rows = [params[i].data.shape[0] for i in now]
-        columns = [params[i].data.size // r if r else 0 for i, r in zip(now, rows)]
-        for r, c in zip(rows, columns):
-            ops._check_products('muon', (r, ops.MOST_ROWS, 'rows'), (c, ops.MOST_ROWS, 'columns'))
-        whole = [k for k in range(count) if rows[k] and columns[k]]
-        count, now = len(whole), [now[k] for k in whole]
-        rows, columns = [rows[k] for k in whole], [columns[k] for k in whole]
-        if count:
+def muon_matrix(param, grad, momentum):
+    """(rows, columns) of a parameter, the first dimension and all others (a convolution's output channels and its taps), whose gradient
+    and momentum (or None, of a first step) fit it, and that fits the kernels (the C ABI takes ints)."""
+    _device(param, grad, momentum)
+    shape = param.data._shape
+    if grad._shape != shape or (momentum is not None and momentum._shape != shape):
+        raise RuntimeError(f"a gradient and a momentum are of their parameter's shape {shape}, got {grad._shape}"
+                           + ('' if momentum is None else f' and {momentum._shape}'))
+    rows, columns = shape[0], prod(shape[1:])
+    if rows > ops.MOST_ROWS or columns > ops.MOST_ROWS or rows * columns > 1 << 32:
+        ops._check_products('muon', (rows, ops.MOST_ROWS, 'rows'), (columns, ops.MOST_ROWS, 'columns'), (rows * columns, 1 << 32, 'values'))
+    return rows, columns
+
+
+def muon(groups):
+    """The matrices of a group share their launches.  ``groups`` holds (params, grads, momenta, matrices, adjust, arguments) of each,
+    the matrices as ``muon_matrix`` has them.  What the library may refuse, and all memory, comes before the first parameter moves: a step
+    that fails can be made again."""
+    for params, _, momenta, _, _, _ in groups:
+        for param, m in zip(params, momenta):       # written in place: nothing may still depend on the old values
+            param.data.own()
+            m.own()
+    calls = []
+    for params, grads, momenta, matrices, adjust, arguments in groups:
+        rest = [k for k, (rows, columns) in enumerate(matrices) if rows and columns]
+        while rest:
+            now, later = rest, []
+            if len(set(map(id, params))) != len(params):
+                # (one that comes twice is stepped twice, one after the other)
+                seen, now = set(), []
+                for k in rest:
+                    (later if id(params[k]) in seen else now).append(k)
+                    seen.add(id(params[k]))
+            count = len(now)
             pointers, ints = ctypes.c_void_p * count, ctypes.c_int * count
-            _hip.call('tt_muon_step_multi_f32', count, pointers(*[params[i].data.ptr for i in now]),
-                      pointers(*[grads[i].ptr for i in now]), pointers(*[momenta[i].ptr for i in now]), ints(*rows),
-                      ints(*columns), (ctypes.c_double * count)(*[adjust(r, c) for r, c in zip(rows, columns)]), lr, momentum,
-                      weight_decay, int(bool(nesterov)), steps, *coefficients, eps)
-        params, grads, momenta = ([some[i] for i in later] for some in (params, grads, momenta))
+            tables = (pointers(*[params[k].data.ptr for k in now]), pointers(*[grads[k].ptr for k in now]),
+                      pointers(*[momenta[k].ptr for k in now]))
+            calls.append((count, tables, (ints(*[matrices[k][0] for k in now]), ints(*[matrices[k][1] for k in now]),
+                                          (ctypes.c_double * count)(*[adjust(*matrices[k]) for k in now]), *arguments)))
+            rest = later
+    if len(calls) > 1:
+        for count, _, arguments in calls:       # (without tables: the scratch memory that the call will need)
+            _hip.call('tt_muon_step_multi_f32', count, None, None, None, *arguments)
+    for count, tables, arguments in calls:
+        _hip.call('tt_muon_step_multi_f32', count, *tables, *arguments)

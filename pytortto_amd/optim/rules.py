@@ -2,6 +2,9 @@
 checks and per-parameter state of the reference; the arithmetic is one kernel launch per parameter
 (``_functional.py`` here).  ``Muon`` and ``orthogonalize`` are not in the reference."""
 import math
+from functools import lru_cache
+
+import numpy as np
 
 from .. import ops
 from ..tensor import Tensor
@@ -93,6 +96,20 @@ def _coefficients(values):
     return values
 
 
+@lru_cache(maxsize=64)
+def _grow(a, b, c, steps):
+    """Whether coefficients let a singular value out of [0, 1], or what a step multiplies it with, out of the kernels' range."""
+    s = np.arange(4097) / 4096.0
+    with np.errstate(all='ignore'):
+        for _ in range(steps):
+            p = b * (s * s) + c * (s * s) * (s * s)
+            grows = not (np.abs(p) <= 15.0).all() or not (np.abs(a + p) <= 15.0).all()
+            s = s * (a + p)
+            if grows or not (np.abs(s) <= 1.9).all():
+                return True
+    return False
+
+
 def orthogonalize(matrix, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     """The nearest semi-orthogonal matrix, roughly: X / max(|X|, eps) (Frobenius norm), then ``steps`` times
     X <- a X + b (X X^T) X + c (X X^T)^2 X, which brings singular values to about 1 and leaves the singular vectors.  ``matrix`` [rows,
@@ -124,30 +141,47 @@ class Muon(Optimizer):
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_coefficients=COEFFICIENTS, eps=1e-7,
                  ns_steps=5, adjust_lr_fn='original'):
-        _check(lr >= 0.0, 'Invalid learning rate: {}', lr)
-        _check(0.0 <= momentum < 1.0, 'Invalid momentum value: {}', momentum)
-        _check(weight_decay >= 0.0, 'Invalid weight_decay value: {}', weight_decay)
-        _check(0.0 < eps <= 1e30, 'Invalid epsilon value: {}', eps)
-        _check(ns_steps.__class__ is int and 1 <= ns_steps <= 100, 'Invalid number of steps: {}', ns_steps)
-        _check(adjust_lr_fn in _ADJUST, 'Invalid adjust_lr_fn: {}', adjust_lr_fn)
-        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov,
-                                      ns_coefficients=_coefficients(ns_coefficients), eps=eps, ns_steps=ns_steps,
-                                      adjust_lr_fn=adjust_lr_fn))
+        options = dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov, ns_coefficients=_coefficients(ns_coefficients),
+                       eps=eps, ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn)
+        self._check_options(options)
+        super().__init__(params, options)
+
+    @staticmethod
+    def _check_options(group):
+        _check(group['lr'] >= 0.0, 'Invalid learning rate: {}', group['lr'])
+        _check(0.0 <= group['momentum'] < 1.0, 'Invalid momentum value: {}', group['momentum'])
+        _check(group['weight_decay'] >= 0.0, 'Invalid weight_decay value: {}', group['weight_decay'])
+        _check(0.0 < group['eps'] <= 1e30, 'Invalid epsilon value: {}', group['eps'])
+        steps, coefficients = group['ns_steps'], _coefficients(group['ns_coefficients'])
+        _check(steps.__class__ is int and 1 <= steps <= 100, 'Invalid number of steps: {}', steps)
+        _check(group['adjust_lr_fn'] in _ADJUST, 'Invalid adjust_lr_fn: {}', group['adjust_lr_fn'])
+        _check(not _grow(*coefficients, steps), 'Newton-Schulz coefficients {} let singular values grow past 1.9', coefficients)
+        return coefficients
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
-        for p in self.param_groups[-1]['params']:
+        group = self.param_groups.pop()
+        for p in group['params']:
             if p.ndim < 2:
-                self.param_groups.pop()
                 raise ValueError(f'Muon takes matrices, got a parameter of shape {p.shape}')
+        self._check_options(group)
+        self.param_groups.append(group)
 
     def step(self):
+        work = []
         for group, members in self._with_grad():
-            states = [self.state[p] for p in members]
-            for p, state in zip(members, states):
-                if 'momentum_buffer' not in state:
-                    F._device(p)
-                    state['momentum_buffer'] = hiparray.zeros(p.data.shape)
-            F.muon(members, [p.grad for p in members], [s['momentum_buffer'] for s in states], group['lr'], group['momentum'],
-                   group['weight_decay'], group['nesterov'], group['ns_steps'], group['ns_coefficients'], group['eps'],
-                   _ADJUST[group['adjust_lr_fn']])
+            coefficients = self._check_options(group)       # (they may have been changed, or loaded)
+            if members:
+                momenta = [self.state[p].get('momentum_buffer') for p in members]
+                work.append((group, members, momenta, [F.muon_matrix(p, p.grad, m) for p, m in zip(members, momenta)], coefficients))
+        groups = []
+        for group, members, momenta, matrices, coefficients in work:
+            if None in momenta:
+                for p in members:
+                    if 'momentum_buffer' not in self.state[p]:
+                        self.state[p]['momentum_buffer'] = hiparray.zeros(p.data.shape)
+                momenta = [self.state[p]['momentum_buffer'] for p in members]
+            arguments = (group['lr'], group['momentum'], group['weight_decay'], int(bool(group['nesterov'])), group['ns_steps'],
+                         *coefficients, group['eps'])
+            groups.append((members, [p.grad for p in members], momenta, matrices, _ADJUST[group['adjust_lr_fn']], arguments))
+        F.muon(groups)

@@ -50,3 +50,36 @@ def test_what_is_not_finite_is_nan_for_any_eps(rows, columns):
             x = _matrix(rows, columns)
             x[3, 4] = value
             assert np.isnan(tt.optim.orthogonalize(_tensor(x), eps=eps).data.get()).all()
+
+
+def test_a_step_has_its_memory_before_it_begins():
+    """Several batches of matrices: asked for without tables, a step's scratch memory does not grow any more."""
+    import ctypes
+
+    from pytortto_amd import _hip
+
+    def taken():
+        sizes = [ctypes.c_size_t() for _ in range(3)]
+        _hip.call('tt_mem_stats', *[ctypes.byref(n) for n in sizes])
+        return sizes[2].value
+
+    shapes = [(3, 5)] * 3 + [(100, 70 + i) for i in range(50)] + [(900, 1000)] * 50
+    leaves = [_tensor(_matrix(*s), True) for s in shapes]
+    opt = tt.optim.Muon([{'params': leaves[:60]}, {'params': leaves[60:], 'lr': 0.25}])
+    before = [leaf.data.get() for leaf in leaves]
+    _hip.call('tt_empty_cache')
+    for i in (slice(0, 60), slice(60, None)):
+        count = len(shapes[i])
+        _hip.call('tt_muon_step_multi_f32', count, None, None, None, (ctypes.c_int * count)(*[s[0] for s in shapes[i]]),
+                  (ctypes.c_int * count)(*[s[1] for s in shapes[i]]), (ctypes.c_double * count)(*[1.0] * count), 0.1, 0.9, 0.0, 1, 5,
+                  3.4445, -4.7750, 2.0315, 1e-7)
+    asked = taken()
+    assert asked > 0
+    for leaf, v in zip(leaves, before):
+        np.testing.assert_array_equal(leaf.data.get(), v)
+        leaf.grad = hiparray(v)
+    opt.step()
+    assert taken() == asked
+    assert all((leaf.data.get() != v).any() for leaf, v in zip(leaves, before))
+    with pytest.raises(RuntimeError, match='null table'):
+        _hip.call('tt_muon_step_multi_f32', 1, leaves[0].data.ptr, None, None, None, None, None, 0.1, 0.9, 0.0, 1, 5, 3.4445, -4.7750, 2.0315, 1e-7)
