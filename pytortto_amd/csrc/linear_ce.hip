@@ -171,14 +171,20 @@ __global__ __launch_bounds__(256) void lce_rows(Rows<T> of_x, Rows<T> of_w, unsi
 
 // x times g, and W, as operands of the gradients' products: float32 with one scale for the whole matrix.  G threads have a row.  Bound
 // by memory: 32768 + 4096 rows of 1024 53 us, 5.7 TB/s.
+struct Again {
+  Rows<float> x, w;
+  const float* g;       // of x's rows
+  unsigned blocks_x, blocks;
+  int columns, ld;
+};
 template <int G>
-__global__ __launch_bounds__(256) void lce_again(Rows<float> of_x, Rows<float> of_w, const float* __restrict__ g, unsigned blocks_x, int columns,
-                                                 int ld, const Control* __restrict__ control) {
-  const bool second = blockIdx.x >= blocks_x;
-  const Rows<float>& q = second ? of_w : of_x;
-  const long long row = (long long)(blockIdx.x - (second ? blocks_x : 0)) * (256 / G) + row_of_block<G>();
+__device__ __forceinline__ void again_rows(const Again& a, unsigned block, const Control* __restrict__ control) {
+  const bool second = block >= a.blocks_x;
+  const Rows<float>& q = second ? a.w : a.x;
+  const long long row = (long long)(block - (second ? a.blocks_x : 0)) * (256 / G) + row_of_block<G>();
   if (row >= q.rows) return;
-  const int quads = (columns + 63) / 64 * 16;
+  const float* g = a.g;
+  const int columns = a.columns, ld = a.ld, quads = (columns + 63) / 64 * 16;
   const float* x = q.from + (size_t)row * columns;
   char* y = q.to + (size_t)row * ld;
   const bool kept = !q.t.at || class_of(q.t, q.first + row) != kIgnored, whole = columns % 4 == 0;
@@ -211,6 +217,13 @@ __global__ __launch_bounds__(256) void lce_again(Rows<float> of_x, Rows<float> o
     store_terms(y, k * 4, v);
   }
 }
+
+constexpr int kAgainWave = 1024;      // columns that a wave takes, 16 a lane; of more a block has a row
+__device__ __forceinline__ void again_block(const Again& a, unsigned block, const Control* __restrict__ control) {
+  if (a.columns <= kAgainWave) again_rows<64>(a, block, control);
+  else again_rows<256>(a, block, control);
+}
+__global__ __launch_bounds__(256) void lce_again(Again a, const Control* __restrict__ control) { again_block(a, blockIdx.x, control); }
 
 // Columns of the logits, or rows of a gradient, that a launch has, and how many blocks of columns are in front of it.
 struct Part {
@@ -547,11 +560,16 @@ __device__ __forceinline__ void few_row(const Logits& q, int rows, int V, const 
   if (!z) return;
   for (int k = threadIdx.x; k < quads; k += 256) store_gradient<TERMS>(floatx4{}, z, k * 4);
 }
+// Blocks behind the rows' bring x and W into the form of the gradients' products: a launch less.
 template <int TERMS>
 __global__ __launch_bounds__(256) void lce_few(Logits q, int rows, int V, const float* __restrict__ g, float* __restrict__ loss,
-                                               const Control* __restrict__ control, Total all) {
+                                               const Control* __restrict__ control, Total all, Again again) {
+  if ((int)blockIdx.x >= rows) {
+    if (TERMS == 2) again_block(again, blockIdx.x - rows, control);
+    return;
+  }
   few_row<TERMS>(q, rows, V, g, loss, control);
-  if (all.to) total_by_last(all, loss, gridDim.x);
+  if (all.to) total_by_last(all, loss, rows);
 }
 
 // What the two gradients' products do with their sums: take the scales back, and store them as float32 (to or on top of what is there)
@@ -752,13 +770,10 @@ void launch_rows(const Rows<T>& x, const Rows<T>& w, int columns, int ld) {
   else lce_rows<T, 256><<<blocks, 256, 0, stream()>>>(x, w, blocks_x, columns, ld);
 }
 
-int launch_again(const Rows<float>& x, const Rows<float>& w, const float* g, int columns, int ld, const Control* control) {
-  const int side = columns <= 1024 ? 4 : 1;
-  const unsigned blocks_x = (unsigned)((x.rows + side - 1) / side), blocks = blocks_x + (unsigned)((w.rows + side - 1) / side);
-  if (side == 4) lce_again<64><<<blocks, 256, 0, stream()>>>(x, w, g, blocks_x, columns, ld, control);
-  else lce_again<256><<<blocks, 256, 0, stream()>>>(x, w, g, blocks_x, columns, ld, control);
-  TT_LAUNCH_CHECK();
-  return 0;
+Again again_of(const Rows<float>& x, const Rows<float>& w, const float* g, int columns, int ld) {
+  const int side = columns <= kAgainWave ? 4 : 1;
+  const unsigned blocks_x = (unsigned)((x.rows + side - 1) / side);
+  return {x, w, g, blocks_x, blocks_x + (unsigned)((w.rows + side - 1) / side), columns, ld};
 }
 
 // Where the tiles are not whole rounds over the compute units and few are left for the last one, the last columns (of n, m the other side)
@@ -916,10 +931,12 @@ int run(const Call& q) {
       lce_begin<<<1, 1024, 0, stream()>>>(q.t, N, first, rows, mean, e, f, q.g, control);
       TT_LAUNCH_CHECK();
     }
+    Again again = {};
     if constexpr (TERMS == 2) {
-      const Rows<float> again_x = {from, base + at_x2, f, q.dw ? rows : 0, q.t, first};
-      const Rows<float> again_w = {(const float*)q.w, base + at_w2, nullptr, q.dx && first == 0 ? V : 0, none, 0};
-      if (again_x.rows + again_w.rows > 0 && launch_again(again_x, again_w, q.g ? q.g + first : nullptr, H, ldx, control)) return -1;
+      again = again_of({from, base + at_x2, f, q.dw ? rows : 0, q.t, first}, {(const float*)q.w, base + at_w2, nullptr, q.dx && first == 0 ? V : 0, none, 0},
+                       q.g ? q.g + first : nullptr, H, ldx);
+      if (again.blocks && splits == 1) lce_again<<<again.blocks, 256, 0, stream()>>>(again, control);
+      TT_LAUNCH_CHECK();
     }
     const Operand x = {base + at_x, (long long)rows * ldx, ldx, kLine};
     float* losses = q.reduction == 0 && q.loss ? q.loss + first : (float*)(base + at_loss);
@@ -927,7 +944,7 @@ int run(const Call& q) {
     const Logits logits = {f, e, q.t, first, z, Vp, stats, own, blocks, partial, per, splits};
     if (launch_logits<TERMS>(size, x, w, rows, V, H, logits, Part{0, V1, 0})) return -1;
     if (V1 < V && launch_logits<TERMS>(left, x, w, rows, V, H, logits, Part{V1, V, blocks1})) return -1;
-    if (splits > 1) lce_few<TERMS><<<(unsigned)rows, 256, 0, stream()>>>(logits, rows, V, q.g, losses, control, by_last);
+    if (splits > 1) lce_few<TERMS><<<(unsigned)rows + again.blocks, 256, 0, stream()>>>(logits, rows, V, q.g, losses, control, by_last, again);
     else lce_join<<<(unsigned)((rows + 3) / 4), 256, 0, stream()>>>(stats, own, z, Vp, of, losses, q.t, first, rows, blocks, by_last);
     TT_LAUNCH_CHECK();
     if (all.to && !at_once) {
