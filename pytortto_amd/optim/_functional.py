@@ -94,19 +94,18 @@ def muon(groups):
             m.own()
     calls = []
     for params, grads, momenta, matrices, adjust, arguments in groups:
-        rest = [k for k, (rows, columns) in enumerate(matrices) if rows and columns]
+        rest, at = [k for k, (rows, columns) in enumerate(matrices) if rows and columns], [param.data.ptr for param in params]
         while rest:
             now, later = rest, []
-            if len(set(map(id, params))) != len(params):
-                # (one that comes twice is stepped twice, one after the other)
+            if len(set(at)) != len(at):
+                # (a parameter that comes twice, or another on the same memory, is stepped again afterwards)
                 seen, now = set(), []
                 for k in rest:
-                    (later if id(params[k]) in seen else now).append(k)
-                    seen.add(id(params[k]))
+                    (later if at[k] in seen else now).append(k)
+                    seen.add(at[k])
             count = len(now)
             pointers, ints = ctypes.c_void_p * count, ctypes.c_int * count
-            tables = (pointers(*[params[k].data.ptr for k in now]), pointers(*[grads[k].ptr for k in now]),
-                      pointers(*[momenta[k].ptr for k in now]))
+            tables = (pointers(*[at[k] for k in now]), pointers(*[grads[k].ptr for k in now]), pointers(*[momenta[k].ptr for k in now]))
             calls.append((count, tables, (ints(*[matrices[k][0] for k in now]), ints(*[matrices[k][1] for k in now]),
                                           (ctypes.c_double * count)(*[adjust(*matrices[k]) for k in now]), *arguments)))
             rest = later

@@ -83,3 +83,19 @@ def test_a_step_has_its_memory_before_it_begins():
     assert all((leaf.data.get() != v).any() for leaf, v in zip(leaves, before))
     with pytest.raises(RuntimeError, match='null table'):
         _hip.call('tt_muon_step_multi_f32', 1, leaves[0].data.ptr, None, None, None, None, None, 0.1, 0.9, 0.0, 1, 5, 3.4445, -4.7750, 2.0315, 1e-7)
+
+
+def test_tied_weights():
+    """Two parameters on one array are stepped one after the other."""
+    for rows, columns in SIZES:
+        w, g = _matrix(rows, columns, scale=1.0), [_matrix(rows, columns, seed=1), _matrix(rows, columns, seed=2)]
+        one, other = _tensor(w, True), _tensor(w, True)
+        tied = tt.nn.Parameter(one)
+        tt_opt, turns = tt.optim.Muon([one, tied], lr=0.1), [tt.optim.Muon([other], lr=0.1) for _ in range(2)]
+        for _ in range(2):
+            one.grad, tied.grad = hiparray(g[0]), hiparray(g[1])
+            tt_opt.step()
+            for k in range(2):
+                other.grad = hiparray(g[k])
+                turns[k].step()
+            np.testing.assert_array_equal(one.data.get(), other.data.get())

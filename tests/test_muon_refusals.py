@@ -1,11 +1,22 @@
 """CPU: ``optim.Muon`` refuses what it cannot do before anything has moved, and asks for a step's memory before its first launch."""
+from itertools import count
+
 import pytest
 
 import pytortto_amd as tt
 from pytortto_amd import _hip
-from tests.test_products_host import _tensor
 
-ABC = (3.4445, -4.7750, 2.0315)
+_addresses = count(1 << 20, 1 << 20)
+
+
+class _Foreign:
+    def __init__(self, shape, kind):
+        self.__cuda_array_interface__ = {'shape': shape, 'typestr': kind, 'data': (next(_addresses), False), 'version': 3}
+
+
+def _tensor(shape, kind='<f4', grad=False):
+    """(No address here is ever followed.)"""
+    return tt.as_tensor(_Foreign(shape, kind), requires_grad=grad)
 
 
 def _leaf(*shape):
@@ -113,6 +124,18 @@ def test_a_parameter_that_comes_twice(calls):
     opt.step()
     made = _steps(calls)
     assert [m[0] for m in made] == [2, 1, 2, 1] and [m[1] is None for m in made] == [True, True, False, False]
+
+
+def test_parameters_on_the_same_memory(calls):
+    """Tied weights: one after the other, as the same parameter twice is."""
+    a, b = _leaf(4, 6), _leaf(5, 3)
+    tied, turned = tt.nn.Parameter(a), tt.Tensor.on(a.data.reshape(6, 4), True)
+    tied.grad, turned.grad = _tensor((4, 6)).data, _tensor((6, 4)).data
+    opt = tt.optim.Muon([a, tied, b, turned])
+    opt.step()
+    made = _steps(calls)
+    assert [m[0] for m in made] == [2, 1, 1] * 2
+    assert all(len(set(m[1])) == m[0] for m in made[3:])
 
 
 def test_nothing_to_do(calls):
