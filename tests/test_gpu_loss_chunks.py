@@ -30,6 +30,16 @@ def _make(rows, width, vocab, half, seed):
     return x, w, target, g
 
 
+def _over_rows(p, a):
+    """p.T @ a, many rows in parts side by side"""
+    parts = len(p) // 16384
+    if parts < 32:
+        return p.T.contiguous() @ a
+    n = parts * 16384
+    sums = torch.bmm(p[:n].view(parts, 16384, -1).transpose(1, 2).contiguous(), a[:n].view(parts, 16384, -1)).sum(0)
+    return sums + p[n:].T.contiguous() @ a[n:]
+
+
 def _want(x, w, target, g, half):
     """(losses, dx, dw, bound of dx, bound of dw) with a weight g of each position, 0 for those without a target.
 
@@ -53,10 +63,10 @@ def _want(x, w, target, g, half):
         p.scatter_add_(1, t[:, None], torch.full((len(t), 1), -1.0, dtype=torch.float64, device='cuda'))
         p *= (g[i:i + step].double() * kept)[:, None]
         dx[i:i + step] = p @ w
-        dw = dw + p.T.contiguous() @ a
+        dw = dw + _over_rows(p, a)
         p.abs_()
         size_x[i:i + step] = p @ w.abs()
-        size_w = size_w + p.T.contiguous() @ a.abs()
+        size_w = size_w + _over_rows(p, a.abs())
     logit = (44 + 6 * x.shape[1] / 32) * U * most
     gradient = 2 * logit + 12 * U + (2.0 ** -11 if half else 0.0)
     least = 2.0 ** -37 * float(g.max())
