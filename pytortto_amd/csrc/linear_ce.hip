@@ -9,7 +9,9 @@
 // has three products and not a fourth for logits that it forgot, and the scratch memory has a bound that the batch does not move: 2 GiB of logits,
 // 2 GiB of features (twice that with gradients of float32), the weight's terms once or twice, and partial sums.
 //
-// float16: the tensors are the products' operands as they are; G is rounded to float16 once, scaled by 2^14.
+// float16: the weight is the products' operand as it is, and so are the features but for positions without a target; G is rounded to float16
+// once, scaled by 2^14.  That is 11 bits of it: gradients are 2.3 to 3.0e-4 off (norms), of which 2.1 are the rounding of the result itself.  A second
+// term would double the gradients' products, 3.5 of 6.4 ms at 4096 x 2048 x 131072.
 // float32: operands have two float16 terms.  For the logits row i of x and row v of W are scaled by powers of two 2^-f_i and 2^-e_v to below
 // 2^15, so that every position and every class has the digits that it would have alone.  In the gradients' products, where these rows are k, a
 // scale of each row's own would have to be G's, and small rows' G would fall out of its range; there W and g x are scaled by one
@@ -103,7 +105,10 @@ __global__ __launch_bounds__(1024) void lce_begin(Targets t, long long positions
 
 // Rows of x or W as the products' operands: two terms of float32, or a copy of float16.  Rows without a target are
 // zeros, whatever they hold.  G threads have a row; of 16 G columns they keep it between its largest value and its terms.
-// Both matrices share a launch: the first blocks have x's rows.  Bound by memory: 50021 + 777 rows of 1024 float32 72 us, 5.8 TB/s.
+// Both matrices share a launch: the first blocks have x's rows.  Bound by memory: 50021 + 777 rows of 1024 float32 69 us, 6.0 TB/s.
+// A wave has a row of up to kWaveColumns, a block one of more (losses of 64 positions, 50021 float32 classes: of 512 features 83 us and 92 with a
+// block, of 768 117 and 119, of 1024 158 and 151, of 2048 304 and 271).
+constexpr int kWaveColumns = 768;
 template <typename T>
 struct Rows {
   const T* from;
@@ -170,7 +175,7 @@ __global__ __launch_bounds__(256) void lce_rows(Rows<T> of_x, Rows<T> of_w, unsi
 }
 
 // x times g, and W, as operands of the gradients' products: float32 with one scale for the whole matrix.  G threads have a row.  Bound
-// by memory: 32768 + 4096 rows of 1024 53 us, 5.7 TB/s.
+// by memory: 32768 + 4096 rows of 1024 49 us, 6.1 TB/s.
 struct Again {
   Rows<float> x, w;
   const float* g;       // of x's rows
@@ -218,9 +223,8 @@ __device__ __forceinline__ void again_rows(const Again& a, unsigned block, const
   }
 }
 
-constexpr int kAgainWave = 1024;      // columns that a wave takes, 16 a lane; of more a block has a row
 __device__ __forceinline__ void again_block(const Again& a, unsigned block, const Control* __restrict__ control) {
-  if (a.columns <= kAgainWave) again_rows<64>(a, block, control);
+  if (a.columns <= kWaveColumns) again_rows<64>(a, block, control);
   else again_rows<256>(a, block, control);
 }
 __global__ __launch_bounds__(256) void lce_again(Again a, const Control* __restrict__ control) { again_block(a, blockIdx.x, control); }
@@ -764,21 +768,23 @@ int launch_scale(const float* from, const float* g, T* to, size_t n) {
 template <typename T>
 void launch_rows(const Rows<T>& x, const Rows<T>& w, int columns, int ld) {
   // (of kMostRows bytes of rows and 2^20 classes: below 2^32 threads, which is all that a launch can have)
-  const int side = columns <= 1024 ? 4 : 1;
+  const int side = columns <= kWaveColumns ? 4 : 1;
   const unsigned blocks_x = (unsigned)((x.rows + side - 1) / side), blocks = blocks_x + (unsigned)((w.rows + side - 1) / side);
   if (side == 4) lce_rows<T, 64><<<blocks, 256, 0, stream()>>>(x, w, blocks_x, columns, ld);
   else lce_rows<T, 256><<<blocks, 256, 0, stream()>>>(x, w, blocks_x, columns, ld);
 }
 
 Again again_of(const Rows<float>& x, const Rows<float>& w, const float* g, int columns, int ld) {
-  const int side = columns <= kAgainWave ? 4 : 1;
+  const int side = columns <= kWaveColumns ? 4 : 1;
   const unsigned blocks_x = (unsigned)((x.rows + side - 1) / side);
   return {x, w, g, blocks_x, blocks_x + (unsigned)((w.rows + side - 1) / side), columns, ld};
 }
 
 // Where the tiles are not whole rounds over the compute units and few are left for the last one, the last columns (of n, m the other side)
 // are left to smaller tiles, in a launch behind the others': the first of these columns.  (777 x 1024 x 50021 float32, 784 tiles of 256 x 256:
-// the logits took 283 us; 768 of them take 232 and 208 of 64 x 64 behind them 16.)
+// the logits took 283 us; 768 of them take 232 and 208 of 64 x 64 behind them 16.)  Few are a quarter of the units at most, and half of them where
+// they begin with a whole column of tiles: losses of 1024 x 512 x 20000 float32, 60 left, 88 us and 106 as they are; of 5000 x 1024 x 7500 float16, 88
+// left, 122 and 116 as they are.
 long long first_left(long long m, long long n, int size) {
   const long long side = kTileSide[size], high = (m + side - 1) / side, wide = (n + side - 1) / side, units = compute_units();
   const long long rounds = high * wide / units, rest = high * wide % units;
@@ -813,10 +819,13 @@ struct Plan {
 Plan plan_product(long long m, long long n, long long pairs) {
   Plan p;
   p.size = tile_size(m, n);
-  // few tiles and a long reduction: large tiles shared by several blocks
+  // Few tiles and a long reduction: large tiles shared by several blocks, sixteen pairs to each unit.  (Losses with gradients: of 8192 x 768 x 2000
+  // float16 185 us, 217 without; of 8192 x 1024 x 512 107, 112 without or from 256 pairs on, 115 where four pairs are enough; of 1024 x 1024 x 2400
+  // float32 107, 105 and 118.)
   while (p.size < 2 && pairs >= 64 && tiles_of(m, n, p.size + 1) * (pairs / 16) >= compute_units() && std::min(m, n) > kTileSide[p.size]) ++p.size;
   const long long tiles = tiles_of(m, n, p.size);
   long long splits = compute_units() / tiles;
+  // (eight pairs or more to a block: of 8192 x 1024 x 512 float16 107 us, 122 with four and 113 with 32; of 4096 x 256 x 512 float32 66, 66 and 71)
   splits = std::max(1LL, std::min(splits, pairs / 8));
   p.per = (int)((pairs + splits - 1) / splits);
   p.splits = (int)((pairs + p.per - 1) / p.per);
@@ -887,7 +896,8 @@ int run(const Call& q) {
   const int pairsV = (int)(Vp / depth), pairsN = (int)((chunk + depth - 1) / depth);
   const int size = tile_size(chunk, V), V1 = (int)first_left(chunk, V, size), left = V1 < V ? size_left(chunk, V - V1, size) : size;
   const int blocks1 = (V1 + kTileSide[size] - 1) / kTileSide[size], blocks = blocks1 + (V - V1 + kTileSide[left] - 1) / kTileSide[left];
-  // (the reduction of few small tiles is shared out, eight pairs or more to a block: fewer would be loads on their way and little else)
+  // (the reduction of few small tiles is shared out, eight pairs or more to a block: fewer would be loads on their way and little else, though a whole call
+  // is as long with two to sixteen)
   const int pairsH = (int)(Hp / depth);
   int splits = size || several ? 1 : (int)std::max(1LL, std::min(compute_units() / tiles_of(chunk, V, 0), (long long)pairsH / 8));
   const int per = (pairsH + splits - 1) / splits;
