@@ -126,5 +126,6 @@ def linear_cross_entropy(input, weight, target, ignore_index=-100, reduction='me
 
     float32 products are computed from two float16 terms of every value, with float32 sums: 22 bits of it, or 2^-40 of the largest
     value of its row (for the logits) or of its matrix (for the gradients; there ``input`` has its losses' weights on it).  softmax(z) - [v =
-    target] is held to 22 bits, or 2^-40."""
+    target] is held to 22 bits, or 2^-40.  Of float16 tensors products are exact but for their float32 sums, and softmax(z) - [v =
+    target] is rounded to float16 once before it meets them."""
     return LinearCrossEntropy.apply(input, weight, target=target, ignore_index=ignore_index, reduction=reduction)
