@@ -3,19 +3,20 @@
 //   z = x W^T     M_i = max_v z_iv     S_i = sum_v e^(z_iv - M_i)     loss_i = ln S_i + M_i - z_i,t(i)
 //   G_iv = g_i (e^(z_iv - M_i) / S_i - [v = t(i)])        dX = G W        dW = G^T x
 //
-// Positions are worked on in chunks.  Their rows come into the products' form; the first product leaves a chunk's logits in scratch memory (none without gradients)
-// and, with the tile still in registers, every row's maximum and sum over a tile's columns; these are joined, and one pass turns the logits
-// into G where they stand.  The two other products read it there: G^T needs no copy, see product.h.  So a training step
-// has three products and not a fourth for logits that it forgot, and the scratch memory has a bound that the batch does not move: 2 GiB of logits,
-// 2 GiB of features (twice that with gradients of float32), the weight's terms once or twice, and partial sums.
+// Positions are worked on in chunks.  Their rows come into the products' form; the first product leaves the logits in scratch memory
+// (none without gradients) and, with the tile still in registers, every row's maximum and sum over a tile's columns; these are joined, and one
+// pass turns the logits into G where they stand.  The two other products read it there: G^T needs no copy, see product.h.  So a
+// training step has three products and not a fourth for logits that it forgot, and the scratch memory has a bound that the batch does not
+// move: 2 GiB of logits, 2 GiB of features (twice that with gradients of float32), the weight's terms once or twice, and partial sums.
 //
-// float16: the weight is the products' operand as it is, and so are the features but for positions without a target; G is rounded to float16
-// once, scaled by 2^14.  That is 11 bits of it: gradients are 2.3 to 3.0e-4 off (norms), of which 2.1 are the rounding of the result itself.  A second
-// term would double the gradients' products, 3.5 of 6.4 ms at 4096 x 2048 x 131072.
-// float32: operands have two float16 terms.  For the logits row i of x and row v of W are scaled by powers of two 2^-f_i and 2^-e_v to below
-// 2^15, so that every position and every class has the digits that it would have alone.  In the gradients' products, where these rows are k, a
-// scale of each row's own would have to be G's, and small rows' G would fall out of its range; there W and g x are scaled by one
-// power of two each, and G is the bare softmax(z) - [v = t], times 2^15: its entries are held to 2^-22 of themselves and to 2^-40, whatever the rows they meet.
+// float16: the weight is the products' operand as it is where its rows are multiples of 16 bytes, and features are but for positions without
+// a target; G is rounded to float16 once, scaled by 2^14.  That is 11 bits of it: gradients are 2.3 to 3.0e-4 off (norms), of which
+// 2.1 are the rounding of the result itself.  A second term would double the gradients' products, 3.5 of 6.4 ms at 4096 x 2048 x 131072.
+// float32: operands have two float16 terms.  For the logits row i of x and row v of W are scaled by powers of two 2^-f_i and 2^-e_v to
+// below 2^15, so that every position and every class has the digits that it would have alone.  In the gradients' products, where these rows
+// are k, a scale of each row's own would have to be G's, and small rows' G would fall out of its range; there W and g x are scaled by one power
+// of two each, and G is the bare softmax(z) - [v = t], times 2^15: its entries are held to 2^-22 of themselves and to 2^-40, whatever the
+// rows they meet.
 #include "product.h"
 #include "rows.h"
 
